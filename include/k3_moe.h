@@ -303,15 +303,17 @@ bool k3_moe_mx8_quantize_rows_bf16(uint8_t *hi_codes, uint8_t *hi_scales, uint8_
  *   output   = bf16(residual + bf16(full + shared))  (residual nullable)
  *
  * x is the post-attention-norm hidden state [T, H]; the shared expert uses
- * the routed shape's activation. Static weights are bf16 or Q8-128
- * (k3_static_store.h's two kinds). Each step is the library's own entry
+ * the routed shape's activation. Static weights are bf16, Q8-128
+ * (k3_static_store.h's two kinds) or FP8-128. Each step is the library's own entry
  * point of the same operation, so every intermediate is bit-identical to
  * calling them in this order. No reference counterpart as one call: the
  * reference engine issues these launches itself.
  */
 typedef enum {
     K3_MOE_STATIC_BF16 = 0,   /* data bf16 [rows, columns] */
-    K3_MOE_STATIC_Q8_128 = 1  /* data int8 [rows, columns], scales f32 [rows, columns / 128] */
+    K3_MOE_STATIC_Q8_128 = 1, /* data int8 [rows, columns], scales f32 [rows, columns / 128] */
+    K3_MOE_STATIC_FP8_128 = 2 /* data e4m3 [rows, columns], scales f32 [ceil(rows / 128), columns / 128]:
+                                 k3_moe_fp8_128_gemm_bf16's weight, its product at every precision */
 } k3_moe_static_kind;
 
 typedef struct {
@@ -319,7 +321,7 @@ typedef struct {
     uint32_t    rows;
     uint32_t    columns;
     const void *data;
-    const void *scales;   /* Q8-128 only */
+    const void *scales;   /* Q8-128 and FP8-128 */
 } k3_moe_static_weight;
 
 typedef struct {
@@ -381,6 +383,135 @@ bool k3_moe_native_forward_bf16(void *output, const void *hidden, const void *re
 bool k3_moe_proj_mfma_bf16(void *output, const void *weights, const float *scales,
                            const void *input, uint32_t vector_count, uint32_t rows,
                            uint32_t columns, bool q8, void *stream);
+
+/* ---- FP8-128: e4m3 codes with an fp32 scale for each block of 128 -------- */
+
+/*
+ * The encoding of a block of bf16 values (128 values of a token row, or 128 x
+ * 128 of a weight):
+ *   a = max(max |v|, 448 * 2^-126), scale = a / 448, inv = 448 / a,
+ *   code = e4m3(v * inv),
+ * every step rounded to nearest even in fp32; a code stands for e4m3 x scale.
+ * The floor of a keeps scale a normal number (a block of zeros has codes 0 and
+ * scale 2^-126). Only the OCP e4m3 format of gfx950 is meant (largest value
+ * 448, no infinities, 0x7f and 0xff NaN). A NaN gets a NaN code; in a block
+ * with an infinity the infinities get NaN codes, the scale is +inf: rows with
+ * either give NaN in every product. No reference counterpart: the reference's
+ * 8-bit weights are Q8-128.
+ */
+
+/* Token rows: codes [rows, columns], scales f32 [rows, columns / 128].
+ * columns % 128 == 0; src 16-byte, codes 8-byte, scales 4-byte aligned. */
+bool k3_moe_fp8_128_quantize_rows_bf16(uint8_t *codes, float *scales, const void *src,
+                                       uint32_t rows, uint32_t columns, void *stream);
+
+/* A weight: codes [rows, columns], scales f32 [ceil(rows / 128), columns /
+ * 128]; the last block of rows may hold fewer than 128. Otherwise as above. */
+bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const void *src,
+                                         uint32_t rows, uint32_t columns, void *stream);
+
+/*
+ * Product of bf16 token rows with an FP8-128 weight:
+ *   output[t, n] = bf16(sum_b sx[t, b] scales[n / 128, b] sum_{k in block b} qx[t, k] codes[n, k])
+ * with qx, sx the encoding of input[t] in blocks of 128 (as
+ * k3_moe_fp8_128_quantize_rows_bf16 gives it). Code products and their sum
+ * over a block run on FP8 MFMA, the scaled blocks add up in fp32; the order of
+ * the blocks depends on the call's sizes only. columns % 128 == 0; input and
+ * codes 16-byte, scales 4-byte, output 2-byte aligned (8-byte stores where the
+ * output and rows allow them); vector_count <= 65535. scratch (256-byte
+ * aligned device memory): k3_moe_fp8_128_scratch_bytes(vector_count, rows,
+ * columns) bytes, 0 where none is needed (scratch may then be NULL).
+ */
+size_t k3_moe_fp8_128_scratch_bytes(uint32_t vector_count, uint32_t rows, uint32_t columns);
+bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, const float *scales,
+                              const void *input, uint32_t vector_count, uint32_t rows,
+                              uint32_t columns, void *scratch, size_t scratch_bytes, void *stream);
+
+/* One routed expert with FP8-128 weights: codes and scales of each matrix.
+ * Codes 16-byte, scales 4-byte aligned. */
+typedef struct {
+    const uint8_t *gate_codes;   /* [ffn, hidden] */
+    const float   *gate_scales;  /* [ffn / 128, hidden / 128] */
+    const uint8_t *down_codes;   /* [hidden, ffn] */
+    const float   *down_scales;  /* [hidden / 128, ffn / 128] */
+    const uint8_t *up_codes;     /* [ffn, hidden] */
+    const float   *up_scales;    /* [ffn / 128, hidden / 128] */
+} k3_moe_fp8_expert;
+
+/*
+ * The expert stage and the whole layer (k3_moe_experts_bf16 and
+ * k3_moe_forward_bf16) with FP8-128 experts:
+ *   h = act(gate_e . q(hidden[t]), up_e . q(hidden[t]))       fp32
+ *   y[t, r] = bf16(down_e . q(h))                             q: blocks of 128
+ *   output[t] = bf16(residual[t] + bf16(sum_r weights[t, r] * y[t, r]))
+ * The products are k3_moe_fp8_128_gemm_bf16's without its bf16 rounding; h is
+ * encoded from fp32. residual may be NULL. experts is a DEVICE array of
+ * expert_count descriptors. A route whose id is not below expert_count, or
+ * repeats an earlier rank's of its token, adds nothing. hidden % 128 == 0 and
+ * ffn % 128 == 0; output, hidden and residual 16-byte aligned; the workspace
+ * 256-byte aligned, k3_moe_fp8_workspace_bytes(shape, T) bytes, no state kept
+ * in it between calls; token_count <= 65535. expert_ids and expert_weights of
+ * the layer are optional copies of the routes.
+ */
+size_t k3_moe_fp8_workspace_bytes(const k3_moe_shape *shape, uint32_t token_count);
+bool k3_moe_fp8_experts_bf16(void *output, const void *hidden, const void *residual,
+                             const void *expert_ids, const void *expert_weights,
+                             const k3_moe_fp8_expert *experts, const k3_moe_shape *shape,
+                             uint32_t token_count, void *workspace, size_t workspace_bytes,
+                             void *stream);
+bool k3_moe_fp8_forward_bf16(void *output, const void *hidden, const void *residual,
+                             const void *router_weight, const void *router_bias,
+                             const k3_moe_fp8_expert *experts, const k3_moe_shape *shape,
+                             uint32_t token_count, void *expert_ids, void *expert_weights,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- the router in training ---------------------------------------------- */
+
+/*
+ * Balance loss of a batch of segments (sequences) of `length` tokens each,
+ * token t = s * length + i, on the router's logits [T, E] and the ids [T, k]
+ * that it chose. With sigma = sigmoid(logits), Z[t] = sum_e sigma[t, e], N[s]
+ * the segment's live tokens (mask[t] != 0; a NULL mask is all ones):
+ *   counts[s, e]      live tokens of s with a route to e
+ *   mean_scores[s, e] = 1 / N[s] sum_{t live} sigma[t, e] / Z[t]
+ *   loss = coefficient / segments * sum_s sum_e E counts[s, e] / (k N[s]) * mean_scores[s, e]
+ *   live_tokens[s] = N[s]
+ * One segment is the loss over the whole batch. A route is counted as
+ * k3_moe_route_plan does: ids from E on and a token's repeated ids are not. A
+ * segment without live tokens has mean scores 0 and adds nothing; a token
+ * whose scores are all 0 (logits below -103 or -inf throughout) has shares 0.
+ * Sums run in an order set by the sizes alone. The reference only
+ * serves; it has no counterpart. segments * length <= 2^24, E <= 1024, k <= 32,
+ * k <= E. scratch: k3_moe_balance_scratch_bytes(segments, length, E) bytes,
+ * 256-byte aligned.
+ */
+size_t k3_moe_balance_scratch_bytes(uint32_t segments, uint32_t length, uint32_t expert_count);
+bool k3_moe_balance_loss_f32(float *loss, uint32_t *counts, float *mean_scores,
+                             uint32_t *live_tokens, const float *logits,
+                             const uint32_t *expert_ids, const uint8_t *mask, uint32_t segments,
+                             uint32_t length, uint32_t expert_count, uint32_t top_k,
+                             float coefficient, void *scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * Gradient by the router's logits of the balance loss (times *loss_gradient;
+ * NULL is 1) and of the route weights that k3_rocm_router_topk_f32_batch
+ * gives, weights[t, r] = scaling_factor sigma[t, ids[t, r]] / (1e-20 + D[t]),
+ * D[t] the sum of the token's chosen sigma, from weight_gradient [T, k] (NULL:
+ * the loss alone; every route counts as above):
+ *   logits_gradient[t, e] = sigma (1 - sigma) (
+ *       g coefficient / (segments N[s] Z[t]) (f[s, e] - sum_j f[s, j] sigma[t, j] / Z[t])
+ *     + [e = ids[t, r]] scaling_factor / (1e-20 + D) (dw[t, r] - sum_q dw[t, q] sigma[t, ids[t, q]] / (1e-20 + D)))
+ * with f[s, e] = E counts[s, e] / (k N[s]); the ids and counts are constants,
+ * as the choice of experts has no gradient. counts and live_tokens are
+ * k3_moe_balance_loss_f32's. Rows of tokens that are not live are 0.
+ */
+bool k3_moe_router_backward_f32(float *logits_gradient, const float *logits,
+                                const uint32_t *expert_ids, const uint32_t *counts,
+                                const uint32_t *live_tokens, const uint8_t *mask,
+                                const float *loss_gradient, const float *weight_gradient,
+                                uint32_t segments, uint32_t length, uint32_t expert_count,
+                                uint32_t top_k, float coefficient, float scaling_factor,
+                                void *stream);
 
 /*
  * Synthetic resident expert store for benchmarks and tests: fills `bytes`

@@ -45,6 +45,13 @@ class K3MoeExpert(ctypes.Structure):
     ]
 
 
+class K3MoeFp8Expert(ctypes.Structure):
+    """k3_moe_fp8_expert (include/k3_moe.h)."""
+
+    _fields_ = [(n, _p) for n in ("gate_codes", "gate_scales", "down_codes", "down_scales",
+                                  "up_codes", "up_scales")]
+
+
 class K3MoeStaticWeight(ctypes.Structure):
     """k3_moe_static_weight (include/k3_moe.h)."""
 
@@ -129,6 +136,20 @@ SIGNATURES = {
     "k3_moe_synth_fill_host": (None, [_p, _u64, _u64, _u64, _u32]),
     "k3_moe_mx8_quantize_bf16": (_b, [_p, _p, _p, _p, _p, _u64, _p]),
     "k3_moe_mx8_quantize_rows_bf16": (_b, [_p, _p, _p, _p, _p, _u32, _u32, _p]),
+    "k3_moe_fp8_128_quantize_rows_bf16": (_b, [_p, _p, _p, _u32, _u32, _p]),
+    "k3_moe_fp8_128_quantize_weight_bf16": (_b, [_p, _p, _p, _u32, _u32, _p]),
+    "k3_moe_fp8_128_scratch_bytes": (_sz, [_u32, _u32, _u32]),
+    "k3_moe_fp8_128_gemm_bf16": (_b, [_p, _p, _p, _p, _u32, _u32, _u32, _p, _sz, _p]),
+    "k3_moe_fp8_workspace_bytes": (_sz, [ctypes.POINTER(K3MoeShape), _u32]),
+    "k3_moe_fp8_experts_bf16": (_b, [_p, _p, _p, _p, _p, _p, ctypes.POINTER(K3MoeShape), _u32,
+                                     _p, _sz, _p]),
+    "k3_moe_fp8_forward_bf16": (_b, [_p, _p, _p, _p, _p, _p, ctypes.POINTER(K3MoeShape), _u32,
+                                     _p, _p, _p, _sz, _p]),
+    "k3_moe_balance_scratch_bytes": (_sz, [_u32, _u32, _u32]),
+    "k3_moe_balance_loss_f32": (_b, [_p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _f, _p,
+                                     _sz, _p]),
+    "k3_moe_router_backward_f32": (_b, [_p, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
+                                        _f, _f, _p]),
 }
 
 _lib = None

@@ -1,0 +1,387 @@
+/*
+ * The router in training: balance loss with per-expert counts, and the gradient
+ * by the router's logits (include/k3_moe.h has the formulas; the reference only
+ * serves and has no counterpart).
+ *
+ *   balance_part_kernel    a block: a run of one segment's tokens, a token a
+ *                          wave at a time; sums of the shares sigma / Z and
+ *                          the counts of its run
+ *   balance_join_kernel    a block: 64 experts of a segment; joins the runs,
+ *                          writes counts and mean scores; the last block to
+ *                          end adds up the loss
+ *   router_backward_kernel a token a wave at a time, the segment's f in
+ *                          registers
+ *
+ * Expert e of a row is slot e / 64 of lane e % 64. All sums run in an order set
+ * by the sizes: counts are whole numbers, and the last block reads every
+ * partial loss in one order whichever block it is.
+ */
+#include "k3_device.h"
+#include "k3_topk.h"
+#include "../../include/k3_moe.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace k3 {
+namespace {
+
+constexpr uint32_t kWaves = 8;
+
+inline size_t align256(size_t v) { return (v + 255u) & ~(size_t)255u; }
+
+/* sigma(x) and 1 - sigma(x), each to a few ulp of itself: the exponential is
+ * taken of -|x|, so neither is a difference. */
+__device__ __forceinline__ float2 sigmoid_pair(float x) {
+    const float t = __builtin_amdgcn_exp2f(__fmul_rn(fabsf(x), -1.44269504088896341f));
+    const float s = __builtin_amdgcn_rcpf(__fadd_rn(1.0f, t)), l = __fmul_rn(t, s);
+    return x >= 0.0f ? make_float2(s, l) : make_float2(l, s);
+}
+
+/* The route of lane r < k of a token: its id, or E where it has none (no such
+ * rank, an id from E on, or one that an earlier rank has). */
+__device__ __forceinline__ uint32_t lane_route(const uint32_t *ids, uint64_t t, uint32_t k,
+                                               uint32_t E) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t id = lane < k ? ids[t * k + lane] : E;
+    bool again = id >= E;
+    for (uint32_t r = 0; r + 1u < k; r++)
+        again |= lane > r && id == (uint32_t)__builtin_amdgcn_readlane((int)id, (int)r);
+    return again ? E : id;
+}
+
+/* The logits of token t (-inf, score 0, past E). */
+template <int J>
+__device__ __forceinline__ void load_row(float (&x)[J], const float *logits, uint64_t t,
+                                         uint32_t E) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const float *row = logits + t * E;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const uint32_t e = lane + 64u * (uint32_t)j;
+        x[j] = e < E ? row[e] : -__builtin_huge_valf();
+    }
+}
+
+struct BalanceArgs {
+    float *loss;
+    uint32_t *counts;
+    float *mean;
+    uint32_t *live;
+    const float *logits;
+    const uint32_t *ids;
+    const uint8_t *mask;
+    uint32_t S, L, E, k;
+    float coef;
+    uint32_t runs, span; /* runs of `span` tokens of a segment */
+    float *part_mean;    /* [S, runs, E] */
+    uint32_t *part_count;
+    uint32_t *part_live; /* [S, runs] */
+    float *part_loss;    /* [S, ceil(E / 64)] */
+    uint32_t *ticket;
+};
+
+template <int J>
+__global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A) {
+    __shared__ float sums[kWaves][64 * J];
+    __shared__ uint32_t hist[64 * J];
+    __shared__ uint32_t lives[kWaves];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
+    const uint32_t s = blockIdx.x / A.runs, run = blockIdx.x % A.runs;
+    const uint32_t i0 = run * A.span, i1 = min(i0 + A.span, A.L);
+    if (blockIdx.x == 0u && threadIdx.x == 0u) *A.ticket = 0u; /* for the next kernel */
+    for (uint32_t e = threadIdx.x; e < 64u * J; e += 64u * kWaves) hist[e] = 0u;
+    __syncthreads();
+    float acc[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) acc[j] = 0.0f;
+    uint32_t live = 0u;
+    for (uint32_t i = i0 + wave; i < i1; i += kWaves) {
+        const uint64_t t = (uint64_t)s * A.L + i;
+        if (A.mask && A.mask[t] == 0u) continue;
+        live++;
+        float x[J];
+        load_row<J>(x, A.logits, t, E);
+        const uint32_t e = lane_route(A.ids, t, A.k, E);
+        if (e < E) atomicAdd(&hist[e], 1u);
+        float z = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            x[j] = sigmoid_pair(x[j]).x;
+            z = __fadd_rn(z, x[j]);
+        }
+        z = wave_sum(z);
+        const float inv = z == 0.0f ? 0.0f : __fdiv_rn(1.0f, z);
+#pragma unroll
+        for (int j = 0; j < J; j++) acc[j] = fmaf(x[j], inv, acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < J; j++) sums[wave][64 * j + lane] = acc[j];
+    if (lane == 0u) lives[wave] = live;
+    __syncthreads();
+    const uint64_t at = (uint64_t)blockIdx.x * E;
+    for (uint32_t e = threadIdx.x; e < E; e += 64u * kWaves) {
+        float v = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) v = __fadd_rn(v, sums[w][e]);
+        A.part_mean[at + e] = v;
+        A.part_count[at + e] = hist[e];
+    }
+    if (threadIdx.x == 0u) {
+        uint32_t n = 0u;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) n += lives[w];
+        A.part_live[blockIdx.x] = n;
+    }
+}
+
+__global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs A) {
+    __shared__ float fsum[16][64];
+    __shared__ uint32_t csum[16][64];
+    __shared__ uint32_t nsum[16];
+    __shared__ uint32_t last;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
+    const uint32_t cols = (E + 63u) / 64u, s = blockIdx.x / cols, e = 64u * (blockIdx.x % cols) + lane;
+    float m = 0.0f;
+    uint32_t c = 0u, n = 0u;
+    for (uint32_t r = threadIdx.x; r < A.runs; r += 1024u) n += A.part_live[s * A.runs + r];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
+    if (e < E) {
+        const uint64_t at = (uint64_t)s * A.runs * E + e;
+#pragma unroll 8
+        for (uint32_t r = wave; r < A.runs; r += 16u) {
+            m = __fadd_rn(m, A.part_mean[at + (uint64_t)r * E]);
+            c += A.part_count[at + (uint64_t)r * E];
+        }
+    }
+    fsum[wave][lane] = m;
+    csum[wave][lane] = c;
+    if (lane == 0u) nsum[wave] = n;
+    __syncthreads();
+    if (wave == 0u) {
+        m = 0.0f, c = 0u, n = 0u;
+#pragma unroll
+        for (uint32_t w = 0; w < 16u; w++) {
+            m = __fadd_rn(m, fsum[w][lane]);
+            c += csum[w][lane];
+            n += nsum[w];
+        }
+        m = n ? __fdiv_rn(m, (float)n) : 0.0f;
+        float l = 0.0f;
+        if (e < E) {
+            A.counts[(uint64_t)s * E + e] = c;
+            A.mean[(uint64_t)s * E + e] = m;
+            if (n) l = __fmul_rn(__fdiv_rn(__fmul_rn((float)c, (float)E), __fmul_rn((float)A.k, (float)n)), m);
+        }
+        if (e == 0u) A.live[s] = n;
+        l = wave_sum(l);
+        if (lane == 0u) {
+            __hip_atomic_store(&A.part_loss[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = __hip_atomic_fetch_add(A.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+                   gridDim.x - 1u;
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    float v = 0.0f;
+    for (uint32_t i = threadIdx.x; i < gridDim.x; i += 1024u)
+        v = __fadd_rn(v, __hip_atomic_load(&A.part_loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    v = wave_sum(v);
+    if (lane == 0u) fsum[wave][0] = v;
+    __syncthreads();
+    if (threadIdx.x == 0u) {
+        v = 0.0f;
+        for (uint32_t w = 0; w < 16u; w++) v = __fadd_rn(v, fsum[w][0]);
+        *A.loss = __fmul_rn(v, __fdiv_rn(A.coef, (float)A.S));
+    }
+}
+
+struct BackwardArgs {
+    float *out;
+    const float *logits;
+    const uint32_t *ids, *counts, *live;
+    const uint8_t *mask;
+    const float *dloss, *dw;
+    uint32_t S, L, E, k;
+    float coef, scale;
+    uint32_t runs, span;
+};
+
+template <int J>
+__global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(BackwardArgs A) {
+    __shared__ float rows[kWaves][64 * J];
+    __shared__ float adds[kWaves][64 * J];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
+    const uint32_t s = blockIdx.x / A.runs, run = blockIdx.x % A.runs;
+    const uint32_t i0 = run * A.span, i1 = min(i0 + A.span, A.L);
+    float *row = rows[wave], *add = adds[wave];
+    const uint32_t n = A.live[s];
+    /* f, and the factor that the loss has in common: both 0 without live tokens */
+    const float per = n ? __fdiv_rn((float)E, __fmul_rn((float)A.k, (float)n)) : 0.0f;
+    float share = n ? __fdiv_rn(__fdiv_rn(A.coef, (float)A.S), (float)n) : 0.0f;
+    if (A.dloss) share = __fmul_rn(share, *A.dloss);
+    float f[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const uint32_t e = lane + 64u * (uint32_t)j;
+        f[j] = e < E ? __fmul_rn((float)A.counts[(uint64_t)s * E + e], per) : 0.0f;
+        add[e] = 0.0f;
+    }
+    for (uint32_t i = i0 + wave; i < i1; i += kWaves) {
+        const uint64_t t = (uint64_t)s * A.L + i;
+        float *out = A.out + t * E;
+        if (A.mask && A.mask[t] == 0u) {
+#pragma unroll
+            for (int j = 0; j < J; j++)
+                if (lane + 64u * (uint32_t)j < E) out[lane + 64u * (uint32_t)j] = 0.0f;
+            continue;
+        }
+        float x[J], d[J];
+        load_row<J>(x, A.logits, t, E);
+        float z = 0.0f, a = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const float2 p = sigmoid_pair(x[j]);
+            x[j] = p.x;
+            d[j] = __fmul_rn(p.x, p.y);
+            z = __fadd_rn(z, p.x);
+            a = fmaf(f[j], p.x, a);
+        }
+        z = wave_sum(z);
+        a = wave_sum(a);
+        const float inv = z == 0.0f ? 0.0f : __fdiv_rn(1.0f, z);
+        const float mean = __fmul_rn(a, inv), by = __fmul_rn(share, inv);
+        uint32_t e = E;
+        if (A.dw) { /* the routes' part, by expert, through LDS */
+#pragma unroll
+            for (int j = 0; j < J; j++) row[64 * j + lane] = x[j];
+            e = lane_route(A.ids, t, A.k, E);
+            const float dw = e < E ? A.dw[t * A.k + lane] : 0.0f;
+            wave_fence();
+            const float sig = e < E ? row[e] : 0.0f;
+            const float den = __fadd_rn(wave_sum(sig), 1e-20f);
+            const float m = __fdiv_rn(wave_sum(__fmul_rn(dw, sig)), den);
+            if (e < E) add[e] = __fmul_rn(__fdiv_rn(A.scale, den), __fsub_rn(dw, m));
+            wave_fence();
+        }
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const uint32_t q = lane + 64u * (uint32_t)j;
+            float v = __fmul_rn(by, __fsub_rn(f[j], mean));
+            if (A.dw) v = __fadd_rn(v, add[q]);
+            if (q < E) out[q] = __fmul_rn(v, d[j]);
+        }
+        if (A.dw) {
+            wave_fence();
+            if (e < E) add[e] = 0.0f;
+            wave_fence();
+        }
+    }
+}
+
+/* Runs a segment is cut into: about 256 blocks in all (two tokens a wave at
+ * least, so that a run's partial sums stay a small part of its reads). */
+void runs_of(uint32_t S, uint32_t L, uint32_t blocks, uint32_t &runs, uint32_t &span) {
+    const uint32_t want = (blocks + S - 1u) / S, most = (L + 2u * kWaves - 1u) / (2u * kWaves);
+    runs = want < most ? want : most;
+    span = (L + runs - 1u) / runs;
+    runs = (L + span - 1u) / span;
+}
+
+bool batch_ok(uint32_t S, uint32_t L, uint32_t E) {
+    return S != 0u && S <= 65535u && L != 0u && (uint64_t)S * L <= (1ull << 24) && E != 0u &&
+           E <= 1024u;
+}
+
+size_t carve(BalanceArgs &A, void *base) {
+    uint8_t *p = (uint8_t *)base;
+    size_t off = 0;
+    auto take = [&](size_t n) {
+        uint8_t *q = p ? p + off : nullptr;
+        off += align256(n);
+        return q;
+    };
+    const size_t parts = (size_t)A.S * A.runs;
+    A.part_mean = (float *)take(4u * parts * A.E);
+    A.part_count = (uint32_t *)take(4u * parts * A.E);
+    A.part_live = (uint32_t *)take(4u * parts);
+    A.part_loss = (float *)take(4u * (size_t)A.S * ((A.E + 63u) / 64u));
+    A.ticket = (uint32_t *)take(4u);
+    return off;
+}
+
+constexpr uint32_t kBlocks = 256;
+
+/* f(integral_constant<int, J>) for the least J of 1, 2, 4, 8, 16 with E <= 64 J */
+template <class F>
+void with_slots(uint32_t E, F &&f) {
+    if (E <= 64u) f(std::integral_constant<int, 1>{});
+    else if (E <= 128u) f(std::integral_constant<int, 2>{});
+    else if (E <= 256u) f(std::integral_constant<int, 4>{});
+    else if (E <= 512u) f(std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, 16>{});
+}
+
+}  // namespace
+}  // namespace k3
+
+using namespace k3;
+
+extern "C" size_t k3_moe_balance_scratch_bytes(uint32_t segments, uint32_t length,
+                                               uint32_t expert_count) {
+    if (!batch_ok(segments, length, expert_count)) return 0u;
+    BalanceArgs A{};
+    A.S = segments, A.L = length, A.E = expert_count;
+    runs_of(segments, length, kBlocks, A.runs, A.span);
+    return carve(A, nullptr);
+}
+
+extern "C" bool k3_moe_balance_loss_f32(float *loss, uint32_t *counts, float *mean_scores,
+                                        uint32_t *live_tokens, const float *logits,
+                                        const uint32_t *expert_ids, const uint8_t *mask,
+                                        uint32_t segments, uint32_t length, uint32_t expert_count,
+                                        uint32_t top_k, float coefficient, void *scratch,
+                                        size_t scratch_bytes, void *stream) {
+    if (!loss || !counts || !mean_scores || !live_tokens || !logits || !expert_ids || !scratch ||
+        !batch_ok(segments, length, expert_count) || top_k == 0u || top_k > 32u ||
+        top_k > expert_count || ((uintptr_t)scratch % 256u) != 0u ||
+        scratch_bytes < k3_moe_balance_scratch_bytes(segments, length, expert_count))
+        return false;
+    BalanceArgs A{loss, counts, mean_scores, live_tokens, logits, expert_ids, mask, segments, length,
+                  expert_count, top_k, coefficient};
+    runs_of(segments, length, kBlocks, A.runs, A.span);
+    carve(A, scratch);
+    const hipStream_t st = (hipStream_t)stream;
+    with_slots(expert_count, [&](auto J) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(balance_part_kernel<decltype(J)::value>),
+                           dim3(segments * A.runs), dim3(64u * kWaves), 0, st, A);
+    });
+    hipLaunchKernelGGL(balance_join_kernel, dim3(segments * ((expert_count + 63u) / 64u)), dim3(1024),
+                       0, st, A);
+    return hipGetLastError() == hipSuccess;
+}
+
+extern "C" bool k3_moe_router_backward_f32(float *logits_gradient, const float *logits,
+                                           const uint32_t *expert_ids, const uint32_t *counts,
+                                           const uint32_t *live_tokens, const uint8_t *mask,
+                                           const float *loss_gradient,
+                                           const float *weight_gradient, uint32_t segments,
+                                           uint32_t length, uint32_t expert_count, uint32_t top_k,
+                                           float coefficient, float scaling_factor, void *stream) {
+    if (!logits_gradient || !logits || !counts || !live_tokens ||
+        (weight_gradient && !expert_ids) || !batch_ok(segments, length, expert_count) ||
+        top_k == 0u || top_k > 32u || top_k > expert_count || !(scaling_factor > 0.0f))
+        return false;
+    BackwardArgs A{logits_gradient, logits, expert_ids, counts, live_tokens, mask, loss_gradient,
+                   weight_gradient, segments, length, expert_count, top_k, coefficient,
+                   scaling_factor, 0u, 0u};
+    runs_of(segments, length, kBlocks, A.runs, A.span);
+    with_slots(expert_count, [&](auto J) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(router_backward_kernel<decltype(J)::value>),
+                           dim3(segments * A.runs), dim3(64u * kWaves), 0, (hipStream_t)stream, A);
+    });
+    return hipGetLastError() == hipSuccess;
+}

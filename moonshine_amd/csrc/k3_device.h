@@ -425,4 +425,25 @@ __device__ __forceinline__ float mx8_inv_scale(uint32_t byte) {
     return __uint_as_float((254u - byte) << 23);
 }
 
+/* ---- routes -------------------------------------------------------------- */
+
+/* Route (t, r) is valid when its id is < E and no earlier rank of token t
+ * chose the same expert (the router never does; external ids might). The
+ * token's k <= K ids are read once into registers (all loads issued
+ * together); invalid routes come back as E. A later duplicate matches the
+ * first occurrence, which stays, so invalidating in place keeps the rule. */
+template <int K>
+__device__ __forceinline__ void token_routes(const uint32_t *ids, uint32_t t, uint32_t k,
+                                             uint32_t E, uint32_t (&e)[K]) {
+#pragma unroll
+    for (int r = 0; r < K; r++) e[r] = (uint32_t)r < k ? ids[(uint64_t)t * k + r] : E;
+#pragma unroll
+    for (int r = 0; r < K; r++) {
+        if (e[r] >= E) e[r] = E;
+#pragma unroll
+        for (int q = 0; q < r; q++)
+            if (e[q] == e[r]) e[r] = E;
+    }
+}
+
 }  // namespace k3

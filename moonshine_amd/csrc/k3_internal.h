@@ -84,6 +84,12 @@ bool launch_router_topk(uint32_t *ids, float *w, uint32_t *ids2, float *w2,
                         uint32_t experts, uint32_t top_k, float scale,
                         hipStream_t stream);
 
+/* out[t] = bf16(residual + bf16(sum_r w[t, r] y[t k + r])) in rank order; routes
+ * with an id from E on are skipped. H % 8 == 0, rows 16-byte aligned. */
+bool launch_combine(void *output, const uint16_t *y, const void *residual, const uint32_t *ids,
+                    const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E,
+                    hipStream_t stream);
+
 /* Counter-based generator of the synthetic expert store. */
 __host__ __device__ inline uint64_t mix64(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;

@@ -141,25 +141,6 @@ Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
 /* routing plan                                                              */
 /* ------------------------------------------------------------------------ */
 
-/* Route (t, r) is valid when its id is < E and no earlier rank of token t
- * chose the same expert (the router never does; external ids might). The
- * token's k <= K ids are read once into registers (all loads issued
- * together); invalid routes come back as E. A later duplicate matches the
- * first occurrence, which stays, so invalidating in place keeps the rule. */
-template <int K>
-__device__ __forceinline__ void token_routes(const uint32_t *ids, uint32_t t, uint32_t k,
-                                             uint32_t E, uint32_t (&e)[K]) {
-#pragma unroll
-    for (int r = 0; r < K; r++) e[r] = (uint32_t)r < k ? ids[(uint64_t)t * k + r] : E;
-#pragma unroll
-    for (int r = 0; r < K; r++) {
-        if (e[r] >= E) e[r] = E;
-#pragma unroll
-        for (int q = 0; q < r; q++)
-            if (e[q] == e[r]) e[r] = E;
-    }
-}
-
 template <int K>
 __global__ __launch_bounds__(256) void plan_count_kernel(uint32_t *__restrict__ chunk_counts,
                                                          const uint32_t *__restrict__ ids,
@@ -343,6 +324,19 @@ __global__ __launch_bounds__(128) void combine_kernel(
     *(uint4 *)(out + o) = make_uint4(ov[0], ov[1], ov[2], ov[3]);
 }
 
+}  // namespace
+
+bool k3::launch_combine(void *output, const uint16_t *y, const void *residual, const uint32_t *ids,
+                        const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E,
+                        hipStream_t st) {
+    hipLaunchKernelGGL(combine_kernel, dim3((H / 8u + kCombineThreads - 1u) / kCombineThreads, T),
+                       dim3(kCombineThreads), 0, st, (uint16_t *)output, y,
+                       (const uint16_t *)residual, ids, weights, H, k, E);
+    return hipGetLastError() == hipSuccess;
+}
+
+namespace {
+
 /* ------------------------------------------------------------------------ */
 /* synthetic store                                                           */
 /* ------------------------------------------------------------------------ */
@@ -449,11 +443,9 @@ bool run_experts(const Workspace &ws, void *output, const void *hidden, const vo
             !launch_exact_down(g, ws.y, ws.act, st))
             return false;
         mark(K3_MOE_STAGE_COMBINE);
-        hipLaunchKernelGGL(combine_kernel, dim3((H / 8u + kCombineThreads - 1u) / kCombineThreads, T),
-                           dim3(kCombineThreads), 0, st, (uint16_t *)output, ws.y,
-                           (const uint16_t *)residual, ws.ids, ws.weights, H, k, E);
+        const bool ok = launch_combine(output, ws.y, residual, ws.ids, ws.weights, T, H, k, E, st);
         mark(K3_MOE_STAGE_END);
-        return hipGetLastError() == hipSuccess;
+        return ok;
     }
     mark(K3_MOE_STAGE_GATE_UP);
     if (!launch_exact_tiles(g, st) ||
@@ -462,11 +454,9 @@ bool run_experts(const Workspace &ws, void *output, const void *hidden, const vo
     mark(K3_MOE_STAGE_DOWN);
     if (!launch_exact_down(g, ws.y, ws.act, st)) return false;
     mark(K3_MOE_STAGE_COMBINE);
-    hipLaunchKernelGGL(combine_kernel, dim3((H / 8u + kCombineThreads - 1u) / kCombineThreads, T),
-                       dim3(kCombineThreads), 0, st, (uint16_t *)output, ws.y,
-                       (const uint16_t *)residual, ws.ids, ws.weights, H, k, E);
+    const bool ok = launch_combine(output, ws.y, residual, ws.ids, ws.weights, T, H, k, E, st);
     mark(K3_MOE_STAGE_END);
-    return hipGetLastError() == hipSuccess;
+    return ok;
 }
 
 }  // namespace

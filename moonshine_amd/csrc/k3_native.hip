@@ -11,6 +11,7 @@
 #include "../../include/k3_moe.h"
 #include "../../include/k3_rocm_ops.h"
 #include "k3_decode.h"
+#include "k3_fp8.h"
 #include "k3_internal.h"
 #include "k3_topk.h"
 
@@ -30,6 +31,8 @@ struct NativeWorkspace {
     uint16_t *latent, *routed, *normed, *full, *gate, *up, *act, *shared, *sum;
     void *experts;
     size_t expert_bytes, bytes;
+    void *fp8[2]; /* scratch of the FP8-128 projections: the side stream's and the main one's */
+    size_t fp8_bytes;
 };
 
 NativeWorkspace carve(void *base, const k3_moe_native_shape &s, uint32_t T) {
@@ -58,6 +61,12 @@ NativeWorkspace carve(void *base, const k3_moe_native_shape &s, uint32_t T) {
     w.sum = (uint16_t *)take(2u * T * H);
     w.expert_bytes = k3_moe_workspace_bytes(&s.routed, T);
     w.experts = take(w.expert_bytes);
+    const size_t fp8[4] = {k3_moe_fp8_128_scratch_bytes(T, (uint32_t)D, (uint32_t)H),
+                           k3_moe_fp8_128_scratch_bytes(T, (uint32_t)H, (uint32_t)D),
+                           k3_moe_fp8_128_scratch_bytes(T, (uint32_t)S, (uint32_t)H),
+                           k3_moe_fp8_128_scratch_bytes(T, (uint32_t)H, (uint32_t)S)};
+    for (size_t n : fp8) w.fp8_bytes = n > w.fp8_bytes ? n : w.fp8_bytes;
+    for (void *&q : w.fp8) q = take(w.fp8_bytes);
     w.bytes = off;
     return w;
 }
@@ -65,7 +74,10 @@ NativeWorkspace carve(void *base, const k3_moe_native_shape &s, uint32_t T) {
 bool static_ok(const k3_moe_static_weight &w, uint32_t rows, uint32_t cols) {
     if (!w.data || w.rows != rows || w.columns != cols) return false;
     if (w.kind == K3_MOE_STATIC_BF16) return true;
-    return w.kind == K3_MOE_STATIC_Q8_128 && w.scales && cols % 128u == 0u;
+    if (w.kind == K3_MOE_STATIC_FP8_128 &&
+        (((uintptr_t)w.data % 16u) != 0u || ((uintptr_t)w.scales % 4u) != 0u))
+        return false; /* as the product would: refused before the block's first launch */
+    return w.kind <= K3_MOE_STATIC_FP8_128 && w.scales && cols % 128u == 0u;
 }
 
 /* out [T, rows] = w . in [T, columns] with the static weight's own kernel */
@@ -76,7 +88,10 @@ bool static_ok(const k3_moe_static_weight &w, uint32_t rows, uint32_t cols) {
 constexpr uint32_t kProjMfmaMinTokens = 32;
 
 bool project(const k3_moe_static_weight &w, void *out, const void *in, uint32_t T,
-             uint32_t precision, hipStream_t st) {
+             uint32_t precision, const NativeWorkspace &ws, int side, hipStream_t st) {
+    if (w.kind == K3_MOE_STATIC_FP8_128)
+        return k3_moe_fp8_128_gemm_bf16(out, (const uint8_t *)w.data, (const float *)w.scales, in, T,
+                                        w.rows, w.columns, ws.fp8[side], ws.fp8_bytes, st);
     const bool q8 = w.kind == K3_MOE_STATIC_Q8_128;
     if (precision != K3_MOE_EXACT && T >= kProjMfmaMinTokens &&
         k3::proj_mfma_supported(T, w.rows, w.columns, q8, w.data, in))
@@ -201,7 +216,7 @@ extern "C" bool k3_moe_native_forward_bf16(void *output, const void *hidden, con
                                                  W.routed_down.data, W.routed_down.scales, D,
                                                  router_in_pair ? &router : nullptr, st);
     } else {
-        ok = ok && project(W.routed_down, ws.latent, hidden, T, precision, side);
+        ok = ok && project(W.routed_down, ws.latent, hidden, T, precision, ws, 0, side);
     }
     if (ev) ok = ok && hipEventRecord(ev->latent, side) == hipSuccess;
     if (pair) {
@@ -210,8 +225,8 @@ extern "C" bool k3_moe_native_forward_bf16(void *output, const void *hidden, con
                                         W.shared_up.data, W.shared_up.scales, hidden, S, H,
                                         s.routed.activation, beta, lb, side);
     } else {
-        ok = ok && project(W.shared_gate, ws.gate, hidden, T, precision, side) &&
-             project(W.shared_up, ws.up, hidden, T, precision, side) &&
+        ok = ok && project(W.shared_gate, ws.gate, hidden, T, precision, ws, 0, side) &&
+             project(W.shared_up, ws.up, hidden, T, precision, ws, 0, side) &&
              (s.routed.activation == K3_MOE_ACT_SWIGLU
                   ? k3_rocm_swiglu_bf16(ws.act, ws.gate, ws.up, sn, side)
                   : k3_rocm_situ_bf16(ws.act, ws.gate, ws.up, sn, s.routed.beta,
@@ -254,7 +269,7 @@ extern "C" bool k3_moe_native_forward_bf16(void *output, const void *hidden, con
         ok = ok &&
              k3_rocm_rms_norm_bf16(ws.normed, ws.routed, W.routed_norm, T, D, s.norm_epsilon,
                                    st) &&
-             project(W.routed_up, ws.full, ws.normed, T, precision, st);
+             project(W.routed_up, ws.full, ws.normed, T, precision, ws, 1, st);
     }
     if (ev) ok = ok && hipStreamWaitEvent(st, ev->act, 0) == hipSuccess;
     if (fused) {
@@ -262,7 +277,7 @@ extern "C" bool k3_moe_native_forward_bf16(void *output, const void *hidden, con
                                       W.shared_down.scales, ws.act, H, S, ws.full,
                                       (const uint16_t *)residual, st);
     } else {
-        ok = ok && project(W.shared_down, ws.shared, ws.act, T, precision, st);
+        ok = ok && project(W.shared_down, ws.shared, ws.act, T, precision, ws, 1, st);
         const uint64_t n = (uint64_t)T * H;
         if (residual) /* output = bf16(residual + bf16(full + shared)) */
             ok = ok && k3_rocm_add_bf16(ws.sum, ws.full, ws.shared, n, st) &&

@@ -3,10 +3,10 @@
 The routed experts (ExpertStore, MXFP4) run on a latent of width D between
 two static projections (routed_down [D, H], routed_up [H, D]) with an RMSNorm
 in between, beside a dense shared expert (gate/up [S, H], down [H, S]); see
-include/k3_moe.h. Static weights are bf16 or Q8-128. Synthetic weights are
-generated on the device from a seeded torch generator (N(0, 0.02) static
-projections, N(1, 0.1) norm weight); Q8-128 codes come from the library's
-own quantizer. torch is used only for device memory and streams.
+include/k3_moe.h. Static weights are bf16, Q8-128 or FP8-128. Synthetic weights
+are generated on the device from a seeded torch generator (N(0, 0.02) static
+projections, N(1, 0.1) norm weight); 8-bit codes come from the library's
+own quantizers. torch is used only for device memory and streams.
 """
 import ctypes
 from dataclasses import dataclass
@@ -14,11 +14,12 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
+from . import fp8
 from ._lib import K3MoeNativeShape, K3MoeNativeWeights, K3MoeShape, K3MoeStaticWeight, lib
 from .layer import ExpertStore, bf16_bits
 from .synth import ACT_SITU, EXACT, f32_to_bf16_bits
 
-STATIC_BF16, STATIC_Q8 = 0, 1
+STATIC_BF16, STATIC_Q8, STATIC_FP8 = 0, 1, 2
 
 
 @dataclass(frozen=True)
@@ -59,6 +60,8 @@ class StaticWeight:
         w = (torch.randn((rows, cols), generator=gen, device=device) * 0.02).to(torch.bfloat16)
         if kind == STATIC_BF16:
             self.data, self.scales = w, None
+        elif kind == STATIC_FP8:
+            self.data, self.scales = fp8.quantize_weight(w)
         else:
             self.data = torch.empty((rows, cols), dtype=torch.int8, device=device)
             self.scales = torch.empty((rows, cols // 128), dtype=torch.float32, device=device)
@@ -75,9 +78,11 @@ class StaticWeight:
                                  None if self.scales is None else self.scales.data_ptr())
 
     def host(self):
-        """(kind, data, scales) as numpy (bf16 bits or int8 codes + f32)."""
+        """(kind, data, scales) as numpy (bf16 bits, int8 or uint8 codes + f32)."""
         if self.kind == STATIC_BF16:
             return self.kind, bf16_bits(self.data), None
+        if self.kind == STATIC_FP8:
+            return self.kind, self.data.view(torch.uint8).cpu().numpy(), self.scales.cpu().numpy()
         return self.kind, self.data.cpu().numpy(), self.scales.cpu().numpy()
 
     @property
@@ -152,4 +157,5 @@ class NativeLayer:
         return out
 
 
-__all__ = ["NativeConfig", "NativeLayer", "K3_NATIVE_LAYER", "STATIC_BF16", "STATIC_Q8"]
+__all__ = ["NativeConfig", "NativeLayer", "K3_NATIVE_LAYER", "STATIC_BF16", "STATIC_Q8",
+           "STATIC_FP8"]
