@@ -416,8 +416,8 @@ bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const vo
  * with qx, sx the encoding of input[t] in blocks of 128 (as
  * k3_moe_fp8_128_quantize_rows_bf16 gives it). Code products and their sum
  * over a block run on FP8 MFMA, the scaled blocks add up in fp32; the order of
- * the blocks depends on the call's sizes only. columns % 128 == 0; input and
- * codes 16-byte, scales 4-byte, output 2-byte aligned (8-byte stores where the
+ * the blocks depends on the call's sizes only. columns % 128 == 0, columns <=
+ * 2^24; input and codes 16-byte, scales 4-byte, output 2-byte aligned (8-byte stores where the
  * output and rows allow them); vector_count <= 65535. scratch (256-byte
  * aligned device memory): k3_moe_fp8_128_scratch_bytes(vector_count, rows,
  * columns) bytes, 0 where none is needed (scratch may then be NULL).
@@ -447,8 +447,8 @@ typedef struct {
  * The products are k3_moe_fp8_128_gemm_bf16's without its bf16 rounding; h is
  * encoded from fp32. residual may be NULL. experts is a DEVICE array of
  * expert_count descriptors. A route whose id is not below expert_count, or
- * repeats an earlier rank's of its token, adds nothing. hidden % 128 == 0 and
- * ffn % 128 == 0; output, hidden and residual 16-byte aligned; the workspace
+ * repeats an earlier rank's of its token, adds nothing. hidden and ffn multiples
+ * of 128 up to 65536; output, hidden and residual 16-byte aligned; the workspace
  * 256-byte aligned, k3_moe_fp8_workspace_bytes(shape, T) bytes, no state kept
  * in it between calls; token_count <= 65535. expert_ids and expert_weights of
  * the layer are optional copies of the routes.

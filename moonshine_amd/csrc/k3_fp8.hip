@@ -4,22 +4,28 @@
  * and the routed experts on it. No reference counterpart; the encoding and the
  * products are defined in include/k3_moe.h.
  *
- *   rows_kernel       token rows (bf16, or fp32 for the experts' activation)
- *   weight_kernel     a weight, one 128 x 128 block a block
- *   product_kernel    output = rows . weight, 16 tokens x 16 rows a wave
- *   gateup_kernel     act(gate . x, up . x) of every selected expert's rows
- *   down_kernel       y[route] = bf16(down . h)
+ *   rows_kernel           token rows
+ *   weight_kernel         a weight, one 128 x 128 block a block
+ *   stream_kernel         products of up to 64 tokens: weights straight to
+ *                         registers, K split over a block's waves
+ *   gateup_stream_kernel  act(gate . x, up . x) of an expert's up to 16 rows,
+ *   down_stream_kernel    and y[route] = bf16(down . h)
+ *   down_one_kernel       down of a single token's routes, and their sum
+ *   tile_kernel           products of many tokens: tiles in LDS; dense, gate/up
+ *                         and down
  *
  * MFMA operands (V_MFMA_F32_16X16X128_F8F6F4): lane 16 g + c holds 32 codes of
- * row c of the 16 x 128 slices. Both operands take the bytes [32 g, 32 g + 32)
- * of their row there: whichever columns the unit takes them for, they are the
- * same in both, and the sum is over all. Weights are the first operand, tokens
- * the second: lane (g, c) of the result holds weight rows 4 g + i (i < 4) of
- * token c, so one factor scales all four.
+ * row c of the 16 x 128 slices: bytes [16 g, 16 g + 16) and [64 + 16 g, 64 +
+ * 16 g + 16) of the row there, in every kernel alike, so an expert's sums have
+ * the same bits in all of them. Weights are the first operand, tokens the
+ * second: lane (g, c) of the result holds weight rows 4 g + i (i < 4) of token
+ * c, so one factor scales all four.
  */
 #include "k3_device.h"
 #include "k3_fp8.h"
 #include "k3_internal.h"
+#include "k3_lds.h"
+#include "k3_topk.h"
 #include "../../include/k3_moe.h"
 
 #include <hip/hip_runtime.h>
@@ -32,10 +38,14 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kBlock = 128;                /* values of a block */
+/* A tile's 256 rows, and a batch's 65535, are addressed by 32 bits. */
+constexpr uint32_t kMostColumns = 1u << 24, kMostWidth = 1u << 16;
 constexpr float kTop = 448.0f;                  /* largest e4m3 */
 constexpr float kLeast = 0x1.cp-118f;           /* 448 * 2^-126 */
 
 inline size_t align256(size_t v) { return (v + 255u) & ~(size_t)255u; }
+/* Scales of a row inside the library: whole groups of four. */
+inline uint32_t scale_stride(uint32_t cols) { return (cols / kBlock + 3u) & ~3u; }
 
 /* Scale and its inverse of a block with maximum a. */
 __device__ __forceinline__ void fp8_scales(float a, float &scale, float &inv) {
@@ -66,12 +76,6 @@ __device__ __forceinline__ void load8(const uint16_t *src, float (&v)[8]) {
         v[2 * i + 1] = bf16_hi(d[i]);
     }
 }
-__device__ __forceinline__ void load8(const float *src, float (&v)[8]) {
-    const float4 a = ((const float4 *)src)[0], b = ((const float4 *)src)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-
 __device__ __forceinline__ float max8(const float (&v)[8]) {
     float m = 0.0f;
 #pragma unroll
@@ -80,11 +84,13 @@ __device__ __forceinline__ float max8(const float (&v)[8]) {
 }
 
 /* Sixteen lanes a block of 128 values, eight values a lane: one 16-byte load
- * (bf16), a maximum within a row of lanes, one 8-byte store. */
+ * (bf16), a maximum within a row of lanes, one 8-byte store. Scales: nblk of a
+ * row, rows `stride` apart. */
 template <class S>
 __global__ __launch_bounds__(256) void rows_kernel(uint8_t *__restrict__ codes,
                                                    float *__restrict__ scales,
-                                                   const S *__restrict__ src, uint64_t blocks) {
+                                                   const S *__restrict__ src, uint64_t blocks,
+                                                   uint32_t nblk, uint32_t stride) {
     const uint64_t q = (uint64_t)blockIdx.x * 16u + (threadIdx.x >> 4);
     if (q >= blocks) return; /* whole rows of 16 lanes */
     const uint32_t l = threadIdx.x & 15u;
@@ -92,7 +98,7 @@ __global__ __launch_bounds__(256) void rows_kernel(uint8_t *__restrict__ codes,
     load8(src + kBlock * q + 8u * l, v);
     fp8_scales(row_group_max<16>(max8(v)), scale, inv);
     *(uint2 *)(codes + kBlock * q + 8u * l) = fp8_codes8(v, inv);
-    if (l == 0u) scales[q] = scale;
+    if (l == 0u) scales[stride == nblk ? q : q / nblk * stride + q % nblk] = scale;
 }
 
 /* One block of 256 threads a 128 x 128 block: thread t holds eight columns of
@@ -127,8 +133,7 @@ __global__ __launch_bounds__(256) void weight_kernel(uint8_t *__restrict__ codes
     if (threadIdx.x == 0u) scales[blockIdx.x] = scale;
 }
 
-__device__ __forceinline__ f32x4 mfma_block(const uint4 &a0, const uint4 &a1, const uint4 &b0,
-                                            const uint4 &b1) {
+__device__ __forceinline__ f32x4 mfma_block(u32x4_t a0, u32x4_t a1, u32x4_t b0, u32x4_t b1) {
     const i32x8 a = {(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w,
                      (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
     const i32x8 b = {(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w,
@@ -138,83 +143,25 @@ __device__ __forceinline__ f32x4 mfma_block(const uint4 &a0, const uint4 &a1, co
                                                             0, 0, 127, 0, 127);
 }
 
-/* acc += sum over the blocks of scale x (weight rows . token rows); w, x: this
- * lane's weight and token row, at byte 32 g of the first block. */
-__device__ __forceinline__ void tile16(f32x4 &acc, const uint8_t *w, const float *sw,
-                                       const uint8_t *x, const float *sx, uint32_t nblk) {
-    for (uint32_t b = 0; b < nblk; b++, w += kBlock, x += kBlock) {
-        const f32x4 p = mfma_block(((const uint4 *)w)[0], ((const uint4 *)w)[1],
-                                   ((const uint4 *)x)[0], ((const uint4 *)x)[1]);
-        const float s = __fmul_rn(sx[b], sw[b]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = fmaf(p[i], s, acc[i]);
-    }
+__device__ __forceinline__ uint2 bf16x4(const f32x4 &v) {
+    return make_uint2(f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
+                      f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16);
 }
-
-__global__ __launch_bounds__(256) void product_kernel(uint16_t *__restrict__ out,
-                                                      const uint8_t *__restrict__ codes,
-                                                      const float *__restrict__ scales,
-                                                      const uint8_t *__restrict__ xq,
-                                                      const float *__restrict__ xs, uint32_t T,
-                                                      uint32_t N, uint32_t K) {
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = K / kBlock;
-    const uint32_t n0 = 64u * blockIdx.x + 16u * (threadIdx.x >> 6), t0 = 16u * blockIdx.y;
-    if (n0 >= N) return;
-    const uint32_t n = min(n0 + c, N - 1u), t = min(t0 + c, T - 1u);
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    tile16(acc, codes + (uint64_t)n * K + 32u * g, scales + (uint64_t)(n0 / kBlock) * nblk,
-           xq + (uint64_t)t * K + 32u * g, xs + (uint64_t)t * nblk, nblk);
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; i++)
-        if (t0 + c < T && n0 + 4u * g + i < N)
-            out[(uint64_t)(t0 + c) * N + n0 + 4u * g + i] = f32_to_bf16(acc[i]);
-}
-
-/* ---------------------------------------------------------------------- */
-/* experts                                                                 */
-/* ---------------------------------------------------------------------- */
-
-/* ids with a token's repeated ones invalidated, as the plan drops them. */
-__global__ __launch_bounds__(256) void routes_kernel(uint32_t *__restrict__ out,
-                                                     const uint32_t *__restrict__ ids, uint32_t T,
-                                                     uint32_t k, uint32_t E) {
-    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
-    if (t >= T) return;
-    uint32_t e[32];
-    token_routes<32>(ids, t, k, E, e);
-#pragma unroll
-    for (uint32_t r = 0; r < 32u; r++)
-        if (r < k) out[(uint64_t)t * k + r] = e[r];
-}
-
-/* One block: the tiles {expert, first row, rows <= 16} in expert order. */
-__global__ __launch_bounds__(1024) void tiles_kernel(uint32_t *__restrict__ tiles,
-                                                     uint32_t *__restrict__ tile_count,
-                                                     const uint32_t *__restrict__ counts,
-                                                     const uint32_t *__restrict__ offsets,
-                                                     uint32_t E) {
-    __shared__ uint32_t tot[16];
-    const uint32_t e = threadIdx.x, lane = e & 63u, wave = e >> 6;
-    const uint32_t n = e < E ? counts[e] : 0u, mine = (n + 15u) / 16u;
-    uint32_t inc = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t a = __shfl_up(inc, o, 64);
-        if ((int)lane >= o) inc += a;
+/* Columns n .. n + 3 of row t of a [T, N] output; wide: N % 4 == 0 and rows
+ * 8-byte aligned. */
+__device__ __forceinline__ void store_rows(uint16_t *out, const f32x4 &v, uint32_t t, uint32_t n,
+                                           uint32_t T, uint32_t N, bool wide) {
+    if (t >= T || n >= N) return;
+    const uint2 u = bf16x4(v);
+    uint16_t *p = out + (uint64_t)t * N + n;
+    if (wide) {
+        *(uint2 *)p = u;
+        return;
     }
-    if (lane == 63u) tot[wave] = inc;
-    __syncthreads();
-    uint32_t at = inc - mine, total = 0u;
-    for (uint32_t w = 0; w < 16u; w++) {
-        if (w < wave) at += tot[w];
-        total += tot[w];
-    }
-    for (uint32_t q = 0; q < mine; q++) {
-        tiles[3u * (at + q)] = e;
-        tiles[3u * (at + q) + 1u] = offsets[e] + 16u * q;
-        tiles[3u * (at + q) + 2u] = min(16u, n - 16u * q);
-    }
-    if (e == 0u) *tile_count = total;
+    p[0] = (uint16_t)u.x;
+    if (n + 1u < N) p[1] = (uint16_t)(u.x >> 16);
+    if (n + 2u < N) p[2] = (uint16_t)u.y;
+    if (n + 3u < N) p[3] = (uint16_t)(u.y >> 16);
 }
 
 /* tanh to a few ulp: its odd series below 1/2, the exponential above. */
@@ -244,56 +191,732 @@ __device__ __forceinline__ float act_f32(float g, float u, uint32_t kind, float 
     return __fmul_rn(__fmul_rn(bg, s), bu);
 }
 
+/* ---------------------------------------------------------------------- */
+/* streams of weights for few tokens                                       */
+/* ---------------------------------------------------------------------- */
+
+/* This lane's codes of a block of 128 columns: 16 at p and 16 at p + 64. */
+struct Frag {
+    u32x4_t lo, hi;
+};
+__device__ __forceinline__ Frag frag(const uint8_t *p) {
+    typedef const __attribute__((address_space(1))) u32x4_t *gp;
+    return Frag{((gp)p)[0], ((gp)p)[4]};
+}
+__device__ __forceinline__ Frag frag_nt(const uint8_t *p) {
+    typedef const __attribute__((address_space(1))) u32x4_t *gp;
+    return Frag{__builtin_nontemporal_load((gp)p), __builtin_nontemporal_load((gp)p + 4)};
+}
+__device__ __forceinline__ f32x4 mfma_block(const Frag &a, const Frag &b) {
+    return mfma_block(a.lo, a.hi, b.lo, b.hi);
+}
+
+struct ProductArgs {
+    uint16_t *out;
+    const uint8_t *codes;
+    const float *scales;
+    const uint16_t *x; /* one token, not encoded */
+    const uint8_t *xq;
+    const float *xs;
+    uint32_t xstride, T, N, K;
+    bool wide;
+};
+
+/*
+ * 16 NI weight rows x up to 16 TI tokens a block; its eight waves take every
+ * eighth block of columns, eight at a time, and add up through LDS in one
+ * order. Weights go straight to registers: each is used once. ONE: a single
+ * token, whose values the wave encodes itself, two a lane, through LDS (no
+ * second launch; all 16 columns of the products are the same token).
+ */
+template <int NI, int TI, bool ONE>
+__global__ __launch_bounds__(512) void stream_kernel(ProductArgs P) {
+    constexpr int G = NI * TI > 4 ? 2 : NI * TI > 1 ? 4 : 8; /* blocks of a wave in flight */
+    __shared__ __attribute__((aligned(16))) float sums[8][NI * TI][64][4];
+    __shared__ __attribute__((aligned(16))) uint8_t xcode[ONE ? 8 : 1][ONE ? 8 : 1][kBlock];
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n0 = 16u * NI * blockIdx.x, nblk = P.K / kBlock;
+    const uint8_t *w[NI], *x[TI];
+    const float *xs[TI], *sw = P.scales + (uint64_t)(n0 / kBlock) * nblk;
+#pragma unroll
+    for (int i = 0; i < NI; i++) w[i] = P.codes + (uint64_t)min(n0 + 16u * i + c, P.N - 1u) * P.K + 16u * g;
+#pragma unroll
+    for (int j = 0; j < TI; j++) {
+        const uint64_t t = ONE ? 0u : min(16u * j + c, P.T - 1u);
+        x[j] = P.xq + t * P.K + 16u * g;
+        xs[j] = P.xs + t * P.xstride;
+    }
+    f32x4 acc[TI][NI];
+#pragma unroll
+    for (int j = 0; j < TI; j++)
+#pragma unroll
+        for (int i = 0; i < NI; i++) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t b0 = wave; b0 < nblk; b0 += 8u * G) {
+        Frag a[G][NI], b[ONE ? 1 : G][TI];
+        float s[G][TI];
+#pragma unroll
+        for (int q = 0; q < G; q++) {
+            const uint32_t k = b0 + 8u * q;
+            if (k >= nblk) break;
+#pragma unroll
+            for (int i = 0; i < NI; i++) a[q][i] = frag_nt(w[i] + kBlock * k);
+            if constexpr (!ONE) {
+#pragma unroll
+                for (int j = 0; j < TI; j++) {
+                    b[q][j] = frag(x[j] + kBlock * k);
+                    s[q][j] = xs[j][k];
+                }
+            }
+        }
+        if constexpr (ONE) {
+            uint32_t v[G];
+            float m[G];
+#pragma unroll
+            for (int q = 0; q < G; q++) {
+                v[q] = ((const uint32_t *)P.x)[64u * min(b0 + 8u * q, nblk - 1u) + lane];
+                m[q] = fmaxf(fabsf(bf16_lo(v[q])), fabsf(bf16_hi(v[q])));
+            }
+#pragma unroll
+            for (int q = 0; q < G; q++) m[q] = row_group_max<16>(m[q]);
+#pragma unroll
+            for (int o = 16; o <= 32; o <<= 1)
+#pragma unroll
+                for (int q = 0; q < G; q++) m[q] = fmaxf(m[q], __shfl_xor(m[q], o, 64));
+#pragma unroll
+            for (int q = 0; q < G; q++) {
+                float inv;
+                fp8_scales(m[q], s[q][0], inv);
+                *(uint16_t *)(xcode[wave][q] + 2u * lane) = (uint16_t)e4m3x2_raw<false>(
+                    __fmul_rn(bf16_lo(v[q]), inv), __fmul_rn(bf16_hi(v[q]), inv), 0u);
+            }
+            wave_fence();
+        }
+#pragma unroll
+        for (int q = 0; q < G; q++) {
+            const uint32_t k = b0 + 8u * q;
+            if (k >= nblk) break;
+            const float wk = sw[k];
+            if constexpr (ONE) {
+                const u32x4_t *p = (const u32x4_t *)(xcode[wave][q] + 16u * g);
+                b[0][0] = Frag{p[0], p[4]};
+            }
+#pragma unroll
+            for (int j = 0; j < TI; j++) {
+                const float f = __fmul_rn(s[q][j], wk);
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const f32x4 p = mfma_block(a[q][i], b[ONE ? 0 : q][j]);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[j][i][r] = fmaf(p[r], f, acc[j][i][r]);
+                }
+            }
+        }
+        if constexpr (ONE) wave_fence(); /* the codes have been read */
+    }
+#pragma unroll
+    for (int j = 0; j < TI; j++)
+#pragma unroll
+        for (int i = 0; i < NI; i++) *(f32x4 *)sums[wave][j * NI + i][lane] = acc[j][i];
+    __syncthreads();
+    for (uint32_t q = wave; q < NI * TI; q += 8u) {
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const f32x4 p = *(const f32x4 *)sums[u][q][lane];
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = __fadd_rn(v[r], p[r]);
+        }
+        store_rows(P.out, v, 16u * (q / NI) + c, n0 + 16u * (q % NI) + 4u * g, P.T, P.N, P.wide);
+    }
+}
+
+/* Route r of a single token: its id, or E (none: from E on, or an earlier one). */
+__device__ __forceinline__ uint32_t one_route(const uint32_t *ids, uint32_t r, uint32_t E) {
+    const uint32_t e = ids[r];
+    if (e >= E) return E;
+    for (uint32_t q = 0; q < r; q++)
+        if (ids[q] == e) return E;
+    return e;
+}
+
 struct ExpertArgs {
     const k3_moe_fp8_expert *experts;
-    const uint32_t *tiles, *tile_count, *token_index, *route_index;
+    const uint32_t *tiles, *tile_count, *token_index, *route_index, *ids;
+    const uint16_t *x; /* one token, not encoded */
     const uint8_t *xq; /* [T, H] */
     const float *xs;
-    float *h; /* [rows, F] in plan order */
-    const uint8_t *hq;
-    const float *hs;
+    uint32_t xstride, hstride;
+    uint8_t *hq; /* [rows, F] in plan order (one token: in rank order) */
+    float *hs;
     uint16_t *y; /* [routes, H] */
-    uint32_t H, F, kind;
+    uint16_t *out;
+    const uint16_t *residual;
+    const float *weights;
+    uint32_t H, F, E, k, kind;
     float beta, lb;
 };
 
-__global__ __launch_bounds__(256) void gateup_kernel(ExpertArgs A) {
-    if (blockIdx.y >= *A.tile_count) return;
-    const uint32_t *tile = A.tiles + 3u * blockIdx.y;
-    const uint32_t row0 = tile[1], rows = tile[2];
-    const k3_moe_fp8_expert ex = A.experts[tile[0]];
+/*
+ * Gate and up of 128 columns of an expert's up to 16 rows: 16 columns of each a
+ * wave over the whole of K, four blocks of columns (16 KB of weights) in flight
+ * a wave. The 128 columns are a scale block of the activation, encoded here.
+ * ONE: a single token, one route a tile, encoded by the block into LDS (H + H /
+ * 32 bytes) under the first weight loads.
+ */
+template <bool ONE>
+__global__ __launch_bounds__(512) void gateup_stream_kernel(ExpertArgs A) {
+    constexpr int G = 4;
+    __shared__ float red[8][16];
+    extern __shared__ __attribute__((aligned(16))) uint8_t xbuf[];
+    const uint32_t cols = A.F / kBlock, tile = blockIdx.x / cols, col = blockIdx.x % cols;
+    uint32_t e, row0, rows;
+    if constexpr (ONE) {
+        e = one_route(A.ids, tile, A.E), row0 = tile, rows = 1u;
+        if (e >= A.E) return;
+    } else {
+        if (tile >= *A.tile_count) return;
+        e = A.tiles[3u * tile], row0 = A.tiles[3u * tile + 1u], rows = A.tiles[3u * tile + 2u];
+    }
+    const k3_moe_fp8_expert ex = A.experts[e];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.H / kBlock;
-    const uint32_t f0 = 64u * blockIdx.x + 16u * (threadIdx.x >> 6);
-    const uint32_t t = A.token_index[row0 + min(c, rows - 1u)];
-    const uint64_t w = (uint64_t)(f0 + c) * A.H + 32u * g, sw = (uint64_t)(f0 / kBlock) * nblk;
-    const uint8_t *x = A.xq + (uint64_t)t * A.H + 32u * g;
-    const float *xs = A.xs + (uint64_t)t * nblk;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t f0 = kBlock * col + 16u * wave;
+    const uint64_t at = (uint64_t)(f0 + c) * A.H + 16u * g;
+    const uint8_t *wg = ex.gate_codes + at, *wu = ex.up_codes + at;
+    const float *sg = ex.gate_scales + (uint64_t)col * nblk, *su = ex.up_scales + (uint64_t)col * nblk;
+    const uint8_t *x = nullptr;
+    const float *xs = nullptr;
+    if constexpr (!ONE) {
+        const uint64_t t = A.token_index[row0 + min(c, rows - 1u)];
+        x = A.xq + t * A.H + 16u * g;
+        xs = A.xs + t * A.xstride;
+    }
     f32x4 gate = {0.0f, 0.0f, 0.0f, 0.0f}, up = gate;
-    tile16(gate, ex.gate_codes + w, ex.gate_scales + sw, x, xs, nblk);
-    tile16(up, ex.up_codes + w, ex.up_scales + sw, x, xs, nblk);
+    Frag ag[G], au[G], b[ONE ? 1 : G];
+    float sx[G];
+    auto load = [&](uint32_t k, int q) {
+        if (k >= nblk) return;
+        ag[q] = frag_nt(wg + kBlock * k);
+        au[q] = frag_nt(wu + kBlock * k);
+        if constexpr (!ONE) {
+            b[q] = frag(x + kBlock * k);
+            sx[q] = xs[k];
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < G; q++) load((uint32_t)q, q);
+    const float *xsc = (const float *)(xbuf + A.H);
+    if constexpr (ONE) {
+        for (uint32_t q = threadIdx.x; q < 16u * nblk; q += 512u) { /* whole rows of 16 lanes */
+            float v[8], scale, inv;
+            load8(A.x + 8u * q, v);
+            fp8_scales(row_group_max<16>(max8(v)), scale, inv);
+            *(uint2 *)(xbuf + 8u * q) = fp8_codes8(v, inv);
+            if ((q & 15u) == 0u) ((float *)(xbuf + A.H))[q >> 4] = scale;
+        }
+        __syncthreads();
+    }
+    for (uint32_t k0 = 0; k0 < nblk; k0 += G) {
+#pragma unroll
+        for (int q = 0; q < G; q++) {
+            const uint32_t k = k0 + (uint32_t)q;
+            if (k < nblk) {
+                Frag xb;
+                float s;
+                if constexpr (ONE) {
+                    const u32x4_t *p = (const u32x4_t *)(xbuf + kBlock * k + 16u * g);
+                    xb = Frag{p[0], p[4]};
+                    s = xsc[k];
+                } else {
+                    xb = b[q];
+                    s = sx[q];
+                }
+                const f32x4 pg = mfma_block(ag[q], xb), pu = mfma_block(au[q], xb);
+                const float fg = __fmul_rn(s, sg[k]), fu = __fmul_rn(s, su[k]);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    gate[r] = fmaf(pg[r], fg, gate[r]);
+                    up[r] = fmaf(pu[r], fu, up[r]);
+                }
+            }
+            load(k + G, q);
+        }
+    }
+    float h[4], m = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        h[r] = act_f32(gate[r], up[r], A.kind, A.beta, A.lb);
+        m = fmaxf(m, fabsf(h[r]));
+    }
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    if (g == 0u) red[wave][c] = m;
+    __syncthreads();
     if (c >= rows) return;
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; i++)
-        A.h[(uint64_t)(row0 + c) * A.F + f0 + 4u * g + i] =
-            act_f32(gate[i], up[i], A.kind, A.beta, A.lb);
+    for (int w = 0; w < 8; w++) m = fmaxf(m, red[w][c]);
+    float scale, inv;
+    fp8_scales(m, scale, inv);
+    *(uint32_t *)(A.hq + (uint64_t)(row0 + c) * A.F + f0 + 4u * g) =
+        e4m3x2_raw<true>(__fmul_rn(h[2], inv), __fmul_rn(h[3], inv),
+                         e4m3x2_raw<false>(__fmul_rn(h[0], inv), __fmul_rn(h[1], inv), 0u));
+    if (wave == 0u && g == 0u) A.hs[(uint64_t)(row0 + c) * A.hstride + col] = scale;
 }
 
-__global__ __launch_bounds__(256) void down_kernel(ExpertArgs A) {
-    if (blockIdx.y >= *A.tile_count) return;
-    const uint32_t *tile = A.tiles + 3u * blockIdx.y;
-    const uint32_t row0 = tile[1], rows = tile[2];
-    const k3_moe_fp8_expert ex = A.experts[tile[0]];
+/* acc[i] = 16 weight rows (w[i], this lane's) . the lane's token row. */
+template <int NI, int G>
+__device__ __forceinline__ void stream_rows(f32x4 (&acc)[NI], const uint8_t *const (&w)[NI],
+                                            const float *sw, const uint8_t *x, const float *xs,
+                                            uint32_t nblk) {
+    Frag a[G][NI], b[G];
+    float sx[G];
+    auto load = [&](uint32_t k, int q) {
+        if (k >= nblk) return;
+#pragma unroll
+        for (int i = 0; i < NI; i++) a[q][i] = frag_nt(w[i] + kBlock * k);
+        b[q] = frag(x + kBlock * k);
+        sx[q] = xs[k];
+    };
+#pragma unroll
+    for (int q = 0; q < G; q++) load((uint32_t)q, q);
+#pragma unroll
+    for (int i = 0; i < NI; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t k0 = 0; k0 < nblk; k0 += G) {
+#pragma unroll
+        for (int q = 0; q < G; q++) {
+            const uint32_t k = k0 + (uint32_t)q;
+            if (k < nblk) {
+                const float f = __fmul_rn(sx[q], sw[k]);
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const f32x4 p = mfma_block(a[q][i], b[q]);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[i][r] = fmaf(p[r], f, acc[i][r]);
+                }
+            }
+            load(k + G, q);
+        }
+    }
+}
+
+/* y of an expert's up to 16 rows: 32 columns a wave, 128 a block. */
+__global__ __launch_bounds__(256) void down_stream_kernel(ExpertArgs A) {
+    const uint32_t cols = A.H / kBlock, tile = blockIdx.x / cols, col = blockIdx.x % cols;
+    if (tile >= *A.tile_count) return;
+    const uint32_t row0 = A.tiles[3u * tile + 1u], rows = A.tiles[3u * tile + 2u];
+    const k3_moe_fp8_expert ex = A.experts[A.tiles[3u * tile]];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.F / kBlock;
-    const uint32_t n0 = 64u * blockIdx.x + 16u * (threadIdx.x >> 6);
-    const uint32_t r = row0 + min(c, rows - 1u);
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    tile16(acc, ex.down_codes + (uint64_t)(n0 + c) * A.F + 32u * g,
-           ex.down_scales + (uint64_t)(n0 / kBlock) * nblk, A.hq + (uint64_t)r * A.F + 32u * g,
-           A.hs + (uint64_t)r * nblk, nblk);
+    const uint32_t n0 = kBlock * col + 32u * (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t r = row0 + min(c, rows - 1u);
+    const uint8_t *w0 = ex.down_codes + (uint64_t)(n0 + c) * A.F + 16u * g;
+    const uint8_t *const w[2] = {w0, w0 + 16ull * A.F};
+    f32x4 acc[2];
+    stream_rows<2, 4>(acc, w, ex.down_scales + (uint64_t)col * nblk, A.hq + r * A.F + 16u * g,
+                      A.hs + r * A.hstride, nblk);
     if (c >= rows) return;
     uint16_t *y = A.y + (uint64_t)A.route_index[r] * A.H + n0 + 4u * g;
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = f32_to_bf16(acc[i]);
+    for (int i = 0; i < 2; i++) *(uint2 *)(y + 16 * i) = bf16x4(acc[i]);
+}
+
+/* A single token's output: 16 columns a block, a route a wave at a time, then
+ * the weighted sum in rank order and the residual (as combine_kernel's). */
+__global__ __launch_bounds__(512) void down_one_kernel(ExpertArgs A) {
+    __shared__ float y[32][16];
+    __shared__ uint32_t live[32];
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.F / kBlock;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = 16u * blockIdx.x;
+    for (uint32_t r = wave; r < A.k; r += 8u) {
+        const uint32_t e = one_route(A.ids, r, A.E);
+        if (lane == 0u) live[r] = e < A.E;
+        if (e >= A.E) continue;
+        const k3_moe_fp8_expert ex = A.experts[e];
+        const uint8_t *const w[1] = {ex.down_codes + (uint64_t)(n0 + c) * A.F + 16u * g};
+        f32x4 acc[1];
+        stream_rows<1, 8>(acc, w, ex.down_scales + (uint64_t)(n0 / kBlock) * nblk,
+                          A.hq + (uint64_t)r * A.F + 16u * g, A.hs + (uint64_t)r * A.hstride, nblk);
+        if (c == 0u)
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[r][4u * g + i] = bf16_to_f32(f32_to_bf16(acc[0][i]));
+    }
+    __syncthreads();
+    if (threadIdx.x >= 16u) return;
+    float v = 0.0f;
+    for (uint32_t r = 0; r < A.k; r++)
+        if (live[r]) v = __fadd_rn(v, __fmul_rn(A.weights[r], y[r][threadIdx.x]));
+    uint16_t o = f32_to_bf16(v);
+    if (A.residual) o = f32_to_bf16(__fadd_rn(bf16_to_f32(A.residual[n0 + threadIdx.x]), bf16_to_f32(o)));
+    A.out[n0 + threadIdx.x] = o;
+}
+
+/* ---------------------------------------------------------------------- */
+/* tiles of many tokens                                                    */
+/* ---------------------------------------------------------------------- */
+
+/*
+ * 256 weight rows x 32 TI tokens a block of eight waves; wave (wn, wt) holds
+ * weight rows 64 wn .. + 64 and the token subtiles (16 tokens) wt, wt + 2, ...:
+ * a tile with fewer tokens costs its 32-token steps, evenly over the waves. A
+ * stage is a block of 128 columns of both operands, in LDS through
+ * direct-to-LDS loads (whole 128-byte lines, XOR-swizzled pieces), STAGES of
+ * them in a ring. A wave keeps its four weight fragments of a stage in
+ * registers and streams the token fragments: four MFMAs with C = 0 each, whose
+ * result goes into the fp32 accumulator with one fma per value under the factor
+ * sx sw; two waves a SIMD hide each other's waits between the two. Token scales
+ * come four blocks at a time (16 bytes a token) into two buffers; the weights'
+ * are held by the lanes of a wave, 64 blocks at a time, and read out by index.
+ */
+template <int TI_, int STAGES_>
+struct Tile {
+    static constexpr int TI = TI_, STAGES = STAGES_;
+    static constexpr uint32_t BN = 256, BT = 32 * TI;
+    static constexpr uint32_t A = BN * kBlock, B = BT * kBlock, STAGE = A + B;
+    static constexpr uint32_t SROWS = BT < 64u ? 64u : BT, SBUF = 16u * SROWS;
+    static constexpr int DA = 4, DB = TI < 2 ? 1 : TI / 2, D = DA + DB; /* loads a wave */
+    static constexpr uint32_t LDS = STAGES * STAGE + 2u * SBUF;
+    static_assert(LDS <= 160u * 1024u, "LDS");
+};
+
+enum TileMode { kDense, kGateUp, kDown };
+
+struct TileArgs {
+    /* dense: the weight; otherwise the experts and the tiles {expert, row, rows} */
+    const uint8_t *codes;
+    const float *scales;
+    const k3_moe_fp8_expert *experts;
+    const uint32_t *tiles, *tile_count, *token_index, *route_index;
+    const uint8_t *xq; /* token rows, K wide */
+    const float *xs;   /* their scales, rows xstride apart */
+    uint32_t xstride;
+    uint16_t *out;     /* dense [T, N]; down y [routes, N] */
+    uint8_t *hq;       /* gate/up: activation rows, N = F wide */
+    float *hs;
+    uint32_t hstride;
+    uint32_t T, N, K, tiles_n, tiles_t;
+    uint32_t kind;
+    float beta, lb;
+    bool wide; /* the output takes 8-byte stores */
+};
+
+/* acc[j][i] += the product over all blocks, for the first TL token subtiles of a
+ * wave (a loop of its own for each TL: a test inside it costs registers). */
+template <class C>
+struct TileRun {
+    const uint8_t *a_base, *b_base; /* the sources of this wave's loads, and this lane's places */
+    uint32_t a[C::DA], b[C::DB];
+    const float *sx;                    /* of the scale loads, for waves that have one */
+    bool has_sx;
+    const float *sw0, *sw1;             /* weight scales of fragments 0, 1 and 2, 3 */
+    uint32_t nblk, wave, lane, wn, wt;
+
+    __device__ __forceinline__ void fetch(uint8_t *smem, uint32_t s, uint32_t slot) const {
+        if (has_sx && s % 4u == 0u && s < nblk)
+            dma<16>((const uint8_t *)(sx + s),
+                    smem + C::STAGES * C::STAGE + C::SBUF * ((s >> 2) & 1u) + 1024u * wave);
+        const uint32_t at = kBlock * (s < nblk ? s : nblk - 1u);
+        const uint8_t *pa = a_base + at, *pb = b_base + at;
+        uint8_t *st = smem + C::STAGE * slot;
+#pragma unroll
+        for (int q = 0; q < C::DA; q++) dma<16>(pa + a[q], st + 1024u * (C::DA * wave + q));
+#pragma unroll
+        for (int q = 0; q < C::DB; q++)
+            dma<16>(pb + b[q], st + C::A + 1024u * (C::TI < 2 ? wave & 3u : C::DB * wave + q));
+    }
+
+    template <int TL, bool Two>
+    __device__ __forceinline__ void run(f32x4 (&acc)[C::TI][4], uint8_t *smem) const {
+        const uint32_t g = lane >> 4, c = lane & 15u;
+        const uint32_t base = lds_addr(smem), lo = a_slot(c, g), hi = a_slot(c, 4u + g);
+        const uint32_t a_at = base + 8192u * wn, b_at = base + C::A + 2048u * wt;
+        const uint32_t s_at = base + C::STAGES * C::STAGE + 16u * (16u * wt + c);
+        float w0 = 0.0f, w1 = 0.0f;
+#pragma unroll
+        for (int s = 0; s < C::STAGES - 1; s++) fetch(smem, (uint32_t)s, (uint32_t)s);
+        uint32_t slot = 0u, next = C::STAGES - 1;
+        for (uint32_t s = 0; s < nblk; s++) {
+            if (s % 64u == 0u) { /* the weight scales of the next 64 blocks */
+                const uint32_t q = s + lane < nblk ? s + lane : nblk - 1u;
+                w0 = sw0[q];
+                if (Two) w1 = sw1[q];
+            }
+            wait_vm<C::D *(C::STAGES - 2)>(); /* this wave's loads of stage s */
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier(); /* everyone's; and stage s - 1 has been read */
+            asm volatile("" ::: "memory");
+            if (C::STAGES > 2 || s + 1u < nblk) fetch(smem, s + C::STAGES - 1u, next);
+            const uint32_t st = C::STAGE * slot, sb = s_at + C::SBUF * ((s >> 2) & 1u) + 4u * (s & 3u);
+            next = slot;
+            slot = slot + 1u == (uint32_t)C::STAGES ? 0u : slot + 1u;
+            const float sw_0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w0), (int)(s & 63u)));
+            const float sw_1 = Two ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w1), (int)(s & 63u))) : sw_0;
+            u32x4_t af[4][2], bf[2][2];
+            uint32_t sx_[2];
+            static_for<4>([&](auto I) {
+                constexpr int i = decltype(I)::value;
+                af[i][0] = ds_read16<2048 * i>(a_at + st + lo);
+                af[i][1] = ds_read16<2048 * i>(a_at + st + hi);
+            });
+            sx_[0] = ds_read4<0>(sb);
+            bf[0][0] = ds_read16<0>(b_at + st + lo);
+            bf[0][1] = ds_read16<0>(b_at + st + hi);
+            static_for<TL>([&](auto J) {
+                constexpr int j = decltype(J)::value;
+                if constexpr (j + 1 < TL) {
+                    sx_[(j + 1) & 1] = ds_read4<512 * (j + 1)>(sb);
+                    bf[(j + 1) & 1][0] = ds_read16<4096 * (j + 1)>(b_at + st + lo);
+                    bf[(j + 1) & 1][1] = ds_read16<4096 * (j + 1)>(b_at + st + hi);
+                    wait_lgkm<3>();
+                } else {
+                    wait_lgkm<0>();
+                }
+                if constexpr (j == 0) {
+                    static_for<4>([&](auto I) {
+                        after_wait(af[decltype(I)::value][0]);
+                        after_wait(af[decltype(I)::value][1]);
+                    });
+                }
+                after_wait(sx_[j & 1]);
+                after_wait(bf[j & 1][0]);
+                after_wait(bf[j & 1][1]);
+                const float sx = __uint_as_float(sx_[j & 1]);
+                const float f0 = __fmul_rn(sx, sw_0), f1 = Two ? __fmul_rn(sx, sw_1) : f0;
+                f32x4 p[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    p[i] = mfma_block(af[i][0], af[i][1], bf[j & 1][0], bf[j & 1][1]);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        acc[j][i][r] = fmaf(p[i][r], i < 2 ? f0 : f1, acc[j][i][r]);
+            });
+        }
+        wait_vm<0>(); /* the loads past the end land before the LDS is used again */
+    }
+};
+
+template <class C, int MODE>
+__global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
+    TileRun<C> R;
+    R.lane = threadIdx.x & 63u;
+    R.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    R.wn = R.wave & 3u, R.wt = R.wave >> 2;
+    const uint32_t L = R.lane, K = P.K, nblk = K / kBlock;
+    /* XCD x (blocks x, x + 8, ...) takes a contiguous range of the works */
+    const uint32_t tiles = MODE == kDense ? P.tiles_t : *P.tile_count;
+    const uint32_t works = tiles * P.tiles_n, per = (works + 7u) / 8u, j8 = blockIdx.x >> 3;
+    const uint32_t w = (blockIdx.x & 7u) * per + j8;
+    if (j8 >= per || w >= works) return;
+    uint32_t tile, col;
+    if constexpr (MODE == kDense) { /* four token tiles at a time, down the weight's rows */
+        const uint32_t grp = w / (4u * P.tiles_n), in = w % (4u * P.tiles_n);
+        const uint32_t high = min(4u, tiles - 4u * grp);
+        tile = 4u * grp + in % high, col = in / high;
+    } else {
+        tile = w / P.tiles_n, col = w % P.tiles_n;
+    }
+    uint32_t row0, rows;
+    const uint8_t *w0, *w1;
+    const uint32_t n0 = (MODE == kGateUp ? 128u : 256u) * col, nb0 = n0 / kBlock;
+    const uint32_t blocks_n = (P.N + kBlock - 1u) / kBlock;
+    if constexpr (MODE == kDense) {
+        row0 = C::BT * tile, rows = min(C::BT, P.T - row0);
+        w0 = w1 = P.codes;
+        const uint32_t nb = min(nb0 + (R.wn >> 1), blocks_n - 1u);
+        R.sw0 = R.sw1 = P.scales + (uint64_t)nb * nblk;
+    } else {
+        const uint32_t *t = P.tiles + 3u * tile;
+        row0 = t[1], rows = t[2];
+        const k3_moe_fp8_expert ex = P.experts[t[0]];
+        if constexpr (MODE == kGateUp) {
+            w0 = ex.gate_codes, w1 = ex.up_codes;
+            R.sw0 = ex.gate_scales + (uint64_t)nb0 * nblk;
+            R.sw1 = ex.up_scales + (uint64_t)nb0 * nblk;
+        } else {
+            w0 = w1 = ex.down_codes;
+            const uint32_t nb = min(nb0 + (R.wn >> 1), blocks_n - 1u);
+            R.sw0 = R.sw1 = ex.down_scales + (uint64_t)nb * nblk;
+        }
+    }
+    R.nblk = nblk;
+    /* chunk q of A: rows 8 q .. + 8 of the tile; gate/up: wave wn's 64 rows are
+     * 32 of gate, then the same 32 of up, so a loading wave has one of them */
+    if constexpr (MODE == kGateUp)
+        R.a_base = (R.wave & 1u ? w1 : w0) + (uint64_t)n0 * K;
+    else
+        R.a_base = w0 + (uint64_t)n0 * K;
+    R.b_base = MODE == kGateUp ? P.xq : P.xq + (uint64_t)row0 * K;
+#pragma unroll
+    for (int q = 0; q < C::DA; q++) {
+        const uint32_t ch = C::DA * R.wave + (uint32_t)q, h = ch & 1u;
+        uint32_t r = 16u * (ch >> 1) + a_dma_row(L, h);
+        if constexpr (MODE == kGateUp)
+            r = 32u * (ch >> 3) + (r & 31u);
+        else
+            r = min(r, P.N - 1u - n0);
+        R.a[q] = r * K + 16u * a_dma_piece(L, h);
+    }
+#pragma unroll
+    for (int q = 0; q < C::DB; q++) {
+        const uint32_t ch = C::TI < 2 ? R.wave & 3u : C::DB * R.wave + (uint32_t)q, h = ch & 1u;
+        uint32_t r = min(16u * (ch >> 1) + a_dma_row(L, h), rows - 1u);
+        if constexpr (MODE == kGateUp) r = P.token_index[row0 + r];
+        R.b[q] = r * K + 16u * a_dma_piece(L, h);
+    }
+    {
+        R.has_sx = 64u * R.wave < C::BT;
+        uint32_t r = row0 + min(64u * R.wave + L, rows - 1u);
+        if constexpr (MODE == kGateUp) r = P.token_index[r];
+        R.sx = P.xs + (uint64_t)r * P.xstride;
+    }
+    f32x4 acc[C::TI][4];
+#pragma unroll
+    for (int j = 0; j < C::TI; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    /* lists hold no tile of fewer than TI / 2 steps of 32 rows */
+    const uint32_t steps = (rows + 31u) / 32u;
+    bool done = false;
+    static_for<C::TI / 2>([&](auto Q) {
+        constexpr int tl = C::TI / 2 + decltype(Q)::value;
+        if (!done && steps <= (uint32_t)tl) {
+            R.template run<tl, MODE == kGateUp>(acc, smem);
+            done = true;
+        }
+    });
+    if (!done) R.template run<C::TI, MODE == kGateUp>(acc, smem);
+    const uint32_t g = L >> 4, c = L & 15u;
+    if constexpr (MODE != kGateUp) {
+        static_for<C::TI>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            const uint32_t r = 16u * (2u * j + R.wt) + c;
+            if (r >= rows) return;
+            uint32_t t = row0 + r;
+            if constexpr (MODE == kDown) t = P.route_index[t];
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++)
+                store_rows(P.out, acc[j][i], t, n0 + 64u * R.wn + 16u * i + 4u * g, ~0u, P.N,
+                           MODE == kDown || P.wide);
+        });
+    } else {
+        /* the block's 128 columns are one scale block of each row: the maximum
+         * over a wave's 32, then over its four neighbours' through LDS; codes
+         * go through LDS too and leave as whole lines */
+        __syncthreads();
+        float *red = (float *)smem;             /* [4][BT] */
+        uint8_t *rowbuf = smem + 16u * C::BT;   /* [BT][128] */
+        static_for<C::TI>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float h = act_f32(acc[j][i][r], acc[j][i + 2][r], P.kind, P.beta, P.lb);
+                    acc[j][i][r] = h;
+                    m = fmaxf(m, fabsf(h));
+                }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            if (g == 0u) red[C::BT * R.wn + 16u * (2u * j + R.wt) + c] = m;
+        });
+        __syncthreads();
+        static_for<C::TI>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            const uint32_t r = 16u * (2u * j + R.wt) + c;
+            float scale, inv;
+            fp8_scales(fmaxf(fmaxf(red[r], red[C::BT + r]), fmaxf(red[2u * C::BT + r], red[3u * C::BT + r])),
+                       scale, inv);
+#pragma unroll
+            for (uint32_t i = 0; i < 2u; i++) {
+                const f32x4 h = acc[j][i];
+                *(uint32_t *)(rowbuf + kBlock * r + 32u * R.wn + 16u * i + 4u * g) =
+                    e4m3x2_raw<true>(__fmul_rn(h[2], inv), __fmul_rn(h[3], inv),
+                                     e4m3x2_raw<false>(__fmul_rn(h[0], inv), __fmul_rn(h[1], inv), 0u));
+            }
+            if (R.wn == 0u && g == 0u && r < rows) P.hs[(uint64_t)(row0 + r) * P.hstride + nb0] = scale;
+        });
+        __syncthreads();
+        for (uint32_t q = threadIdx.x; q < 8u * rows; q += 512u)
+            *(uint4 *)(P.hq + (uint64_t)(row0 + (q >> 3)) * P.N + n0 + 16u * (q & 7u)) =
+                *(const uint4 *)(rowbuf + 16u * q);
+    }
+}
+
+template <class C, int MODE>
+bool launch_tile(const TileArgs &A, uint32_t works, hipStream_t st) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<C, MODE>), dim3(8u * ((works + 7u) / 8u)),
+                       dim3(512), 0, st, A);
+    return hipGetLastError() == hipSuccess;
+}
+
+/* ---------------------------------------------------------------------- */
+/* routes and tiles of the experts                                         */
+/* ---------------------------------------------------------------------- */
+
+/* ids with a token's repeated ones invalidated, as the plan drops them. */
+__global__ __launch_bounds__(256) void routes_kernel(uint32_t *__restrict__ out,
+                                                     const uint32_t *__restrict__ ids, uint32_t T,
+                                                     uint32_t k, uint32_t E) {
+    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+    if (t >= T) return;
+    uint32_t e[32];
+    token_routes<32>(ids, t, k, E, e);
+#pragma unroll
+    for (uint32_t r = 0; r < 32u; r++)
+        if (r < k) out[(uint64_t)t * k + r] = e[r];
+}
+
+/* Tile classes by an expert's rows: up to 16 (streams), up to 64 and up to 128
+ * (one tile), more (tiles of up to 256, of equal length in 32-row steps). */
+constexpr int kClasses = 4;
+
+/* One block of 1024 threads (thread e: expert e): each class's tiles {expert,
+ * first row, rows} in expert order, from its own base on. */
+struct TileLists {
+    uint32_t *tiles[kClasses];
+    uint32_t *count; /* [kClasses] */
+};
+__global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t *__restrict__ counts,
+                                                     const uint32_t *__restrict__ offsets,
+                                                     uint32_t E) {
+    __shared__ uint32_t tot[kClasses][16];
+    const uint32_t e = threadIdx.x, lane = e & 63u, wave = e >> 6;
+    const uint32_t n = e < E ? counts[e] : 0u;
+    const uint32_t steps = (n + 31u) / 32u, many = (n + 255u) / 256u;
+    const uint32_t height = n > 128u ? 32u * ((steps + many - 1u) / many) : n;
+    const uint32_t mine = n == 0u ? 0u : (n + height - 1u) / height;
+    const int cls = n <= 16u ? 0 : n <= 64u ? 1 : n <= 128u ? 2 : 3;
+    uint32_t inc[kClasses];
+#pragma unroll
+    for (int q = 0; q < kClasses; q++) {
+        inc[q] = cls == q ? mine : 0u;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t a = __shfl_up(inc[q], o, 64);
+            if ((int)lane >= o) inc[q] += a;
+        }
+        if (lane == 63u) tot[q][wave] = inc[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kClasses; q++) {
+        uint32_t at = inc[q] - mine, total = 0u;
+        for (uint32_t w = 0; w < 16u; w++) {
+            if (w < wave) at += tot[q][w];
+            total += tot[q][w];
+        }
+        if (cls == q)
+            for (uint32_t i = 0; i < mine; i++) {
+                uint32_t *t = Q.tiles[q] + 3u * (at + i);
+                t[0] = e;
+                t[1] = offsets[e] + height * i;
+                t[2] = min(height, n - height * i);
+            }
+        if (e == 0u) Q.count[q] = total;
+    }
 }
 
 struct Fp8Workspace {
@@ -302,10 +925,10 @@ struct Fp8Workspace {
     uint32_t *counts, *offsets, *unique, *summary, *token_index, *route_index;
     void *plan;
     size_t plan_bytes;
-    uint32_t *tiles, *tile_count;
-    uint32_t tile_cap;
+    TileLists lists;
+    uint32_t cap[kClasses]; /* most tiles of a class; 0: no expert can be of it */
     uint8_t *xq, *hq;
-    float *xs, *hs, *h;
+    float *xs, *hs;
     uint16_t *y;
     void *router;
     size_t router_bytes, bytes;
@@ -331,14 +954,18 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
     w.route_index = (uint32_t *)take(4u * routes);
     w.plan_bytes = k3_moe_plan_scratch_bytes(T, s.expert_count);
     w.plan = take(w.plan_bytes);
-    w.tile_cap = (uint32_t)(routes / 16u + (E < routes ? E : routes));
-    w.tiles = (uint32_t *)take(12u * (size_t)w.tile_cap);
-    w.tile_count = (uint32_t *)take(4u);
+    /* an expert has a token's route at most once: T rows at most */
+    static constexpr size_t least[kClasses] = {1u, 17u, 65u, 128u};
+    for (int q = 0; q < kClasses; q++) {
+        const size_t n = routes / least[q];
+        w.cap[q] = T < least[q] ? 0u : (uint32_t)(q < 3 && n > E ? E : n);
+        w.lists.tiles[q] = (uint32_t *)take(12u * (size_t)w.cap[q]);
+    }
+    w.lists.count = (uint32_t *)take(4u * kClasses);
     w.xq = take((size_t)T * s.hidden);
-    w.xs = (float *)take((size_t)T * s.hidden / 32u);
-    w.h = (float *)take(4u * routes * s.ffn);
+    w.xs = (float *)take(4u * (size_t)T * scale_stride(s.hidden));
     w.hq = take(routes * s.ffn);
-    w.hs = (float *)take(routes * s.ffn / 32u);
+    w.hs = (float *)take(4u * routes * scale_stride(s.ffn));
     w.y = (uint16_t *)take(2u * routes * s.hidden);
     w.router_bytes = k3_moe_router_scratch_bytes(T, s.expert_count);
     w.router = take(w.router_bytes);
@@ -348,38 +975,86 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
 
 bool fp8_shape_ok(const k3_moe_shape *s, uint32_t T) {
     return s && T != 0u && T <= 65535u && s->hidden != 0u && s->hidden % kBlock == 0u &&
-           s->ffn != 0u && s->ffn % kBlock == 0u && s->expert_count != 0u &&
+           s->hidden <= kMostWidth && s->ffn != 0u && s->ffn % kBlock == 0u &&
+           s->ffn <= kMostWidth && s->expert_count != 0u &&
            s->expert_count <= 1024u && s->top_k != 0u && s->top_k <= 32u &&
            s->top_k <= s->expert_count && s->scaling_factor > 0.0f && s->activation <= 1u &&
            (s->activation == K3_MOE_ACT_SWIGLU || (s->beta > 0.0f && s->linear_beta > 0.0f));
 }
 
-bool launch_rows(uint8_t *codes, float *scales, const uint16_t *src, uint64_t blocks,
-                 hipStream_t st) {
+/* Encodes rows of `cols` bf16 values; scales of a row `stride` apart. */
+bool launch_rows(uint8_t *codes, float *scales, const void *src, uint32_t rows, uint32_t cols,
+                 uint32_t stride, hipStream_t st) {
+    const uint32_t nblk = cols / kBlock;
+    const uint64_t blocks = (uint64_t)rows * nblk;
     hipLaunchKernelGGL(rows_kernel<uint16_t>, dim3((uint32_t)((blocks + 15u) / 16u)), dim3(256), 0,
-                       st, codes, scales, src, blocks);
+                       st, codes, scales, (const uint16_t *)src, blocks, nblk, stride);
     return hipGetLastError() == hipSuccess;
 }
 
-/* The expert stage on routes in ws.ids (weights: wts). */
+template <int NI, int TI, bool ONE>
+bool launch_stream(const ProductArgs &A, hipStream_t st) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(stream_kernel<NI, TI, ONE>),
+                       dim3((A.N + 16u * NI - 1u) / (16u * NI)), dim3(512), 0, st, A);
+    return hipGetLastError() == hipSuccess;
+}
+
+using Tile64 = Tile<2, 3>;
+using Tile128 = Tile<4, 3>;
+using Tile256 = Tile<8, 2>;
+
+template <class C>
+bool launch_dense(TileArgs A, hipStream_t st) {
+    A.tiles_t = (A.T + C::BT - 1u) / C::BT;
+    A.tiles_n = (A.N + C::BN - 1u) / C::BN;
+    return launch_tile<C, kDense>(A, A.tiles_t * A.tiles_n, st);
+}
+
+/* Gate/up and down of one class of tiles. */
+template <class C>
+bool launch_class(TileArgs A, const Fp8Workspace &ws, int cls, const k3_moe_shape &s, hipStream_t st) {
+    if (ws.cap[cls] == 0u) return true;
+    A.tiles = ws.lists.tiles[cls], A.tile_count = ws.lists.count + cls;
+    A.N = s.ffn, A.K = s.hidden, A.tiles_n = s.ffn / kBlock;
+    if (!launch_tile<C, kGateUp>(A, ws.cap[cls] * A.tiles_n, st)) return false;
+    A.xq = ws.hq, A.xs = ws.hs, A.xstride = scale_stride(s.ffn);
+    A.N = s.hidden, A.K = s.ffn, A.tiles_n = (s.hidden + C::BN - 1u) / C::BN;
+    return launch_tile<C, kDown>(A, ws.cap[cls] * A.tiles_n, st);
+}
+
+/* A token's codes and scales in LDS, beside the block's other arrays. */
+bool one_token_fits(const k3_moe_shape &s) { return s.hidden <= 32768u; }
+
+/* The expert stage on routes in ids (T > 1: ws.ids, repeated ones taken out). */
 bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, const void *residual,
-                     const float *wts, const k3_moe_fp8_expert *experts, const k3_moe_shape &s,
-                     uint32_t T, hipStream_t st) {
+                     const uint32_t *ids, const float *wts, const k3_moe_fp8_expert *experts,
+                     const k3_moe_shape &s, uint32_t T, hipStream_t st) {
     const uint32_t H = s.hidden, F = s.ffn, E = s.expert_count, k = s.top_k;
-    if (!launch_rows(ws.xq, ws.xs, (const uint16_t *)hidden, (uint64_t)T * (H / kBlock), st) ||
+    ExpertArgs A{experts, ws.lists.tiles[0], ws.lists.count, ws.token_index, ws.route_index, ids,
+                 (const uint16_t *)hidden, ws.xq, ws.xs, scale_stride(H), scale_stride(F), ws.hq,
+                 ws.hs, ws.y, (uint16_t *)output, (const uint16_t *)residual, wts, H, F, E, k,
+                 s.activation, s.beta, s.linear_beta};
+    if (T == 1u && one_token_fits(s)) {
+        hipLaunchKernelGGL(gateup_stream_kernel<true>, dim3(k * (F / kBlock)), dim3(512), H + H / 32u,
+                           st, A);
+        hipLaunchKernelGGL(down_one_kernel, dim3(H / 16u), dim3(512), 0, st, A);
+        return hipGetLastError() == hipSuccess;
+    }
+    hipLaunchKernelGGL(routes_kernel, dim3((T + 255u) / 256u), dim3(256), 0, st, ws.ids, ids, T, k, E);
+    if (!launch_rows(ws.xq, ws.xs, hidden, T, H, A.xstride, st) ||
         !k3_moe_route_plan(ws.counts, ws.offsets, ws.unique, ws.summary, ws.token_index,
                            ws.route_index, ws.ids, T, k, E, ws.plan, ws.plan_bytes, st))
         return false;
-    hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(1024), 0, st, ws.tiles, ws.tile_count, ws.counts,
-                       ws.offsets, E);
-    const ExpertArgs A{experts, ws.tiles, ws.tile_count, ws.token_index, ws.route_index, ws.xq,
-                       ws.xs, ws.h, ws.hq, ws.hs, ws.y, H, F, s.activation, s.beta, s.linear_beta};
-    hipLaunchKernelGGL(gateup_kernel, dim3(F / 64u, ws.tile_cap), dim3(256), 0, st, A);
-    const uint64_t blocks = (uint64_t)T * k * (F / kBlock);
-    hipLaunchKernelGGL(rows_kernel<float>, dim3((uint32_t)((blocks + 15u) / 16u)), dim3(256), 0, st,
-                       ws.hq, ws.hs, ws.h, blocks);
-    hipLaunchKernelGGL(down_kernel, dim3(H / 64u, ws.tile_cap), dim3(256), 0, st, A);
-    return hipGetLastError() == hipSuccess &&
+    hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(1024), 0, st, ws.lists, ws.counts, ws.offsets, E);
+    hipLaunchKernelGGL(gateup_stream_kernel<false>, dim3(ws.cap[0] * (F / kBlock)), dim3(512), 0, st, A);
+    hipLaunchKernelGGL(down_stream_kernel, dim3(ws.cap[0] * (H / kBlock)), dim3(256), 0, st, A);
+    TileArgs B{};
+    B.experts = experts, B.token_index = ws.token_index, B.route_index = ws.route_index;
+    B.xq = ws.xq, B.xs = ws.xs, B.xstride = A.xstride;
+    B.out = ws.y, B.hq = ws.hq, B.hs = ws.hs, B.hstride = A.hstride;
+    B.kind = s.activation, B.beta = s.beta, B.lb = s.linear_beta;
+    return hipGetLastError() == hipSuccess && launch_class<Tile64>(B, ws, 1, s, st) &&
+           launch_class<Tile128>(B, ws, 2, s, st) && launch_class<Tile256>(B, ws, 3, s, st) &&
            launch_combine(output, ws.y, residual, ws.ids, wts, T, H, k, E, st);
 }
 
@@ -387,7 +1062,8 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
 
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
     (void)rows;
-    return align256((size_t)T * cols) + align256((size_t)T * (cols / kBlock) * 4u);
+    if (T == 1u) return 0u; /* encoded by the product's own kernel */
+    return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols));
 }
 
 }  // namespace k3
@@ -398,10 +1074,10 @@ extern "C" bool k3_moe_fp8_128_quantize_rows_bf16(uint8_t *codes, float *scales,
                                                   uint32_t rows, uint32_t columns, void *stream) {
     const uint64_t blocks = (uint64_t)rows * (columns / kBlock);
     if (!codes || !scales || !src || rows == 0u || columns == 0u || columns % kBlock != 0u ||
-        blocks > (1ull << 34) || ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
+        blocks > (1ull << 34) || /* the grid */ ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
         ((uintptr_t)scales % 4u) != 0u)
         return false;
-    return launch_rows(codes, scales, (const uint16_t *)src, blocks, (hipStream_t)stream);
+    return launch_rows(codes, scales, src, rows, columns, columns / kBlock, (hipStream_t)stream);
 }
 
 extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const void *src,
@@ -420,7 +1096,7 @@ extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scale
 extern "C" size_t k3_moe_fp8_128_scratch_bytes(uint32_t vector_count, uint32_t rows,
                                                uint32_t columns) {
     if (vector_count == 0u || vector_count > 65535u || rows == 0u || columns == 0u ||
-        columns % kBlock != 0u)
+        columns % kBlock != 0u || columns > kMostColumns)
         return 0u;
     return fp8_scratch_bytes(vector_count, rows, columns);
 }
@@ -430,7 +1106,7 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
                                          uint32_t columns, void *scratch, size_t scratch_bytes,
                                          void *stream) {
     if (!output || !codes || !scales || !input || vector_count == 0u || vector_count > 65535u ||
-        rows == 0u || columns == 0u || columns % kBlock != 0u ||
+        rows == 0u || columns == 0u || columns % kBlock != 0u || columns > kMostColumns ||
         (((uintptr_t)codes | (uintptr_t)input) % 16u) != 0u || ((uintptr_t)scales % 4u) != 0u ||
         ((uintptr_t)output % 2u) != 0u)
         return false;
@@ -438,15 +1114,22 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
     if (need != 0u && (!scratch || scratch_bytes < need || ((uintptr_t)scratch % 256u) != 0u))
         return false;
     const hipStream_t st = (hipStream_t)stream;
+    const bool wide = rows % 4u == 0u && ((uintptr_t)output % 8u) == 0u;
+    ProductArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, nullptr, nullptr, 0u,
+                  vector_count, rows, columns, wide};
+    if (vector_count == 1u) return launch_stream<1, 1, true>(A, st);
     uint8_t *xq = (uint8_t *)scratch;
     float *xs = (float *)(xq + align256((size_t)vector_count * columns));
-    if (!launch_rows(xq, xs, (const uint16_t *)input, (uint64_t)vector_count * (columns / kBlock),
-                     st))
-        return false;
-    hipLaunchKernelGGL(product_kernel, dim3((rows + 63u) / 64u, (vector_count + 15u) / 16u),
-                       dim3(256), 0, st, (uint16_t *)output, codes, scales, xq, xs, vector_count,
-                       rows, columns);
-    return hipGetLastError() == hipSuccess;
+    A.xq = xq, A.xs = xs, A.xstride = scale_stride(columns);
+    if (!launch_rows(xq, xs, input, vector_count, columns, A.xstride, st)) return false;
+    if (vector_count <= 16u) return launch_stream<1, 1, false>(A, st);
+    if (vector_count <= 32u) return launch_stream<2, 2, false>(A, st);
+    if (vector_count <= 48u) return launch_stream<2, 3, false>(A, st);
+    if (vector_count <= 64u) return launch_stream<2, 4, false>(A, st);
+    TileArgs B{};
+    B.codes = codes, B.scales = scales, B.xq = xq, B.xs = xs, B.xstride = A.xstride;
+    B.out = A.out, B.T = vector_count, B.N = rows, B.K = columns, B.wide = wide;
+    return vector_count <= 512u ? launch_dense<Tile128>(B, st) : launch_dense<Tile256>(B, st);
 }
 
 extern "C" size_t k3_moe_fp8_workspace_bytes(const k3_moe_shape *shape, uint32_t token_count) {
@@ -475,13 +1158,9 @@ extern "C" bool k3_moe_fp8_experts_bf16(void *output, const void *hidden, const 
         return false;
     const Fp8Workspace ws = carve(workspace, *shape, token_count);
     if (workspace_bytes < ws.bytes) return false;
-    const hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(routes_kernel, dim3((token_count + 255u) / 256u), dim3(256), 0, st, ws.ids,
-                       (const uint32_t *)expert_ids, token_count, shape->top_k,
-                       shape->expert_count);
-    return hipGetLastError() == hipSuccess &&
-           run_fp8_experts(ws, output, hidden, residual, (const float *)expert_weights, experts,
-                           *shape, token_count, st);
+    return run_fp8_experts(ws, output, hidden, residual, (const uint32_t *)expert_ids,
+                           (const float *)expert_weights, experts, *shape, token_count,
+                           (hipStream_t)stream);
 }
 
 extern "C" bool k3_moe_fp8_forward_bf16(void *output, const void *hidden, const void *residual,
@@ -506,5 +1185,6 @@ extern "C" bool k3_moe_fp8_forward_bf16(void *output, const void *hidden, const 
         (expert_weights && hipMemcpyAsync(expert_weights, ws.weights, route_bytes,
                                           hipMemcpyDefault, st) != hipSuccess))
         return false;
-    return run_fp8_experts(ws, output, hidden, residual, ws.weights, experts, s, token_count, st);
+    return run_fp8_experts(ws, output, hidden, residual, ws.ids, ws.weights, experts, s, token_count,
+                           st);
 }
