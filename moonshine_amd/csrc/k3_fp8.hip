@@ -138,9 +138,10 @@ __device__ __forceinline__ f32x4 mfma_block(u32x4_t a0, u32x4_t a1, u32x4_t b0, 
                      (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
     const i32x8 b = {(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w,
                      (int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w};
-    /* both scale operands 2^0 */
+    /* no block scales: with constant zeros the unscaled form of the instruction
+     * (alone on the part 4993 TFLOP/s, with scales of 2^0 4594) */
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0,
-                                                            0, 0, 127, 0, 127);
+                                                            0, 0, 0, 0, 0);
 }
 
 __device__ __forceinline__ uint2 bf16x4(const f32x4 &v) {
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(512) void gateup_stream_kernel(ExpertArgs A) {
         if (e >= A.E) return;
     } else {
         if (tile >= *A.tile_count) return;
-        e = A.tiles[3u * tile], row0 = A.tiles[3u * tile + 1u], rows = A.tiles[3u * tile + 2u];
+        e = A.tiles[4u * tile], row0 = A.tiles[4u * tile + 1u], rows = A.tiles[4u * tile + 2u];
     }
     const k3_moe_fp8_expert ex = A.experts[e];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.H / kBlock;
@@ -504,8 +505,8 @@ __device__ __forceinline__ void stream_rows(f32x4 (&acc)[NI], const uint8_t *con
 __global__ __launch_bounds__(256) void down_stream_kernel(ExpertArgs A) {
     const uint32_t cols = A.H / kBlock, tile = blockIdx.x / cols, col = blockIdx.x % cols;
     if (tile >= *A.tile_count) return;
-    const uint32_t row0 = A.tiles[3u * tile + 1u], rows = A.tiles[3u * tile + 2u];
-    const k3_moe_fp8_expert ex = A.experts[A.tiles[3u * tile]];
+    const uint32_t row0 = A.tiles[4u * tile + 1u], rows = A.tiles[4u * tile + 2u];
+    const k3_moe_fp8_expert ex = A.experts[A.tiles[4u * tile]];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.F / kBlock;
     const uint32_t n0 = kBlock * col + 32u * (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t r = row0 + min(c, rows - 1u);
@@ -563,7 +564,7 @@ __global__ __launch_bounds__(512) void down_one_kernel(ExpertArgs A) {
  * them in a ring. A wave keeps its four weight fragments of a stage in
  * registers and streams the token fragments: four MFMAs with C = 0 each, whose
  * result goes into the fp32 accumulator with one fma per value under the factor
- * sx sw; two waves a SIMD hide each other's waits between the two. Token scales
+ * sx sw, one subtile later. Token scales
  * come four blocks at a time (16 bytes a token) into two buffers; the weights'
  * are held by the lanes of a wave, 64 blocks at a time, and read out by index.
  */
@@ -576,12 +577,16 @@ struct Tile {
     static constexpr int DA = 4, DB = TI < 2 ? 1 : TI / 2, D = DA + DB; /* loads a wave */
     static constexpr uint32_t LDS = STAGES * STAGE + 2u * SBUF;
     static_assert(LDS <= 160u * 1024u, "LDS");
+    /* Two stages: a stage's weights have been read once its first subtile is
+     * under way, so after a second barrier in mid-stage their place takes the
+     * weights of two stages on (they come from HBM, the tokens from the L2). */
+    static constexpr bool EARLY = STAGES == 2;
 };
 
 enum TileMode { kDense, kGateUp, kDown };
 
 struct TileArgs {
-    /* dense: the weight; otherwise the experts and the tiles {expert, row, rows} */
+    /* dense: the weight; otherwise the experts and the tiles */
     const uint8_t *codes;
     const float *scales;
     const k3_moe_fp8_expert *experts;
@@ -610,18 +615,31 @@ struct TileRun {
     const float *sw0, *sw1;             /* weight scales of fragments 0, 1 and 2, 3 */
     uint32_t nblk, wave, lane, wn, wt;
 
-    __device__ __forceinline__ void fetch(uint8_t *smem, uint32_t s, uint32_t slot) const {
+    __device__ __forceinline__ void fetch_scales(uint8_t *smem, uint32_t s) const {
         if (has_sx && s % 4u == 0u && s < nblk)
             dma<16>((const uint8_t *)(sx + s),
                     smem + C::STAGES * C::STAGE + C::SBUF * ((s >> 2) & 1u) + 1024u * wave);
+    }
+    /* Load Q of stage s; past the end the last stage again, so that the counts
+     * of the waits stay. */
+    template <int Q>
+    __device__ __forceinline__ void fetch_one(uint8_t *smem, uint32_t s, uint32_t slot) const {
         const uint32_t at = kBlock * (s < nblk ? s : nblk - 1u);
-        const uint8_t *pa = a_base + at, *pb = b_base + at;
         uint8_t *st = smem + C::STAGE * slot;
+        if constexpr (Q < C::DA)
+            dma<16>(a_base + at + a[Q], st + 1024u * (C::DA * wave + Q));
+        else
+            dma<16>(b_base + at + b[Q - C::DA],
+                    st + C::A + 1024u * (C::TI < 2 ? wave & 3u : C::DB * wave + (Q - C::DA)));
+    }
+    template <int FROM, int TO>
+    __device__ __forceinline__ void fetch(uint8_t *smem, uint32_t s, uint32_t slot) const {
+        static_for<TO - FROM>([&](auto Q) { fetch_one<FROM + decltype(Q)::value>(smem, s, slot); });
+    }
+
+    static __device__ __forceinline__ void scale_in(f32x4 &acc, const f32x4 &p, float f) {
 #pragma unroll
-        for (int q = 0; q < C::DA; q++) dma<16>(pa + a[q], st + 1024u * (C::DA * wave + q));
-#pragma unroll
-        for (int q = 0; q < C::DB; q++)
-            dma<16>(pb + b[q], st + C::A + 1024u * (C::TI < 2 ? wave & 3u : C::DB * wave + q));
+        for (int r = 0; r < 4; r++) acc[r] = fmaf(p[r], f, acc[r]);
     }
 
     template <int TL, bool Two>
@@ -631,20 +649,33 @@ struct TileRun {
         const uint32_t a_at = base + 8192u * wn, b_at = base + C::A + 2048u * wt;
         const uint32_t s_at = base + C::STAGES * C::STAGE + 16u * (16u * wt + c);
         float w0 = 0.0f, w1 = 0.0f;
+        f32x4 p[2][4]; /* the products of a subtile and of the one before, and their factors */
+        float f[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll
-        for (int s = 0; s < C::STAGES - 1; s++) fetch(smem, (uint32_t)s, (uint32_t)s);
+        for (int i = 0; i < 4; i++) p[1][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < C::STAGES - 1; s++) {
+            fetch_scales(smem, (uint32_t)s);
+            fetch<0, C::D>(smem, (uint32_t)s, (uint32_t)s);
+        }
+        if constexpr (C::EARLY) fetch<0, C::DA>(smem, 1u, 1u);
         uint32_t slot = 0u, next = C::STAGES - 1;
         for (uint32_t s = 0; s < nblk; s++) {
             if (s % 64u == 0u) { /* the weight scales of the next 64 blocks */
                 const uint32_t q = s + lane < nblk ? s + lane : nblk - 1u;
                 w0 = sw0[q];
                 if (Two) w1 = sw1[q];
+                /* waited for here: at its use the wait would drain the loads
+                 * ahead in every stage */
+                asm volatile("" : "+v"(w0), "+v"(w1));
             }
-            wait_vm<C::D *(C::STAGES - 2)>(); /* this wave's loads of stage s */
+            /* this wave's loads of stage s; later ones stay out */
+            wait_vm<C::EARLY ? C::DA : C::D *(C::STAGES - 2)>();
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier(); /* everyone's; and stage s - 1 has been read */
             asm volatile("" ::: "memory");
-            if (C::STAGES > 2 || s + 1u < nblk) fetch(smem, s + C::STAGES - 1u, next);
+            const uint32_t ahead = s + C::STAGES - 1u, to = next;
+            fetch_scales(smem, ahead);
             const uint32_t st = C::STAGE * slot, sb = s_at + C::SBUF * ((s >> 2) & 1u) + 4u * (s & 3u);
             next = slot;
             slot = slot + 1u == (uint32_t)C::STAGES ? 0u : slot + 1u;
@@ -652,46 +683,81 @@ struct TileRun {
             const float sw_1 = Two ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w1), (int)(s & 63u))) : sw_0;
             u32x4_t af[4][2], bf[2][2];
             uint32_t sx_[2];
+            auto read_b = [&](auto J) {
+                constexpr int j = decltype(J)::value;
+                sx_[j & 1] = ds_read4<512 * j>(sb);
+                bf[j & 1][0] = ds_read16<4096 * j>(b_at + st + lo);
+                bf[j & 1][1] = ds_read16<4096 * j>(b_at + st + hi);
+            };
+            read_b(std::integral_constant<int, 0>{});
             static_for<4>([&](auto I) {
                 constexpr int i = decltype(I)::value;
                 af[i][0] = ds_read16<2048 * i>(a_at + st + lo);
                 af[i][1] = ds_read16<2048 * i>(a_at + st + hi);
             });
-            sx_[0] = ds_read4<0>(sb);
-            bf[0][0] = ds_read16<0>(b_at + st + lo);
-            bf[0][1] = ds_read16<0>(b_at + st + hi);
             static_for<TL>([&](auto J) {
                 constexpr int j = decltype(J)::value;
-                if constexpr (j + 1 < TL) {
-                    sx_[(j + 1) & 1] = ds_read4<512 * (j + 1)>(sb);
-                    bf[(j + 1) & 1][0] = ds_read16<4096 * (j + 1)>(b_at + st + lo);
-                    bf[(j + 1) & 1][1] = ds_read16<4096 * (j + 1)>(b_at + st + hi);
-                    wait_lgkm<3>();
-                } else {
-                    wait_lgkm<0>();
-                }
+                /* the next subtile's reads stay out; in the first one the weight
+                 * fragments are waited for one by one */
+                constexpr int out = j + 1 < TL ? 3 : 0;
+                if constexpr (j + 1 < TL) read_b(std::integral_constant<int, j + 1>{});
+                wait_lgkm<(j == 0 ? 6 : 0) + out>();
                 if constexpr (j == 0) {
-                    static_for<4>([&](auto I) {
-                        after_wait(af[decltype(I)::value][0]);
-                        after_wait(af[decltype(I)::value][1]);
-                    });
+                    after_wait(af[0][0]);
+                    after_wait(af[0][1]);
                 }
                 after_wait(sx_[j & 1]);
                 after_wait(bf[j & 1][0]);
                 after_wait(bf[j & 1][1]);
                 const float sx = __uint_as_float(sx_[j & 1]);
-                const float f0 = __fmul_rn(sx, sw_0), f1 = Two ? __fmul_rn(sx, sw_1) : f0;
-                f32x4 p[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    p[i] = mfma_block(af[i][0], af[i][1], bf[j & 1][0], bf[j & 1][1]);
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        acc[j][i][r] = fmaf(p[i][r], i < 2 ? f0 : f1, acc[j][i][r]);
+                f[j & 1][0] = __fmul_rn(sx, sw_0);
+                f[j & 1][1] = Two ? __fmul_rn(sx, sw_1) : f[j & 1][0];
+                /* a product, then the four fmas of the subtile before: they run
+                 * while the matrix unit is busy */
+                constexpr int q = (j + TL - 1) % TL;
+                static_for<4>([&](auto I) {
+                    constexpr int i = decltype(I)::value;
+                    if constexpr (j == 0 && i > 0) {
+                        wait_lgkm<6 - 2 * i + out>();
+                        after_wait(af[i][0]);
+                        after_wait(af[i][1]);
+                    }
+                    p[j & 1][i] = mfma_block(af[i][0], af[i][1], bf[j & 1][0], bf[j & 1][1]);
+                    scale_in(acc[q][i], p[(j + 1) & 1][i], f[(j + 1) & 1][i >> 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    /* the loads ahead, spread over the products: at once they
+                     * would keep the waves from their first reads */
+                    constexpr int half = 4 * ((TL + 1) / 2), at = 4 * j + i;
+                    if constexpr (C::EARLY) {
+                        if constexpr (at == half - 1) {
+                            asm volatile("" ::: "memory");
+                            __builtin_amdgcn_s_barrier();
+                            asm volatile("" ::: "memory");
+                        }
+                        static_for<C::DB>([&](auto Q) {
+                            if constexpr (decltype(Q)::value * (half - 1) / C::DB == at)
+                                fetch_one<C::DA + decltype(Q)::value>(smem, ahead, to);
+                        });
+                        static_for<C::DA>([&](auto Q) {
+                            if constexpr (half - 1 + decltype(Q)::value * (4 * TL - half) / C::DA == at)
+                                fetch_one<decltype(Q)::value>(smem, s + 2u, to ^ 1u);
+                        });
+                    } else {
+                        static_for<C::D>([&](auto Q) {
+                            if constexpr (decltype(Q)::value * half / C::D == at)
+                                fetch_one<decltype(Q)::value>(smem, ahead, to);
+                        });
+                    }
+                });
             });
+            if constexpr (TL % 2 != 0) { /* the next stage's first subtile has the same parity */
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[1][i] = p[0][i];
+                f[1][0] = f[0][0], f[1][1] = f[0][1];
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++) scale_in(acc[TL - 1][i], p[1][i], f[1][i >> 1]);
         wait_vm<0>(); /* the loads past the end land before the LDS is used again */
     }
 };
@@ -715,7 +781,11 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
         const uint32_t high = min(4u, tiles - 4u * grp);
         tile = 4u * grp + in % high, col = in / high;
     } else {
-        tile = w / P.tiles_n, col = w % P.tiles_n;
+        /* an expert's tiles of one column block are neighbours: they read the
+         * same weights at about the same time, through the same L2 */
+        const uint32_t t = w / P.tiles_n, in = P.tiles[4u * t + 3u];
+        const uint32_t many = in >> 16, local = (in & 0xffffu) * P.tiles_n + w % P.tiles_n;
+        tile = t - (in & 0xffffu) + local % many, col = local / many;
     }
     uint32_t row0, rows;
     const uint8_t *w0, *w1;
@@ -727,7 +797,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
         const uint32_t nb = min(nb0 + (R.wn >> 1), blocks_n - 1u);
         R.sw0 = R.sw1 = P.scales + (uint64_t)nb * nblk;
     } else {
-        const uint32_t *t = P.tiles + 3u * tile;
+        const uint32_t *t = P.tiles + 4u * tile;
         row0 = t[1], rows = t[2];
         const k3_moe_fp8_expert ex = P.experts[t[0]];
         if constexpr (MODE == kGateUp) {
@@ -874,7 +944,8 @@ __global__ __launch_bounds__(256) void routes_kernel(uint32_t *__restrict__ out,
 constexpr int kClasses = 4;
 
 /* One block of 1024 threads (thread e: expert e): each class's tiles {expert,
- * first row, rows} in expert order, from its own base on. */
+ * first row, rows, index among the expert's tiles | their number << 16} in
+ * expert order. */
 struct TileLists {
     uint32_t *tiles[kClasses];
     uint32_t *count; /* [kClasses] */
@@ -910,10 +981,11 @@ __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t
         }
         if (cls == q)
             for (uint32_t i = 0; i < mine; i++) {
-                uint32_t *t = Q.tiles[q] + 3u * (at + i);
+                uint32_t *t = Q.tiles[q] + 4u * (at + i);
                 t[0] = e;
                 t[1] = offsets[e] + height * i;
                 t[2] = min(height, n - height * i);
+                t[3] = i | mine << 16;
             }
         if (e == 0u) Q.count[q] = total;
     }
@@ -959,7 +1031,7 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
     for (int q = 0; q < kClasses; q++) {
         const size_t n = routes / least[q];
         w.cap[q] = T < least[q] ? 0u : (uint32_t)(q < 3 && n > E ? E : n);
-        w.lists.tiles[q] = (uint32_t *)take(12u * (size_t)w.cap[q]);
+        w.lists.tiles[q] = (uint32_t *)take(16u * (size_t)w.cap[q]);
     }
     w.lists.count = (uint32_t *)take(4u * kClasses);
     w.xq = take((size_t)T * s.hidden);
