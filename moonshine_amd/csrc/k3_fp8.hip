@@ -6,13 +6,12 @@
  *
  *   rows_kernel           token rows
  *   weight_kernel         a weight, one 128 x 128 block a block
- *   stream_kernel         products of up to 64 tokens: weights straight to
- *                         registers, K split over a block's waves
- *   gateup_stream_kernel  act(gate . x, up . x) of an expert's up to 16 rows,
- *   down_stream_kernel    and y[route] = bf16(down . h)
- *   down_one_kernel       down of a single token's routes, and their sum
- *   tile_kernel           products of many tokens: tiles in LDS; dense, gate/up
- *                         and down
+ *   product_one_kernel    one token's product,
+ *   gateup_one_kernel     act(gate . x, up . x) of its routes,
+ *   down_one_kernel       their down products and weighted sum
+ *   tile_kernel           more tokens, tiles in LDS: dense, gate/up of the
+ *                         experts, y[route] = bf16(down . h)
+ *   join_kernel           a dense product's parts of K
  *
  * MFMA operands (V_MFMA_F32_16X16X128_F8F6F4): lane 16 g + c holds 32 codes of
  * row c of the 16 x 128 slices: bytes [16 g, 16 g + 16) and [64 + 16 g, 64 +
@@ -67,8 +66,7 @@ __device__ __forceinline__ uint2 fp8_codes8(const float (&v)[8], float inv) {
     return make_uint2(w[0], w[1]);
 }
 
-__device__ __forceinline__ void load8(const uint16_t *src, float (&v)[8]) {
-    const uint4 p = *(const uint4 *)src;
+__device__ __forceinline__ void unpack8(const uint4 &p, float (&v)[8]) {
     const uint32_t d[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -76,6 +74,10 @@ __device__ __forceinline__ void load8(const uint16_t *src, float (&v)[8]) {
         v[2 * i + 1] = bf16_hi(d[i]);
     }
 }
+__device__ __forceinline__ void load8(const uint16_t *src, float (&v)[8]) {
+    unpack8(*(const uint4 *)src, v);
+}
+
 __device__ __forceinline__ float max8(const float (&v)[8]) {
     float m = 0.0f;
 #pragma unroll
@@ -193,353 +195,331 @@ __device__ __forceinline__ float act_f32(float g, float u, uint32_t kind, float 
 }
 
 /* ---------------------------------------------------------------------- */
-/* streams of weights for few tokens                                       */
+/* one token                                                               */
 /* ---------------------------------------------------------------------- */
 
-/* This lane's codes of a block of 128 columns: 16 at p and 16 at p + 64. */
-struct Frag {
-    u32x4_t lo, hi;
-};
-__device__ __forceinline__ Frag frag(const uint8_t *p) {
-    typedef const __attribute__((address_space(1))) u32x4_t *gp;
-    return Frag{((gp)p)[0], ((gp)p)[4]};
+/* A row of scales, 64 at a time by the lanes of a wave (those from base on):
+ * loaded one by one, each block of columns would wait for its own. */
+__device__ __forceinline__ float lane_scales(const float *row, uint32_t base, uint32_t n) {
+    const uint32_t k = base + (threadIdx.x & 63u);
+    return row[k < n ? k : n - 1u];
 }
-__device__ __forceinline__ Frag frag_nt(const uint8_t *p) {
-    typedef const __attribute__((address_space(1))) u32x4_t *gp;
-    return Frag{__builtin_nontemporal_load((gp)p), __builtin_nontemporal_load((gp)p + 4)};
-}
-__device__ __forceinline__ f32x4 mfma_block(const Frag &a, const Frag &b) {
-    return mfma_block(a.lo, a.hi, b.lo, b.hi);
+__device__ __forceinline__ float scale_at(float scales, uint32_t k) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), (int)(k & 63u)));
 }
 
-struct ProductArgs {
+/*
+ * A wave's own ring of weights in LDS: M matrices x 16 rows x 128 columns a
+ * stage. Direct-to-LDS loads take whole 128-byte lines (eight rows an
+ * instruction); straight into the registers of the MFMA layout a load touches
+ * 16 rows in 16-byte pieces, which holds a CU to about 10 bytes a clock (61
+ * tokens' gate/up: 4.8 TB/s so, 6.1 TB/s through LDS). No wave waits for
+ * another. Loads past the end take the last block again: the waits count them.
+ */
+template <int M, int R>
+struct WaveRing {
+    static constexpr uint32_t STAGE = 2048u * M, BYTES = STAGE * R;
+    const uint8_t *src[M]; /* row 0 of the 16, at column 0 */
+    uint32_t off[2];       /* this lane's place in the two loads of a matrix */
+    uint8_t *smem;
+    uint32_t base;
+
+    __device__ __forceinline__ void init(uint8_t *lds, const uint8_t *const (&w)[M], uint32_t rows,
+                                         uint32_t K) {
+        const uint32_t L = threadIdx.x & 63u;
+        smem = lds, base = lds_addr(lds);
+#pragma unroll
+        for (int m = 0; m < M; m++) src[m] = w[m];
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; h++)
+            off[h] = min(a_dma_row(L, h), rows - 1u) * K + 16u * a_dma_piece(L, h);
+    }
+    __device__ __forceinline__ void fetch(uint32_t block, uint32_t slot) const {
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++)
+                dma<16>(src[m] + kBlock * block + off[h], smem + STAGE * slot + 2048u * m + 1024u * h);
+    }
+    /* The products of the stage in `slot` with the token codes at LDS address x. */
+    __device__ __forceinline__ void products(f32x4 (&p)[M], uint32_t slot, uint32_t x) const {
+        const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u;
+        const uint32_t at = base + STAGE * slot;
+        u32x4_t a[M][2], b[2];
+        wait_vm<2 * M *(R - 1)>();
+        asm volatile("" ::: "memory");
+        static_for<M>([&](auto Q) {
+            constexpr int m = decltype(Q)::value;
+            a[m][0] = ds_read16<2048 * m>(at + a_slot(c, g));
+            a[m][1] = ds_read16<2048 * m>(at + a_slot(c, 4u + g));
+        });
+        b[0] = ds_read16<0>(x + 16u * g);
+        b[1] = ds_read16<64>(x + 16u * g);
+        wait_lgkm<0>();
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            after_wait(a[m][0]);
+            after_wait(a[m][1]);
+        }
+        after_wait(b[0]);
+        after_wait(b[1]);
+#pragma unroll
+        for (int m = 0; m < M; m++) p[m] = mfma_block(a[m][0], a[m][1], b[0], b[1]);
+        asm volatile("" ::: "memory");
+    }
+};
+
+__device__ __forceinline__ void ds_write8(uint32_t addr, uint2 v) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 w = {v.x, v.y};
+    asm volatile("ds_write_b64 %0, %1" ::"v"(addr), "v"(w) : "memory");
+}
+__device__ __forceinline__ void ds_write4(uint32_t addr, uint32_t v) {
+    asm volatile("ds_write_b32 %0, %1" ::"v"(addr), "v"(v) : "memory");
+}
+/* Between LDS writes and other waves' reads, with loads to LDS still out. */
+__device__ __forceinline__ void lds_barrier() {
+    wait_lgkm<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+/* A block of 512 threads encodes up to 64 blocks of 128 values into LDS: codes at
+ * `codes`, scales at `scales` (LDS addresses). Loads first, so that what is
+ * issued between the two halves does not stand in their way. */
+struct TokenPart {
+    uint4 v[2];
+    __device__ __forceinline__ void load(const uint16_t *x, uint32_t n) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2u; i++)
+            v[i] = ((const uint4 *)x)[min(threadIdx.x + 512u * i, 16u * n - 1u)];
+    }
+    __device__ __forceinline__ void encode(uint32_t n, uint32_t codes, uint32_t scales) const {
+#pragma unroll
+        for (uint32_t i = 0; i < 2u; i++) {
+            const uint32_t q = threadIdx.x + 512u * i;
+            if (q >= 16u * n) continue; /* whole rows of 16 lanes */
+            float u[8], scale, inv;
+            unpack8(v[i], u);
+            fp8_scales(row_group_max<16>(max8(u)), scale, inv);
+            ds_write8(codes + 8u * q, fp8_codes8(u, inv));
+            if ((q & 15u) == 0u) ds_write4(scales + (q >> 2), __float_as_uint(scale));
+        }
+    }
+};
+
+struct OneArgs {
     uint16_t *out;
     const uint8_t *codes;
     const float *scales;
-    const uint16_t *x; /* one token, not encoded */
-    const uint8_t *xq;
-    const float *xs;
-    uint32_t xstride, T, N, K;
-    bool wide;
+    const uint16_t *x;
+    uint32_t N, K;
 };
 
 /*
- * 16 NI weight rows x up to 16 TI tokens a block; its eight waves take every
- * eighth block of columns, eight at a time, and add up through LDS in one
- * order. Weights go straight to registers: each is used once. ONE: a single
- * token, whose values the wave encodes itself, two a lane, through LDS (no
- * second launch; all 16 columns of the products are the same token).
+ * One token times a weight, 16 rows a block: its eight waves take every eighth
+ * block of columns and add up through LDS in one order. The token is encoded
+ * 64 blocks of columns at a time, by the block, under the first weight loads.
  */
-template <int NI, int TI, bool ONE>
-__global__ __launch_bounds__(512) void stream_kernel(ProductArgs P) {
-    constexpr int G = NI * TI > 4 ? 2 : NI * TI > 1 ? 4 : 8; /* blocks of a wave in flight */
-    __shared__ __attribute__((aligned(16))) float sums[8][NI * TI][64][4];
-    __shared__ __attribute__((aligned(16))) uint8_t xcode[ONE ? 8 : 1][ONE ? 8 : 1][kBlock];
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u;
+constexpr int kOneRing = 4;
+__global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
+    using Ring = WaveRing<1, kOneRing>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * Ring::BYTES + 64u * (kBlock + 4u)];
+    __shared__ float sums[8][16];
+    const uint32_t lane = threadIdx.x & 63u, nblk = P.K / kBlock, n0 = 16u * blockIdx.x;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t n0 = 16u * NI * blockIdx.x, nblk = P.K / kBlock;
-    const uint8_t *w[NI], *x[TI];
-    const float *xs[TI], *sw = P.scales + (uint64_t)(n0 / kBlock) * nblk;
+    const uint32_t codes = lds_addr(smem) + 8u * Ring::BYTES, scales = codes + 64u * kBlock;
+    const float *ws = P.scales + (uint64_t)(n0 / kBlock) * nblk;
+    /* lane q: the scale of the wave's q-th block of 64 */
+    float sw = ws[min(wave + 8u * (lane & 7u), nblk - 1u)];
+    TokenPart x;
+    x.load(P.x, min(64u, nblk));
+    asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
+    Ring ring;
+    const uint8_t *const w[1] = {P.codes + (uint64_t)n0 * P.K};
+    ring.init(smem + Ring::BYTES * wave, w, P.N - n0, P.K);
 #pragma unroll
-    for (int i = 0; i < NI; i++) w[i] = P.codes + (uint64_t)min(n0 + 16u * i + c, P.N - 1u) * P.K + 16u * g;
+    for (uint32_t q = 0; q < kOneRing; q++) ring.fetch(min(wave + 8u * q, nblk - 1u), q);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t slot = 0u;
+    for (uint32_t base = 0; base < nblk; base += 64u) {
+        const uint32_t n = min(64u, nblk - base);
+        if (base != 0u) {
+            sw = ws[min(base + wave + 8u * (lane & 7u), nblk - 1u)];
+            x.load(P.x + kBlock * base, n);
+            lds_barrier(); /* the codes before have been read */
+        }
+        x.encode(n, codes, scales);
+        asm volatile("" : "+v"(sw)); /* waited for here, not in the loop */
+        lds_barrier();
+        for (uint32_t k = wave, q = 0; k < n; k += 8u, q++) {
+            f32x4 p[1];
+            uint32_t sx = ds_read4<0>(scales + 4u * k);
+            ring.products(p, slot, codes + kBlock * k); /* waits for sx too */
+            after_wait(sx);
+            const float f = __fmul_rn(__uint_as_float(sx), scale_at(sw, q));
 #pragma unroll
-    for (int j = 0; j < TI; j++) {
-        const uint64_t t = ONE ? 0u : min(16u * j + c, P.T - 1u);
-        x[j] = P.xq + t * P.K + 16u * g;
-        xs[j] = P.xs + t * P.xstride;
+            for (int r = 0; r < 4; r++) acc[r] = fmaf(p[0][r], f, acc[r]);
+            ring.fetch(min(base + k + 8u * kOneRing, nblk - 1u), slot);
+            slot = slot + 1u == (uint32_t)kOneRing ? 0u : slot + 1u;
+        }
     }
-    f32x4 acc[TI][NI];
+    wait_vm<0>();
+    if ((lane & 15u) == 0u)
 #pragma unroll
-    for (int j = 0; j < TI; j++)
-#pragma unroll
-        for (int i = 0; i < NI; i++) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t b0 = wave; b0 < nblk; b0 += 8u * G) {
-        Frag a[G][NI], b[ONE ? 1 : G][TI];
-        float s[G][TI];
-#pragma unroll
-        for (int q = 0; q < G; q++) {
-            const uint32_t k = b0 + 8u * q;
-            if (k >= nblk) break;
-#pragma unroll
-            for (int i = 0; i < NI; i++) a[q][i] = frag_nt(w[i] + kBlock * k);
-            if constexpr (!ONE) {
-#pragma unroll
-                for (int j = 0; j < TI; j++) {
-                    b[q][j] = frag(x[j] + kBlock * k);
-                    s[q][j] = xs[j][k];
-                }
-            }
-        }
-        if constexpr (ONE) {
-            uint32_t v[G];
-            float m[G];
-#pragma unroll
-            for (int q = 0; q < G; q++) {
-                v[q] = ((const uint32_t *)P.x)[64u * min(b0 + 8u * q, nblk - 1u) + lane];
-                m[q] = fmaxf(fabsf(bf16_lo(v[q])), fabsf(bf16_hi(v[q])));
-            }
-#pragma unroll
-            for (int q = 0; q < G; q++) m[q] = row_group_max<16>(m[q]);
-#pragma unroll
-            for (int o = 16; o <= 32; o <<= 1)
-#pragma unroll
-                for (int q = 0; q < G; q++) m[q] = fmaxf(m[q], __shfl_xor(m[q], o, 64));
-#pragma unroll
-            for (int q = 0; q < G; q++) {
-                float inv;
-                fp8_scales(m[q], s[q][0], inv);
-                *(uint16_t *)(xcode[wave][q] + 2u * lane) = (uint16_t)e4m3x2_raw<false>(
-                    __fmul_rn(bf16_lo(v[q]), inv), __fmul_rn(bf16_hi(v[q]), inv), 0u);
-            }
-            wave_fence();
-        }
-#pragma unroll
-        for (int q = 0; q < G; q++) {
-            const uint32_t k = b0 + 8u * q;
-            if (k >= nblk) break;
-            const float wk = sw[k];
-            if constexpr (ONE) {
-                const u32x4_t *p = (const u32x4_t *)(xcode[wave][q] + 16u * g);
-                b[0][0] = Frag{p[0], p[4]};
-            }
-#pragma unroll
-            for (int j = 0; j < TI; j++) {
-                const float f = __fmul_rn(s[q][j], wk);
-#pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const f32x4 p = mfma_block(a[q][i], b[ONE ? 0 : q][j]);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) acc[j][i][r] = fmaf(p[r], f, acc[j][i][r]);
-                }
-            }
-        }
-        if constexpr (ONE) wave_fence(); /* the codes have been read */
-    }
-#pragma unroll
-    for (int j = 0; j < TI; j++)
-#pragma unroll
-        for (int i = 0; i < NI; i++) *(f32x4 *)sums[wave][j * NI + i][lane] = acc[j][i];
+        for (uint32_t r = 0; r < 4u; r++) sums[wave][(lane >> 2) + r] = acc[r];
     __syncthreads();
-    for (uint32_t q = wave; q < NI * TI; q += 8u) {
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (threadIdx.x < 16u && n0 + threadIdx.x < P.N) {
+        float v = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-            const f32x4 p = *(const f32x4 *)sums[u][q][lane];
-#pragma unroll
-            for (int r = 0; r < 4; r++) v[r] = __fadd_rn(v[r], p[r]);
-        }
-        store_rows(P.out, v, 16u * (q / NI) + c, n0 + 16u * (q % NI) + 4u * g, P.T, P.N, P.wide);
+        for (int u = 0; u < 8; u++) v = __fadd_rn(v, sums[u][threadIdx.x]);
+        P.out[n0 + threadIdx.x] = f32_to_bf16(v);
     }
 }
 
-/* Route r of a single token: its id, or E (none: from E on, or an earlier one). */
-__device__ __forceinline__ uint32_t one_route(const uint32_t *ids, uint32_t r, uint32_t E) {
-    const uint32_t e = ids[r];
-    if (e >= E) return E;
-    for (uint32_t q = 0; q < r; q++)
-        if (ids[q] == e) return E;
-    return e;
+/* Route r of a single token: its id, or E (none: from E on, or an earlier
+ * one's). All ids come with one load. */
+__device__ __forceinline__ uint32_t one_route(const uint32_t *ids, uint32_t r, uint32_t k, uint32_t E) {
+    const uint32_t lane = threadIdx.x & 63u, id = lane < k ? ids[lane] : E;
+    const uint32_t e = (uint32_t)__builtin_amdgcn_readlane((int)id, (int)r);
+    return e >= E || __any(lane < r && id == e) ? E : e;
 }
 
-struct ExpertArgs {
+struct OneExpertArgs {
     const k3_moe_fp8_expert *experts;
-    const uint32_t *tiles, *tile_count, *token_index, *route_index, *ids;
-    const uint16_t *x; /* one token, not encoded */
-    const uint8_t *xq; /* [T, H] */
-    const float *xs;
-    uint32_t xstride, hstride;
-    uint8_t *hq; /* [rows, F] in plan order (one token: in rank order) */
-    float *hs;
-    uint16_t *y; /* [routes, H] */
-    uint16_t *out;
-    const uint16_t *residual;
+    const uint32_t *ids;
     const float *weights;
-    uint32_t H, F, E, k, kind;
+    const uint16_t *x, *residual;
+    uint16_t *out;
+    uint8_t *hq; /* [k, F] */
+    float *hs;   /* [k], hstride apart */
+    uint32_t hstride, H, F, E, k, kind;
     float beta, lb;
 };
 
 /*
- * Gate and up of 128 columns of an expert's up to 16 rows: 16 columns of each a
- * wave over the whole of K, four blocks of columns (16 KB of weights) in flight
- * a wave. The 128 columns are a scale block of the activation, encoded here.
- * ONE: a single token, one route a tile, encoded by the block into LDS (H + H /
- * 32 bytes) under the first weight loads.
+ * Gate and up of 128 columns for one route of a single token: 16 columns of each
+ * a wave over the whole of K, 16 KB of weights in flight a wave. The 128 columns
+ * are a scale block of the activation, encoded here. LDS: the rings, then the
+ * token's codes and scales.
  */
-template <bool ONE>
-__global__ __launch_bounds__(512) void gateup_stream_kernel(ExpertArgs A) {
-    constexpr int G = 4;
-    __shared__ float red[8][16];
-    extern __shared__ __attribute__((aligned(16))) uint8_t xbuf[];
-    const uint32_t cols = A.F / kBlock, tile = blockIdx.x / cols, col = blockIdx.x % cols;
-    uint32_t e, row0, rows;
-    if constexpr (ONE) {
-        e = one_route(A.ids, tile, A.E), row0 = tile, rows = 1u;
-        if (e >= A.E) return;
-    } else {
-        if (tile >= *A.tile_count) return;
-        e = A.tiles[4u * tile], row0 = A.tiles[4u * tile + 1u], rows = A.tiles[4u * tile + 2u];
-    }
+constexpr int kGateUpRing = 4;
+constexpr uint32_t kOneHidden = 8192, kOneFfn = 4096; /* widths that a token's kernels hold in LDS */
+__global__ __launch_bounds__(512) void gateup_one_kernel(OneExpertArgs A) {
+    using Ring = WaveRing<2, kGateUpRing>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * Ring::BYTES + kOneHidden + kOneHidden / 32u];
+    __shared__ float red[8];
+    const uint32_t cols = A.F / kBlock, r = blockIdx.x / cols, col = blockIdx.x % cols;
+    TokenPart x;
+    x.load(A.x, A.H / kBlock);
+    const uint32_t e = one_route(A.ids, r, A.k, A.E);
+    if (e >= A.E) return;
     const k3_moe_fp8_expert ex = A.experts[e];
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.H / kBlock;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, nblk = A.H / kBlock;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t f0 = kBlock * col + 16u * wave;
-    const uint64_t at = (uint64_t)(f0 + c) * A.H + 16u * g;
-    const uint8_t *wg = ex.gate_codes + at, *wu = ex.up_codes + at;
-    const float *sg = ex.gate_scales + (uint64_t)col * nblk, *su = ex.up_scales + (uint64_t)col * nblk;
-    const uint8_t *x = nullptr;
-    const float *xs = nullptr;
-    if constexpr (!ONE) {
-        const uint64_t t = A.token_index[row0 + min(c, rows - 1u)];
-        x = A.xq + t * A.H + 16u * g;
-        xs = A.xs + t * A.xstride;
-    }
+    const uint32_t codes = lds_addr(smem) + 8u * Ring::BYTES, scales = codes + A.H;
+    const float *gs = ex.gate_scales + (uint64_t)col * nblk, *us = ex.up_scales + (uint64_t)col * nblk;
+    float sg = lane_scales(gs, 0u, nblk), su = lane_scales(us, 0u, nblk);
+    asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
+    Ring ring;
+    const uint8_t *const w[2] = {ex.gate_codes + (uint64_t)f0 * A.H, ex.up_codes + (uint64_t)f0 * A.H};
+    ring.init(smem + Ring::BYTES * wave, w, 16u, A.H);
+#pragma unroll
+    for (uint32_t q = 0; q < kGateUpRing; q++) ring.fetch(min(q, nblk - 1u), q);
+    x.encode(nblk, codes, scales);
+    asm volatile("" : "+v"(sg), "+v"(su)); /* waited for here, not in the loop */
+    lds_barrier();
     f32x4 gate = {0.0f, 0.0f, 0.0f, 0.0f}, up = gate;
-    Frag ag[G], au[G], b[ONE ? 1 : G];
-    float sx[G];
-    auto load = [&](uint32_t k, int q) {
-        if (k >= nblk) return;
-        ag[q] = frag_nt(wg + kBlock * k);
-        au[q] = frag_nt(wu + kBlock * k);
-        if constexpr (!ONE) {
-            b[q] = frag(x + kBlock * k);
-            sx[q] = xs[k];
-        }
-    };
+    uint32_t slot = 0u;
+    for (uint32_t k = 0; k < nblk; k++) { /* nblk <= 64 */
+        f32x4 p[2];
+        uint32_t sx = ds_read4<0>(scales + 4u * k);
+        ring.products(p, slot, codes + kBlock * k); /* waits for sx too */
+        after_wait(sx);
+        const float fg = __fmul_rn(__uint_as_float(sx), scale_at(sg, k));
+        const float fu = __fmul_rn(__uint_as_float(sx), scale_at(su, k));
+        ring.fetch(min(k + kGateUpRing, nblk - 1u), slot);
 #pragma unroll
-    for (int q = 0; q < G; q++) load((uint32_t)q, q);
-    const float *xsc = (const float *)(xbuf + A.H);
-    if constexpr (ONE) {
-        for (uint32_t q = threadIdx.x; q < 16u * nblk; q += 512u) { /* whole rows of 16 lanes */
-            float v[8], scale, inv;
-            load8(A.x + 8u * q, v);
-            fp8_scales(row_group_max<16>(max8(v)), scale, inv);
-            *(uint2 *)(xbuf + 8u * q) = fp8_codes8(v, inv);
-            if ((q & 15u) == 0u) ((float *)(xbuf + A.H))[q >> 4] = scale;
+        for (int i = 0; i < 4; i++) {
+            gate[i] = fmaf(p[0][i], fg, gate[i]);
+            up[i] = fmaf(p[1][i], fu, up[i]);
         }
-        __syncthreads();
+        slot = slot + 1u == (uint32_t)kGateUpRing ? 0u : slot + 1u;
     }
-    for (uint32_t k0 = 0; k0 < nblk; k0 += G) {
-#pragma unroll
-        for (int q = 0; q < G; q++) {
-            const uint32_t k = k0 + (uint32_t)q;
-            if (k < nblk) {
-                Frag xb;
-                float s;
-                if constexpr (ONE) {
-                    const u32x4_t *p = (const u32x4_t *)(xbuf + kBlock * k + 16u * g);
-                    xb = Frag{p[0], p[4]};
-                    s = xsc[k];
-                } else {
-                    xb = b[q];
-                    s = sx[q];
-                }
-                const f32x4 pg = mfma_block(ag[q], xb), pu = mfma_block(au[q], xb);
-                const float fg = __fmul_rn(s, sg[k]), fu = __fmul_rn(s, su[k]);
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    gate[r] = fmaf(pg[r], fg, gate[r]);
-                    up[r] = fmaf(pu[r], fu, up[r]);
-                }
-            }
-            load(k + G, q);
-        }
-    }
+    wait_vm<0>();
     float h[4], m = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        h[r] = act_f32(gate[r], up[r], A.kind, A.beta, A.lb);
-        m = fmaxf(m, fabsf(h[r]));
+    for (int i = 0; i < 4; i++) {
+        h[i] = act_f32(gate[i], up[i], A.kind, A.beta, A.lb);
+        m = fmaxf(m, fabsf(h[i]));
     }
     m = fmaxf(m, __shfl_xor(m, 16, 64));
     m = fmaxf(m, __shfl_xor(m, 32, 64));
-    if (g == 0u) red[wave][c] = m;
+    if (lane == 0u) red[wave] = m;
     __syncthreads();
-    if (c >= rows) return;
+    if ((lane & 15u) != 0u) return;
 #pragma unroll
-    for (int w = 0; w < 8; w++) m = fmaxf(m, red[w][c]);
+    for (int u = 0; u < 8; u++) m = fmaxf(m, red[u]);
     float scale, inv;
     fp8_scales(m, scale, inv);
-    *(uint32_t *)(A.hq + (uint64_t)(row0 + c) * A.F + f0 + 4u * g) =
+    *(uint32_t *)(A.hq + (uint64_t)r * A.F + f0 + 4u * g) =
         e4m3x2_raw<true>(__fmul_rn(h[2], inv), __fmul_rn(h[3], inv),
                          e4m3x2_raw<false>(__fmul_rn(h[0], inv), __fmul_rn(h[1], inv), 0u));
-    if (wave == 0u && g == 0u) A.hs[(uint64_t)(row0 + c) * A.hstride + col] = scale;
+    if (threadIdx.x == 0u) A.hs[(uint64_t)r * A.hstride + col] = scale;
 }
 
-/* acc[i] = 16 weight rows (w[i], this lane's) . the lane's token row. */
-template <int NI, int G>
-__device__ __forceinline__ void stream_rows(f32x4 (&acc)[NI], const uint8_t *const (&w)[NI],
-                                            const float *sw, const uint8_t *x, const float *xs,
-                                            uint32_t nblk) {
-    Frag a[G][NI], b[G];
-    float sx[G];
-    auto load = [&](uint32_t k, int q) {
-        if (k >= nblk) return;
-#pragma unroll
-        for (int i = 0; i < NI; i++) a[q][i] = frag_nt(w[i] + kBlock * k);
-        b[q] = frag(x + kBlock * k);
-        sx[q] = xs[k];
-    };
-#pragma unroll
-    for (int q = 0; q < G; q++) load((uint32_t)q, q);
-#pragma unroll
-    for (int i = 0; i < NI; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t k0 = 0; k0 < nblk; k0 += G) {
-#pragma unroll
-        for (int q = 0; q < G; q++) {
-            const uint32_t k = k0 + (uint32_t)q;
-            if (k < nblk) {
-                const float f = __fmul_rn(sx[q], sw[k]);
-#pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const f32x4 p = mfma_block(a[q][i], b[q]);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) acc[i][r] = fmaf(p[r], f, acc[i][r]);
-                }
-            }
-            load(k + G, q);
-        }
-    }
-}
-
-/* y of an expert's up to 16 rows: 32 columns a wave, 128 a block. */
-__global__ __launch_bounds__(256) void down_stream_kernel(ExpertArgs A) {
-    const uint32_t cols = A.H / kBlock, tile = blockIdx.x / cols, col = blockIdx.x % cols;
-    if (tile >= *A.tile_count) return;
-    const uint32_t row0 = A.tiles[4u * tile + 1u], rows = A.tiles[4u * tile + 2u];
-    const k3_moe_fp8_expert ex = A.experts[A.tiles[4u * tile]];
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.F / kBlock;
-    const uint32_t n0 = kBlock * col + 32u * (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint64_t r = row0 + min(c, rows - 1u);
-    const uint8_t *w0 = ex.down_codes + (uint64_t)(n0 + c) * A.F + 16u * g;
-    const uint8_t *const w[2] = {w0, w0 + 16ull * A.F};
-    f32x4 acc[2];
-    stream_rows<2, 4>(acc, w, ex.down_scales + (uint64_t)col * nblk, A.hq + r * A.F + 16u * g,
-                      A.hs + r * A.hstride, nblk);
-    if (c >= rows) return;
-    uint16_t *y = A.y + (uint64_t)A.route_index[r] * A.H + n0 + 4u * g;
-#pragma unroll
-    for (int i = 0; i < 2; i++) *(uint2 *)(y + 16 * i) = bf16x4(acc[i]);
-}
-
-/* A single token's output: 16 columns a block, a route a wave at a time, then
- * the weighted sum in rank order and the residual (as combine_kernel's). */
-__global__ __launch_bounds__(512) void down_one_kernel(ExpertArgs A) {
+/*
+ * A single token's output: 16 columns a block, a route a wave at a time (its
+ * activation's codes in the wave's LDS), then the weighted
+ * sum in rank order and the residual (as the batch's combine).
+ */
+constexpr int kDownRing = 3;
+template <uint32_t MOST> /* F at most: 2048 lets a CU hold two blocks */
+__global__ __launch_bounds__(512) void down_one_kernel(OneExpertArgs A) {
+    using Ring = WaveRing<1, kDownRing>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * (Ring::BYTES + MOST)];
     __shared__ float y[32][16];
     __shared__ uint32_t live[32];
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, nblk = A.F / kBlock;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, nblk = A.F / kBlock;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = 16u * blockIdx.x;
+    uint8_t *mine = smem + (Ring::BYTES + MOST) * wave;
+    const uint32_t codes = lds_addr(mine) + Ring::BYTES;
     for (uint32_t r = wave; r < A.k; r += 8u) {
-        const uint32_t e = one_route(A.ids, r, A.E);
+        const uint32_t e = one_route(A.ids, r, A.k, A.E);
         if (lane == 0u) live[r] = e < A.E;
         if (e >= A.E) continue;
+        const uint8_t *h = A.hq + (uint64_t)r * A.F;
         const k3_moe_fp8_expert ex = A.experts[e];
-        const uint8_t *const w[1] = {ex.down_codes + (uint64_t)(n0 + c) * A.F + 16u * g};
-        f32x4 acc[1];
-        stream_rows<1, 8>(acc, w, ex.down_scales + (uint64_t)(n0 / kBlock) * nblk,
-                          A.hq + (uint64_t)r * A.F + 16u * g, A.hs + (uint64_t)r * A.hstride, nblk);
-        if (c == 0u)
+        const float *ws = ex.down_scales + (uint64_t)(n0 / kBlock) * nblk;
+        float f = lane_scales(ws, 0u, nblk); /* nblk <= 64 */
+        const float sx = lane_scales(A.hs + (uint64_t)r * A.hstride, 0u, nblk);
+        asm volatile("" ::: "memory"); /* issued before the weights, so that their wait leaves those out */
+        for (uint32_t o = 0; o < A.F; o += 1024u)
+            dma<16>(h + min(o + 16u * lane, A.F - 16u), mine + Ring::BYTES + o);
+        Ring ring;
+        const uint8_t *const w[1] = {ex.down_codes + (uint64_t)n0 * A.F};
+        ring.init(mine, w, 16u, A.F);
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[r][4u * g + i] = bf16_to_f32(f32_to_bf16(acc[0][i]));
+        for (uint32_t q = 0; q < kDownRing; q++) ring.fetch(min(q, nblk - 1u), q);
+        f = __fmul_rn(sx, f);
+        asm volatile("" : "+v"(f)); /* waited for here, not in the loop */
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t slot = 0u;
+        for (uint32_t k = 0; k < nblk; k++) {
+            f32x4 p[1];
+            ring.products(p, slot, codes + kBlock * k);
+            ring.fetch(min(k + kDownRing, nblk - 1u), slot);
+            const float s = scale_at(f, k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(p[0][i], s, acc[i]);
+            slot = slot + 1u == (uint32_t)kDownRing ? 0u : slot + 1u;
+        }
+        wait_vm<0>(); /* before the wave's next route, or the block's end */
+        if ((lane & 15u) == 0u)
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[r][4u * g + i] = bf16_to_f32(f32_to_bf16(acc[i]));
     }
     __syncthreads();
     if (threadIdx.x >= 16u) return;
@@ -551,12 +531,25 @@ __global__ __launch_bounds__(512) void down_one_kernel(ExpertArgs A) {
     A.out[n0 + threadIdx.x] = o;
 }
 
+/* One of the `many` row tiles of an expert with n rows from `row` on: all that
+ * a block needs to know comes with one read. */
+struct ExpertTile {
+    uint32_t row, n, index, many;
+    k3_moe_fp8_expert ex;
+};
+/* Rows of each but the last of an expert's tiles: all of up to 128 rows in one,
+ * more in equal steps of 32 rows, at most 256. */
+__device__ __forceinline__ uint32_t tile_height(uint32_t n) {
+    const uint32_t steps = (n + 31u) / 32u, many = (n + 255u) / 256u;
+    return n > 128u ? 32u * ((steps + many - 1u) / many) : n;
+}
+
 /* ---------------------------------------------------------------------- */
 /* tiles of many tokens                                                    */
 /* ---------------------------------------------------------------------- */
 
 /*
- * 256 weight rows x 32 TI tokens a block of eight waves; wave (wn, wt) holds
+ * 64 WN weight rows x 32 TI tokens a block of 2 WN waves; wave (wn, wt) holds
  * weight rows 64 wn .. + 64 and the token subtiles (16 tokens) wt, wt + 2, ...:
  * a tile with fewer tokens costs its 32-token steps, evenly over the waves. A
  * stage is a block of 128 columns of both operands, in LDS through
@@ -568,19 +561,24 @@ __global__ __launch_bounds__(512) void down_one_kernel(ExpertArgs A) {
  * come four blocks at a time (16 bytes a token) into two buffers; the weights'
  * are held by the lanes of a wave, 64 blocks at a time, and read out by index.
  */
-template <int TI_, int STAGES_>
+template <int WN_, int TI_, int STAGES_>
 struct Tile {
-    static constexpr int TI = TI_, STAGES = STAGES_;
-    static constexpr uint32_t BN = 256, BT = 32 * TI;
+    static constexpr int WN = WN_, TI = TI_, STAGES = STAGES_, WAVES = 2 * WN, THREADS = 64 * WAVES;
+    static constexpr uint32_t BN = 64 * WN, BT = 32 * TI;
     static constexpr uint32_t A = BN * kBlock, B = BT * kBlock, STAGE = A + B;
     static constexpr uint32_t SROWS = BT < 64u ? 64u : BT, SBUF = 16u * SROWS;
-    static constexpr int DA = 4, DB = TI < 2 ? 1 : TI / 2, D = DA + DB; /* loads a wave */
+    static constexpr uint32_t B_CHUNKS = 4 * TI; /* of 8 rows, 1 KB; fewer than the waves: some load the same */
+    static constexpr int DA = 4, DB = B_CHUNKS < WAVES ? 1 : B_CHUNKS / WAVES, D = DA + DB; /* loads a wave */
     static constexpr uint32_t LDS = STAGES * STAGE + 2u * SBUF;
     static_assert(LDS <= 160u * 1024u, "LDS");
+    static_assert(STAGES <= 5, "a buffer of scales is read for four stages, and the next but one comes after");
     /* Two stages: a stage's weights have been read once its first subtile is
      * under way, so after a second barrier in mid-stage their place takes the
      * weights of two stages on (they come from HBM, the tokens from the L2). */
     static constexpr bool EARLY = STAGES == 2;
+    static __device__ __forceinline__ uint32_t b_chunk(uint32_t wave, uint32_t q) {
+        return B_CHUNKS < WAVES ? wave % B_CHUNKS : DB * wave + q;
+    }
 };
 
 enum TileMode { kDense, kGateUp, kDown };
@@ -589,8 +587,8 @@ struct TileArgs {
     /* dense: the weight; otherwise the experts and the tiles */
     const uint8_t *codes;
     const float *scales;
-    const k3_moe_fp8_expert *experts;
-    const uint32_t *tiles, *tile_count, *token_index, *route_index;
+    const ExpertTile *tiles;
+    const uint32_t *tile_count, *token_index, *route_index;
     const uint8_t *xq; /* token rows, K wide */
     const float *xs;   /* their scales, rows xstride apart */
     uint32_t xstride;
@@ -599,9 +597,11 @@ struct TileArgs {
     float *hs;
     uint32_t hstride;
     uint32_t T, N, K, tiles_n, tiles_t;
+    uint32_t splits, span; /* dense: K in `splits` parts of `span` blocks (a multiple of 4) */
+    f32x4 *part;           /* their sums, of more than one */
     uint32_t kind;
     float beta, lb;
-    bool wide; /* the output takes 8-byte stores */
+    bool wide, wide16; /* the output takes 8-byte, 16-byte stores */
 };
 
 /* acc[j][i] += the product over all blocks, for the first TL token subtiles of a
@@ -630,7 +630,7 @@ struct TileRun {
             dma<16>(a_base + at + a[Q], st + 1024u * (C::DA * wave + Q));
         else
             dma<16>(b_base + at + b[Q - C::DA],
-                    st + C::A + 1024u * (C::TI < 2 ? wave & 3u : C::DB * wave + (Q - C::DA)));
+                    st + C::A + 1024u * C::b_chunk(wave, Q - C::DA));
     }
     template <int FROM, int TO>
     __device__ __forceinline__ void fetch(uint8_t *smem, uint32_t s, uint32_t slot) const {
@@ -763,61 +763,60 @@ struct TileRun {
 };
 
 template <class C, int MODE>
-__global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
+__global__ __launch_bounds__(C::THREADS, C::WAVES / 4) void tile_kernel(TileArgs P) {
+    static_assert(MODE != kGateUp || C::WN == 4, "a gate/up block holds whole scale blocks");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
     TileRun<C> R;
     R.lane = threadIdx.x & 63u;
     R.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    R.wn = R.wave & 3u, R.wt = R.wave >> 2;
+    R.wn = R.wave % C::WN, R.wt = R.wave / C::WN;
     const uint32_t L = R.lane, K = P.K, nblk = K / kBlock;
     /* XCD x (blocks x, x + 8, ...) takes a contiguous range of the works */
     const uint32_t tiles = MODE == kDense ? P.tiles_t : *P.tile_count;
-    const uint32_t works = tiles * P.tiles_n, per = (works + 7u) / 8u, j8 = blockIdx.x >> 3;
-    const uint32_t w = (blockIdx.x & 7u) * per + j8;
+    const uint32_t works = tiles * P.tiles_n * (MODE == kDense ? P.splits : 1u);
+    const uint32_t per = (works + 7u) / 8u, j8 = blockIdx.x >> 3;
+    uint32_t w = (blockIdx.x & 7u) * per + j8;
     if (j8 >= per || w >= works) return;
-    uint32_t tile, col;
+    const uint32_t split = MODE == kDense ? w % P.splits : 0u; /* a part of K */
+    if constexpr (MODE == kDense) w /= P.splits;
+    uint32_t row0, rows, col;
+    const uint8_t *w0, *w1;
     if constexpr (MODE == kDense) { /* four token tiles at a time, down the weight's rows */
         const uint32_t grp = w / (4u * P.tiles_n), in = w % (4u * P.tiles_n);
         const uint32_t high = min(4u, tiles - 4u * grp);
-        tile = 4u * grp + in % high, col = in / high;
+        col = in / high;
+        row0 = C::BT * (4u * grp + in % high), rows = min(C::BT, P.T - row0);
+        w0 = w1 = P.codes;
+        R.sw0 = R.sw1 = P.scales;
     } else {
         /* an expert's tiles of one column block are neighbours: they read the
          * same weights at about the same time, through the same L2 */
-        const uint32_t t = w / P.tiles_n, in = P.tiles[4u * t + 3u];
-        const uint32_t many = in >> 16, local = (in & 0xffffu) * P.tiles_n + w % P.tiles_n;
-        tile = t - (in & 0xffffu) + local % many, col = local / many;
+        const ExpertTile &t = P.tiles[w / P.tiles_n];
+        const uint32_t local = t.index * P.tiles_n + w % P.tiles_n, height = tile_height(t.n);
+        const uint32_t q = local % t.many;
+        col = local / t.many;
+        row0 = t.row + height * q, rows = min(height, t.n - height * q);
+        w0 = MODE == kGateUp ? t.ex.gate_codes : t.ex.down_codes;
+        w1 = t.ex.up_codes;
+        R.sw0 = MODE == kGateUp ? t.ex.gate_scales : t.ex.down_scales;
+        R.sw1 = MODE == kGateUp ? t.ex.up_scales : R.sw0;
     }
-    uint32_t row0, rows;
-    const uint8_t *w0, *w1;
-    const uint32_t n0 = (MODE == kGateUp ? 128u : 256u) * col, nb0 = n0 / kBlock;
-    const uint32_t blocks_n = (P.N + kBlock - 1u) / kBlock;
-    if constexpr (MODE == kDense) {
-        row0 = C::BT * tile, rows = min(C::BT, P.T - row0);
-        w0 = w1 = P.codes;
-        const uint32_t nb = min(nb0 + (R.wn >> 1), blocks_n - 1u);
-        R.sw0 = R.sw1 = P.scales + (uint64_t)nb * nblk;
-    } else {
-        const uint32_t *t = P.tiles + 4u * tile;
-        row0 = t[1], rows = t[2];
-        const k3_moe_fp8_expert ex = P.experts[t[0]];
-        if constexpr (MODE == kGateUp) {
-            w0 = ex.gate_codes, w1 = ex.up_codes;
-            R.sw0 = ex.gate_scales + (uint64_t)nb0 * nblk;
-            R.sw1 = ex.up_scales + (uint64_t)nb0 * nblk;
-        } else {
-            w0 = w1 = ex.down_codes;
-            const uint32_t nb = min(nb0 + (R.wn >> 1), blocks_n - 1u);
-            R.sw0 = R.sw1 = ex.down_scales + (uint64_t)nb * nblk;
-        }
+    const uint32_t n0 = (MODE == kGateUp ? 128u : C::BN) * col, nb0 = n0 / kBlock;
+    {
+        const uint32_t nb = MODE == kGateUp ? nb0 : min(nb0 + (R.wn >> 1), (P.N + kBlock - 1u) / kBlock - 1u);
+        R.sw0 += (uint64_t)nb * nblk;
+        R.sw1 += (uint64_t)nb * nblk;
     }
-    R.nblk = nblk;
+    const uint32_t k0 = MODE == kDense ? P.span * split : 0u; /* a multiple of 4 */
+    R.nblk = MODE == kDense ? min(P.span, nblk - k0) : nblk;
+    R.sw0 += k0, R.sw1 += k0;
     /* chunk q of A: rows 8 q .. + 8 of the tile; gate/up: wave wn's 64 rows are
      * 32 of gate, then the same 32 of up, so a loading wave has one of them */
     if constexpr (MODE == kGateUp)
         R.a_base = (R.wave & 1u ? w1 : w0) + (uint64_t)n0 * K;
     else
-        R.a_base = w0 + (uint64_t)n0 * K;
-    R.b_base = MODE == kGateUp ? P.xq : P.xq + (uint64_t)row0 * K;
+        R.a_base = w0 + (uint64_t)n0 * K + kBlock * k0;
+    R.b_base = MODE == kGateUp ? P.xq : P.xq + (uint64_t)row0 * K + kBlock * k0;
 #pragma unroll
     for (int q = 0; q < C::DA; q++) {
         const uint32_t ch = C::DA * R.wave + (uint32_t)q, h = ch & 1u;
@@ -830,7 +829,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
     }
 #pragma unroll
     for (int q = 0; q < C::DB; q++) {
-        const uint32_t ch = C::TI < 2 ? R.wave & 3u : C::DB * R.wave + (uint32_t)q, h = ch & 1u;
+        const uint32_t ch = C::b_chunk(R.wave, (uint32_t)q), h = ch & 1u;
         uint32_t r = min(16u * (ch >> 1) + a_dma_row(L, h), rows - 1u);
         if constexpr (MODE == kGateUp) r = P.token_index[row0 + r];
         R.b[q] = r * K + 16u * a_dma_piece(L, h);
@@ -839,7 +838,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
         R.has_sx = 64u * R.wave < C::BT;
         uint32_t r = row0 + min(64u * R.wave + L, rows - 1u);
         if constexpr (MODE == kGateUp) r = P.token_index[r];
-        R.sx = P.xs + (uint64_t)r * P.xstride;
+        R.sx = P.xs + (uint64_t)r * P.xstride + k0;
     }
     f32x4 acc[C::TI][4];
 #pragma unroll
@@ -859,17 +858,47 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
     if (!done) R.template run<C::TI, MODE == kGateUp>(acc, smem);
     const uint32_t g = L >> 4, c = L & 15u;
     if constexpr (MODE != kGateUp) {
-        static_for<C::TI>([&](auto J) {
-            constexpr int j = decltype(J)::value;
-            const uint32_t r = 16u * (2u * j + R.wt) + c;
-            if (r >= rows) return;
-            uint32_t t = row0 + r;
-            if constexpr (MODE == kDown) t = P.route_index[t];
+        if (MODE == kDense && P.splits > 1u) { /* as they lie: join_kernel knows the layout */
+            f32x4 *part = P.part + ((uint64_t)split * (tiles * P.tiles_n) + w) * (4u * C::TI * C::THREADS);
 #pragma unroll
-            for (uint32_t i = 0; i < 4u; i++)
-                store_rows(P.out, acc[j][i], t, n0 + 64u * R.wn + 16u * i + 4u * g, ~0u, P.N,
-                           MODE == kDown || P.wide);
-        });
+            for (int j = 0; j < C::TI; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) part[(4u * j + i) * C::THREADS + threadIdx.x] = acc[j][i];
+        } else if (MODE == kDown || P.wide16) {
+            /* the tile goes through LDS, 2 BN bytes a token, and leaves in
+             * 16-byte pieces of whole rows; piece p of token r lies at p ^ r
+             * modulo their number */
+            constexpr uint32_t PIECES = C::BN / 8u;
+            __syncthreads();
+            static_for<C::TI>([&](auto J) {
+                constexpr int j = decltype(J)::value;
+                const uint32_t r = 16u * (2u * j + R.wt) + c;
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) {
+                    const uint32_t p = 8u * R.wn + 2u * i + (g >> 1);
+                    *(uint2 *)(smem + 16u * (PIECES * r + (p ^ (r & (PIECES - 1u)))) + 8u * (g & 1u)) =
+                        bf16x4(acc[j][i]);
+                }
+            });
+            __syncthreads();
+            const uint32_t width = min(C::BN, P.N - n0); /* a multiple of 8 */
+            const uint32_t p = threadIdx.x % PIECES;
+            if (8u * p < width)
+                for (uint32_t r = threadIdx.x / PIECES; r < rows; r += C::THREADS / PIECES) {
+                    const uint32_t t = MODE == kDown ? P.route_index[row0 + r] : row0 + r;
+                    *(uint4 *)(P.out + (uint64_t)t * P.N + n0 + 8u * p) =
+                        *(const uint4 *)(smem + 16u * (PIECES * r + (p ^ (r & (PIECES - 1u)))));
+                }
+        } else {
+            static_for<C::TI>([&](auto J) {
+                constexpr int j = decltype(J)::value;
+                const uint32_t r = 16u * (2u * j + R.wt) + c;
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++)
+                    store_rows(P.out, acc[j][i], row0 + r, n0 + 64u * R.wn + 16u * i + 4u * g, P.T, P.N,
+                               P.wide);
+            });
+        }
     } else {
         /* the block's 128 columns are one scale block of each row: the maximum
          * over a wave's 32, then over its four neighbours' through LDS; codes
@@ -918,8 +947,31 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(TileArgs P) {
 template <class C, int MODE>
 bool launch_tile(const TileArgs &A, uint32_t works, hipStream_t st) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<C, MODE>), dim3(8u * ((works + 7u) / 8u)),
-                       dim3(512), 0, st, A);
+                       dim3(C::THREADS), 0, st, A);
     return hipGetLastError() == hipSuccess;
+}
+
+/* Output of a product whose K was split: the parts in their order. A block adds
+ * one accumulator (token subtile j, fragment i) of every wave of a tile. */
+template <class C>
+__global__ __launch_bounds__(C::THREADS) void join_kernel(TileArgs P) {
+    const uint32_t w = blockIdx.x / (4u * C::TI), ji = blockIdx.x % (4u * C::TI);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wn = wave % C::WN, wt = wave / C::WN;
+    const uint32_t grp = w / (4u * P.tiles_n), in = w % (4u * P.tiles_n);
+    const uint32_t high = min(4u, P.tiles_t - 4u * grp);
+    const uint32_t t = C::BT * (4u * grp + in % high) + 16u * (2u * (ji >> 2) + wt) + (lane & 15u);
+    const uint32_t n = C::BN * (in / high) + 64u * wn + 16u * (ji & 3u) + 4u * (lane >> 4);
+    if (t >= P.T || n >= P.N) return;
+    const uint64_t works = P.tiles_t * P.tiles_n, stride = works * (4u * C::TI * C::THREADS);
+    const f32x4 *part = P.part + ((uint64_t)w * (4u * C::TI) + ji) * C::THREADS + threadIdx.x;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t z = 0; z < P.splits; z++) {
+        const f32x4 p = part[stride * z];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = __fadd_rn(v[r], p[r]);
+    }
+    store_rows(P.out, v, t, n, P.T, P.N, P.wide);
 }
 
 /* ---------------------------------------------------------------------- */
@@ -939,31 +991,34 @@ __global__ __launch_bounds__(256) void routes_kernel(uint32_t *__restrict__ out,
         if (r < k) out[(uint64_t)t * k + r] = e[r];
 }
 
-/* Tile classes by an expert's rows: up to 16 (streams), up to 64 and up to 128
- * (one tile), more (tiles of up to 256, of equal length in 32-row steps). */
+/* Tile classes by an expert's rows: up to 32, 64 and 128 (one tile), more (tiles
+ * of up to 256, of equal length in 32-row steps). */
 constexpr int kClasses = 4;
 
-/* One block of 1024 threads (thread e: expert e): each class's tiles {expert,
- * first row, rows, index among the expert's tiles | their number << 16} in
- * expert order. */
+/* One block of 1024 threads (thread e: expert e): each class's tiles in expert
+ * order. */
 struct TileLists {
-    uint32_t *tiles[kClasses];
+    ExpertTile *tiles[kClasses];
     uint32_t *count; /* [kClasses] */
 };
 __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t *__restrict__ counts,
                                                      const uint32_t *__restrict__ offsets,
+                                                     const k3_moe_fp8_expert *__restrict__ experts,
                                                      uint32_t E) {
     __shared__ uint32_t tot[kClasses][16];
     const uint32_t e = threadIdx.x, lane = e & 63u, wave = e >> 6;
     const uint32_t n = e < E ? counts[e] : 0u;
-    const uint32_t steps = (n + 31u) / 32u, many = (n + 255u) / 256u;
-    const uint32_t height = n > 128u ? 32u * ((steps + many - 1u) / many) : n;
-    const uint32_t mine = n == 0u ? 0u : (n + height - 1u) / height;
-    const int cls = n <= 16u ? 0 : n <= 64u ? 1 : n <= 128u ? 2 : 3;
+    ExpertTile mine{0u, n, 0u, 0u, {}};
+    if (n != 0u) {
+        mine.row = offsets[e];
+        mine.many = (n + tile_height(n) - 1u) / tile_height(n);
+        mine.ex = experts[e];
+    }
+    const int cls = n <= 32u ? 0 : n <= 64u ? 1 : n <= 128u ? 2 : 3;
     uint32_t inc[kClasses];
 #pragma unroll
     for (int q = 0; q < kClasses; q++) {
-        inc[q] = cls == q ? mine : 0u;
+        inc[q] = cls == q ? mine.many : 0u;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t a = __shfl_up(inc[q], o, 64);
@@ -974,19 +1029,13 @@ __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kClasses; q++) {
-        uint32_t at = inc[q] - mine, total = 0u;
+        uint32_t at = inc[q] - mine.many, total = 0u;
         for (uint32_t w = 0; w < 16u; w++) {
             if (w < wave) at += tot[q][w];
             total += tot[q][w];
         }
         if (cls == q)
-            for (uint32_t i = 0; i < mine; i++) {
-                uint32_t *t = Q.tiles[q] + 4u * (at + i);
-                t[0] = e;
-                t[1] = offsets[e] + height * i;
-                t[2] = min(height, n - height * i);
-                t[3] = i | mine << 16;
-            }
+            for (; mine.index < mine.many; mine.index++) Q.tiles[q][at + mine.index] = mine;
         if (e == 0u) Q.count[q] = total;
     }
 }
@@ -1027,11 +1076,11 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
     w.plan_bytes = k3_moe_plan_scratch_bytes(T, s.expert_count);
     w.plan = take(w.plan_bytes);
     /* an expert has a token's route at most once: T rows at most */
-    static constexpr size_t least[kClasses] = {1u, 17u, 65u, 128u};
+    static constexpr size_t least[kClasses] = {1u, 33u, 65u, 128u};
     for (int q = 0; q < kClasses; q++) {
         const size_t n = routes / least[q];
         w.cap[q] = T < least[q] ? 0u : (uint32_t)(q < 3 && n > E ? E : n);
-        w.lists.tiles[q] = (uint32_t *)take(16u * (size_t)w.cap[q]);
+        w.lists.tiles[q] = (ExpertTile *)take(sizeof(ExpertTile) * (size_t)w.cap[q]);
     }
     w.lists.count = (uint32_t *)take(4u * kClasses);
     w.xq = take((size_t)T * s.hidden);
@@ -1064,22 +1113,55 @@ bool launch_rows(uint8_t *codes, float *scales, const void *src, uint32_t rows, 
     return hipGetLastError() == hipSuccess;
 }
 
-template <int NI, int TI, bool ONE>
-bool launch_stream(const ProductArgs &A, hipStream_t st) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(stream_kernel<NI, TI, ONE>),
-                       dim3((A.N + 16u * NI - 1u) / (16u * NI)), dim3(512), 0, st, A);
-    return hipGetLastError() == hipSuccess;
-}
+using Tile32 = Tile<4, 1, 4>;
+using Tile64 = Tile<4, 2, 3>;
+using Tile128 = Tile<4, 4, 3>;
+using Tile256 = Tile<4, 8, 2>;
+/* half as many rows: few tokens' products */
+using Half32 = Tile<2, 1, 5>;
+using Half64 = Tile<2, 2, 5>;
+using Half128 = Tile<2, 4, 4>;
 
-using Tile64 = Tile<2, 3>;
-using Tile128 = Tile<4, 3>;
-using Tile256 = Tile<8, 2>;
+/* How a product of T > 1 tokens is cut. */
+struct Cut {
+    int tile; /* 0 .. 3: Half32, Half64, Half128, Tile256 */
+    uint32_t tiles_t, tiles_n, splits, span;
+    size_t part_bytes;
+};
 
 template <class C>
-bool launch_dense(TileArgs A, hipStream_t st) {
-    A.tiles_t = (A.T + C::BT - 1u) / C::BT;
-    A.tiles_n = (A.N + C::BN - 1u) / C::BN;
-    return launch_tile<C, kDense>(A, A.tiles_t * A.tiles_n, st);
+void cut_as(Cut &q, uint32_t T, uint32_t N, uint32_t K) {
+    const uint32_t groups = (K / kBlock + 3u) / 4u;
+    q.tiles_t = (T + C::BT - 1u) / C::BT, q.tiles_n = (N + C::BN - 1u) / C::BN;
+    const uint64_t tiles = (uint64_t)q.tiles_t * q.tiles_n;
+    uint32_t want = tiles >= 256u ? 1u : (uint32_t)(256u / tiles);
+    want = want < groups ? want : groups;
+    q.span = 4u * ((groups + want - 1u) / want);
+    q.splits = (4u * groups + q.span - 1u) / q.span;
+    q.part_bytes = q.splits > 1u ? align256((size_t)q.splits * tiles * C::BT * C::BN * 4u) : 0u;
+}
+
+Cut cut_of(uint32_t T, uint32_t N, uint32_t K) {
+    Cut q{};
+    q.tile = T <= 32u ? 0 : T <= 64u ? 1 : T <= 512u ? 2 : 3;
+    switch (q.tile) {
+    case 0: cut_as<Half32>(q, T, N, K); break;
+    case 1: cut_as<Half64>(q, T, N, K); break;
+    case 2: cut_as<Half128>(q, T, N, K); break;
+    default: cut_as<Tile256>(q, T, N, K);
+    }
+    return q;
+}
+
+template <class C>
+bool launch_dense(TileArgs A, const Cut &q, hipStream_t st) {
+    A.tiles_t = q.tiles_t, A.tiles_n = q.tiles_n, A.splits = q.splits, A.span = q.span;
+    const uint32_t tiles = q.tiles_t * q.tiles_n;
+    if (!launch_tile<C, kDense>(A, tiles * q.splits, st)) return false;
+    if (q.splits == 1u) return true;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(join_kernel<C>), dim3(tiles * 4u * C::TI), dim3(C::THREADS), 0,
+                       st, A);
+    return hipGetLastError() == hipSuccess;
 }
 
 /* Gate/up and down of one class of tiles. */
@@ -1094,38 +1176,35 @@ bool launch_class(TileArgs A, const Fp8Workspace &ws, int cls, const k3_moe_shap
     return launch_tile<C, kDown>(A, ws.cap[cls] * A.tiles_n, st);
 }
 
-/* A token's codes and scales in LDS, beside the block's other arrays. */
-bool one_token_fits(const k3_moe_shape &s) { return s.hidden <= 32768u; }
-
 /* The expert stage on routes in ids (T > 1: ws.ids, repeated ones taken out). */
 bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, const void *residual,
                      const uint32_t *ids, const float *wts, const k3_moe_fp8_expert *experts,
                      const k3_moe_shape &s, uint32_t T, hipStream_t st) {
     const uint32_t H = s.hidden, F = s.ffn, E = s.expert_count, k = s.top_k;
-    ExpertArgs A{experts, ws.lists.tiles[0], ws.lists.count, ws.token_index, ws.route_index, ids,
-                 (const uint16_t *)hidden, ws.xq, ws.xs, scale_stride(H), scale_stride(F), ws.hq,
-                 ws.hs, ws.y, (uint16_t *)output, (const uint16_t *)residual, wts, H, F, E, k,
-                 s.activation, s.beta, s.linear_beta};
-    if (T == 1u && one_token_fits(s)) {
-        hipLaunchKernelGGL(gateup_stream_kernel<true>, dim3(k * (F / kBlock)), dim3(512), H + H / 32u,
-                           st, A);
-        hipLaunchKernelGGL(down_one_kernel, dim3(H / 16u), dim3(512), 0, st, A);
+    if (T == 1u && H <= kOneHidden && F <= kOneFfn) {
+        const OneExpertArgs A{experts, ids, wts, (const uint16_t *)hidden, (const uint16_t *)residual,
+                              (uint16_t *)output, ws.hq, ws.hs, scale_stride(F), H, F, E, k,
+                              s.activation, s.beta, s.linear_beta};
+        hipLaunchKernelGGL(gateup_one_kernel, dim3(k * (F / kBlock)), dim3(512), 0, st, A);
+        if (F <= 2048u)
+            hipLaunchKernelGGL(down_one_kernel<2048u>, dim3(H / 16u), dim3(512), 0, st, A);
+        else
+            hipLaunchKernelGGL(down_one_kernel<kOneFfn>, dim3(H / 16u), dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
     hipLaunchKernelGGL(routes_kernel, dim3((T + 255u) / 256u), dim3(256), 0, st, ws.ids, ids, T, k, E);
-    if (!launch_rows(ws.xq, ws.xs, hidden, T, H, A.xstride, st) ||
+    if (!launch_rows(ws.xq, ws.xs, hidden, T, H, scale_stride(H), st) ||
         !k3_moe_route_plan(ws.counts, ws.offsets, ws.unique, ws.summary, ws.token_index,
                            ws.route_index, ws.ids, T, k, E, ws.plan, ws.plan_bytes, st))
         return false;
-    hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(1024), 0, st, ws.lists, ws.counts, ws.offsets, E);
-    hipLaunchKernelGGL(gateup_stream_kernel<false>, dim3(ws.cap[0] * (F / kBlock)), dim3(512), 0, st, A);
-    hipLaunchKernelGGL(down_stream_kernel, dim3(ws.cap[0] * (H / kBlock)), dim3(256), 0, st, A);
+    hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(1024), 0, st, ws.lists, ws.counts, ws.offsets,
+                       experts, E);
     TileArgs B{};
-    B.experts = experts, B.token_index = ws.token_index, B.route_index = ws.route_index;
-    B.xq = ws.xq, B.xs = ws.xs, B.xstride = A.xstride;
-    B.out = ws.y, B.hq = ws.hq, B.hs = ws.hs, B.hstride = A.hstride;
+    B.token_index = ws.token_index, B.route_index = ws.route_index;
+    B.xq = ws.xq, B.xs = ws.xs, B.xstride = scale_stride(H);
+    B.out = ws.y, B.hq = ws.hq, B.hs = ws.hs, B.hstride = scale_stride(F);
     B.kind = s.activation, B.beta = s.beta, B.lb = s.linear_beta;
-    return hipGetLastError() == hipSuccess && launch_class<Tile64>(B, ws, 1, s, st) &&
+    return hipGetLastError() == hipSuccess && launch_class<Tile32>(B, ws, 0, s, st) && launch_class<Tile64>(B, ws, 1, s, st) &&
            launch_class<Tile128>(B, ws, 2, s, st) && launch_class<Tile256>(B, ws, 3, s, st) &&
            launch_combine(output, ws.y, residual, ws.ids, wts, T, H, k, E, st);
 }
@@ -1133,9 +1212,9 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
 }  // namespace
 
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
-    (void)rows;
     if (T == 1u) return 0u; /* encoded by the product's own kernel */
-    return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols));
+    return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols)) +
+           cut_of(T, rows, cols).part_bytes;
 }
 
 }  // namespace k3
@@ -1187,21 +1266,26 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
         return false;
     const hipStream_t st = (hipStream_t)stream;
     const bool wide = rows % 4u == 0u && ((uintptr_t)output % 8u) == 0u;
-    ProductArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, nullptr, nullptr, 0u,
-                  vector_count, rows, columns, wide};
-    if (vector_count == 1u) return launch_stream<1, 1, true>(A, st);
+    if (vector_count == 1u) {
+        const OneArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, rows, columns};
+        hipLaunchKernelGGL(product_one_kernel, dim3((rows + 15u) / 16u), dim3(512), 0, st, A);
+        return hipGetLastError() == hipSuccess;
+    }
+    TileArgs B{};
     uint8_t *xq = (uint8_t *)scratch;
     float *xs = (float *)(xq + align256((size_t)vector_count * columns));
-    A.xq = xq, A.xs = xs, A.xstride = scale_stride(columns);
-    if (!launch_rows(xq, xs, input, vector_count, columns, A.xstride, st)) return false;
-    if (vector_count <= 16u) return launch_stream<1, 1, false>(A, st);
-    if (vector_count <= 32u) return launch_stream<2, 2, false>(A, st);
-    if (vector_count <= 48u) return launch_stream<2, 3, false>(A, st);
-    if (vector_count <= 64u) return launch_stream<2, 4, false>(A, st);
-    TileArgs B{};
-    B.codes = codes, B.scales = scales, B.xq = xq, B.xs = xs, B.xstride = A.xstride;
-    B.out = A.out, B.T = vector_count, B.N = rows, B.K = columns, B.wide = wide;
-    return vector_count <= 512u ? launch_dense<Tile128>(B, st) : launch_dense<Tile256>(B, st);
+    B.codes = codes, B.scales = scales, B.xq = xq, B.xs = xs, B.xstride = scale_stride(columns);
+    B.part = (f32x4 *)((uint8_t *)xs + align256(4u * (size_t)vector_count * B.xstride));
+    B.out = (uint16_t *)output, B.T = vector_count, B.N = rows, B.K = columns, B.wide = wide;
+    B.wide16 = rows % 8u == 0u && ((uintptr_t)output % 16u) == 0u;
+    if (!launch_rows(xq, xs, input, vector_count, columns, B.xstride, st)) return false;
+    const Cut q = cut_of(vector_count, rows, columns);
+    switch (q.tile) {
+    case 0: return launch_dense<Half32>(B, q, st);
+    case 1: return launch_dense<Half64>(B, q, st);
+    case 2: return launch_dense<Half128>(B, q, st);
+    default: return launch_dense<Tile256>(B, q, st);
+    }
 }
 
 extern "C" size_t k3_moe_fp8_workspace_bytes(const k3_moe_shape *shape, uint32_t token_count) {
