@@ -6,7 +6,7 @@
  *   balance_part_kernel    a block: a run of one segment's tokens, a token a
  *                          wave at a time; sums of the shares sigma / Z and
  *                          the counts of its run
- *   balance_join_kernel    a block: 64 experts of a segment; joins the runs,
+ *   balance_join_kernel    a block: 16 experts of a segment; joins the runs,
  *                          writes counts and mean scores; the last block to
  *                          end adds up the loss
  *   router_backward_kernel a token a wave at a time, the segment's f in
@@ -28,7 +28,9 @@
 namespace k3 {
 namespace {
 
-constexpr uint32_t kWaves = 8;
+constexpr uint32_t kWaves = 8;  /* of a block of balance_part_kernel */
+constexpr uint32_t kJoin = 16;  /* experts of a block of balance_join_kernel */
+constexpr uint32_t kBackWaves = 4;
 
 inline size_t align256(size_t v) { return (v + 255u) & ~(size_t)255u; }
 
@@ -79,7 +81,7 @@ struct BalanceArgs {
     float *part_mean;    /* [S, runs, E] */
     uint32_t *part_count;
     uint32_t *part_live; /* [S, runs] */
-    float *part_loss;    /* [S, ceil(E / 64)] */
+    float *part_loss;    /* [S, ceil(E / kJoin)] */
     uint32_t *ticket;
 };
 
@@ -138,12 +140,13 @@ __global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A
 }
 
 __global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs A) {
-    __shared__ float fsum[16][64];
-    __shared__ uint32_t csum[16][64];
+    __shared__ float fsum[16][kJoin];
+    __shared__ uint32_t csum[16][kJoin];
     __shared__ uint32_t nsum[16];
     __shared__ uint32_t last;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
-    const uint32_t cols = (E + 63u) / 64u, s = blockIdx.x / cols, e = 64u * (blockIdx.x % cols) + lane;
+    const uint32_t cols = (E + kJoin - 1u) / kJoin, s = blockIdx.x / cols;
+    const uint32_t i = lane % kJoin, e = kJoin * (blockIdx.x % cols) + i;
     float m = 0.0f;
     uint32_t c = 0u, n = 0u;
     for (uint32_t r = threadIdx.x; r < A.runs; r += 1024u) n += A.part_live[s * A.runs + r];
@@ -152,31 +155,35 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs A) {
     if (e < E) {
         const uint64_t at = (uint64_t)s * A.runs * E + e;
 #pragma unroll 8
-        for (uint32_t r = wave; r < A.runs; r += 16u) {
+        for (uint32_t r = threadIdx.x / kJoin; r < A.runs; r += 1024u / kJoin) {
             m = __fadd_rn(m, A.part_mean[at + (uint64_t)r * E]);
             c += A.part_count[at + (uint64_t)r * E];
         }
     }
-    fsum[wave][lane] = m;
-    csum[wave][lane] = c;
+#pragma unroll
+    for (int o = kJoin; o < 64; o <<= 1) {
+        m = __fadd_rn(m, __shfl_xor(m, o, 64));
+        c += __shfl_xor(c, o, 64);
+    }
+    if (lane < kJoin) fsum[wave][i] = m, csum[wave][i] = c;
     if (lane == 0u) nsum[wave] = n;
     __syncthreads();
     if (wave == 0u) {
         m = 0.0f, c = 0u, n = 0u;
 #pragma unroll
         for (uint32_t w = 0; w < 16u; w++) {
-            m = __fadd_rn(m, fsum[w][lane]);
-            c += csum[w][lane];
+            m = __fadd_rn(m, fsum[w][i]);
+            c += csum[w][i];
             n += nsum[w];
         }
         m = n ? __fdiv_rn(m, (float)n) : 0.0f;
         float l = 0.0f;
-        if (e < E) {
+        if (e < E && lane < kJoin) {
             A.counts[(uint64_t)s * E + e] = c;
             A.mean[(uint64_t)s * E + e] = m;
             if (n) l = __fmul_rn(__fdiv_rn(__fmul_rn((float)c, (float)E), __fmul_rn((float)A.k, (float)n)), m);
         }
-        if (e == 0u) A.live[s] = n;
+        if (e == 0u && lane == 0u) A.live[s] = n;
         l = wave_sum(l);
         if (lane == 0u) {
             __hip_atomic_store(&A.part_loss[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -187,8 +194,8 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs A) {
     __syncthreads();
     if (!last) return;
     float v = 0.0f;
-    for (uint32_t i = threadIdx.x; i < gridDim.x; i += 1024u)
-        v = __fadd_rn(v, __hip_atomic_load(&A.part_loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    for (uint32_t q = threadIdx.x; q < gridDim.x; q += 1024u)
+        v = __fadd_rn(v, __hip_atomic_load(&A.part_loss[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     v = wave_sum(v);
     if (lane == 0u) fsum[wave][0] = v;
     __syncthreads();
@@ -210,15 +217,17 @@ struct BackwardArgs {
     uint32_t runs, span;
 };
 
+/* A row is stored twice over: its lanes store every expert that the token did
+ * not choose, and lane r the one of route r, whose score it reads again (from
+ * the cache) rather than through LDS: 27 us so with LDS rows of 64 KB a block
+ * (two blocks a CU), 8192 tokens of 896 experts. */
 template <int J>
-__global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(BackwardArgs A) {
-    __shared__ float rows[kWaves][64 * J];
-    __shared__ float adds[kWaves][64 * J];
+__global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(BackwardArgs A) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
     const uint32_t s = blockIdx.x / A.runs, run = blockIdx.x % A.runs;
     const uint32_t i0 = run * A.span, i1 = min(i0 + A.span, A.L);
-    float *row = rows[wave], *add = adds[wave];
     const uint32_t n = A.live[s];
+    const uint32_t *counts = A.counts + (uint64_t)s * E;
     /* f, and the factor that the loss has in common: both 0 without live tokens */
     const float per = n ? __fdiv_rn((float)E, __fmul_rn((float)A.k, (float)n)) : 0.0f;
     float share = n ? __fdiv_rn(__fdiv_rn(A.coef, (float)A.S), (float)n) : 0.0f;
@@ -227,10 +236,9 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(BackwardAr
 #pragma unroll
     for (int j = 0; j < J; j++) {
         const uint32_t e = lane + 64u * (uint32_t)j;
-        f[j] = e < E ? __fmul_rn((float)A.counts[(uint64_t)s * E + e], per) : 0.0f;
-        add[e] = 0.0f;
+        f[j] = e < E ? __fmul_rn((float)counts[e], per) : 0.0f;
     }
-    for (uint32_t i = i0 + wave; i < i1; i += kWaves) {
+    for (uint32_t i = i0 + wave; i < i1; i += kBackWaves) {
         const uint64_t t = (uint64_t)s * A.L + i;
         float *out = A.out + t * E;
         if (A.mask && A.mask[t] == 0u) {
@@ -241,11 +249,21 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(BackwardAr
         }
         float x[J], d[J];
         load_row<J>(x, A.logits, t, E);
+        /* lane r: route r's expert (E: none), its logit, f and gradient */
+        uint32_t e = E;
+        float xe = -__builtin_huge_valf(), fe = 0.0f, dw = 0.0f;
+        if (A.dw) {
+            e = lane_route(A.ids, t, A.k, E);
+            if (e < E) {
+                xe = A.logits[t * E + e];
+                fe = __fmul_rn((float)counts[e], per);
+                dw = A.dw[t * A.k + lane];
+            }
+        }
         float z = 0.0f, a = 0.0f;
 #pragma unroll
         for (int j = 0; j < J; j++) {
             const float2 p = sigmoid_pair(x[j]);
-            x[j] = p.x;
             d[j] = __fmul_rn(p.x, p.y);
             z = __fadd_rn(z, p.x);
             a = fmaf(f[j], p.x, a);
@@ -254,38 +272,31 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(BackwardAr
         a = wave_sum(a);
         const float inv = z == 0.0f ? 0.0f : __fdiv_rn(1.0f, z);
         const float mean = __fmul_rn(a, inv), by = __fmul_rn(share, inv);
-        uint32_t e = E;
-        if (A.dw) { /* the routes' part, by expert, through LDS */
-#pragma unroll
-            for (int j = 0; j < J; j++) row[64 * j + lane] = x[j];
-            e = lane_route(A.ids, t, A.k, E);
-            const float dw = e < E ? A.dw[t * A.k + lane] : 0.0f;
-            wave_fence();
-            const float sig = e < E ? row[e] : 0.0f;
-            const float den = __fadd_rn(wave_sum(sig), 1e-20f);
-            const float m = __fdiv_rn(wave_sum(__fmul_rn(dw, sig)), den);
-            if (e < E) add[e] = __fmul_rn(__fdiv_rn(A.scale, den), __fsub_rn(dw, m));
-            wave_fence();
+        uint32_t chosen = 0u; /* the slots of this lane that a route has */
+        if (A.dw) {
+            for (uint32_t r = 0; r < A.k; r++) {
+                const uint32_t er = (uint32_t)__builtin_amdgcn_readlane((int)e, (int)r);
+                if (er < E && (er & 63u) == lane) chosen |= 1u << (er >> 6);
+            }
+            const float2 p = sigmoid_pair(xe); /* 0 without a route */
+            const float den = __fadd_rn(wave_sum(p.x), 1e-20f);
+            const float m = __fdiv_rn(wave_sum(__fmul_rn(dw, p.x)), den);
+            const float add = __fmul_rn(__fdiv_rn(A.scale, den), __fsub_rn(dw, m));
+            const float v = __fadd_rn(__fmul_rn(by, __fsub_rn(fe, mean)), add);
+            if (e < E) out[e] = __fmul_rn(v, __fmul_rn(p.x, p.y));
         }
 #pragma unroll
         for (int j = 0; j < J; j++) {
             const uint32_t q = lane + 64u * (uint32_t)j;
-            float v = __fmul_rn(by, __fsub_rn(f[j], mean));
-            if (A.dw) v = __fadd_rn(v, add[q]);
-            if (q < E) out[q] = __fmul_rn(v, d[j]);
-        }
-        if (A.dw) {
-            wave_fence();
-            if (e < E) add[e] = 0.0f;
-            wave_fence();
+            if (q < E && !(chosen >> j & 1u)) out[q] = __fmul_rn(__fmul_rn(by, __fsub_rn(f[j], mean)), d[j]);
         }
     }
 }
 
-/* Runs a segment is cut into: about 256 blocks in all (two tokens a wave at
- * least, so that a run's partial sums stay a small part of its reads). */
-void runs_of(uint32_t S, uint32_t L, uint32_t blocks, uint32_t &runs, uint32_t &span) {
-    const uint32_t want = (blocks + S - 1u) / S, most = (L + 2u * kWaves - 1u) / (2u * kWaves);
+/* Runs a segment is cut into: about `blocks` in all, of `waves` tokens at
+ * least. */
+void runs_of(uint32_t S, uint32_t L, uint32_t blocks, uint32_t waves, uint32_t &runs, uint32_t &span) {
+    const uint32_t want = (blocks + S - 1u) / S, most = (L + waves - 1u) / waves;
     runs = want < most ? want : most;
     span = (L + runs - 1u) / runs;
     runs = (L + span - 1u) / span;
@@ -308,21 +319,23 @@ size_t carve(BalanceArgs &A, void *base) {
     A.part_mean = (float *)take(4u * parts * A.E);
     A.part_count = (uint32_t *)take(4u * parts * A.E);
     A.part_live = (uint32_t *)take(4u * parts);
-    A.part_loss = (float *)take(4u * (size_t)A.S * ((A.E + 63u) / 64u));
+    A.part_loss = (float *)take(4u * (size_t)A.S * ((A.E + kJoin - 1u) / kJoin));
     A.ticket = (uint32_t *)take(4u);
     return off;
 }
 
-constexpr uint32_t kBlocks = 256;
+/* Two blocks a CU read a batch (their partial sums are another eighth of the
+ * reads at 8192 tokens), eight write its gradient. */
+constexpr uint32_t kPartBlocks = 512, kBackBlocks = 2048;
 
-/* f(integral_constant<int, J>) for the least J of 1, 2, 4, 8, 16 with E <= 64 J */
-template <class F>
+/* f(integral_constant<int, J>) for the least J here with E <= 64 J */
+template <int J = 1, class F>
 void with_slots(uint32_t E, F &&f) {
-    if (E <= 64u) f(std::integral_constant<int, 1>{});
-    else if (E <= 128u) f(std::integral_constant<int, 2>{});
-    else if (E <= 256u) f(std::integral_constant<int, 4>{});
-    else if (E <= 512u) f(std::integral_constant<int, 8>{});
-    else f(std::integral_constant<int, 16>{});
+    constexpr int next = J < 4 ? J + 1 : J + 2;
+    if constexpr (J < 16) {
+        if (E > 64u * J) return with_slots<next>(E, f);
+    }
+    f(std::integral_constant<int, J>{});
 }
 
 }  // namespace
@@ -335,7 +348,7 @@ extern "C" size_t k3_moe_balance_scratch_bytes(uint32_t segments, uint32_t lengt
     if (!batch_ok(segments, length, expert_count)) return 0u;
     BalanceArgs A{};
     A.S = segments, A.L = length, A.E = expert_count;
-    runs_of(segments, length, kBlocks, A.runs, A.span);
+    runs_of(segments, length, kPartBlocks, kWaves, A.runs, A.span);
     return carve(A, nullptr);
 }
 
@@ -352,14 +365,14 @@ extern "C" bool k3_moe_balance_loss_f32(float *loss, uint32_t *counts, float *me
         return false;
     BalanceArgs A{loss, counts, mean_scores, live_tokens, logits, expert_ids, mask, segments, length,
                   expert_count, top_k, coefficient};
-    runs_of(segments, length, kBlocks, A.runs, A.span);
+    runs_of(segments, length, kPartBlocks, kWaves, A.runs, A.span);
     carve(A, scratch);
     const hipStream_t st = (hipStream_t)stream;
     with_slots(expert_count, [&](auto J) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(balance_part_kernel<decltype(J)::value>),
                            dim3(segments * A.runs), dim3(64u * kWaves), 0, st, A);
     });
-    hipLaunchKernelGGL(balance_join_kernel, dim3(segments * ((expert_count + 63u) / 64u)), dim3(1024),
+    hipLaunchKernelGGL(balance_join_kernel, dim3(segments * ((expert_count + kJoin - 1u) / kJoin)), dim3(1024),
                        0, st, A);
     return hipGetLastError() == hipSuccess;
 }
@@ -378,10 +391,10 @@ extern "C" bool k3_moe_router_backward_f32(float *logits_gradient, const float *
     BackwardArgs A{logits_gradient, logits, expert_ids, counts, live_tokens, mask, loss_gradient,
                    weight_gradient, segments, length, expert_count, top_k, coefficient,
                    scaling_factor, 0u, 0u};
-    runs_of(segments, length, kBlocks, A.runs, A.span);
+    runs_of(segments, length, kBackBlocks, kBackWaves, A.runs, A.span);
     with_slots(expert_count, [&](auto J) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(router_backward_kernel<decltype(J)::value>),
-                           dim3(segments * A.runs), dim3(64u * kWaves), 0, (hipStream_t)stream, A);
+                           dim3(segments * A.runs), dim3(64u * kBackWaves), 0, (hipStream_t)stream, A);
     });
     return hipGetLastError() == hipSuccess;
 }

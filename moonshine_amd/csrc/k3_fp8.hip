@@ -763,7 +763,7 @@ struct TileRun {
 };
 
 template <class C, int MODE>
-__global__ __launch_bounds__(C::THREADS, C::WAVES / 4) void tile_kernel(TileArgs P) {
+__global__ __launch_bounds__(C::THREADS, 2) void tile_kernel(TileArgs P) {
     static_assert(MODE != kGateUp || C::WN == 4, "a gate/up block holds whole scale blocks");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
     TileRun<C> R;
@@ -1118,9 +1118,9 @@ using Tile64 = Tile<4, 2, 3>;
 using Tile128 = Tile<4, 4, 3>;
 using Tile256 = Tile<4, 8, 2>;
 /* half as many rows: few tokens' products */
-using Half32 = Tile<2, 1, 5>;
-using Half64 = Tile<2, 2, 5>;
-using Half128 = Tile<2, 4, 4>;
+using Half32 = Tile<2, 1, 3>;
+using Half64 = Tile<2, 2, 3>;
+using Half128 = Tile<2, 4, 2>;
 
 /* How a product of T > 1 tokens is cut. */
 struct Cut {

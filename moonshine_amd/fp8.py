@@ -18,90 +18,83 @@ from .synth import Config
 
 BLOCK = 128
 _CODES = (torch.float8_e4m3fn, torch.uint8)
-
-
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+_BF16, _F32, _I32, _I64, _U8 = (torch.bfloat16,), (torch.float32,), (torch.int32,), (torch.int64,), (torch.uint8,)
 
 
 def _dense(t, name, dtypes, dim, device=None):
-    """A contiguous device tensor of one of `dtypes` (and on `device`)."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a tensor on the GPU is wanted")
-    _need(t.dtype in dtypes, f"{name}: {t.dtype}, wanted {' or '.join(map(str, dtypes))}")
-    _need(t.dim() == dim and t.is_contiguous(), f"{name}: a contiguous tensor of {dim} dimensions is wanted")
-    _need(device is None or t.device == device, f"{name}: on {t.device}, not {device}")
-    return t
+    """The address of a contiguous tensor of one of `dtypes` on GPU `device` (any, if None)."""
+    if (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and t.is_contiguous()
+            and t.is_cuda and (device is None or t.get_device() == device)):
+        return t.data_ptr()
+    raise ValueError(
+        f"{name}: a contiguous tensor of {dim} dimensions and {' or '.join(map(str, dtypes))} on GPU "
+        f"{'' if device is None else device} is wanted"
+        + (f", not {t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else ""))
 
 
-class _On:
-    """The tensors' device made current for a launch (nothing if it is)."""
-
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+# a call costs the host several microseconds, so device and stream are asked for directly
+_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _scratch(n, device):
-    """n bytes for one call (None for 0) and its address."""
+def _call(fn, device, *args):
+    """fn(*args, stream) on `device`, made current for the call if it is not."""
+    if _device() == device:
+        ok = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            ok = fn(*args, _stream(device))
+    if not ok:
+        raise RuntimeError(f"{fn.__name__} rejected its arguments or failed to launch")
+
+
+def _scratch(like, n):
+    """n bytes for one call (None for 0) and their address."""
     if n == 0:
         return None, None
-    t = torch.empty(n, dtype=torch.uint8, device=device)
+    t = like.new_empty((n,), dtype=torch.uint8)
     return t, t.data_ptr()
 
 
-def _quantize(fn, name, x, block_rows):
-    _dense(x, "x", (torch.bfloat16,), 2)
+def _quantize(fn, x, block_rows):
+    at = _dense(x, "x", _BF16, 2)
     rows, cols = x.shape
-    _need(rows > 0 and cols > 0 and cols % BLOCK == 0, f"{name}: columns in blocks of {BLOCK} are wanted")
-    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((-(-rows // block_rows), cols // BLOCK), dtype=torch.float32, device=x.device)
-    with _On(x.device) as st:
-        if not fn(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, cols, st):
-            raise RuntimeError(f"{name} rejected its arguments or failed to launch")
+    if rows == 0 or cols == 0 or cols % BLOCK != 0:
+        raise ValueError(f"x: {tuple(x.shape)}, columns in blocks of {BLOCK} are wanted")
+    codes = x.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((-(-rows // block_rows), cols // BLOCK), dtype=torch.float32)
+    _call(fn, x.get_device(), codes.data_ptr(), scales.data_ptr(), at, rows, cols)
     return codes, scales
 
 
 def quantize_rows(x):
     """bf16 [rows, cols] -> codes [rows, cols], scales [rows, cols / 128]."""
-    return _quantize(lib().k3_moe_fp8_128_quantize_rows_bf16, "k3_moe_fp8_128_quantize_rows_bf16", x, 1)
+    return _quantize(lib().k3_moe_fp8_128_quantize_rows_bf16, x, 1)
 
 
 def quantize_weight(w):
     """bf16 [rows, cols] -> codes [rows, cols], scales [ceil(rows / 128), cols / 128]."""
-    return _quantize(lib().k3_moe_fp8_128_quantize_weight_bf16,
-                     "k3_moe_fp8_128_quantize_weight_bf16", w, BLOCK)
+    return _quantize(lib().k3_moe_fp8_128_quantize_weight_bf16, w, BLOCK)
 
 
 def product(x, codes, scales, out=None):
     """bf16 [T, cols] times an encoded weight [rows, cols] -> bf16 [T, rows]."""
-    _dense(x, "x", (torch.bfloat16,), 2)
-    _dense(codes, "codes", _CODES, 2, x.device)
-    _dense(scales, "scales", (torch.float32,), 2, x.device)
+    at = _dense(x, "x", _BF16, 2)
+    device = x.get_device()
+    w, s = _dense(codes, "codes", _CODES, 2, device), _dense(scales, "scales", _F32, 2, device)
     (T, K), (N, K2) = x.shape, codes.shape
-    _need(K == K2 and scales.shape == (-(-N // BLOCK), K // BLOCK),
-          f"product of {tuple(x.shape)} with {tuple(codes.shape)}, scales {tuple(scales.shape)}")
+    if K != K2 or scales.shape != (-(-N // BLOCK), K // BLOCK):
+        raise ValueError(f"product of {tuple(x.shape)} with {tuple(codes.shape)}, scales {tuple(scales.shape)}")
     if out is None:
-        out = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((T, N))
+        to = out.data_ptr()
     else:
-        _dense(out, "out", (torch.bfloat16,), 2, x.device)
-        _need(out.shape == (T, N), f"out: {tuple(out.shape)}, wanted {(T, N)}")
+        to = _dense(out, "out", _BF16, 2, device)
+        if out.shape != (T, N):
+            raise ValueError(f"out: {tuple(out.shape)}, wanted {(T, N)}")
     L = lib()
-    n = L.k3_moe_fp8_128_scratch_bytes(T, N, K)
-    keep, at = _scratch(n, x.device)
-    with _On(x.device) as st:
-        if not L.k3_moe_fp8_128_gemm_bf16(out.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-                                          x.data_ptr(), T, N, K, at, n, st):
-            raise RuntimeError("k3_moe_fp8_128_gemm_bf16 rejected its arguments or failed to launch")
+    n = L.k3_moe_fp8_128_scratch_bytes(T, N, K) if T > 1 else 0
+    keep, room = _scratch(x, n)
+    _call(L.k3_moe_fp8_128_gemm_bf16, device, to, w, s, at, T, N, K, room, n)
     return out
 
 
@@ -110,18 +103,21 @@ def shape(hidden, experts, top_k, ffn, scaling_factor, activation, beta=4.0, lin
     return K3MoeShape(hidden, experts, top_k, ffn, scaling_factor, activation, beta, linear_beta)
 
 
-def _rows(t, name, T, H, like):
-    if t is not None:
-        _dense(t, name, (torch.bfloat16,), 2, like.device)
-        _need(t.shape == (T, H), f"{name}: {tuple(t.shape)}, wanted {(T, H)}")
-    return None if t is None else t.data_ptr()
+def _rows(t, name, shape, device):
+    """The address of a bf16 tensor of `shape` (None: none)."""
+    if t is None:
+        return None
+    at = _dense(t, name, _BF16, 2, device)
+    if t.shape != shape:
+        raise ValueError(f"{name}: {tuple(t.shape)}, wanted {tuple(shape)}")
+    return at
 
 
-def _workspace(shape, T, device):
+def _workspace(shape, T, like):
     n = lib().k3_moe_fp8_workspace_bytes(ctypes.byref(shape), T)
-    _need(n != 0, "unsupported shape or token count")
-    keep, at = _scratch(n, device)
-    return keep, at, n
+    if n == 0:
+        raise ValueError("unsupported shape or token count")
+    return (*_scratch(like, n), n)
 
 
 def experts(hidden, ids, weights, table, shape, residual=None, out=None):
@@ -129,24 +125,23 @@ def experts(hidden, ids, weights, table, shape, residual=None, out=None):
 
     ids (int32) and weights (float32): [T, top_k]; table: int64 [E, 6] device
     tensor of the experts' addresses (Fp8ExpertStore.table)."""
-    _dense(hidden, "hidden", (torch.bfloat16,), 2)
+    x = _dense(hidden, "hidden", _BF16, 2)
     T, H = hidden.shape
-    _need(H == shape.hidden, f"hidden: {H} wide, the shape {shape.hidden}")
-    for t, name, dtype in ((ids, "ids", torch.int32), (weights, "weights", torch.float32)):
-        _dense(t, name, (dtype,), 2, hidden.device)
-        _need(t.shape == (T, shape.top_k), f"{name}: {tuple(t.shape)}, wanted {(T, shape.top_k)}")
-    _dense(table, "table", (torch.int64,), 2, hidden.device)
-    _need(table.shape == (shape.expert_count, 6), "table: [experts, 6] is wanted")
-    res = _rows(residual, "residual", T, H, hidden)
+    device = hidden.get_device()
+    if H != shape.hidden:
+        raise ValueError(f"hidden: {H} wide, the shape {shape.hidden}")
+    i, w = _dense(ids, "ids", _I32, 2, device), _dense(weights, "weights", _F32, 2, device)
+    if ids.shape != (T, shape.top_k) or weights.shape != (T, shape.top_k):
+        raise ValueError(f"ids {tuple(ids.shape)}, weights {tuple(weights.shape)}, wanted {(T, shape.top_k)}")
+    t = _dense(table, "table", _I64, 2, device)
+    if table.shape != (shape.expert_count, 6):
+        raise ValueError("table: [experts, 6] is wanted")
+    res = _rows(residual, "residual", hidden.shape, device)
     if out is None:
-        out = torch.empty_like(hidden)
-    to = _rows(out, "out", T, H, hidden)
-    keep, at, n = _workspace(shape, T, hidden.device)
-    with _On(hidden.device) as st:
-        if not lib().k3_moe_fp8_experts_bf16(to, hidden.data_ptr(), res, ids.data_ptr(),
-                                             weights.data_ptr(), table.data_ptr(),
-                                             ctypes.byref(shape), T, at, n, st):
-            raise RuntimeError("k3_moe_fp8_experts_bf16 rejected its arguments or failed to launch")
+        out = hidden.new_empty((T, H))
+    to = _rows(out, "out", hidden.shape, device)
+    keep, room, n = _workspace(shape, T, hidden)
+    _call(lib().k3_moe_fp8_experts_bf16, device, to, x, res, i, w, t, ctypes.byref(shape), T, room, n)
     return out
 
 
@@ -160,11 +155,11 @@ class Fp8ExpertStore:
         E, F, H = gate[0].shape
         for (codes, scales), name, rows, cols in ((gate, "gate", F, H), (down, "down", H, F),
                                                   (up, "up", F, H)):
-            _dense(codes, name, _CODES, 3, gate[0].device)
-            _dense(scales, name + " scales", (torch.float32,), 3, gate[0].device)
-            _need(rows % BLOCK == 0 and cols % BLOCK == 0 and codes.shape == (E, rows, cols)
-                  and scales.shape == (E, rows // BLOCK, cols // BLOCK),
-                  f"{name}: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
+            _dense(codes, name, _CODES, 3, gate[0].get_device())
+            _dense(scales, name + " scales", _F32, 3, gate[0].get_device())
+            if (rows % BLOCK != 0 or cols % BLOCK != 0 or codes.shape != (E, rows, cols)
+                    or scales.shape != (E, rows // BLOCK, cols // BLOCK)):
+                raise ValueError(f"{name}: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
         self.experts, self.ffn, self.hidden = E, F, H
         self.gate, self.down, self.up = gate, down, up
         each = torch.arange(E, dtype=torch.int64)
@@ -194,31 +189,34 @@ class Fp8RoutedMoE:
 
     def __init__(self, cfg: Config, router_weight, router_bias, store: Fp8ExpertStore):
         self.cfg, self.shape, self.store = cfg, make_shape(cfg), store
-        _need((store.experts, store.hidden, store.ffn) == (cfg.experts, cfg.hidden, cfg.ffn),
-              "the store's sizes are not the configuration's")
-        self.router_weight = _dense(router_weight, "router_weight", (torch.bfloat16,), 2)
-        self.router_bias = _dense(router_bias, "router_bias", (torch.float32,), 1)
+        if (store.experts, store.hidden, store.ffn) != (cfg.experts, cfg.hidden, cfg.ffn):
+            raise ValueError("the store's sizes are not the configuration's")
+        _dense(router_weight, "router_weight", _BF16, 2)
+        _dense(router_bias, "router_bias", _F32, 1, router_weight.get_device())
+        if router_weight.shape != (cfg.experts, cfg.hidden) or router_bias.shape != (cfg.experts,):
+            raise ValueError(f"router_weight {tuple(router_weight.shape)}, router_bias {tuple(router_bias.shape)}")
+        self.router_weight, self.router_bias = router_weight, router_bias
 
     def forward(self, hidden, residual=None, out=None, ids=None, weights=None):
         """ids, weights: optional [T, top_k] tensors that receive the routes."""
-        _dense(hidden, "hidden", (torch.bfloat16,), 2, self.router_weight.device)
+        device = self.router_weight.get_device()
+        x = _dense(hidden, "hidden", _BF16, 2, device)
         T, H = hidden.shape
-        _need(H == self.shape.hidden, f"hidden: {H} wide, the shape {self.shape.hidden}")
-        res = _rows(residual, "residual", T, H, hidden)
+        if H != self.shape.hidden:
+            raise ValueError(f"hidden: {H} wide, the shape {self.shape.hidden}")
+        res = _rows(residual, "residual", hidden.shape, device)
         if out is None:
-            out = torch.empty_like(hidden)
-        to = _rows(out, "out", T, H, hidden)
-        for t in (ids, weights):
-            _need(t is None or t.shape == (T, self.shape.top_k) and t.element_size() == 4
-                  and t.is_contiguous(), "ids, weights: contiguous [T, top_k] of 32 bits are wanted")
-        keep, at, n = _workspace(self.shape, T, hidden.device)
-        with _On(hidden.device) as st:
-            if not lib().k3_moe_fp8_forward_bf16(
-                    to, hidden.data_ptr(), res, self.router_weight.data_ptr(),
-                    self.router_bias.data_ptr(), self.store.table.data_ptr(),
-                    ctypes.byref(self.shape), T, None if ids is None else ids.data_ptr(),
-                    None if weights is None else weights.data_ptr(), at, n, st):
-                raise RuntimeError("k3_moe_fp8_forward_bf16 rejected its arguments or failed to launch")
+            out = hidden.new_empty((T, H))
+        to = _rows(out, "out", hidden.shape, device)
+        copies = []
+        for t, name, dtypes in ((ids, "ids", _I32), (weights, "weights", _F32)):
+            copies.append(None if t is None else _dense(t, name, dtypes, 2, device))
+            if t is not None and t.shape != (T, self.shape.top_k):
+                raise ValueError(f"{name}: [T, top_k] is wanted")
+        keep, room, n = _workspace(self.shape, T, hidden)
+        _call(lib().k3_moe_fp8_forward_bf16, device, to, x, res, self.router_weight.data_ptr(),
+              self.router_bias.data_ptr(), self.store.table.data_ptr(), ctypes.byref(self.shape), T,
+              *copies, room, n)
         return out
 
     def experts_only(self, hidden, ids, weights, residual=None, out=None):
