@@ -479,7 +479,7 @@ bool k3_moe_fp8_forward_bf16(void *output, const void *hidden, const void *resid
  * One segment is the loss over the whole batch. A route is counted as
  * k3_moe_route_plan does: ids from E on and a token's repeated ids are not. A
  * segment without live tokens has mean scores 0 and adds nothing; a token
- * whose scores are all 0 (logits below -103 or -inf throughout) has shares 0.
+ * whose scores are all 0 (logits below -88.7 or -inf throughout) has shares 0.
  * Sums run in an order set by the sizes alone. The reference only
  * serves; it has no counterpart. segments * length <= 2^24, E <= 1024, k <= 32,
  * k <= E. scratch: k3_moe_balance_scratch_bytes(segments, length, E) bytes,

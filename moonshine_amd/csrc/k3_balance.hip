@@ -34,25 +34,37 @@ constexpr uint32_t kBackWaves = 4;
 
 inline size_t align256(size_t v) { return (v + 255u) & ~(size_t)255u; }
 
-/* sigma(x) and 1 - sigma(x), each to a few ulp of itself: the exponential is
- * taken of -|x|, so neither is a difference. */
-__device__ __forceinline__ float2 sigmoid_pair(float x) {
-    const float t = __builtin_amdgcn_exp2f(__fmul_rn(fabsf(x), -1.44269504088896341f));
-    const float s = __builtin_amdgcn_rcpf(__fadd_rn(1.0f, t)), l = __fmul_rn(t, s);
-    return x >= 0.0f ? make_float2(s, l) : make_float2(l, s);
+/* sigma(x) = 1 / (1 + t), t = e^-x, to a few ulp of itself; 0 where t overflows
+ * (x < -88.7). */
+__device__ __forceinline__ float exp_neg(float x) {
+    return __builtin_amdgcn_exp2f(__fmul_rn(x, -1.44269504088896341f));
+}
+__device__ __forceinline__ float sigma_of(float t) {
+    return __builtin_amdgcn_rcpf(__fadd_rn(1.0f, t));
+}
+/* sigma (1 - sigma) = t sigma^2: no difference of near values, and 0 where sigma
+ * is 0. */
+__device__ __forceinline__ float slope_of(float t, float sigma) {
+    return __fmul_rn(__fmul_rn(fminf(t, 0x1p126f), sigma), sigma);
 }
 
-/* The route of lane r < k of a token: its id, or E where it has none (no such
- * rank, an id from E on, or one that an earlier rank has). */
-__device__ __forceinline__ uint32_t lane_route(const uint32_t *ids, uint64_t t, uint32_t k,
-                                               uint32_t E) {
+/* Lane r < k: the id of route r of a token; E past them. */
+__device__ __forceinline__ uint32_t load_ids(const uint32_t *ids, uint64_t t, uint32_t k, uint32_t E) {
     const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t id = lane < k ? ids[t * k + lane] : E;
+    return lane < k ? ids[t * k + lane] : E;
+}
+/* The route of lane r < k of a token by load_ids: its id, or E where it has none
+ * (no such rank, an id from E on, or one that an earlier rank has). */
+__device__ __forceinline__ uint32_t lane_route(uint32_t id, uint32_t k, uint32_t E) {
+    const uint32_t lane = threadIdx.x & 63u;
     bool again = id >= E;
     for (uint32_t r = 0; r + 1u < k; r++)
         again |= lane > r && id == (uint32_t)__builtin_amdgcn_readlane((int)id, (int)r);
     return again ? E : id;
 }
+
+/* Slots of a row of J that are whole wherever with_slots picks J. */
+constexpr int whole_slots(int J) { return J <= 4 ? J - 1 : J - 2; }
 
 /* The logits of token t (-inf, score 0, past E). */
 template <int J>
@@ -63,7 +75,7 @@ __device__ __forceinline__ void load_row(float (&x)[J], const float *logits, uin
 #pragma unroll
     for (int j = 0; j < J; j++) {
         const uint32_t e = lane + 64u * (uint32_t)j;
-        x[j] = e < E ? row[e] : -__builtin_huge_valf();
+        x[j] = j < whole_slots(J) || e < E ? row[e] : -__builtin_huge_valf();
     }
 }
 
@@ -105,13 +117,14 @@ __global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A
         if (A.mask && A.mask[t] == 0u) continue;
         live++;
         float x[J];
+        const uint32_t id = load_ids(A.ids, t, A.k, E);
         load_row<J>(x, A.logits, t, E);
-        const uint32_t e = lane_route(A.ids, t, A.k, E);
+        const uint32_t e = lane_route(id, A.k, E);
         if (e < E) atomicAdd(&hist[e], 1u);
         float z = 0.0f;
 #pragma unroll
         for (int j = 0; j < J; j++) {
-            x[j] = sigmoid_pair(x[j]).x;
+            x[j] = sigma_of(exp_neg(x[j]));
             z = __fadd_rn(z, x[j]);
         }
         z = wave_sum(z);
@@ -248,12 +261,15 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
             continue;
         }
         float x[J], d[J];
+        /* the ids first: the loads that go by them wait for nothing else */
+        const uint32_t id = A.dw ? load_ids(A.ids, t, A.k, E) : E;
+        asm volatile("" ::: "memory");
         load_row<J>(x, A.logits, t, E);
         /* lane r: route r's expert (E: none), its logit, f and gradient */
         uint32_t e = E;
         float xe = -__builtin_huge_valf(), fe = 0.0f, dw = 0.0f;
         if (A.dw) {
-            e = lane_route(A.ids, t, A.k, E);
+            e = lane_route(id, A.k, E);
             if (e < E) {
                 xe = A.logits[t * E + e];
                 fe = __fmul_rn((float)counts[e], per);
@@ -263,10 +279,10 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
         float z = 0.0f, a = 0.0f;
 #pragma unroll
         for (int j = 0; j < J; j++) {
-            const float2 p = sigmoid_pair(x[j]);
-            d[j] = __fmul_rn(p.x, p.y);
-            z = __fadd_rn(z, p.x);
-            a = fmaf(f[j], p.x, a);
+            const float u = exp_neg(x[j]), p = sigma_of(u);
+            d[j] = slope_of(u, p);
+            z = __fadd_rn(z, p);
+            a = fmaf(f[j], p, a);
         }
         z = wave_sum(z);
         a = wave_sum(a);
@@ -276,19 +292,19 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
         if (A.dw) {
             for (uint32_t r = 0; r < A.k; r++) {
                 const uint32_t er = (uint32_t)__builtin_amdgcn_readlane((int)e, (int)r);
-                if (er < E && (er & 63u) == lane) chosen |= 1u << (er >> 6);
+                chosen |= er < E && (er & 63u) == lane ? 1u << (er >> 6) : 0u;
             }
-            const float2 p = sigmoid_pair(xe); /* 0 without a route */
-            const float den = __fadd_rn(wave_sum(p.x), 1e-20f);
-            const float m = __fdiv_rn(wave_sum(__fmul_rn(dw, p.x)), den);
+            const float u = exp_neg(xe), p = sigma_of(u); /* 0 without a route */
+            const float den = __fadd_rn(wave_sum(p), 1e-20f);
+            const float m = __fdiv_rn(wave_sum(__fmul_rn(dw, p)), den);
             const float add = __fmul_rn(__fdiv_rn(A.scale, den), __fsub_rn(dw, m));
             const float v = __fadd_rn(__fmul_rn(by, __fsub_rn(fe, mean)), add);
-            if (e < E) out[e] = __fmul_rn(v, __fmul_rn(p.x, p.y));
+            if (e < E) out[e] = __fmul_rn(v, slope_of(u, p));
         }
 #pragma unroll
         for (int j = 0; j < J; j++) {
             const uint32_t q = lane + 64u * (uint32_t)j;
-            if (q < E && !(chosen >> j & 1u)) out[q] = __fmul_rn(__fmul_rn(by, __fsub_rn(f[j], mean)), d[j]);
+            if ((j < whole_slots(J) || q < E) && !(chosen >> j & 1u)) out[q] = __fmul_rn(__fmul_rn(by, __fsub_rn(f[j], mean)), d[j]);
         }
     }
 }
@@ -325,8 +341,8 @@ size_t carve(BalanceArgs &A, void *base) {
 }
 
 /* Two blocks a CU read a batch (their partial sums are another eighth of the
- * reads at 8192 tokens), eight write its gradient. */
-constexpr uint32_t kPartBlocks = 512, kBackBlocks = 2048;
+ * reads at 8192 tokens), four write its gradient. */
+constexpr uint32_t kPartBlocks = 512, kBackBlocks = 1024;
 
 /* f(integral_constant<int, J>) for the least J here with E <= 64 J */
 template <int J = 1, class F>
