@@ -978,47 +978,29 @@ __global__ __launch_bounds__(C::THREADS) void join_kernel(TileArgs P) {
 /* routes and tiles of the experts                                         */
 /* ---------------------------------------------------------------------- */
 
-/* ids with a token's repeated ones invalidated, as the plan drops them. */
-__global__ __launch_bounds__(256) void routes_kernel(uint32_t *__restrict__ out,
-                                                     const uint32_t *__restrict__ ids, uint32_t T,
-                                                     uint32_t k, uint32_t E) {
-    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
-    if (t >= T) return;
-    uint32_t e[32];
-    token_routes<32>(ids, t, k, E, e);
-#pragma unroll
-    for (uint32_t r = 0; r < 32u; r++)
-        if (r < k) out[(uint64_t)t * k + r] = e[r];
-}
-
 /* Tile classes by an expert's rows: up to 32, 64 and 128 (one tile), more (tiles
  * of up to 256, of equal length in 32-row steps). */
 constexpr int kClasses = 4;
 
-/* One block of 1024 threads (thread e: expert e): each class's tiles in expert
- * order. */
 struct TileLists {
     ExpertTile *tiles[kClasses];
     uint32_t *count; /* [kClasses] */
 };
-__global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t *__restrict__ counts,
-                                                     const uint32_t *__restrict__ offsets,
-                                                     const k3_moe_fp8_expert *__restrict__ experts,
-                                                     uint32_t E) {
+
+/* By a block of 1024 threads, thread e with expert e's rows [row, row + n): each
+ * class's tiles in expert order. */
+__device__ __forceinline__ void list_tiles(const TileLists &Q, uint32_t row, uint32_t n,
+                                           const k3_moe_fp8_expert *experts) {
     __shared__ uint32_t tot[kClasses][16];
     const uint32_t e = threadIdx.x, lane = e & 63u, wave = e >> 6;
-    const uint32_t n = e < E ? counts[e] : 0u;
-    ExpertTile mine{0u, n, 0u, 0u, {}};
-    if (n != 0u) {
-        mine.row = offsets[e];
-        mine.many = (n + tile_height(n) - 1u) / tile_height(n);
-        mine.ex = experts[e];
-    }
     const int cls = n <= 32u ? 0 : n <= 64u ? 1 : n <= 128u ? 2 : 3;
+    const uint32_t height = n ? tile_height(n) : 1u, many = (n + height - 1u) / height;
+    k3_moe_fp8_expert ex{};
+    if (n != 0u) ex = experts[e];
     uint32_t inc[kClasses];
 #pragma unroll
     for (int q = 0; q < kClasses; q++) {
-        inc[q] = cls == q ? mine.many : 0u;
+        inc[q] = cls == q ? many : 0u;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t a = __shfl_up(inc[q], o, 64);
@@ -1029,14 +1011,72 @@ __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kClasses; q++) {
-        uint32_t at = inc[q] - mine.many, total = 0u;
+        uint32_t at = inc[q] - many, total = 0u;
         for (uint32_t w = 0; w < 16u; w++) {
             if (w < wave) at += tot[q][w];
             total += tot[q][w];
         }
         if (cls == q)
-            for (; mine.index < mine.many; mine.index++) Q.tiles[q][at + mine.index] = mine;
+            for (uint32_t i = 0; i < many; i++) Q.tiles[q][at + i] = ExpertTile{row, n, i, many, ex};
         if (e == 0u) Q.count[q] = total;
+    }
+}
+
+__global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t *__restrict__ counts,
+                                                     const uint32_t *__restrict__ offsets,
+                                                     const k3_moe_fp8_expert *__restrict__ experts,
+                                                     uint32_t E) {
+    const uint32_t e = threadIdx.x;
+    list_tiles(Q, e < E ? offsets[e] : 0u, e < E ? counts[e] : 0u, experts);
+}
+
+/* The plan (k3_moe_route_plan's order) and the tiles of up to 256 tokens as one
+ * block's work: four launches less. Thread t < T holds token t's routes; an
+ * expert's rows are the set bits of its masks. */
+constexpr uint32_t kSmallPlan = 256;
+template <int K>
+__global__ __launch_bounds__(1024) void small_plan_kernel(TileLists Q, uint32_t *__restrict__ token_index,
+                                                          uint32_t *__restrict__ route_index,
+                                                          const uint32_t *__restrict__ ids,
+                                                          const k3_moe_fp8_expert *__restrict__ experts,
+                                                          uint32_t T, uint32_t k, uint32_t E) {
+    __shared__ unsigned long long masks[kSmallPlan / 64u][1024];
+    __shared__ uint32_t first[1024], wave_tot[16];
+    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+#pragma unroll
+    for (uint32_t w = 0; w < kSmallPlan / 64u; w++) masks[w][t] = 0ull;
+    __syncthreads();
+    uint32_t e[K];
+    if (t < T) {
+        token_routes<K>(ids, t, k, E, e);
+#pragma unroll
+        for (int r = 0; r < K; r++)
+            if (e[r] < E) atomicOr(&masks[wave][e[r]], 1ull << lane);
+    }
+    __syncthreads();
+    uint32_t n = 0u;
+#pragma unroll
+    for (uint32_t w = 0; w < kSmallPlan / 64u; w++) n += (uint32_t)__popcll(masks[w][t]);
+    uint32_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t a = __shfl_up(inc, o, 64);
+        if ((int)lane >= o) inc += a;
+    }
+    if (lane == 63u) wave_tot[wave] = inc;
+    __syncthreads();
+    uint32_t row = inc - n;
+    for (uint32_t w = 0; w < wave; w++) row += wave_tot[w];
+    first[t] = row;
+    list_tiles(Q, row, n, experts); /* a barrier inside: `first` is whole */
+    if (t >= T) return;
+#pragma unroll
+    for (int r = 0; r < K; r++) {
+        if (e[r] >= E) continue;
+        uint32_t at = first[e[r]] + (uint32_t)__popcll(masks[wave][e[r]] & ((1ull << lane) - 1ull));
+        for (uint32_t w = 0; w < wave; w++) at += (uint32_t)__popcll(masks[w][e[r]]);
+        token_index[at] = t;
+        route_index[at] = t * k + (uint32_t)r;
     }
 }
 
@@ -1176,7 +1216,7 @@ bool launch_class(TileArgs A, const Fp8Workspace &ws, int cls, const k3_moe_shap
     return launch_tile<C, kDown>(A, ws.cap[cls] * A.tiles_n, st);
 }
 
-/* The expert stage on routes in ids (T > 1: ws.ids, repeated ones taken out). */
+/* The expert stage on given routes. */
 bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, const void *residual,
                      const uint32_t *ids, const float *wts, const k3_moe_fp8_expert *experts,
                      const k3_moe_shape &s, uint32_t T, hipStream_t st) {
@@ -1192,13 +1232,21 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
             hipLaunchKernelGGL(down_one_kernel<kOneFfn>, dim3(H / 16u), dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
-    hipLaunchKernelGGL(routes_kernel, dim3((T + 255u) / 256u), dim3(256), 0, st, ws.ids, ids, T, k, E);
-    if (!launch_rows(ws.xq, ws.xs, hidden, T, H, scale_stride(H), st) ||
-        !k3_moe_route_plan(ws.counts, ws.offsets, ws.unique, ws.summary, ws.token_index,
-                           ws.route_index, ws.ids, T, k, E, ws.plan, ws.plan_bytes, st))
-        return false;
-    hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(1024), 0, st, ws.lists, ws.counts, ws.offsets,
-                       experts, E);
+    if (!launch_rows(ws.xq, ws.xs, hidden, T, H, scale_stride(H), st)) return false;
+    if (T <= kSmallPlan) {
+        if (k <= 8u)
+            hipLaunchKernelGGL(small_plan_kernel<8>, dim3(1), dim3(1024), 0, st, ws.lists,
+                               ws.token_index, ws.route_index, ids, experts, T, k, E);
+        else
+            hipLaunchKernelGGL(small_plan_kernel<32>, dim3(1), dim3(1024), 0, st, ws.lists,
+                               ws.token_index, ws.route_index, ids, experts, T, k, E);
+    } else {
+        if (!k3_moe_route_plan(ws.counts, ws.offsets, ws.unique, ws.summary, ws.token_index,
+                               ws.route_index, ids, T, k, E, ws.plan, ws.plan_bytes, st))
+            return false;
+        hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(1024), 0, st, ws.lists, ws.counts, ws.offsets,
+                           experts, E);
+    }
     TileArgs B{};
     B.token_index = ws.token_index, B.route_index = ws.route_index;
     B.xq = ws.xq, B.xs = ws.xs, B.xstride = scale_stride(H);
@@ -1206,7 +1254,7 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
     B.kind = s.activation, B.beta = s.beta, B.lb = s.linear_beta;
     return hipGetLastError() == hipSuccess && launch_class<Tile32>(B, ws, 0, s, st) && launch_class<Tile64>(B, ws, 1, s, st) &&
            launch_class<Tile128>(B, ws, 2, s, st) && launch_class<Tile256>(B, ws, 3, s, st) &&
-           launch_combine(output, ws.y, residual, ws.ids, wts, T, H, k, E, st);
+           launch_combine(output, ws.y, residual, ids, wts, T, H, k, E, true, st);
 }
 
 }  // namespace

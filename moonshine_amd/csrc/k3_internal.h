@@ -85,9 +85,10 @@ bool launch_router_topk(uint32_t *ids, float *w, uint32_t *ids2, float *w2,
                         hipStream_t stream);
 
 /* out[t] = bf16(residual + bf16(sum_r w[t, r] y[t k + r])) in rank order; routes
- * with an id from E on are skipped. H % 8 == 0, rows 16-byte aligned. */
+ * with an id from E on are skipped, with `once` also those that repeat an id of
+ * their token. H % 8 == 0, rows 16-byte aligned. */
 bool launch_combine(void *output, const uint16_t *y, const void *residual, const uint32_t *ids,
-                    const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E,
+                    const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E, bool once,
                     hipStream_t stream);
 
 /* Counter-based generator of the synthetic expert store. */

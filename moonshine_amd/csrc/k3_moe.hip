@@ -277,23 +277,34 @@ __device__ __forceinline__ float bf16_round(float v) { return bf16_to_f32(f32_to
  * a token costs one memory round trip. H % 8 == 0, rows 16-byte aligned. */
 constexpr uint32_t kCombineThreads = 128;
 
+/* ONCE: a token's repeated ids are skipped too (the plan gives them no row). */
+template <bool ONCE>
 __global__ __launch_bounds__(128) void combine_kernel(
         uint16_t *__restrict__ out, const uint16_t *__restrict__ y,
         const uint16_t *__restrict__ residual, const uint32_t *__restrict__ ids,
         const float *__restrict__ wts, uint32_t H, uint32_t k, uint32_t E) {
     const uint32_t t = blockIdx.y;
     const uint32_t d = 8u * (blockIdx.x * kCombineThreads + threadIdx.x);
-    if (d >= H) return;
+    if (!ONCE && d >= H) return;
     const uint64_t r0 = (uint64_t)t * k;
     uint4 yv[32];
     float w[32];
     bool live[32];
+    uint32_t again = 0u; /* ranks that repeat an earlier one's id */
+    if constexpr (ONCE) {
+        const uint32_t lane = threadIdx.x & 63u, id = lane < k ? ids[r0 + lane] : E;
+        bool same = false;
+        for (uint32_t r = 0; r + 1u < k; r++)
+            same |= lane > r && id == (uint32_t)__builtin_amdgcn_readlane((int)id, (int)r);
+        again = (uint32_t)__ballot(same && lane < k);
+        if (d >= H) return;
+    }
 #pragma unroll
     for (int r = 0; r < 32; r++) { /* route 0 stands in for r >= k */
         const uint64_t route = r0 + ((uint32_t)r < k ? (uint32_t)r : 0u);
         yv[r] = *(const uint4 *)(y + route * H + d);
         w[r] = wts[route];
-        live[r] = ((uint32_t)r < k) & (ids[route] < E);
+        live[r] = ((uint32_t)r < k) & (ids[route] < E) & !(again >> r & 1u);
     }
     const uint64_t o = (uint64_t)t * H + d;
     const uint4 rv = residual ? *(const uint4 *)(residual + o) : make_uint4(0u, 0u, 0u, 0u);
@@ -328,10 +339,14 @@ __global__ __launch_bounds__(128) void combine_kernel(
 
 bool k3::launch_combine(void *output, const uint16_t *y, const void *residual, const uint32_t *ids,
                         const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E,
-                        hipStream_t st) {
-    hipLaunchKernelGGL(combine_kernel, dim3((H / 8u + kCombineThreads - 1u) / kCombineThreads, T),
-                       dim3(kCombineThreads), 0, st, (uint16_t *)output, y,
-                       (const uint16_t *)residual, ids, weights, H, k, E);
+                        bool once, hipStream_t st) {
+    const dim3 grid((H / 8u + kCombineThreads - 1u) / kCombineThreads, T);
+    if (once)
+        hipLaunchKernelGGL(combine_kernel<true>, grid, dim3(kCombineThreads), 0, st, (uint16_t *)output,
+                           y, (const uint16_t *)residual, ids, weights, H, k, E);
+    else
+        hipLaunchKernelGGL(combine_kernel<false>, grid, dim3(kCombineThreads), 0, st,
+                           (uint16_t *)output, y, (const uint16_t *)residual, ids, weights, H, k, E);
     return hipGetLastError() == hipSuccess;
 }
 
@@ -443,7 +458,7 @@ bool run_experts(const Workspace &ws, void *output, const void *hidden, const vo
             !launch_exact_down(g, ws.y, ws.act, st))
             return false;
         mark(K3_MOE_STAGE_COMBINE);
-        const bool ok = launch_combine(output, ws.y, residual, ws.ids, ws.weights, T, H, k, E, st);
+        const bool ok = launch_combine(output, ws.y, residual, ws.ids, ws.weights, T, H, k, E, false, st);
         mark(K3_MOE_STAGE_END);
         return ok;
     }
@@ -454,7 +469,7 @@ bool run_experts(const Workspace &ws, void *output, const void *hidden, const vo
     mark(K3_MOE_STAGE_DOWN);
     if (!launch_exact_down(g, ws.y, ws.act, st)) return false;
     mark(K3_MOE_STAGE_COMBINE);
-    const bool ok = launch_combine(output, ws.y, residual, ws.ids, ws.weights, T, H, k, E, st);
+    const bool ok = launch_combine(output, ws.y, residual, ws.ids, ws.weights, T, H, k, E, false, st);
     mark(K3_MOE_STAGE_END);
     return ok;
 }
