@@ -642,6 +642,14 @@ struct TileRun {
         for (int r = 0; r < 4; r++) acc[r] = fmaf(p[r], f, acc[r]);
     }
 
+    /*
+     * Step s of the loop, token subtile j: the reads of subtile j + 1, the wait
+     * for those of j, four products. Before the last subtile's products the
+     * stage's LDS has been read by this wave; behind a barrier there (all waves
+     * have, and stage s + 1 has landed for all) its products run over the reads
+     * of the next stage's first fragments, so that no step begins with an empty
+     * matrix unit.
+     */
     template <int TL, bool Two>
     __device__ __forceinline__ void run(f32x4 (&acc)[C::TI][4], uint8_t *smem) const {
         const uint32_t g = lane >> 4, c = lane & 15u;
@@ -651,6 +659,25 @@ struct TileRun {
         float w0 = 0.0f, w1 = 0.0f;
         f32x4 p[2][4]; /* the products of a subtile and of the one before, and their factors */
         float f[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+        u32x4_t af[4][2], bf[2][2];
+        uint32_t sx_[2];
+        uint32_t st = 0u, sb = s_at; /* the stage's place, its scales' */
+        auto read_a = [&](auto I) {
+            constexpr int i = decltype(I)::value;
+            af[i][0] = ds_read16<2048 * i>(a_at + st + lo);
+            af[i][1] = ds_read16<2048 * i>(a_at + st + hi);
+        };
+        auto read_b = [&](auto J) {
+            constexpr int j = decltype(J)::value;
+            sx_[j & 1] = ds_read4<512 * j>(sb);
+            bf[j & 1][0] = ds_read16<4096 * j>(b_at + st + lo);
+            bf[j & 1][1] = ds_read16<4096 * j>(b_at + st + hi);
+        };
+        auto barrier = [] {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
 #pragma unroll
         for (int i = 0; i < 4; i++) p[1][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -659,6 +686,11 @@ struct TileRun {
             fetch<0, C::D>(smem, (uint32_t)s, (uint32_t)s);
         }
         if constexpr (C::EARLY) fetch<0, C::DA>(smem, 1u, 1u);
+        /* stage 0: what was issued after it may stay out */
+        wait_vm<C::EARLY ? C::DA : C::D *(C::STAGES - 2)>();
+        barrier();
+        static_for<4>(read_a);
+        read_b(std::integral_constant<int, 0>{});
         uint32_t slot = 0u, next = C::STAGES - 1;
         for (uint32_t s = 0; s < nblk; s++) {
             if (s % 64u == 0u) { /* the weight scales of the next 64 blocks */
@@ -669,42 +701,23 @@ struct TileRun {
                  * ahead in every stage */
                 asm volatile("" : "+v"(w0), "+v"(w1));
             }
-            /* this wave's loads of stage s; later ones stay out */
-            wait_vm<C::EARLY ? C::DA : C::D *(C::STAGES - 2)>();
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_barrier(); /* everyone's; and stage s - 1 has been read */
-            asm volatile("" ::: "memory");
             const uint32_t ahead = s + C::STAGES - 1u, to = next;
             fetch_scales(smem, ahead);
-            const uint32_t st = C::STAGE * slot, sb = s_at + C::SBUF * ((s >> 2) & 1u) + 4u * (s & 3u);
+            if constexpr (TL == 1) fetch<0, C::D>(smem, ahead, to);
             next = slot;
             slot = slot + 1u == (uint32_t)C::STAGES ? 0u : slot + 1u;
             const float sw_0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w0), (int)(s & 63u)));
             const float sw_1 = Two ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w1), (int)(s & 63u))) : sw_0;
-            u32x4_t af[4][2], bf[2][2];
-            uint32_t sx_[2];
-            auto read_b = [&](auto J) {
-                constexpr int j = decltype(J)::value;
-                sx_[j & 1] = ds_read4<512 * j>(sb);
-                bf[j & 1][0] = ds_read16<4096 * j>(b_at + st + lo);
-                bf[j & 1][1] = ds_read16<4096 * j>(b_at + st + hi);
-            };
-            read_b(std::integral_constant<int, 0>{});
-            static_for<4>([&](auto I) {
-                constexpr int i = decltype(I)::value;
-                af[i][0] = ds_read16<2048 * i>(a_at + st + lo);
-                af[i][1] = ds_read16<2048 * i>(a_at + st + hi);
-            });
             static_for<TL>([&](auto J) {
                 constexpr int j = decltype(J)::value;
-                /* the next subtile's reads stay out; in the first one the weight
-                 * fragments are waited for one by one */
-                constexpr int out = j + 1 < TL ? 3 : 0;
-                if constexpr (j + 1 < TL) read_b(std::integral_constant<int, j + 1>{});
-                wait_lgkm<(j == 0 ? 6 : 0) + out>();
+                constexpr bool last = j + 1 == TL;
+                if constexpr (!last) read_b(std::integral_constant<int, j + 1>{});
+                wait_lgkm<last ? 0 : 3>(); /* the next subtile's reads stay out */
                 if constexpr (j == 0) {
-                    after_wait(af[0][0]);
-                    after_wait(af[0][1]);
+                    static_for<4>([&](auto I) {
+                        after_wait(af[decltype(I)::value][0]);
+                        after_wait(af[decltype(I)::value][1]);
+                    });
                 }
                 after_wait(sx_[j & 1]);
                 after_wait(bf[j & 1][0]);
@@ -712,34 +725,34 @@ struct TileRun {
                 const float sx = __uint_as_float(sx_[j & 1]);
                 f[j & 1][0] = __fmul_rn(sx, sw_0);
                 f[j & 1][1] = Two ? __fmul_rn(sx, sw_1) : f[j & 1][0];
+                if constexpr (last) {
+                    /* this wave's loads of stage s + 1; later ones stay out */
+                    wait_vm<C::EARLY ? C::DA : C::D *(C::STAGES - 2)>();
+                    barrier();
+                    st = C::STAGE * slot;
+                    sb = s_at + C::SBUF * (((s + 1u) >> 2) & 1u) + 4u * ((s + 1u) & 3u);
+                }
                 /* a product, then the four fmas of the subtile before: they run
                  * while the matrix unit is busy */
                 constexpr int q = (j + TL - 1) % TL;
                 static_for<4>([&](auto I) {
                     constexpr int i = decltype(I)::value;
-                    if constexpr (j == 0 && i > 0) {
-                        wait_lgkm<6 - 2 * i + out>();
-                        after_wait(af[i][0]);
-                        after_wait(af[i][1]);
-                    }
                     p[j & 1][i] = mfma_block(af[i][0], af[i][1], bf[j & 1][0], bf[j & 1][1]);
+                    if constexpr (last) read_a(I);
                     scale_in(acc[q][i], p[(j + 1) & 1][i], f[(j + 1) & 1][i >> 1]);
                     __builtin_amdgcn_sched_barrier(0);
-                    /* the loads ahead, spread over the products: at once they
-                     * would keep the waves from their first reads */
+                    /* the loads ahead, spread over the products before the last
+                     * subtile's: at once they would keep the waves from their reads */
                     constexpr int half = 4 * ((TL + 1) / 2), at = 4 * j + i;
-                    if constexpr (C::EARLY) {
-                        if constexpr (at == half - 1) {
-                            asm volatile("" ::: "memory");
-                            __builtin_amdgcn_s_barrier();
-                            asm volatile("" ::: "memory");
-                        }
+                    if constexpr (TL == 1) {
+                    } else if constexpr (C::EARLY) {
+                        if constexpr (at == half - 1) barrier();
                         static_for<C::DB>([&](auto Q) {
                             if constexpr (decltype(Q)::value * (half - 1) / C::DB == at)
                                 fetch_one<C::DA + decltype(Q)::value>(smem, ahead, to);
                         });
                         static_for<C::DA>([&](auto Q) {
-                            if constexpr (half - 1 + decltype(Q)::value * (4 * TL - half) / C::DA == at)
+                            if constexpr (half - 1 + decltype(Q)::value * (4 * (TL - 1) - half) / C::DA == at)
                                 fetch_one<decltype(Q)::value>(smem, s + 2u, to ^ 1u);
                         });
                     } else {
@@ -749,6 +762,7 @@ struct TileRun {
                         });
                     }
                 });
+                if constexpr (last) read_b(std::integral_constant<int, 0>{});
             });
             if constexpr (TL % 2 != 0) { /* the next stage's first subtile has the same parity */
 #pragma unroll
@@ -756,6 +770,14 @@ struct TileRun {
                 f[1][0] = f[0][0], f[1][1] = f[0][1];
             }
         }
+        wait_lgkm<0>(); /* the reads past the end: their registers stay taken till here */
+        static_for<4>([&](auto I) {
+            after_wait(af[decltype(I)::value][0]);
+            after_wait(af[decltype(I)::value][1]);
+        });
+        after_wait(sx_[0]);
+        after_wait(bf[0][0]);
+        after_wait(bf[0][1]);
 #pragma unroll
         for (int i = 0; i < 4; i++) scale_in(acc[TL - 1][i], p[1][i], f[1][i >> 1]);
         wait_vm<0>(); /* the loads past the end land before the LDS is used again */
