@@ -292,7 +292,7 @@ struct TokenPart {
     uint4 v[2];
     __device__ __forceinline__ void load(const uint16_t *x, uint32_t n) {
 #pragma unroll
-        for (uint32_t i = 0; i < 2u; i++)
+        for (uint32_t i = 0; i < 2u; i++) /* past the end the last ones again */
             v[i] = ((const uint4 *)x)[min(threadIdx.x + 512u * i, 16u * n - 1u)];
     }
     __device__ __forceinline__ void encode(uint32_t n, uint32_t codes, uint32_t scales) const {
@@ -314,27 +314,39 @@ struct OneArgs {
     const uint8_t *codes;
     const float *scales;
     const uint16_t *x;
-    uint32_t N, K;
+    uint32_t T, N, K;
 };
 
 /*
- * One token times a weight, 16 rows a block: its eight waves take every eighth
- * block of columns and add up through LDS in one order. The token is encoded
- * 64 blocks of columns at a time, by the block, under the first weight loads.
+ * T <= NT tokens times a weight, 16 rows a block: its eight waves take every
+ * eighth block of columns and add up through LDS in one order. The tokens are
+ * encoded 64 blocks of columns at a time, by the block, under the first weight
+ * loads; column c of the products is token min(c, NT - 1). Each block encodes the
+ * tokens anew, which costs more the more blocks and tokens there are. us, here
+ * and by tiles with a launch for the codes and one for the parts of K: 2048 x
+ * 7168, 1 token 5.7 and 12.4, 4 tokens 7.4 and 12.4, 8 tokens 9.8 and 12.4; 7168
+ * x 7168 12.7, 17.5, 22.6 and 20.3 (one token's weights at 4.1 TB/s and, of 2048
+ * rows, 2.6: the first loads' latency is half of it).
  */
 constexpr int kOneRing = 4;
+constexpr uint32_t kOneTokens = 8;
+inline bool one_launch(uint32_t T, uint32_t N) { return T <= 4u || (T <= kOneTokens && N <= 4096u); }
+template <uint32_t NT>
 __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
     using Ring = WaveRing<1, kOneRing>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * Ring::BYTES + 64u * (kBlock + 4u)];
-    __shared__ float sums[8][16];
+    constexpr uint32_t TOKEN = 64u * (kBlock + 4u); /* codes, then scales */
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * Ring::BYTES + NT * TOKEN];
+    __shared__ float sums[8][NT][16];
     const uint32_t lane = threadIdx.x & 63u, nblk = P.K / kBlock, n0 = 16u * blockIdx.x;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t codes = lds_addr(smem) + 8u * Ring::BYTES, scales = codes + 64u * kBlock;
+    const uint32_t c = lane & 15u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t codes = lds_addr(smem) + 8u * Ring::BYTES;
+    const uint32_t mine = codes + TOKEN * min(c, NT - 1u);
     const float *ws = P.scales + (uint64_t)(n0 / kBlock) * nblk;
     /* lane q: the scale of the wave's q-th block of 64 */
     float sw = ws[min(wave + 8u * (lane & 7u), nblk - 1u)];
-    TokenPart x;
-    x.load(P.x, min(64u, nblk));
+    TokenPart x[NT];
+#pragma unroll
+    for (uint32_t t = 0; t < NT; t++) x[t].load(P.x + (uint64_t)min(t, P.T - 1u) * P.K, min(64u, nblk));
     asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
     Ring ring;
     const uint8_t *const w[1] = {P.codes + (uint64_t)n0 * P.K};
@@ -347,16 +359,19 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
         const uint32_t n = min(64u, nblk - base);
         if (base != 0u) {
             sw = ws[min(base + wave + 8u * (lane & 7u), nblk - 1u)];
-            x.load(P.x + kBlock * base, n);
+#pragma unroll
+            for (uint32_t t = 0; t < NT; t++)
+                x[t].load(P.x + (uint64_t)min(t, P.T - 1u) * P.K + kBlock * base, n);
             lds_barrier(); /* the codes before have been read */
         }
-        x.encode(n, codes, scales);
+#pragma unroll
+        for (uint32_t t = 0; t < NT; t++) x[t].encode(n, codes + TOKEN * t, codes + TOKEN * t + 64u * kBlock);
         asm volatile("" : "+v"(sw)); /* waited for here, not in the loop */
         lds_barrier();
         for (uint32_t k = wave, q = 0; k < n; k += 8u, q++) {
             f32x4 p[1];
-            uint32_t sx = ds_read4<0>(scales + 4u * k);
-            ring.products(p, slot, codes + kBlock * k); /* waits for sx too */
+            uint32_t sx = ds_read4<64 * kBlock>(mine + 4u * k);
+            ring.products(p, slot, mine + kBlock * k); /* waits for sx too */
             after_wait(sx);
             const float f = __fmul_rn(__uint_as_float(sx), scale_at(sw, q));
 #pragma unroll
@@ -366,15 +381,16 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
         }
     }
     wait_vm<0>();
-    if ((lane & 15u) == 0u)
+    if (c < NT)
 #pragma unroll
-        for (uint32_t r = 0; r < 4u; r++) sums[wave][(lane >> 2) + r] = acc[r];
+        for (uint32_t r = 0; r < 4u; r++) sums[wave][c][4u * (lane >> 4) + r] = acc[r];
     __syncthreads();
-    if (threadIdx.x < 16u && n0 + threadIdx.x < P.N) {
+    const uint32_t t = threadIdx.x >> 4, n = n0 + (threadIdx.x & 15u);
+    if (t < NT && t < P.T && n < P.N) {
         float v = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 8; u++) v = __fadd_rn(v, sums[u][threadIdx.x]);
-        P.out[n0 + threadIdx.x] = f32_to_bf16(v);
+        for (int u = 0; u < 8; u++) v = __fadd_rn(v, sums[u][t][threadIdx.x & 15u]);
+        P.out[(uint64_t)t * P.N + n] = f32_to_bf16(v);
     }
 }
 
@@ -1184,35 +1200,51 @@ using Half32 = Tile<2, 1, 3>;
 using Half64 = Tile<2, 2, 3>;
 using Half128 = Tile<2, 4, 2>;
 
-/* How a product of T > 1 tokens is cut. */
+/* How a product of more tokens is cut: its tile, and K in `splits` parts of `span`
+ * blocks. */
 struct Cut {
-    int tile; /* 0 .. 3: Half32, Half64, Half128, Tile256 */
+    int tile; /* 0 .. 4: Half32, Half64, Half128, Tile128, Tile256 */
     uint32_t tiles_t, tiles_n, splits, span;
     size_t part_bytes;
 };
 
-template <class C>
-void cut_as(Cut &q, uint32_t T, uint32_t N, uint32_t K) {
-    const uint32_t groups = (K / kBlock + 3u) / 4u;
-    q.tiles_t = (T + C::BT - 1u) / C::BT, q.tiles_n = (N + C::BN - 1u) / C::BN;
-    const uint64_t tiles = (uint64_t)q.tiles_t * q.tiles_n;
-    uint32_t want = tiles >= 256u ? 1u : (uint32_t)(256u / tiles);
-    want = want < groups ? want : groups;
-    q.span = 4u * ((groups + want - 1u) / want);
-    q.splits = (4u * groups + q.span - 1u) / q.span;
-    q.part_bytes = q.splits > 1u ? align256((size_t)q.splits * tiles * C::BT * C::BN * 4u) : 0u;
-}
+/*
+ * The cheapest of all cuts, by what tiles cost on the part: nanoseconds of a
+ * stage (128 columns) of a block that has a CU to itself, and a block's share
+ * with several (tiles of 128 rows lie two a CU); a part of K in memory at 5
+ * TB/s, written and read, and 3 us for the launch that adds them. (us, 2048 x
+ * 7168, the tiles of 128 x 64, 128 x 128, 256 x 128 and 256 x 256: 512 tokens 25.1,
+ * 26.5, 26.3, 34.3; 1024 tokens 35.2, 37.9, 39.4, 43.6; 4096 tokens 103, 85, 82, 94;
+ * 7168 x 7168: 300 tokens 44.9, 45.9, 39.6, 46.4; 4096 tokens 301, 245, 254, 214.)
+ */
+struct TileCost {
+    uint32_t bn, bt, alone, shared;
+};
+constexpr TileCost kTileCost[5] = {{128, 32, 420, 340}, {128, 64, 490, 390}, {128, 128, 750, 590},
+                                   {256, 128, 1160, 1060}, {256, 256, 1900, 1800}};
 
 Cut cut_of(uint32_t T, uint32_t N, uint32_t K) {
-    Cut q{};
-    q.tile = T <= 32u ? 0 : T <= 64u ? 1 : T <= 512u ? 2 : 3;
-    switch (q.tile) {
-    case 0: cut_as<Half32>(q, T, N, K); break;
-    case 1: cut_as<Half64>(q, T, N, K); break;
-    case 2: cut_as<Half128>(q, T, N, K); break;
-    default: cut_as<Tile256>(q, T, N, K);
+    const uint32_t groups = (K / kBlock + 3u) / 4u;
+    Cut best{};
+    uint64_t least = ~0ull;
+    for (int i = 0; i < 5; i++) {
+        const TileCost &c = kTileCost[i];
+        const uint32_t tt = (T + c.bt - 1u) / c.bt, tn = (N + c.bn - 1u) / c.bn;
+        const uint64_t tiles = (uint64_t)tt * tn, padded = tiles * c.bt * c.bn;
+        for (uint32_t want = 1u; want <= groups && want <= 16u && (want == 1u || tiles * want <= 768u); want++) {
+            const uint32_t span = 4u * ((groups + want - 1u) / want);
+            const uint32_t splits = (4u * groups + span - 1u) / span;
+            if (splits != want) continue; /* the same cut as a smaller number's */
+            const uint64_t each = (tiles * splits + 255u) / 256u;
+            uint64_t ns = each * span * (each == 1u ? c.alone : c.shared);
+            if (splits > 1u) ns += 3000u + padded * splits * 8u / 5000u;
+            if (ns < least) {
+                least = ns;
+                best = Cut{i, tt, tn, splits, span, splits > 1u ? align256(padded * splits * 4u) : 0u};
+            }
+        }
     }
-    return q;
+    return best;
 }
 
 template <class C>
@@ -1282,7 +1314,7 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
 }  // namespace
 
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
-    if (T == 1u) return 0u; /* encoded by the product's own kernel */
+    if (one_launch(T, rows)) return 0u; /* encoded by the product's own kernel */
     return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols)) +
            cut_of(T, rows, cols).part_bytes;
 }
@@ -1336,9 +1368,18 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
         return false;
     const hipStream_t st = (hipStream_t)stream;
     const bool wide = rows % 4u == 0u && ((uintptr_t)output % 8u) == 0u;
-    if (vector_count == 1u) {
-        const OneArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, rows, columns};
-        hipLaunchKernelGGL(product_one_kernel, dim3((rows + 15u) / 16u), dim3(512), 0, st, A);
+    if (one_launch(vector_count, rows)) {
+        const OneArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, vector_count, rows,
+                        columns};
+        const dim3 grid((rows + 15u) / 16u);
+        if (vector_count == 1u)
+            hipLaunchKernelGGL(product_one_kernel<1u>, grid, dim3(512), 0, st, A);
+        else if (vector_count == 2u)
+            hipLaunchKernelGGL(product_one_kernel<2u>, grid, dim3(512), 0, st, A);
+        else if (vector_count <= 4u)
+            hipLaunchKernelGGL(product_one_kernel<4u>, grid, dim3(512), 0, st, A);
+        else
+            hipLaunchKernelGGL(product_one_kernel<8u>, grid, dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
     TileArgs B{};
@@ -1354,6 +1395,7 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
     case 0: return launch_dense<Half32>(B, q, st);
     case 1: return launch_dense<Half64>(B, q, st);
     case 2: return launch_dense<Half128>(B, q, st);
+    case 3: return launch_dense<Tile128>(B, q, st);
     default: return launch_dense<Tile256>(B, q, st);
     }
 }
