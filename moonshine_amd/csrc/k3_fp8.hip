@@ -560,6 +560,15 @@ __device__ __forceinline__ uint32_t tile_height(uint32_t n) {
     return n > 128u ? 32u * ((steps + many - 1u) / many) : n;
 }
 
+/* Tile classes by an expert's rows: up to 32, 64 and 128 (one tile), more (tiles
+ * of up to 256, of equal length in 32-row steps). */
+constexpr int kClasses = 4;
+
+struct TileLists {
+    ExpertTile *tiles[kClasses];
+    uint32_t *count; /* [kClasses] */
+};
+
 /* ---------------------------------------------------------------------- */
 /* tiles of many tokens                                                    */
 /* ---------------------------------------------------------------------- */
@@ -603,8 +612,8 @@ struct TileArgs {
     /* dense: the weight; otherwise the experts and the tiles */
     const uint8_t *codes;
     const float *scales;
-    const ExpertTile *tiles;
-    const uint32_t *tile_count, *token_index, *route_index;
+    TileLists lists;
+    const uint32_t *token_index, *route_index;
     const uint8_t *xq; /* token rows, K wide */
     const float *xs;   /* their scales, rows xstride apart */
     uint32_t xstride;
@@ -800,21 +809,26 @@ struct TileRun {
     }
 };
 
+/* Work L of `works` (blocks L, L + 8, ... lie on one XCD): XCD x takes a
+ * contiguous range of them. Returns false past the end. */
+__device__ __forceinline__ bool xcd_work(uint32_t L, uint32_t works, uint32_t &w) {
+    const uint32_t per = (works + 7u) / 8u, j8 = L >> 3;
+    w = (L & 7u) * per + j8;
+    return j8 < per && w < works;
+}
+
+/* Block L of the `tiles` row tiles (list: the experts') x P.tiles_n column blocks. */
 template <class C, int MODE>
-__global__ __launch_bounds__(C::THREADS, 2) void tile_kernel(TileArgs P) {
+__device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uint32_t L8, uint32_t tiles,
+                                           const ExpertTile *list) {
     static_assert(MODE != kGateUp || C::WN == 4, "a gate/up block holds whole scale blocks");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
     TileRun<C> R;
     R.lane = threadIdx.x & 63u;
     R.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     R.wn = R.wave % C::WN, R.wt = R.wave / C::WN;
     const uint32_t L = R.lane, K = P.K, nblk = K / kBlock;
-    /* XCD x (blocks x, x + 8, ...) takes a contiguous range of the works */
-    const uint32_t tiles = MODE == kDense ? P.tiles_t : *P.tile_count;
-    const uint32_t works = tiles * P.tiles_n * (MODE == kDense ? P.splits : 1u);
-    const uint32_t per = (works + 7u) / 8u, j8 = blockIdx.x >> 3;
-    uint32_t w = (blockIdx.x & 7u) * per + j8;
-    if (j8 >= per || w >= works) return;
+    uint32_t w;
+    if (!xcd_work(L8, tiles * P.tiles_n * (MODE == kDense ? P.splits : 1u), w)) return;
     const uint32_t split = MODE == kDense ? w % P.splits : 0u; /* a part of K */
     if constexpr (MODE == kDense) w /= P.splits;
     uint32_t row0, rows, col;
@@ -829,7 +843,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void tile_kernel(TileArgs P) {
     } else {
         /* an expert's tiles of one column block are neighbours: they read the
          * same weights at about the same time, through the same L2 */
-        const ExpertTile &t = P.tiles[w / P.tiles_n];
+        const ExpertTile &t = list[w / P.tiles_n];
         const uint32_t local = t.index * P.tiles_n + w % P.tiles_n, height = tile_height(t.n);
         const uint32_t q = local % t.many;
         col = local / t.many;
@@ -982,11 +996,47 @@ __global__ __launch_bounds__(C::THREADS, 2) void tile_kernel(TileArgs P) {
     }
 }
 
-template <class C, int MODE>
-bool launch_tile(const TileArgs &A, uint32_t works, hipStream_t st) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<C, MODE>), dim3(8u * ((works + 7u) / 8u)),
-                       dim3(C::THREADS), 0, st, A);
-    return hipGetLastError() == hipSuccess;
+template <class C>
+__global__ __launch_bounds__(C::THREADS, 2) void product_tile_kernel(TileArgs P) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
+    tile_block<C, kDense>(P, smem, blockIdx.x, P.tiles_t, nullptr);
+}
+
+using Tile32 = Tile<4, 1, 4>;
+using Tile64 = Tile<4, 2, 3>;
+using Tile128 = Tile<4, 4, 3>;
+using Tile256 = Tile<4, 8, 2>;
+/* half as many rows: few tokens' products */
+using Half32 = Tile<2, 1, 3>;
+using Half64 = Tile<2, 2, 3>;
+using Half128 = Tile<2, 4, 2>;
+
+/* All tiles of the experts' gate/up, or down, in one launch: the classes one
+ * behind the other, the largest tiles first, each on whole groups of eight
+ * blocks. A CU holds one block of any class, so the largest's registers and LDS
+ * cost the others nothing (a launch for each class took 3 to 5 us where it had no
+ * tile). */
+template <int MODE>
+__global__ __launch_bounds__(512, 2) void experts_tile_kernel(TileArgs P) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[Tile128::LDS];
+    static_assert(Tile128::LDS >= Tile256::LDS && Tile128::LDS >= Tile64::LDS &&
+                  Tile128::LDS >= Tile32::LDS, "LDS of every class");
+    const uint4 count = *(const uint4 *)P.lists.count;
+    const uint32_t n[kClasses] = {count.x, count.y, count.z, count.w};
+    uint32_t b = blockIdx.x, cls = kClasses;
+#pragma unroll
+    for (int q = kClasses - 1; q >= 0; q--) {
+        const uint32_t blocks = 8u * ((n[q] * P.tiles_n + 7u) / 8u);
+        if (cls != (uint32_t)kClasses) continue;
+        if (b < blocks) cls = (uint32_t)q;
+        else b -= blocks;
+    }
+    switch (cls) {
+    case 0: tile_block<Tile32, MODE>(P, smem, b, n[0], P.lists.tiles[0]); break;
+    case 1: tile_block<Tile64, MODE>(P, smem, b, n[1], P.lists.tiles[1]); break;
+    case 2: tile_block<Tile128, MODE>(P, smem, b, n[2], P.lists.tiles[2]); break;
+    case 3: tile_block<Tile256, MODE>(P, smem, b, n[3], P.lists.tiles[3]); break;
+    }
 }
 
 /* Output of a product whose K was split: the parts in their order. A block adds
@@ -1015,15 +1065,6 @@ __global__ __launch_bounds__(C::THREADS) void join_kernel(TileArgs P) {
 /* ---------------------------------------------------------------------- */
 /* routes and tiles of the experts                                         */
 /* ---------------------------------------------------------------------- */
-
-/* Tile classes by an expert's rows: up to 32, 64 and 128 (one tile), more (tiles
- * of up to 256, of equal length in 32-row steps). */
-constexpr int kClasses = 4;
-
-struct TileLists {
-    ExpertTile *tiles[kClasses];
-    uint32_t *count; /* [kClasses] */
-};
 
 /* By a block of 1024 threads, thread e with expert e's rows [row, row + n): each
  * class's tiles in expert order. */
@@ -1125,7 +1166,7 @@ struct Fp8Workspace {
     void *plan;
     size_t plan_bytes;
     TileLists lists;
-    uint32_t cap[kClasses]; /* most tiles of a class; 0: no expert can be of it */
+    uint32_t tile_cap; /* most tiles of all classes */
     uint8_t *xq, *hq;
     float *xs, *hs;
     uint16_t *y;
@@ -1153,13 +1194,15 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
     w.route_index = (uint32_t *)take(4u * routes);
     w.plan_bytes = k3_moe_plan_scratch_bytes(T, s.expert_count);
     w.plan = take(w.plan_bytes);
-    /* an expert has a token's route at most once: T rows at most */
+    /* an expert has a token's route at most once: T rows at most; n rows are
+     * cut into at most 1 + n / 256 tiles, of the last class into at most n / 128 */
     static constexpr size_t least[kClasses] = {1u, 33u, 65u, 128u};
+    const size_t used = E < routes ? E : routes;
     for (int q = 0; q < kClasses; q++) {
-        const size_t n = routes / least[q];
-        w.cap[q] = T < least[q] ? 0u : (uint32_t)(q < 3 && n > E ? E : n);
-        w.lists.tiles[q] = (ExpertTile *)take(sizeof(ExpertTile) * (size_t)w.cap[q]);
+        const size_t n = T < least[q] ? 0u : routes / least[q];
+        w.lists.tiles[q] = (ExpertTile *)take(sizeof(ExpertTile) * (q < 3 && n > E ? E : n));
     }
+    w.tile_cap = (uint32_t)(used + routes / 256u);
     w.lists.count = (uint32_t *)take(4u * kClasses);
     w.xq = take((size_t)T * s.hidden);
     w.xs = (float *)take(4u * (size_t)T * scale_stride(s.hidden));
@@ -1190,15 +1233,6 @@ bool launch_rows(uint8_t *codes, float *scales, const void *src, uint32_t rows, 
                        st, codes, scales, (const uint16_t *)src, blocks, nblk, stride);
     return hipGetLastError() == hipSuccess;
 }
-
-using Tile32 = Tile<4, 1, 4>;
-using Tile64 = Tile<4, 2, 3>;
-using Tile128 = Tile<4, 4, 3>;
-using Tile256 = Tile<4, 8, 2>;
-/* half as many rows: few tokens' products */
-using Half32 = Tile<2, 1, 3>;
-using Half64 = Tile<2, 2, 3>;
-using Half128 = Tile<2, 4, 2>;
 
 /* How a product of more tokens is cut: its tile, and K in `splits` parts of `span`
  * blocks. */
@@ -1251,23 +1285,12 @@ template <class C>
 bool launch_dense(TileArgs A, const Cut &q, hipStream_t st) {
     A.tiles_t = q.tiles_t, A.tiles_n = q.tiles_n, A.splits = q.splits, A.span = q.span;
     const uint32_t tiles = q.tiles_t * q.tiles_n;
-    if (!launch_tile<C, kDense>(A, tiles * q.splits, st)) return false;
-    if (q.splits == 1u) return true;
+    hipLaunchKernelGGL(product_tile_kernel<C>, dim3(8u * ((tiles * q.splits + 7u) / 8u)),
+                       dim3(C::THREADS), 0, st, A);
+    if (q.splits == 1u) return hipGetLastError() == hipSuccess;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(join_kernel<C>), dim3(tiles * 4u * C::TI), dim3(C::THREADS), 0,
                        st, A);
     return hipGetLastError() == hipSuccess;
-}
-
-/* Gate/up and down of one class of tiles. */
-template <class C>
-bool launch_class(TileArgs A, const Fp8Workspace &ws, int cls, const k3_moe_shape &s, hipStream_t st) {
-    if (ws.cap[cls] == 0u) return true;
-    A.tiles = ws.lists.tiles[cls], A.tile_count = ws.lists.count + cls;
-    A.N = s.ffn, A.K = s.hidden, A.tiles_n = s.ffn / kBlock;
-    if (!launch_tile<C, kGateUp>(A, ws.cap[cls] * A.tiles_n, st)) return false;
-    A.xq = ws.hq, A.xs = ws.hs, A.xstride = scale_stride(s.ffn);
-    A.N = s.hidden, A.K = s.ffn, A.tiles_n = (s.hidden + C::BN - 1u) / C::BN;
-    return launch_tile<C, kDown>(A, ws.cap[cls] * A.tiles_n, st);
 }
 
 /* The expert stage on given routes. */
@@ -1302,12 +1325,19 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
                            experts, E);
     }
     TileArgs B{};
-    B.token_index = ws.token_index, B.route_index = ws.route_index;
+    B.lists = ws.lists, B.token_index = ws.token_index, B.route_index = ws.route_index;
     B.xq = ws.xq, B.xs = ws.xs, B.xstride = scale_stride(H);
     B.out = ws.y, B.hq = ws.hq, B.hs = ws.hs, B.hstride = scale_stride(F);
     B.kind = s.activation, B.beta = s.beta, B.lb = s.linear_beta;
-    return hipGetLastError() == hipSuccess && launch_class<Tile32>(B, ws, 0, s, st) && launch_class<Tile64>(B, ws, 1, s, st) &&
-           launch_class<Tile128>(B, ws, 2, s, st) && launch_class<Tile256>(B, ws, 3, s, st) &&
+    B.N = F, B.K = H, B.tiles_n = F / kBlock;
+    /* the classes' blocks are rounded up to eights */
+    hipLaunchKernelGGL(experts_tile_kernel<kGateUp>, dim3(ws.tile_cap * B.tiles_n + 8u * kClasses),
+                       dim3(512), 0, st, B);
+    B.xq = ws.hq, B.xs = ws.hs, B.xstride = scale_stride(F);
+    B.N = H, B.K = F, B.tiles_n = (H + 255u) / 256u;
+    hipLaunchKernelGGL(experts_tile_kernel<kDown>, dim3(ws.tile_cap * B.tiles_n + 8u * kClasses),
+                       dim3(512), 0, st, B);
+    return hipGetLastError() == hipSuccess &&
            launch_combine(output, ws.y, residual, ids, wts, T, H, k, E, true, st);
 }
 

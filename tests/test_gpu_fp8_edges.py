@@ -1,0 +1,150 @@
+"""FP8-128 products and experts on the GPU where one kernel hands over to the next:
+few tokens in one launch or in tiles, K in one part or several, an expert's rows at
+its tiles' heights, a plan in one launch or several, the widest and longest calls.
+Bounds as in tests/_fp8.py."""
+import pytest
+import torch
+
+import _fp8 as R
+from moonshine_amd import fp8
+from moonshine_amd.synth import ACT_SITU, ACT_SWIGLU
+from test_gpu_fp8 import check_experts, check_product, make_store, normal
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- product -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("T", [2, 3, 4, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize("rows,cols", [(16, 384), (4096, 256), (4100, 896), (33, 8320)])
+def test_product_of_few_tokens(cuda, T, rows, cols):
+    check_product(cuda, T, rows, cols, 7 * T + rows)
+
+
+# K whole and in 2 to 16 parts, the last one shorter; every height of tile
+@pytest.mark.parametrize("T,rows,cols", [
+    (9, 130, 16384), (20, 257, 7296), (33, 1030, 2176), (37, 4100, 4224), (70, 129, 8192), (97, 2050, 1664),
+    (129, 513, 4736), (140, 5000, 640), (260, 300, 6272), (300, 4100, 2176), (515, 1030, 1152),
+    (1030, 1300, 2176), (2050, 1030, 384), (65535, 130, 128)])
+def test_product_cuts(cuda, T, rows, cols):
+    check_product(cuda, T, rows, cols, T + 3 * rows + cols)
+
+
+def test_product_of_many_parts_in_graphs(cuda):
+    """Two graphs whose products cut K, replayed in turn with eager calls between."""
+    wq, ws = fp8.quantize_weight(normal((1100, 7168), 3, 0.02).to(cuda))
+    xs = [normal((T, 7168), T).to(cuda) for T in (37, 150)]
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(fp8.product(x, wq, ws))
+        graphs.append(g)
+    for n in range(4):
+        new = [normal(x.shape, 40 + n).to(cuda) for x in xs]
+        for x, v, g in zip(xs, new, graphs):
+            x.copy_(v)
+            g.replay()
+        want = [fp8.product(v, wq, ws) for v in new]
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    store = make_store(cuda, 16, 512, 256, 8)
+    sh = fp8.shape(512, 16, 4, 256, 1.0, ACT_SWIGLU)
+    wq, ws = fp8.quantize_weight(normal((700, 512), 3, 0.02).to(cuda))
+    g = torch.Generator().manual_seed(3)
+    sets = []
+    for T in (1, 6, 60, 300):
+        x = normal((T, 512), T).to(cuda)
+        ids = torch.stack([torch.randperm(16, generator=g)[:4] for _ in range(T)]).to(torch.int32).to(cuda)
+        sets.append((x, ids, torch.rand((T, 4), generator=g).to(cuda)))
+
+    def run(x, ids, w):
+        return fp8.product(x, wq, ws), fp8.experts(x, ids, w, store.table, sh)
+
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] += [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    for lane in got:
+        for n, pair in enumerate(lane):
+            for a, b in zip(pair, want[n % len(sets)]):
+                assert torch.equal(a, b)
+
+
+# ---- experts -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("T", [255, 256, 257, 300])
+@pytest.mark.parametrize("E,k", [(6, 4), (64, 8), (40, 32), (1024, 3)])
+def test_experts_plan(cuda, T, E, k):
+    """Any ids: valid ones, repeats and ids of no expert."""
+    store = make_store(cuda, E, 128, 128, 4)
+    ids = torch.randint(-1, E + 1, (T, k), generator=torch.Generator().manual_seed(T + E),
+                        dtype=torch.int32)
+    ids[3] = E
+    check_experts(cuda, store, T, k, ACT_SWIGLU, T, ids=ids)
+
+
+@pytest.mark.parametrize("rows", [31, 95, 96, 255, 256, 257, 288, 384, 385, 511, 512, 513, 700, 1025])
+def test_experts_tile_heights(cuda, rows):
+    """`rows` tokens at expert 1, a third and a tenth of them at experts 0 and 3."""
+    store = make_store(cuda, 5, 256, 384, 3)
+    ids = torch.full((rows, 3), 1, dtype=torch.int32)
+    ids[:, 1:] = -5
+    ids[: rows // 3, 1] = 0
+    ids[rows - rows // 10:, 2] = 3
+    check_experts(cuda, store, rows, 3, ACT_SITU, rows, ids=ids)
+
+
+@pytest.mark.parametrize("H,F", [(8192, 256), (8320, 256), (256, 2048), (256, 2176), (256, 4096), (256, 4224),
+                                 (384, 128), (128, 640)])
+@pytest.mark.parametrize("T", [1, 3])
+def test_experts_widths(cuda, H, F, T):
+    check_experts(cuda, make_store(cuda, 3, H, F, 9), T, 2, ACT_SWIGLU, H + F)
+
+
+@pytest.mark.parametrize("H,F", [(512, 256), (1152, 640)])
+def test_experts_bits_do_not_depend_on_the_batch(cuda, H, F):
+    """A token alone, in a small and in a large batch."""
+    E, k, T = 12, 4, 400
+    store = make_store(cuda, E, H, F, 8)
+    g = torch.Generator().manual_seed(5)
+    x, r = normal((T, H), 4).to(cuda), normal((T, H), 5).to(cuda)
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).to(torch.int32).to(cuda)
+    w = torch.rand((T, k), generator=g).to(cuda)
+    sh = fp8.shape(H, E, k, F, 1.0, ACT_SITU)
+    want = fp8.experts(x, ids, w, store.table, sh, r)
+    for n in (1, 2, 30, 100, 256):
+        got = fp8.experts(x[:n].contiguous(), ids[:n].contiguous(), w[:n].contiguous(), store.table, sh,
+                          r[:n].contiguous())
+        assert torch.equal(got, want[:n]), n
+    for t in (7, 399):
+        got = fp8.experts(x[t:t + 1], ids[t:t + 1], w[t:t + 1], store.table, sh, r[t:t + 1])
+        assert torch.equal(got[0], want[t])
+
+
+def test_experts_of_the_most_tokens(cuda):
+    """65535 tokens: a sample of them against the same tokens in a small batch."""
+    E, H, F, k, T = 8, 128, 128, 2, 65535
+    store = make_store(cuda, E, H, F, 8)
+    g = torch.Generator().manual_seed(6)
+    x = normal((T, H), 4).to(cuda)
+    ids = torch.randint(0, E + 1, (T, k), generator=g, dtype=torch.int32).to(cuda)
+    w = torch.rand((T, k), generator=g).to(cuda)
+    sh = fp8.shape(H, E, k, F, 1.0, ACT_SWIGLU)
+    out = fp8.experts(x, ids, w, store.table, sh)
+    some = torch.cat([torch.arange(0, T, 331), torch.tensor([T - 2, T - 1])]).to(cuda)
+    got = fp8.experts(x[some], ids[some], w[some], store.table, sh)
+    assert torch.equal(got, out[some])
+    a = some[:40].cpu()
+    check_experts(cuda, store, 40, k, ACT_SWIGLU, 7, ids=ids.cpu()[a])
