@@ -416,9 +416,10 @@ bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const vo
  * with qx, sx the encoding of input[t] in blocks of 128 (as
  * k3_moe_fp8_128_quantize_rows_bf16 gives it). Code products and their sum
  * over a block run on FP8 MFMA, the scaled blocks add up in fp32; the order of
- * the blocks depends on the call's sizes only. columns % 128 == 0, columns <=
- * 2^24; input and codes 16-byte, scales 4-byte, output 2-byte aligned (8-byte stores where the
- * output and rows allow them); vector_count <= 65535. scratch (256-byte
+ * the blocks depends on the call's sizes only. columns % 128 == 0; rows and
+ * columns <= 2^24; input and codes 16-byte, scales 4-byte, output 2-byte
+ * aligned (wider stores where the output and rows allow them); vector_count <=
+ * 65535. scratch (256-byte
  * aligned device memory): k3_moe_fp8_128_scratch_bytes(vector_count, rows,
  * columns) bytes, 0 where none is needed (scratch may then be NULL).
  */

@@ -38,7 +38,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kBlock = 128;                /* values of a block */
 /* A tile's 256 rows, and a batch's 65535, are addressed by 32 bits. */
-constexpr uint32_t kMostColumns = 1u << 24, kMostWidth = 1u << 16;
+constexpr uint32_t kMostAxis = 1u << 24, kMostWidth = 1u << 16;
 constexpr float kTop = 448.0f;                  /* largest e4m3 */
 constexpr float kLeast = 0x1.cp-118f;           /* 448 * 2^-126 */
 
@@ -87,20 +87,32 @@ __device__ __forceinline__ float max8(const float (&v)[8]) {
 
 /* Sixteen lanes a block of 128 values, eight values a lane: one 16-byte load
  * (bf16), a maximum within a row of lanes, one 8-byte store. Scales: nblk of a
- * row, rows `stride` apart. */
-template <class S>
-__global__ __launch_bounds__(256) void rows_kernel(uint8_t *__restrict__ codes,
-                                                   float *__restrict__ scales,
-                                                   const S *__restrict__ src, uint64_t blocks,
-                                                   uint32_t nblk, uint32_t stride) {
-    const uint64_t q = (uint64_t)blockIdx.x * 16u + (threadIdx.x >> 4);
-    if (q >= blocks) return; /* whole rows of 16 lanes */
+ * row, rows `stride` apart. Block q of the `blocks`, a row of lanes each. */
+struct RowArgs {
+    uint8_t *codes;
+    float *scales;
+    const uint16_t *src;
+    uint64_t blocks;
+    uint32_t nblk, stride;
+};
+__device__ __forceinline__ void encode_block(const RowArgs &A, uint64_t q) {
+    if (q >= A.blocks) return; /* whole rows of 16 lanes */
     const uint32_t l = threadIdx.x & 15u;
+    const uint64_t at = kBlock * q + 8u * l;
     float v[8], scale, inv;
-    load8(src + kBlock * q + 8u * l, v);
+    load8(A.src + at, v);
     fp8_scales(row_group_max<16>(max8(v)), scale, inv);
-    *(uint2 *)(codes + kBlock * q + 8u * l) = fp8_codes8(v, inv);
-    if (l == 0u) scales[stride == nblk ? q : q / nblk * stride + q % nblk] = scale;
+    *(uint2 *)(A.codes + at) = fp8_codes8(v, inv);
+    if (l != 0u) return;
+    uint64_t to = q;
+    if (A.stride != A.nblk) { /* a short division where it does */
+        const uint64_t row = A.blocks >> 32 ? q / A.nblk : (uint32_t)q / A.nblk;
+        to = q + row * (A.stride - A.nblk);
+    }
+    A.scales[to] = scale;
+}
+__global__ __launch_bounds__(256) void rows_kernel(RowArgs A) {
+    encode_block(A, ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16u + (threadIdx.x >> 4));
 }
 
 /* One block of 256 threads a 128 x 128 block: thread t holds eight columns of
@@ -1066,38 +1078,53 @@ __global__ __launch_bounds__(C::THREADS) void join_kernel(TileArgs P) {
 /* routes and tiles of the experts                                         */
 /* ---------------------------------------------------------------------- */
 
-/* By a block of 1024 threads, thread e with expert e's rows [row, row + n): each
- * class's tiles in expert order. */
-__device__ __forceinline__ void list_tiles(const TileLists &Q, uint32_t row, uint32_t n,
-                                           const k3_moe_fp8_expert *experts) {
-    __shared__ uint32_t tot[kClasses][16];
+typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8))); /* two addresses */
+
+/* By a block of 1024 threads, thread e with expert e's n rows and descriptor (ex):
+ * each class's tiles in expert order. `row` is the expert's first row; FIRST: it is the sum of the
+ * earlier experts' n, and set here. The four classes' tiles are counted in 16
+ * bits each of one word (65535 tokens of 32 routes are 9215 tiles at most). */
+template <bool FIRST>
+__device__ __forceinline__ void list_tiles(const TileLists &Q, uint32_t &row, uint32_t n,
+                                           u32x4_8 ex0, u32x4_8 ex1, u32x4_8 ex2) {
+    static_assert(sizeof(ExpertTile) == 64 && sizeof(k3_moe_fp8_expert) == 48, "four stores");
+    static_assert(kClasses == 4, "16 bits each");
+    __shared__ unsigned long long tiles_of[16];
+    __shared__ uint32_t rows_of[16];
     const uint32_t e = threadIdx.x, lane = e & 63u, wave = e >> 6;
-    const int cls = n <= 32u ? 0 : n <= 64u ? 1 : n <= 128u ? 2 : 3;
+    const uint32_t cls = n <= 32u ? 0u : n <= 64u ? 1u : n <= 128u ? 2u : 3u;
     const uint32_t height = n ? tile_height(n) : 1u, many = (n + height - 1u) / height;
-    k3_moe_fp8_expert ex{};
-    if (n != 0u) ex = experts[e];
-    uint32_t inc[kClasses];
+    unsigned long long inc = (unsigned long long)many << (16u * cls);
+    uint32_t rows = n;
 #pragma unroll
-    for (int q = 0; q < kClasses; q++) {
-        inc[q] = cls == q ? many : 0u;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t a = __shfl_up(inc[q], o, 64);
-            if ((int)lane >= o) inc[q] += a;
-        }
-        if (lane == 63u) tot[q][wave] = inc[q];
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned long long a = __shfl_up(inc, o, 64);
+        const uint32_t r = FIRST ? __shfl_up(rows, o, 64) : 0u;
+        if ((int)lane >= o) inc += a, rows += r;
     }
+    if (lane == 63u) tiles_of[wave] = inc, rows_of[wave] = rows;
     __syncthreads();
+    unsigned long long at = inc - ((unsigned long long)many << (16u * cls)), total = 0ull;
+    if (FIRST) row = rows - n;
 #pragma unroll
-    for (int q = 0; q < kClasses; q++) {
-        uint32_t at = inc[q] - many, total = 0u;
-        for (uint32_t w = 0; w < 16u; w++) {
-            if (w < wave) at += tot[q][w];
-            total += tot[q][w];
+    for (uint32_t w = 0; w < 16u; w++) {
+        if (w < wave) {
+            at += tiles_of[w];
+            if (FIRST) row += rows_of[w];
         }
-        if (cls == q)
-            for (uint32_t i = 0; i < many; i++) Q.tiles[q][at + i] = ExpertTile{row, n, i, many, ex};
-        if (e == 0u) Q.count[q] = total;
+        total += tiles_of[w];
+    }
+    const uint32_t to = (uint32_t)(at >> (16u * cls)) & 0xffffu;
+    ExpertTile *const low = cls & 1u ? Q.tiles[1] : Q.tiles[0], *const high = cls & 1u ? Q.tiles[3] : Q.tiles[2];
+    ExpertTile *const list = cls & 2u ? high : low;
+    for (uint32_t i = 0; i < many; i++) {
+        u32x4_8 *const t = (u32x4_8 *)(list + to + i);
+        t[0] = u32x4_8{row, n, i, many};
+        t[1] = ex0, t[2] = ex1, t[3] = ex2;
+    }
+    if (e == 0u) {
+#pragma unroll
+        for (int q = 0; q < kClasses; q++) Q.count[q] = (uint32_t)(total >> (16 * q)) & 0xffffu;
     }
 }
 
@@ -1106,56 +1133,59 @@ __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t
                                                      const k3_moe_fp8_expert *__restrict__ experts,
                                                      uint32_t E) {
     const uint32_t e = threadIdx.x;
-    list_tiles(Q, e < E ? offsets[e] : 0u, e < E ? counts[e] : 0u, experts);
+    const u32x4_8 *const ex = (const u32x4_8 *)(experts + min(e, E - 1u));
+    uint32_t row = offsets[min(e, E - 1u)], n = e < E ? counts[e] : 0u;
+    list_tiles<false>(Q, row, n, ex[0], ex[1], ex[2]);
 }
 
-/* The plan (k3_moe_route_plan's order) and the tiles of up to 256 tokens as one
- * block's work: four launches less. Thread t < T holds token t's routes; an
- * expert's rows are the set bits of its masks. */
+/* Up to 256 tokens: the plan (k3_moe_route_plan's order) and the tiles as block
+ * 0's work, while the others encode the tokens' rows: five launches in one. Thread
+ * t < T of block 0 holds token t's routes; an expert's rows are the set bits of
+ * its masks. */
 constexpr uint32_t kSmallPlan = 256;
+struct PlanArgs {
+    TileLists lists;
+    uint32_t *token_index, *route_index;
+    const uint32_t *ids;
+    const k3_moe_fp8_expert *experts;
+    uint32_t T, k, E;
+    RowArgs rows;
+};
 template <int K>
-__global__ __launch_bounds__(1024) void small_plan_kernel(TileLists Q, uint32_t *__restrict__ token_index,
-                                                          uint32_t *__restrict__ route_index,
-                                                          const uint32_t *__restrict__ ids,
-                                                          const k3_moe_fp8_expert *__restrict__ experts,
-                                                          uint32_t T, uint32_t k, uint32_t E) {
+__global__ __launch_bounds__(1024) void small_plan_kernel(PlanArgs A) {
     __shared__ unsigned long long masks[kSmallPlan / 64u][1024];
-    __shared__ uint32_t first[1024], wave_tot[16];
-    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-#pragma unroll
-    for (uint32_t w = 0; w < kSmallPlan / 64u; w++) masks[w][t] = 0ull;
-    __syncthreads();
+    __shared__ uint32_t first[1024];
+    if (blockIdx.x != 0u) {
+        encode_block(A.rows, (blockIdx.x - 1u) * 64u + (threadIdx.x >> 4));
+        return;
+    }
+    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, waves = (A.T + 63u) / 64u;
+    const u32x4_8 *const ex = (const u32x4_8 *)(A.experts + min(t, A.E - 1u));
+    const u32x4_8 ex0 = ex[0], ex1 = ex[1], ex2 = ex[2];
+    asm volatile("" ::: "memory"); /* issued here, before the routes are waited for */
     uint32_t e[K];
-    if (t < T) {
-        token_routes<K>(ids, t, k, E, e);
+    if (t < A.T) token_routes<K>(A.ids, t, A.k, A.E, e);
+    for (uint32_t w = 0; w < waves; w++) masks[w][t] = 0ull;
+    __syncthreads();
+    if (t < A.T) {
 #pragma unroll
         for (int r = 0; r < K; r++)
-            if (e[r] < E) atomicOr(&masks[wave][e[r]], 1ull << lane);
+            if (e[r] < A.E) atomicOr(&masks[wave][e[r]], 1ull << lane);
     }
     __syncthreads();
-    uint32_t n = 0u;
-#pragma unroll
-    for (uint32_t w = 0; w < kSmallPlan / 64u; w++) n += (uint32_t)__popcll(masks[w][t]);
-    uint32_t inc = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t a = __shfl_up(inc, o, 64);
-        if ((int)lane >= o) inc += a;
-    }
-    if (lane == 63u) wave_tot[wave] = inc;
-    __syncthreads();
-    uint32_t row = inc - n;
-    for (uint32_t w = 0; w < wave; w++) row += wave_tot[w];
+    uint32_t n = 0u, row = 0u;
+    for (uint32_t w = 0; w < waves; w++) n += (uint32_t)__popcll(masks[w][t]);
+    list_tiles<true>(A.lists, row, n, ex0, ex1, ex2);
     first[t] = row;
-    list_tiles(Q, row, n, experts); /* a barrier inside: `first` is whole */
-    if (t >= T) return;
+    __syncthreads();
+    if (t >= A.T) return;
 #pragma unroll
     for (int r = 0; r < K; r++) {
-        if (e[r] >= E) continue;
+        if (e[r] >= A.E) continue;
         uint32_t at = first[e[r]] + (uint32_t)__popcll(masks[wave][e[r]] & ((1ull << lane) - 1ull));
         for (uint32_t w = 0; w < wave; w++) at += (uint32_t)__popcll(masks[w][e[r]]);
-        token_index[at] = t;
-        route_index[at] = t * k + (uint32_t)r;
+        A.token_index[at] = t;
+        A.route_index[at] = t * A.k + (uint32_t)r;
     }
 }
 
@@ -1224,13 +1254,17 @@ bool fp8_shape_ok(const k3_moe_shape *s, uint32_t T) {
            (s->activation == K3_MOE_ACT_SWIGLU || (s->beta > 0.0f && s->linear_beta > 0.0f));
 }
 
-/* Encodes rows of `cols` bf16 values; scales of a row `stride` apart. */
-bool launch_rows(uint8_t *codes, float *scales, const void *src, uint32_t rows, uint32_t cols,
-                 uint32_t stride, hipStream_t st) {
-    const uint32_t nblk = cols / kBlock;
-    const uint64_t blocks = (uint64_t)rows * nblk;
-    hipLaunchKernelGGL(rows_kernel<uint16_t>, dim3((uint32_t)((blocks + 15u) / 16u)), dim3(256), 0,
-                       st, codes, scales, (const uint16_t *)src, blocks, nblk, stride);
+/* Rows of `cols` bf16 values to encode; scales of a row `stride` apart. */
+constexpr uint64_t kMostGrid = 1u << 20; /* a launch's x axis is under 2^32 threads */
+RowArgs row_args(uint8_t *codes, float *scales, const void *src, uint32_t rows, uint32_t cols,
+                 uint32_t stride) {
+    return RowArgs{codes, scales, (const uint16_t *)src, (uint64_t)rows * (cols / kBlock), cols / kBlock,
+                   stride};
+}
+bool launch_rows(const RowArgs &A, hipStream_t st) {
+    const uint64_t n = (A.blocks + 15u) / 16u;
+    const uint32_t x = (uint32_t)(n < kMostGrid ? n : kMostGrid);
+    hipLaunchKernelGGL(rows_kernel, dim3(x, (uint32_t)((n + x - 1u) / x)), dim3(256), 0, st, A);
     return hipGetLastError() == hipSuccess;
 }
 
@@ -1285,6 +1319,7 @@ template <class C>
 bool launch_dense(TileArgs A, const Cut &q, hipStream_t st) {
     A.tiles_t = q.tiles_t, A.tiles_n = q.tiles_n, A.splits = q.splits, A.span = q.span;
     const uint32_t tiles = q.tiles_t * q.tiles_n;
+    if ((uint64_t)tiles * q.splits >= (1u << 23)) return false; /* 2^32 threads: outputs of 2^33 values */
     hipLaunchKernelGGL(product_tile_kernel<C>, dim3(8u * ((tiles * q.splits + 7u) / 8u)),
                        dim3(C::THREADS), 0, st, A);
     if (q.splits == 1u) return hipGetLastError() == hipSuccess;
@@ -1309,15 +1344,16 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
             hipLaunchKernelGGL(down_one_kernel<kOneFfn>, dim3(H / 16u), dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
-    if (!launch_rows(ws.xq, ws.xs, hidden, T, H, scale_stride(H), st)) return false;
+    const RowArgs R = row_args(ws.xq, ws.xs, hidden, T, H, scale_stride(H));
     if (T <= kSmallPlan) {
+        const PlanArgs A{ws.lists, ws.token_index, ws.route_index, ids, experts, T, k, E, R};
+        const dim3 grid(1u + (uint32_t)((R.blocks + 63u) / 64u));
         if (k <= 8u)
-            hipLaunchKernelGGL(small_plan_kernel<8>, dim3(1), dim3(1024), 0, st, ws.lists,
-                               ws.token_index, ws.route_index, ids, experts, T, k, E);
+            hipLaunchKernelGGL(small_plan_kernel<8>, grid, dim3(1024), 0, st, A);
         else
-            hipLaunchKernelGGL(small_plan_kernel<32>, dim3(1), dim3(1024), 0, st, ws.lists,
-                               ws.token_index, ws.route_index, ids, experts, T, k, E);
+            hipLaunchKernelGGL(small_plan_kernel<32>, grid, dim3(1024), 0, st, A);
     } else {
+        if (!launch_rows(R, st)) return false;
         if (!k3_moe_route_plan(ws.counts, ws.offsets, ws.unique, ws.summary, ws.token_index,
                                ws.route_index, ids, T, k, E, ws.plan, ws.plan_bytes, st))
             return false;
@@ -1357,10 +1393,10 @@ extern "C" bool k3_moe_fp8_128_quantize_rows_bf16(uint8_t *codes, float *scales,
                                                   uint32_t rows, uint32_t columns, void *stream) {
     const uint64_t blocks = (uint64_t)rows * (columns / kBlock);
     if (!codes || !scales || !src || rows == 0u || columns == 0u || columns % kBlock != 0u ||
-        blocks > (1ull << 34) || /* the grid */ ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
+        blocks > (1ull << 34) || ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
         ((uintptr_t)scales % 4u) != 0u)
         return false;
-    return launch_rows(codes, scales, src, rows, columns, columns / kBlock, (hipStream_t)stream);
+    return launch_rows(row_args(codes, scales, src, rows, columns, columns / kBlock), (hipStream_t)stream);
 }
 
 extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const void *src,
@@ -1368,7 +1404,7 @@ extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scale
                                                     void *stream) {
     const uint64_t blocks = ((uint64_t)rows + kBlock - 1u) / kBlock * (columns / kBlock);
     if (!codes || !scales || !src || rows == 0u || columns == 0u || columns % kBlock != 0u ||
-        blocks > 0x7fffffffull || ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
+        blocks >= (1ull << 24) || /* 2^32 threads */ ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
         ((uintptr_t)scales % 4u) != 0u)
         return false;
     hipLaunchKernelGGL(weight_kernel, dim3((uint32_t)blocks), dim3(256), 0, (hipStream_t)stream,
@@ -1378,8 +1414,8 @@ extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scale
 
 extern "C" size_t k3_moe_fp8_128_scratch_bytes(uint32_t vector_count, uint32_t rows,
                                                uint32_t columns) {
-    if (vector_count == 0u || vector_count > 65535u || rows == 0u || columns == 0u ||
-        columns % kBlock != 0u || columns > kMostColumns)
+    if (vector_count == 0u || vector_count > 65535u || rows == 0u || rows > kMostAxis ||
+        columns == 0u || columns % kBlock != 0u || columns > kMostAxis)
         return 0u;
     return fp8_scratch_bytes(vector_count, rows, columns);
 }
@@ -1389,7 +1425,8 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
                                          uint32_t columns, void *scratch, size_t scratch_bytes,
                                          void *stream) {
     if (!output || !codes || !scales || !input || vector_count == 0u || vector_count > 65535u ||
-        rows == 0u || columns == 0u || columns % kBlock != 0u || columns > kMostColumns ||
+        rows == 0u || rows > kMostAxis || columns == 0u || columns % kBlock != 0u ||
+        columns > kMostAxis ||
         (((uintptr_t)codes | (uintptr_t)input) % 16u) != 0u || ((uintptr_t)scales % 4u) != 0u ||
         ((uintptr_t)output % 2u) != 0u)
         return false;
@@ -1419,7 +1456,7 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
     B.part = (f32x4 *)((uint8_t *)xs + align256(4u * (size_t)vector_count * B.xstride));
     B.out = (uint16_t *)output, B.T = vector_count, B.N = rows, B.K = columns, B.wide = wide;
     B.wide16 = rows % 8u == 0u && ((uintptr_t)output % 16u) == 0u;
-    if (!launch_rows(xq, xs, input, vector_count, columns, B.xstride, st)) return false;
+    if (!launch_rows(row_args(xq, xs, input, vector_count, columns, B.xstride), st)) return false;
     const Cut q = cut_of(vector_count, rows, columns);
     switch (q.tile) {
     case 0: return launch_dense<Half32>(B, q, st);
@@ -1441,7 +1478,7 @@ bool fp8_args_ok(const void *output, const void *hidden, const void *residual,
                  const void *workspace) {
     return output && hidden && experts && workspace && fp8_shape_ok(shape, T) &&
            (((uintptr_t)output | (uintptr_t)hidden | (uintptr_t)residual) % 16u) == 0u &&
-           ((uintptr_t)workspace % 256u) == 0u;
+           ((uintptr_t)experts % 8u) == 0u && ((uintptr_t)workspace % 256u) == 0u;
 }
 
 }  // namespace
@@ -1452,6 +1489,7 @@ extern "C" bool k3_moe_fp8_experts_bf16(void *output, const void *hidden, const 
                                         const k3_moe_shape *shape, uint32_t token_count,
                                         void *workspace, size_t workspace_bytes, void *stream) {
     if (!expert_ids || !expert_weights ||
+        (((uintptr_t)expert_ids | (uintptr_t)expert_weights) % 4u) != 0u ||
         !fp8_args_ok(output, hidden, residual, experts, shape, token_count, workspace))
         return false;
     const Fp8Workspace ws = carve(workspace, *shape, token_count);

@@ -35,7 +35,7 @@ def test_scratch_holds_the_encoded_rows(T, N, K):
 
 def test_scratch_refuses():
     f = _lib.lib().k3_moe_fp8_128_scratch_bytes
-    for bad in ((0, 1, 128), (65536, 1, 128), (1, 0, 128), (1, 1, 0), (1, 1, 64), (1, 1, 192)):
+    for bad in ((0, 1, 128), (65536, 1, 128), (1, 0, 128), (20, (1 << 24) + 1, 128), (20, 1, (1 << 24) + 128), (1, 1, 0), (1, 1, 64), (1, 1, 192)):
         assert f(*bad) == 0
 
 
@@ -53,7 +53,7 @@ def test_product_refuses():
     L = _lib.lib()
     big = 1 << 40
     good = [P, P, P, P, 5, 64, 256, P, big]
-    for at, bad in ((0, None), (1, None), (2, None), (3, None), (4, 0), (4, 65536), (5, 0), (6, 0),
+    for at, bad in ((0, None), (1, None), (2, None), (3, None), (4, 0), (4, 65536), (5, 0), (5, (1 << 24) + 1), (6, 0),
                     (6, 64), (6, 200), (0, P.value + 1), (1, P.value + 8), (2, P.value + 2),
                     (3, P.value + 8)):
         args = list(good)
@@ -80,13 +80,13 @@ def test_experts_refuse():
     args = [P, P, P, P, P, P, s, 5, P, n]
     for at, bad in ((0, None), (1, None), (3, None), (4, None), (5, None), (6, None), (7, 0),
                     (8, None), (9, n - 1), (0, P.value + 8), (1, P.value + 8), (2, P.value + 8),
-                    (8, P.value + 128)):
+                    (3, P.value + 2), (4, P.value + 2), (5, P.value + 4), (8, P.value + 128)):
         a = list(args)
         a[at] = bad
         assert not L.k3_moe_fp8_experts_bf16(*a, None), (at, bad)
     args = [P, P, P, P, P, P, s, 5, None, None, P, n]
     for at, bad in ((0, None), (1, None), (3, None), (4, None), (5, None), (6, None), (7, 0),
-                    (10, None), (11, n - 1), (3, P.value + 8), (10, P.value + 64)):
+                    (10, None), (11, n - 1), (3, P.value + 8), (5, P.value + 4), (10, P.value + 64)):
         a = list(args)
         a[at] = bad
         assert not L.k3_moe_fp8_forward_bf16(*a, None), (at, bad)
