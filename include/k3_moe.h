@@ -419,9 +419,10 @@ bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const vo
  * the blocks depends on the call's sizes only. columns % 128 == 0; rows and
  * columns <= 2^24; input and codes 16-byte, scales 4-byte, output 2-byte
  * aligned (wider stores where the output and rows allow them); vector_count <=
- * 65535. scratch (256-byte
- * aligned device memory): k3_moe_fp8_128_scratch_bytes(vector_count, rows,
- * columns) bytes, 0 where none is needed (scratch may then be NULL).
+ * 65535. scratch (256-byte aligned device memory):
+ * k3_moe_fp8_128_scratch_bytes(vector_count, rows, columns) bytes, 0 where none
+ * is needed (scratch may then be NULL). An output that overlaps the input is
+ * refused.
  */
 size_t k3_moe_fp8_128_scratch_bytes(uint32_t vector_count, uint32_t rows, uint32_t columns);
 bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, const float *scales,
@@ -448,7 +449,8 @@ typedef struct {
  * The products are k3_moe_fp8_128_gemm_bf16's without its bf16 rounding; h is
  * encoded from fp32. residual may be NULL. experts is a DEVICE array of
  * expert_count descriptors. A route whose id is not below expert_count, or
- * repeats an earlier rank's of its token, adds nothing. hidden and ffn multiples
+ * repeats an earlier rank's of its token, adds nothing, whatever its weight.
+ * output may be hidden or residual itself. hidden and ffn multiples
  * of 128 up to 65536; output, hidden and residual 16-byte aligned; the workspace
  * 256-byte aligned, k3_moe_fp8_workspace_bytes(shape, T) bytes, no state kept
  * in it between calls; token_count <= 65535. expert_ids and expert_weights of
@@ -505,6 +507,7 @@ bool k3_moe_balance_loss_f32(float *loss, uint32_t *counts, float *mean_scores,
  * with f[s, e] = E counts[s, e] / (k N[s]); the ids and counts are constants,
  * as the choice of experts has no gradient. counts and live_tokens are
  * k3_moe_balance_loss_f32's. Rows of tokens that are not live are 0.
+ * logits_gradient may be logits itself.
  */
 bool k3_moe_router_backward_f32(float *logits_gradient, const float *logits,
                                 const uint32_t *expert_ids, const uint32_t *counts,

@@ -17,7 +17,6 @@
  * partial loss in one order whichever block it is.
  */
 #include "k3_device.h"
-#include "k3_topk.h"
 #include "../../include/k3_moe.h"
 
 #include <hip/hip_runtime.h>

@@ -6,12 +6,14 @@
  *
  *   rows_kernel           token rows
  *   weight_kernel         a weight, one 128 x 128 block a block
- *   product_one_kernel    one token's product,
- *   gateup_one_kernel     act(gate . x, up . x) of its routes,
+ *   product_one_kernel    few tokens' product
+ *   product_tile_kernel   more tokens', tiles in LDS
+ *   join_kernel           the parts of K of a product that was cut
+ *   gateup_one_kernel     one token: act(gate . x, up . x) of its routes,
  *   down_one_kernel       their down products and weighted sum
- *   tile_kernel           more tokens, tiles in LDS: dense, gate/up of the
- *                         experts, y[route] = bf16(down . h)
- *   join_kernel           a dense product's parts of K
+ *   small_plan_kernel     up to 256 tokens: their rows, and the experts' tiles
+ *   tiles_kernel          the experts' tiles by k3_moe_route_plan's counts
+ *   experts_tile_kernel   gate/up of all tiles; y[route] = bf16(down . h)
  *
  * MFMA operands (V_MFMA_F32_16X16X128_F8F6F4): lane 16 g + c holds 32 codes of
  * row c of the 16 x 128 slices: bytes [16 g, 16 g + 16) and [64 + 16 g, 64 +
@@ -24,7 +26,6 @@
 #include "k3_fp8.h"
 #include "k3_internal.h"
 #include "k3_lds.h"
-#include "k3_topk.h"
 #include "../../include/k3_moe.h"
 
 #include <hip/hip_runtime.h>
@@ -1081,8 +1082,8 @@ __global__ __launch_bounds__(C::THREADS) void join_kernel(TileArgs P) {
 typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8))); /* two addresses */
 
 /* By a block of 1024 threads, thread e with expert e's n rows and descriptor (ex):
- * each class's tiles in expert order. `row` is the expert's first row; FIRST: it is the sum of the
- * earlier experts' n, and set here. The four classes' tiles are counted in 16
+ * each class's tiles in expert order. `row` is the expert's first row; FIRST: it is
+ * the sum of the earlier experts' n, and set here. The four classes' tiles are counted in 16
  * bits each of one word (65535 tokens of 32 routes are 9215 tiles at most). */
 template <bool FIRST>
 __device__ __forceinline__ void list_tiles(const TileLists &Q, uint32_t &row, uint32_t n,
@@ -1430,6 +1431,9 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
         (((uintptr_t)codes | (uintptr_t)input) % 16u) != 0u || ((uintptr_t)scales % 4u) != 0u ||
         ((uintptr_t)output % 2u) != 0u)
         return false;
+    /* blocks of one launch read all of the input and write their own columns */
+    const uintptr_t in = (uintptr_t)input, to = (uintptr_t)output;
+    if (to < in + 2u * (uint64_t)vector_count * columns && in < to + 2u * (uint64_t)vector_count * rows) return false;
     const size_t need = fp8_scratch_bytes(vector_count, rows, columns);
     if (need != 0u && (!scratch || scratch_bytes < need || ((uintptr_t)scratch % 256u) != 0u))
         return false;

@@ -75,7 +75,8 @@ bool static_ok(const k3_moe_static_weight &w, uint32_t rows, uint32_t cols) {
     if (!w.data || w.rows != rows || w.columns != cols) return false;
     if (w.kind == K3_MOE_STATIC_BF16) return true;
     if (w.kind == K3_MOE_STATIC_FP8_128 &&
-        (((uintptr_t)w.data % 16u) != 0u || ((uintptr_t)w.scales % 4u) != 0u))
+        (((uintptr_t)w.data % 16u) != 0u || ((uintptr_t)w.scales % 4u) != 0u ||
+         rows > (1u << 24) || cols > (1u << 24)))
         return false; /* as the product would: refused before the block's first launch */
     return w.kind <= K3_MOE_STATIC_FP8_128 && w.scales && cols % 128u == 0u;
 }

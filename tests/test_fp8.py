@@ -59,6 +59,8 @@ def test_product_refuses():
         args = list(good)
         args[at] = bad
         assert not L.k3_moe_fp8_128_gemm_bf16(*args, None), (at, bad)
+    for at in (P.value + 16, P.value - 2, P.value + 2 * 5 * 256 - 2):  # an output over the input
+        assert not L.k3_moe_fp8_128_gemm_bf16(at, P, P, P, 5, 64, 256, P, big, None), at
     need = L.k3_moe_fp8_128_scratch_bytes(300, 64, 256)
     assert need > 0
     for at, n in ((None, need), (P, need - 1), (P.value + 128, need)):

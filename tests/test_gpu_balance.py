@@ -285,3 +285,27 @@ def test_a_training_step_of_the_router(cuda):
     # the weighted rows are the layer's output without its residual's rounding
     back = sum(w[:, r:r + 1] * v.float() for r, v in enumerate(rows)) + x.float()
     assert torch.linalg.norm(back - y.float()) <= 2.0 ** -7 * torch.linalg.norm(y.float())
+
+
+def test_many_segments(cuda):
+    """A segment a block; the last block adds up thousands of partial losses."""
+    logits, ids, dw = case(4096, 64, 4, 21)
+    check(cuda, logits, ids, dw, 1024, None)
+    S, E, k = 65535, 8, 2
+    logits, ids, _ = case(S, E, k, 22)
+    got = balance.balance_loss(logits.to(cuda), ids.to(cuda), 0.3, segments=S)
+    loss, counts, mean, n, *_ = forward64(logits.double(), ids, 0.3, S, None)
+    assert torch.equal(got[1].cpu().double(), counts) and torch.equal(got[3].cpu().double(), n)
+    assert ((got[2].cpu().double() - mean).abs() <= 230 * U * mean + 1e-38).all()
+    # 64 terms a lane, 6 levels and 16 waves behind a term's own 234 u, and 2 more
+    assert abs(got[0].item() - loss.item()) <= (234 + 64 + 6 + 16 + 2) * U * loss.item()
+
+
+def test_gradient_into_the_logits(cuda):
+    """The gradient may take the logits' place."""
+    for E, T in ((64, 200), (896, 3000)):
+        logits, ids, dw = (t.to(cuda) for t in case(T, E, 4, E))
+        _, counts, _, live = balance.balance_loss(logits, ids, 0.3)
+        want = balance.router_backward(logits, ids, counts, live, 0.3, dweights=dw)
+        got = balance.router_backward(logits, ids, counts, live, 0.3, dweights=dw, out=logits)
+        assert got is logits and torch.equal(got, want)

@@ -148,3 +148,46 @@ def test_experts_of_the_most_tokens(cuda):
     assert torch.equal(got, out[some])
     a = some[:40].cpu()
     check_experts(cuda, store, 40, k, ACT_SWIGLU, 7, ids=ids.cpu()[a])
+
+
+@pytest.mark.parametrize("T", [1, 4, 300])
+def test_experts_in_place(cuda, T):
+    """The output in the place of the hidden rows, and of the residual's."""
+    store = make_store(cuda, 8, 256, 128, 2)
+    g = torch.Generator().manual_seed(9)
+    ids = torch.stack([torch.randperm(8, generator=g)[:3] for _ in range(T)]).to(torch.int32).to(cuda)
+    w = torch.rand((T, 3), generator=g).to(cuda)
+    sh = fp8.shape(256, 8, 3, 128, 1.0, ACT_SWIGLU)
+    x, r = normal((T, 256), 4).to(cuda), normal((T, 256), 5).to(cuda)
+    want, alone = fp8.experts(x, ids, w, store.table, sh, r), fp8.experts(x, ids, w, store.table, sh, x)
+    a, b, c = x.clone(), r.clone(), x.clone()
+    assert torch.equal(fp8.experts(a, ids, w, store.table, sh, r, out=a), want)
+    assert torch.equal(fp8.experts(x, ids, w, store.table, sh, b, out=b), want)
+    assert torch.equal(fp8.experts(c, ids, w, store.table, sh, c, out=c), alone)
+
+
+@pytest.mark.parametrize("T", [1, 5, 280])
+def test_experts_weights_of_routes_that_are_none(cuda, T):
+    """A route that is left out adds nothing, whatever its weight."""
+    store = make_store(cuda, 6, 128, 128, 2)
+    ids = torch.tensor([[4, 6, 4, 1]], dtype=torch.int32).repeat(T, 1)
+    w = torch.tensor([[0.5, float("nan"), float("inf"), -2.0]]).repeat(T, 1)
+    sh = fp8.shape(128, 6, 4, 128, 1.0, ACT_SWIGLU)
+    x = normal((T, 128), 4).to(cuda)
+    got = fp8.experts(x, ids.to(cuda), w.to(cuda), store.table, sh)
+    w[:, 1:3] = 0
+    want = fp8.experts(x, ids.to(cuda), w.to(cuda), store.table, sh)
+    assert torch.isfinite(got).all() and torch.equal(got, want)
+
+
+def test_product_refuses_an_output_over_its_input(cuda):
+    wq, ws = fp8.quantize_weight(normal((256, 256), 3, 0.02).to(cuda))
+    room = normal((12, 256), 4).to(cuda)
+    before = room.clone()
+    for T in (1, 3, 6):
+        for to in (0, T - 1):
+            with pytest.raises(RuntimeError):
+                fp8.product(room[:T], wq, ws, out=room[to:to + T])
+    assert torch.equal(room, before)
+    fp8.product(room[:3], wq, ws, out=room[3:6])
+    assert torch.equal(room[3:6], fp8.product(before[:3], wq, ws))
