@@ -180,30 +180,40 @@ __device__ __forceinline__ void store_rows(uint16_t *out, const f32x4 &v, uint32
     if (n + 3u < N) p[3] = (uint16_t)(u.y >> 16);
 }
 
-/* tanh to a few ulp: its odd series below 1/2, the exponential above. */
+/* tanh within 16 u of itself (u = 2^-24): its odd series below 1/4 (the term left
+ * out is under u / 6 there), the exponential above (2 / (e + 1) to 3.6 u, of 0.245). */
 __device__ __forceinline__ float tanh_f32(float y) {
     const float a = fabsf(y), z = __fmul_rn(a, a);
-    float p = -1.4558343870513183e-3f;
-    p = fmaf(p, z, 3.5921280365724811e-3f);
-    p = fmaf(p, z, -8.8632355299021966e-3f);
-    p = fmaf(p, z, 2.1869488536155203e-2f);
+    float p = 2.1869488536155203e-2f;
     p = fmaf(p, z, -5.3968253968253968e-2f);
     p = fmaf(p, z, 1.3333333333333333e-1f);
     p = fmaf(p, z, -3.3333333333333333e-1f);
     const float lo = fmaf(__fmul_rn(a, z), p, a);
     const float e = __builtin_amdgcn_exp2f(__fmul_rn(a, 2.88539008177792681f)); /* e^2a */
     const float hi = fmaf(-2.0f, __builtin_amdgcn_rcpf(__fadd_rn(e, 1.0f)), 1.0f);
-    return copysignf(a < 0.5f ? lo : hi, y);
+    return copysignf(a < 0.25f ? lo : hi, y);
 }
 
-/* The activation in fp32: it is encoded in e4m3 next, and exp2 and the
- * reciprocal of the hardware (1 ulp) are far inside that. */
-__device__ __forceinline__ float act_f32(float g, float u, uint32_t kind, float beta, float lb) {
+/* The activation and SiTU's constants: by = 1 / beta (at most the largest number,
+ * so that 0 stays 0), by_linear = 1 / linear_beta. */
+struct Activation {
+    uint32_t kind;
+    float beta, linear, by, by_linear;
+};
+Activation activation_of(const k3_moe_shape &s) {
+    const auto inverse = [](float v) { return v < 0x1p-127f ? 0x1.fffffep127f : 1.0f / v; };
+    return Activation{s.activation, s.beta, s.linear_beta, inverse(s.beta), inverse(s.linear_beta)};
+}
+
+/* In fp32: it is encoded in e4m3 next, and exp2 and the reciprocal of the hardware
+ * (1 ulp), products with reciprocals and tanh_f32 are far inside that. SiTU costs
+ * some 60 vector cycles a value: a division by each beta would be 30 more. */
+__device__ __forceinline__ float act_f32(float g, float u, const Activation &A) {
     const float e = __builtin_amdgcn_exp2f(__fmul_rn(g, -1.44269504088896341f));
     const float s = __builtin_amdgcn_rcpf(__fadd_rn(1.0f, e));
-    if (kind == K3_MOE_ACT_SWIGLU) return __fmul_rn(__fmul_rn(g, s), u);
-    const float bg = __fmul_rn(beta, tanh_f32(__fdiv_rn(g, beta)));
-    const float bu = __fmul_rn(lb, tanh_f32(__fdiv_rn(u, lb)));
+    if (A.kind == K3_MOE_ACT_SWIGLU) return __fmul_rn(__fmul_rn(g, s), u);
+    const float bg = __fmul_rn(A.beta, tanh_f32(__fmul_rn(g, A.by)));
+    const float bu = __fmul_rn(A.linear, tanh_f32(__fmul_rn(u, A.by_linear)));
     return __fmul_rn(__fmul_rn(bg, s), bu);
 }
 
@@ -423,8 +433,8 @@ struct OneExpertArgs {
     uint16_t *out;
     uint8_t *hq; /* [k, F] */
     float *hs;   /* [k], hstride apart */
-    uint32_t hstride, H, F, E, k, kind;
-    float beta, lb;
+    uint32_t hstride, H, F, E, k;
+    Activation act;
 };
 
 /*
@@ -439,10 +449,10 @@ __global__ __launch_bounds__(512) void gateup_one_kernel(OneExpertArgs A) {
     using Ring = WaveRing<2, kGateUpRing>;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * Ring::BYTES + kOneHidden + kOneHidden / 32u];
     __shared__ float red[8];
-    const uint32_t cols = A.F / kBlock, r = blockIdx.x / cols, col = blockIdx.x % cols;
+    const uint32_t cols = A.F / kBlock, r = blockIdx.x / cols, col = blockIdx.x % cols, t = r / A.k;
     TokenPart x;
-    x.load(A.x, A.H / kBlock);
-    const uint32_t e = one_route(A.ids, r, A.k, A.E);
+    x.load(A.x + (uint64_t)t * A.H, A.H / kBlock);
+    const uint32_t e = one_route(A.ids + t * A.k, r - t * A.k, A.k, A.E);
     if (e >= A.E) return;
     const k3_moe_fp8_expert ex = A.experts[e];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, nblk = A.H / kBlock;
@@ -481,7 +491,7 @@ __global__ __launch_bounds__(512) void gateup_one_kernel(OneExpertArgs A) {
     float h[4], m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        h[i] = act_f32(gate[i], up[i], A.kind, A.beta, A.lb);
+        h[i] = act_f32(gate[i], up[i], A.act);
         m = fmaxf(m, fabsf(h[i]));
     }
     m = fmaxf(m, __shfl_xor(m, 16, 64));
@@ -515,15 +525,16 @@ __global__ __launch_bounds__(512) void down_one_kernel(OneExpertArgs A) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = 16u * blockIdx.x;
     uint8_t *mine = smem + (Ring::BYTES + MOST) * wave;
     const uint32_t codes = lds_addr(mine) + Ring::BYTES;
+    const uint32_t r0 = blockIdx.y * A.k; /* the token's first route */
     for (uint32_t r = wave; r < A.k; r += 8u) {
-        const uint32_t e = one_route(A.ids, r, A.k, A.E);
+        const uint32_t e = one_route(A.ids + r0, r, A.k, A.E);
         if (lane == 0u) live[r] = e < A.E;
         if (e >= A.E) continue;
-        const uint8_t *h = A.hq + (uint64_t)r * A.F;
+        const uint8_t *h = A.hq + (uint64_t)(r0 + r) * A.F;
         const k3_moe_fp8_expert ex = A.experts[e];
         const float *ws = ex.down_scales + (uint64_t)(n0 / kBlock) * nblk;
         float f = lane_scales(ws, 0u, nblk); /* nblk <= 64 */
-        const float sx = lane_scales(A.hs + (uint64_t)r * A.hstride, 0u, nblk);
+        const float sx = lane_scales(A.hs + (uint64_t)(r0 + r) * A.hstride, 0u, nblk);
         asm volatile("" ::: "memory"); /* issued before the weights, so that their wait leaves those out */
         for (uint32_t o = 0; o < A.F; o += 1024u)
             dma<16>(h + min(o + 16u * lane, A.F - 16u), mine + Ring::BYTES + o);
@@ -554,10 +565,11 @@ __global__ __launch_bounds__(512) void down_one_kernel(OneExpertArgs A) {
     if (threadIdx.x >= 16u) return;
     float v = 0.0f;
     for (uint32_t r = 0; r < A.k; r++)
-        if (live[r]) v = __fadd_rn(v, __fmul_rn(A.weights[r], y[r][threadIdx.x]));
+        if (live[r]) v = __fadd_rn(v, __fmul_rn(A.weights[r0 + r], y[r][threadIdx.x]));
     uint16_t o = f32_to_bf16(v);
-    if (A.residual) o = f32_to_bf16(__fadd_rn(bf16_to_f32(A.residual[n0 + threadIdx.x]), bf16_to_f32(o)));
-    A.out[n0 + threadIdx.x] = o;
+    const uint64_t at = (uint64_t)blockIdx.y * A.H + n0 + threadIdx.x;
+    if (A.residual) o = f32_to_bf16(__fadd_rn(bf16_to_f32(A.residual[at]), bf16_to_f32(o)));
+    A.out[at] = o;
 }
 
 /* One of the `many` row tiles of an expert with n rows from `row` on: all that
@@ -637,8 +649,7 @@ struct TileArgs {
     uint32_t T, N, K, tiles_n, tiles_t;
     uint32_t splits, span; /* dense: K in `splits` parts of `span` blocks (a multiple of 4) */
     f32x4 *part;           /* their sums, of more than one */
-    uint32_t kind;
-    float beta, lb;
+    Activation act;
     bool wide, wide16; /* the output takes 8-byte, 16-byte stores */
 };
 
@@ -978,7 +989,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float h = act_f32(acc[j][i][r], acc[j][i + 2][r], P.kind, P.beta, P.lb);
+                    const float h = act_f32(acc[j][i][r], acc[j][i + 2][r], P.act);
                     acc[j][i][r] = h;
                     m = fmaxf(m, fabsf(h));
                 }
@@ -1139,11 +1150,11 @@ __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t
     list_tiles<false>(Q, row, n, ex[0], ex[1], ex[2]);
 }
 
-/* Up to 256 tokens: the plan (k3_moe_route_plan's order) and the tiles as block
+/* Up to 1024 tokens: the plan (k3_moe_route_plan's order) and the tiles as block
  * 0's work, while the others encode the tokens' rows: five launches in one. Thread
  * t < T of block 0 holds token t's routes; an expert's rows are the set bits of
- * its masks. */
-constexpr uint32_t kSmallPlan = 256;
+ * its masks, a word for each 64 tokens: WORDS of them at most. */
+constexpr uint32_t kSmallPlan = 1024, kFewWords = 4096, kMostWords = 16384;
 struct PlanArgs {
     TileLists lists;
     uint32_t *token_index, *route_index;
@@ -1152,9 +1163,9 @@ struct PlanArgs {
     uint32_t T, k, E;
     RowArgs rows;
 };
-template <int K>
+template <int K, uint32_t WORDS>
 __global__ __launch_bounds__(1024) void small_plan_kernel(PlanArgs A) {
-    __shared__ unsigned long long masks[kSmallPlan / 64u][1024];
+    __shared__ unsigned long long masks[WORDS]; /* [waves][E] */
     __shared__ uint32_t first[1024];
     if (blockIdx.x != 0u) {
         encode_block(A.rows, (blockIdx.x - 1u) * 64u + (threadIdx.x >> 4));
@@ -1166,16 +1177,17 @@ __global__ __launch_bounds__(1024) void small_plan_kernel(PlanArgs A) {
     asm volatile("" ::: "memory"); /* issued here, before the routes are waited for */
     uint32_t e[K];
     if (t < A.T) token_routes<K>(A.ids, t, A.k, A.E, e);
-    for (uint32_t w = 0; w < waves; w++) masks[w][t] = 0ull;
+    for (uint32_t i = t; i < waves * A.E; i += 1024u) masks[i] = 0ull;
     __syncthreads();
     if (t < A.T) {
 #pragma unroll
         for (int r = 0; r < K; r++)
-            if (e[r] < A.E) atomicOr(&masks[wave][e[r]], 1ull << lane);
+            if (e[r] < A.E) atomicOr(&masks[wave * A.E + e[r]], 1ull << lane);
     }
     __syncthreads();
     uint32_t n = 0u, row = 0u;
-    for (uint32_t w = 0; w < waves; w++) n += (uint32_t)__popcll(masks[w][t]);
+    if (t < A.E)
+        for (uint32_t w = 0; w < waves; w++) n += (uint32_t)__popcll(masks[w * A.E + t]);
     list_tiles<true>(A.lists, row, n, ex0, ex1, ex2);
     first[t] = row;
     __syncthreads();
@@ -1183,8 +1195,8 @@ __global__ __launch_bounds__(1024) void small_plan_kernel(PlanArgs A) {
 #pragma unroll
     for (int r = 0; r < K; r++) {
         if (e[r] >= A.E) continue;
-        uint32_t at = first[e[r]] + (uint32_t)__popcll(masks[wave][e[r]] & ((1ull << lane) - 1ull));
-        for (uint32_t w = 0; w < wave; w++) at += (uint32_t)__popcll(masks[w][e[r]]);
+        uint32_t at = first[e[r]] + (uint32_t)__popcll(masks[wave * A.E + e[r]] & ((1ull << lane) - 1ull));
+        for (uint32_t w = 0; w < wave; w++) at += (uint32_t)__popcll(masks[w * A.E + e[r]]);
         A.token_index[at] = t;
         A.route_index[at] = t * A.k + (uint32_t)r;
     }
@@ -1329,30 +1341,45 @@ bool launch_dense(TileArgs A, const Cut &q, hipStream_t st) {
     return hipGetLastError() == hipSuccess;
 }
 
+/* Whether a few tokens go through the experts one by one, in two launches. Tiles
+ * take four and read an expert once however many tokens chose it: 14 us or some
+ * 64 MB of weights read again, by the number of experts that T tokens choose if
+ * each chooses at random. (us, one by one and by tiles; hidden 2048, ffn 512, 4 of 64
+ * experts: 2 tokens 11.1 and 26.1, 8 tokens 22.4 and 32.1; 7168, 2048, 8 of 128:
+ * 2 tokens 126 and 134, 4 tokens level, 8 tokens 451 and 413.) */
+bool one_by_one(uint32_t T, const k3_moe_shape &s) {
+    if (T > 64u || s.hidden > kOneHidden || s.ffn > kOneFfn) return false;
+    double miss = 1.0; /* of an expert by all tokens */
+    for (uint32_t t = 0; t < T; t++) miss *= 1.0 - (double)s.top_k / s.expert_count;
+    const double again = (double)T * s.top_k - s.expert_count * (1.0 - miss);
+    return T == 1u || again * 3.0 * s.hidden * s.ffn < 64e6;
+}
+
 /* The expert stage on given routes. */
 bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, const void *residual,
                      const uint32_t *ids, const float *wts, const k3_moe_fp8_expert *experts,
                      const k3_moe_shape &s, uint32_t T, hipStream_t st) {
     const uint32_t H = s.hidden, F = s.ffn, E = s.expert_count, k = s.top_k;
-    if (T == 1u && H <= kOneHidden && F <= kOneFfn) {
+    if (one_by_one(T, s)) {
         const OneExpertArgs A{experts, ids, wts, (const uint16_t *)hidden, (const uint16_t *)residual,
                               (uint16_t *)output, ws.hq, ws.hs, scale_stride(F), H, F, E, k,
-                              s.activation, s.beta, s.linear_beta};
-        hipLaunchKernelGGL(gateup_one_kernel, dim3(k * (F / kBlock)), dim3(512), 0, st, A);
+                              activation_of(s)};
+        hipLaunchKernelGGL(gateup_one_kernel, dim3(T * k * (F / kBlock)), dim3(512), 0, st, A);
         if (F <= 2048u)
-            hipLaunchKernelGGL(down_one_kernel<2048u>, dim3(H / 16u), dim3(512), 0, st, A);
+            hipLaunchKernelGGL(down_one_kernel<2048u>, dim3(H / 16u, T), dim3(512), 0, st, A);
         else
-            hipLaunchKernelGGL(down_one_kernel<kOneFfn>, dim3(H / 16u), dim3(512), 0, st, A);
+            hipLaunchKernelGGL(down_one_kernel<kOneFfn>, dim3(H / 16u, T), dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
     const RowArgs R = row_args(ws.xq, ws.xs, hidden, T, H, scale_stride(H));
     if (T <= kSmallPlan) {
         const PlanArgs A{ws.lists, ws.token_index, ws.route_index, ids, experts, T, k, E, R};
         const dim3 grid(1u + (uint32_t)((R.blocks + 63u) / 64u));
-        if (k <= 8u)
-            hipLaunchKernelGGL(small_plan_kernel<8>, grid, dim3(1024), 0, st, A);
-        else
-            hipLaunchKernelGGL(small_plan_kernel<32>, grid, dim3(1024), 0, st, A);
+        const bool few = (T + 63u) / 64u * E <= kFewWords;
+        const auto plan = k <= 8u ? few ? small_plan_kernel<8, kFewWords> : small_plan_kernel<8, kMostWords>
+                          : few   ? small_plan_kernel<32, kFewWords>
+                                  : small_plan_kernel<32, kMostWords>;
+        hipLaunchKernelGGL(plan, grid, dim3(1024), 0, st, A);
     } else {
         if (!launch_rows(R, st)) return false;
         if (!k3_moe_route_plan(ws.counts, ws.offsets, ws.unique, ws.summary, ws.token_index,
@@ -1365,7 +1392,7 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
     B.lists = ws.lists, B.token_index = ws.token_index, B.route_index = ws.route_index;
     B.xq = ws.xq, B.xs = ws.xs, B.xstride = scale_stride(H);
     B.out = ws.y, B.hq = ws.hq, B.hs = ws.hs, B.hstride = scale_stride(F);
-    B.kind = s.activation, B.beta = s.beta, B.lb = s.linear_beta;
+    B.act = activation_of(s);
     B.N = F, B.K = H, B.tiles_n = F / kBlock;
     /* the classes' blocks are rounded up to eights */
     hipLaunchKernelGGL(experts_tile_kernel<kGateUp>, dim3(ws.tile_cap * B.tiles_n + 8u * kClasses),

@@ -84,7 +84,7 @@ def test_calls_on_two_streams_at_once(cuda):
 # ---- experts -------------------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("T", [255, 256, 257, 300])
+@pytest.mark.parametrize("T", [255, 256, 257, 300, 1000, 1024, 1025])
 @pytest.mark.parametrize("E,k", [(6, 4), (64, 8), (40, 32), (1024, 3)])
 def test_experts_plan(cuda, T, E, k):
     """Any ids: valid ones, repeats and ids of no expert."""
@@ -113,6 +113,16 @@ def test_experts_widths(cuda, H, F, T):
     check_experts(cuda, make_store(cuda, 3, H, F, 9), T, 2, ACT_SWIGLU, H + F)
 
 
+@pytest.mark.parametrize("T", [2, 8, 16, 31, 64, 65])
+@pytest.mark.parametrize("E,H,F,k", [(8, 256, 128, 8), (3, 2048, 1024, 2), (40, 384, 256, 9)])
+def test_experts_one_by_one_or_in_tiles(cuda, E, H, F, k, T):
+    """Any ids: valid ones, repeats and ids of no expert."""
+    ids = torch.randint(-1, E + 1, (T, k), generator=torch.Generator().manual_seed(T + E),
+                        dtype=torch.int32)
+    ids[T // 2] = E
+    check_experts(cuda, make_store(cuda, E, H, F, 9), T, k, ACT_SITU, H + T, ids=ids)
+
+
 @pytest.mark.parametrize("H,F", [(512, 256), (1152, 640)])
 def test_experts_bits_do_not_depend_on_the_batch(cuda, H, F):
     """A token alone, in a small and in a large batch."""
@@ -124,7 +134,7 @@ def test_experts_bits_do_not_depend_on_the_batch(cuda, H, F):
     w = torch.rand((T, k), generator=g).to(cuda)
     sh = fp8.shape(H, E, k, F, 1.0, ACT_SITU)
     want = fp8.experts(x, ids, w, store.table, sh, r)
-    for n in (1, 2, 30, 100, 256):
+    for n in (1, 2, 30, 100, 256, 399):
         got = fp8.experts(x[:n].contiguous(), ids[:n].contiguous(), w[:n].contiguous(), store.table, sh,
                           r[:n].contiguous())
         assert torch.equal(got, want[:n]), n
