@@ -1140,14 +1140,20 @@ __device__ __forceinline__ void list_tiles(const TileLists &Q, uint32_t &row, ui
     }
 }
 
+/* By the plan's counts and first rows, in block 0; the others encode the tokens'
+ * rows meanwhile. */
 __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t *__restrict__ counts,
                                                      const uint32_t *__restrict__ offsets,
                                                      const k3_moe_fp8_expert *__restrict__ experts,
-                                                     uint32_t E) {
+                                                     uint32_t E, RowArgs R) {
+    if (blockIdx.x != 0u) {
+        encode_block(R, (blockIdx.x - 1u) * 64u + (threadIdx.x >> 4));
+        return;
+    }
     const uint32_t e = threadIdx.x;
     const u32x4_8 *const ex = (const u32x4_8 *)(experts + min(e, E - 1u));
-    uint32_t row = offsets[min(e, E - 1u)], n = e < E ? counts[e] : 0u;
-    list_tiles<false>(Q, row, n, ex[0], ex[1], ex[2]);
+    uint32_t row = offsets[min(e, E - 1u)];
+    list_tiles<false>(Q, row, e < E ? counts[e] : 0u, ex[0], ex[1], ex[2]);
 }
 
 /* Up to 1024 tokens: the plan (k3_moe_route_plan's order) and the tiles as block
@@ -1372,21 +1378,20 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
         return hipGetLastError() == hipSuccess;
     }
     const RowArgs R = row_args(ws.xq, ws.xs, hidden, T, H, scale_stride(H));
+    const dim3 grid(1u + (uint32_t)((R.blocks + 63u) / 64u)); /* the plan's block, 64 blocks of rows each */
     if (T <= kSmallPlan) {
         const PlanArgs A{ws.lists, ws.token_index, ws.route_index, ids, experts, T, k, E, R};
-        const dim3 grid(1u + (uint32_t)((R.blocks + 63u) / 64u));
         const bool few = (T + 63u) / 64u * E <= kFewWords;
         const auto plan = k <= 8u ? few ? small_plan_kernel<8, kFewWords> : small_plan_kernel<8, kMostWords>
                           : few   ? small_plan_kernel<32, kFewWords>
                                   : small_plan_kernel<32, kMostWords>;
         hipLaunchKernelGGL(plan, grid, dim3(1024), 0, st, A);
     } else {
-        if (!launch_rows(R, st)) return false;
         if (!k3_moe_route_plan(ws.counts, ws.offsets, ws.unique, ws.summary, ws.token_index,
                                ws.route_index, ids, T, k, E, ws.plan, ws.plan_bytes, st))
             return false;
-        hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(1024), 0, st, ws.lists, ws.counts, ws.offsets,
-                           experts, E);
+        hipLaunchKernelGGL(tiles_kernel, grid, dim3(1024), 0, st, ws.lists, ws.counts, ws.offsets,
+                           experts, E, R);
     }
     TileArgs B{};
     B.lists = ws.lists, B.token_index = ws.token_index, B.route_index = ws.route_index;
