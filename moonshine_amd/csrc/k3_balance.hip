@@ -6,9 +6,9 @@
  *   balance_part_kernel    a block: a run of one segment's tokens, a token a
  *                          wave at a time; sums of the shares sigma / Z and
  *                          the counts of its run
- *   balance_join_kernel    a block: 16 experts of a segment; joins the runs,
- *                          writes counts and mean scores; the last block to
- *                          end adds up the loss
+ *   balance_join_kernel    joins the runs, writes counts and mean scores; the
+ *                          last block to end adds up the loss
+ *   balance_loss_kernel    adds up the loss of segments of one run each
  *   router_backward_kernel a token a wave at a time, the segment's f in
  *                          registers
  *
@@ -96,7 +96,39 @@ struct BalanceArgs {
     uint32_t *ticket;
 };
 
-template <int J>
+/* Expert e of segment s, with the sum m of its shares and its count c: written, and
+ * its term of the loss. n: the segment's live tokens. */
+__device__ __forceinline__ float close_expert(const BalanceArgs &A, uint32_t s, uint32_t e, float m,
+                                              uint32_t c, uint32_t n) {
+    m = n ? __fdiv_rn(m, (float)n) : 0.0f;
+    A.counts[(uint64_t)s * A.E + e] = c;
+    A.mean[(uint64_t)s * A.E + e] = m;
+    return n ? __fmul_rn(__fdiv_rn(__fmul_rn((float)c, (float)A.E), __fmul_rn((float)A.k, (float)n)), m)
+             : 0.0f;
+}
+/* The sum of v over a block of WAVES waves, in thread 0. */
+template <uint32_t WAVES>
+__device__ __forceinline__ float block_sum(float v) {
+    __shared__ float part[WAVES];
+    v = wave_sum(v);
+    if ((threadIdx.x & 63u) == 0u) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; w++) v = __fadd_rn(v, part[w]);
+    return v;
+}
+/* The loss from `n` partial ones, by a block of 1024 threads. */
+__device__ __forceinline__ void close_loss(const BalanceArgs &A, uint32_t n) {
+    float v = 0.0f;
+    for (uint32_t q = threadIdx.x; q < n; q += 1024u)
+        v = __fadd_rn(v, __hip_atomic_load(&A.part_loss[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    v = block_sum<16>(v);
+    if (threadIdx.x == 0u) *A.loss = __fmul_rn(v, __fdiv_rn(A.coef, (float)A.S));
+}
+
+/* WHOLE: a run is a segment, and the block writes what is the segment's. */
+template <int J, bool WHOLE>
 __global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A) {
     __shared__ float sums[kWaves][64 * J];
     __shared__ uint32_t hist[64 * J];
@@ -104,7 +136,7 @@ __global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
     const uint32_t s = blockIdx.x / A.runs, run = blockIdx.x % A.runs;
     const uint32_t i0 = run * A.span, i1 = min(i0 + A.span, A.L);
-    if (blockIdx.x == 0u && threadIdx.x == 0u) *A.ticket = 0u; /* for the next kernel */
+    if (!WHOLE && blockIdx.x == 0u && threadIdx.x == 0u) *A.ticket = 0u; /* for the next kernel */
     for (uint32_t e = threadIdx.x; e < 64u * J; e += 64u * kWaves) hist[e] = 0u;
     __syncthreads();
     float acc[J];
@@ -135,87 +167,106 @@ __global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A
     for (int j = 0; j < J; j++) sums[wave][64 * j + lane] = acc[j];
     if (lane == 0u) lives[wave] = live;
     __syncthreads();
+    uint32_t n = 0u;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; w++) n += lives[w];
     const uint64_t at = (uint64_t)blockIdx.x * E;
+    float l = 0.0f;
     for (uint32_t e = threadIdx.x; e < E; e += 64u * kWaves) {
         float v = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; w++) v = __fadd_rn(v, sums[w][e]);
-        A.part_mean[at + e] = v;
-        A.part_count[at + e] = hist[e];
+        if constexpr (WHOLE) {
+            l = __fadd_rn(l, close_expert(A, s, e, v, hist[e], n));
+        } else {
+            A.part_mean[at + e] = v;
+            A.part_count[at + e] = hist[e];
+        }
     }
-    if (threadIdx.x == 0u) {
-        uint32_t n = 0u;
-#pragma unroll
-        for (uint32_t w = 0; w < kWaves; w++) n += lives[w];
+    if constexpr (WHOLE) l = block_sum<kWaves>(l);
+    if (threadIdx.x != 0u) return;
+    if constexpr (WHOLE) {
+        A.live[s] = n;
+        if (A.S == 1u)
+            *A.loss = __fmul_rn(l, A.coef);
+        else
+            A.part_loss[s] = l;
+    } else {
         A.part_live[blockIdx.x] = n;
     }
 }
 
+/* The loss of segments whose blocks were whole: thousands of tickets would cost
+ * more than this launch (4096 segments of 64 tokens: 353 us with tickets). */
+__global__ __launch_bounds__(1024) void balance_loss_kernel(BalanceArgs A) { close_loss(A, A.S); }
+
+/* Joins the runs of a segment: 16 experts a block, 64 runs at a time, or (WIDE) all
+ * experts of a segment a block; the last block to end closes the loss. */
+template <bool WIDE>
 __global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs A) {
     __shared__ float fsum[16][kJoin];
     __shared__ uint32_t csum[16][kJoin];
     __shared__ uint32_t nsum[16];
     __shared__ uint32_t last;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
-    const uint32_t cols = (E + kJoin - 1u) / kJoin, s = blockIdx.x / cols;
-    const uint32_t i = lane % kJoin, e = kJoin * (blockIdx.x % cols) + i;
-    float m = 0.0f;
+    float m = 0.0f, l = 0.0f;
     uint32_t c = 0u, n = 0u;
-    for (uint32_t r = threadIdx.x; r < A.runs; r += 1024u) n += A.part_live[s * A.runs + r];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
-    if (e < E) {
+    if constexpr (WIDE) {
+        const uint32_t s = blockIdx.x, e = threadIdx.x;
         const uint64_t at = (uint64_t)s * A.runs * E + e;
+        for (uint32_t r = 0; r < A.runs; r++) n += A.part_live[s * A.runs + r];
+        if (e < E) {
 #pragma unroll 8
-        for (uint32_t r = threadIdx.x / kJoin; r < A.runs; r += 1024u / kJoin) {
-            m = __fadd_rn(m, A.part_mean[at + (uint64_t)r * E]);
-            c += A.part_count[at + (uint64_t)r * E];
+            for (uint32_t r = 0; r < A.runs; r++) {
+                m = __fadd_rn(m, A.part_mean[at + (uint64_t)r * E]);
+                c += A.part_count[at + (uint64_t)r * E];
+            }
+            l = close_expert(A, s, e, m, c, n);
         }
-    }
+        if (e == 0u) A.live[s] = n;
+        l = block_sum<16>(l);
+    } else {
+        const uint32_t cols = (E + kJoin - 1u) / kJoin, s = blockIdx.x / cols;
+        const uint32_t i = lane % kJoin, e = kJoin * (blockIdx.x % cols) + i;
+        for (uint32_t r = threadIdx.x; r < A.runs; r += 1024u) n += A.part_live[s * A.runs + r];
 #pragma unroll
-    for (int o = kJoin; o < 64; o <<= 1) {
-        m = __fadd_rn(m, __shfl_xor(m, o, 64));
-        c += __shfl_xor(c, o, 64);
-    }
-    if (lane < kJoin) fsum[wave][i] = m, csum[wave][i] = c;
-    if (lane == 0u) nsum[wave] = n;
-    __syncthreads();
-    if (wave == 0u) {
-        m = 0.0f, c = 0u, n = 0u;
+        for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
+        if (e < E) {
+            const uint64_t at = (uint64_t)s * A.runs * E + e;
+#pragma unroll 8
+            for (uint32_t r = threadIdx.x / kJoin; r < A.runs; r += 1024u / kJoin) {
+                m = __fadd_rn(m, A.part_mean[at + (uint64_t)r * E]);
+                c += A.part_count[at + (uint64_t)r * E];
+            }
+        }
 #pragma unroll
-        for (uint32_t w = 0; w < 16u; w++) {
-            m = __fadd_rn(m, fsum[w][i]);
-            c += csum[w][i];
-            n += nsum[w];
+        for (int o = kJoin; o < 64; o <<= 1) {
+            m = __fadd_rn(m, __shfl_xor(m, o, 64));
+            c += __shfl_xor(c, o, 64);
         }
-        m = n ? __fdiv_rn(m, (float)n) : 0.0f;
-        float l = 0.0f;
-        if (e < E && lane < kJoin) {
-            A.counts[(uint64_t)s * E + e] = c;
-            A.mean[(uint64_t)s * E + e] = m;
-            if (n) l = __fmul_rn(__fdiv_rn(__fmul_rn((float)c, (float)E), __fmul_rn((float)A.k, (float)n)), m);
-        }
-        if (e == 0u && lane == 0u) A.live[s] = n;
-        l = wave_sum(l);
-        if (lane == 0u) {
-            __hip_atomic_store(&A.part_loss[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            last = __hip_atomic_fetch_add(A.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-                   gridDim.x - 1u;
+        if (lane < kJoin) fsum[wave][i] = m, csum[wave][i] = c;
+        if (lane == 0u) nsum[wave] = n;
+        __syncthreads();
+        if (wave == 0u) {
+            m = 0.0f, c = 0u, n = 0u;
+#pragma unroll
+            for (uint32_t w = 0; w < 16u; w++) {
+                m = __fadd_rn(m, fsum[w][i]);
+                c += csum[w][i];
+                n += nsum[w];
+            }
+            if (e < E && lane < kJoin) l = close_expert(A, s, e, m, c, n);
+            if (e == 0u && lane == 0u) A.live[s] = n;
+            l = wave_sum(l);
         }
     }
-    __syncthreads();
-    if (!last) return;
-    float v = 0.0f;
-    for (uint32_t q = threadIdx.x; q < gridDim.x; q += 1024u)
-        v = __fadd_rn(v, __hip_atomic_load(&A.part_loss[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    v = wave_sum(v);
-    if (lane == 0u) fsum[wave][0] = v;
-    __syncthreads();
     if (threadIdx.x == 0u) {
-        v = 0.0f;
-        for (uint32_t w = 0; w < 16u; w++) v = __fadd_rn(v, fsum[w][0]);
-        *A.loss = __fmul_rn(v, __fdiv_rn(A.coef, (float)A.S));
+        __hip_atomic_store(&A.part_loss[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(A.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+               gridDim.x - 1u;
     }
+    __syncthreads();
+    if (last) close_loss(A, gridDim.x);
 }
 
 struct BackwardArgs {
@@ -342,6 +393,10 @@ size_t carve(BalanceArgs &A, void *base) {
 /* Two blocks a CU read a batch (their partial sums are another eighth of the
  * reads at 8192 tokens), four write its gradient. */
 constexpr uint32_t kPartBlocks = 512, kBackBlocks = 1024;
+/* Joins of a whole segment a block: of up to 16 runs, and where 16 experts a block
+ * would be more blocks than the chip holds at once (30 segments of 300 tokens,
+ * 1024 experts: loss 54 us so, 18.5 here). */
+constexpr uint32_t kFewRuns = 16, kJoinBlocks = 512;
 
 /* f(integral_constant<int, J>) for the least J here with E <= 64 J */
 template <int J = 1, class F>
@@ -384,11 +439,18 @@ extern "C" bool k3_moe_balance_loss_f32(float *loss, uint32_t *counts, float *me
     carve(A, scratch);
     const hipStream_t st = (hipStream_t)stream;
     with_slots(expert_count, [&](auto J) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(balance_part_kernel<decltype(J)::value>),
-                           dim3(segments * A.runs), dim3(64u * kWaves), 0, st, A);
+        constexpr int j = decltype(J)::value;
+        const auto part = A.runs == 1u ? balance_part_kernel<j, true> : balance_part_kernel<j, false>;
+        hipLaunchKernelGGL(part, dim3(segments * A.runs), dim3(64u * kWaves), 0, st, A);
     });
-    hipLaunchKernelGGL(balance_join_kernel, dim3(segments * ((expert_count + kJoin - 1u) / kJoin)), dim3(1024),
-                       0, st, A);
+    const uint32_t blocks = segments * ((expert_count + kJoin - 1u) / kJoin); /* of 16 experts */
+    if (A.runs == 1u) {
+        if (segments > 1u) hipLaunchKernelGGL(balance_loss_kernel, dim3(1), dim3(1024), 0, st, A);
+    } else if (A.runs <= kFewRuns || blocks > kJoinBlocks) {
+        hipLaunchKernelGGL(balance_join_kernel<true>, dim3(segments), dim3(1024), 0, st, A);
+    } else {
+        hipLaunchKernelGGL(balance_join_kernel<false>, dim3(blocks), dim3(1024), 0, st, A);
+    }
     return hipGetLastError() == hipSuccess;
 }
 

@@ -101,7 +101,8 @@ def test_one_segment(cuda, T, E, k):
 
 
 @pytest.mark.parametrize("segments,length,E,k", [(3, 17, 64, 4), (2, 1, 16, 2), (40, 9, 130, 6),
-                                                 (300, 5, 24, 3), (5, 333, 64, 4)])
+                                                 (300, 5, 24, 3), (5, 333, 64, 4), (30, 144, 1000, 8),
+                                                 (70, 40, 64, 6)])
 def test_masked_segments(cuda, segments, length, E, k):
     """Padded sequences: one whole, one empty, one of holes; a loss for each."""
     T = segments * length
