@@ -705,7 +705,10 @@ struct TileRun {
         const uint32_t base = lds_addr(smem), lo = a_slot(c, g), hi = a_slot(c, 4u + g);
         const uint32_t a_at = base + 8192u * wn, b_at = base + C::A + 2048u * wt;
         const uint32_t s_at = base + C::STAGES * C::STAGE + 16u * (16u * wt + c);
-        float w0 = 0.0f, w1 = 0.0f;
+        /* the weight scales of 64 blocks, in front of the loads whose waits they
+         * would otherwise drain */
+        float w0 = sw0[min(lane, nblk - 1u)], w1 = Two ? sw1[min(lane, nblk - 1u)] : 0.0f;
+        asm volatile("" ::: "memory");
         f32x4 p[2][4]; /* the products of a subtile and of the one before, and their factors */
         float f[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
         u32x4_t af[4][2], bf[2][2];
@@ -737,12 +740,13 @@ struct TileRun {
         if constexpr (C::EARLY) fetch<0, C::DA>(smem, 1u, 1u);
         /* stage 0: what was issued after it may stay out */
         wait_vm<C::EARLY ? C::DA : C::D *(C::STAGES - 2)>();
+        asm volatile("" : "+v"(w0), "+v"(w1));
         barrier();
         static_for<4>(read_a);
         read_b(std::integral_constant<int, 0>{});
         uint32_t slot = 0u, next = C::STAGES - 1;
         for (uint32_t s = 0; s < nblk; s++) {
-            if (s % 64u == 0u) { /* the weight scales of the next 64 blocks */
+            if (s % 64u == 0u && s != 0u) { /* of the next 64 blocks */
                 const uint32_t q = s + lane < nblk ? s + lane : nblk - 1u;
                 w0 = sw0[q];
                 if (Two) w1 = sw1[q];
@@ -842,7 +846,7 @@ __device__ __forceinline__ bool xcd_work(uint32_t L, uint32_t works, uint32_t &w
 }
 
 /* Block L of the `tiles` row tiles (list: the experts') x P.tiles_n column blocks. */
-template <class C, int MODE>
+template <class C, int MODE, uint32_t LDS>
 __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uint32_t L8, uint32_t tiles,
                                            const ExpertTile *list) {
     static_assert(MODE != kGateUp || C::WN == 4, "a gate/up block holds whole scale blocks");
@@ -945,6 +949,10 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
              * 16-byte pieces of whole rows; piece p of token r lies at p ^ r
              * modulo their number */
             constexpr uint32_t PIECES = C::BN / 8u;
+            /* read here once: a load in the loop of stores would wait for each */
+            static_assert(MODE != kDown || 2u * C::BN * C::BT + 4u * C::BT <= LDS, "tile and routes");
+            uint32_t *const route = (uint32_t *)(smem + 2u * C::BN * C::BT);
+            const uint32_t mine = MODE == kDown && threadIdx.x < rows ? P.route_index[row0 + threadIdx.x] : 0u;
             __syncthreads();
             static_for<C::TI>([&](auto J) {
                 constexpr int j = decltype(J)::value;
@@ -956,12 +964,13 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
                         bf16x4(acc[j][i]);
                 }
             });
+            if (MODE == kDown && threadIdx.x < C::BT) route[threadIdx.x] = mine;
             __syncthreads();
             const uint32_t width = min(C::BN, P.N - n0); /* a multiple of 8 */
             const uint32_t p = threadIdx.x % PIECES;
             if (8u * p < width)
                 for (uint32_t r = threadIdx.x / PIECES; r < rows; r += C::THREADS / PIECES) {
-                    const uint32_t t = MODE == kDown ? P.route_index[row0 + r] : row0 + r;
+                    const uint32_t t = MODE == kDown ? route[r] : row0 + r;
                     *(uint4 *)(P.out + (uint64_t)t * P.N + n0 + 8u * p) =
                         *(const uint4 *)(smem + 16u * (PIECES * r + (p ^ (r & (PIECES - 1u)))));
                 }
@@ -1023,7 +1032,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
 template <class C>
 __global__ __launch_bounds__(C::THREADS, 2) void product_tile_kernel(TileArgs P) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
-    tile_block<C, kDense>(P, smem, blockIdx.x, P.tiles_t, nullptr);
+    tile_block<C, kDense, C::LDS>(P, smem, blockIdx.x, P.tiles_t, nullptr);
 }
 
 using Tile32 = Tile<4, 1, 4>;
@@ -1056,10 +1065,10 @@ __global__ __launch_bounds__(512, 2) void experts_tile_kernel(TileArgs P) {
         else b -= blocks;
     }
     switch (cls) {
-    case 0: tile_block<Tile32, MODE>(P, smem, b, n[0], P.lists.tiles[0]); break;
-    case 1: tile_block<Tile64, MODE>(P, smem, b, n[1], P.lists.tiles[1]); break;
-    case 2: tile_block<Tile128, MODE>(P, smem, b, n[2], P.lists.tiles[2]); break;
-    case 3: tile_block<Tile256, MODE>(P, smem, b, n[3], P.lists.tiles[3]); break;
+    case 0: tile_block<Tile32, MODE, sizeof smem>(P, smem, b, n[0], P.lists.tiles[0]); break;
+    case 1: tile_block<Tile64, MODE, sizeof smem>(P, smem, b, n[1], P.lists.tiles[1]); break;
+    case 2: tile_block<Tile128, MODE, sizeof smem>(P, smem, b, n[2], P.lists.tiles[2]); break;
+    case 3: tile_block<Tile256, MODE, sizeof smem>(P, smem, b, n[3], P.lists.tiles[3]); break;
     }
 }
 
