@@ -127,7 +127,10 @@ __device__ __forceinline__ void close_loss(const BalanceArgs &A, uint32_t n) {
     if (threadIdx.x == 0u) *A.loss = __fmul_rn(v, __fdiv_rn(A.coef, (float)A.S));
 }
 
-/* WHOLE: a run is a segment, and the block writes what is the segment's. */
+/* WHOLE: a run is a segment, and the block writes what is the segment's. A row is
+ * read once into registers, where the wave adds up its scores and scales them.
+ * 8192 tokens of 896 experts: 11.5 us, 2.6 TB/s; of 64 experts the wave's sums over
+ * its lanes bound it (262144 tokens 54 us). */
 template <int J, bool WHOLE>
 __global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A) {
     __shared__ float sums[kWaves][64 * J];
@@ -201,7 +204,9 @@ __global__ __launch_bounds__(64 * kWaves) void balance_part_kernel(BalanceArgs A
 __global__ __launch_bounds__(1024) void balance_loss_kernel(BalanceArgs A) { close_loss(A, A.S); }
 
 /* Joins the runs of a segment: 16 experts a block, 64 runs at a time, or (WIDE) all
- * experts of a segment a block; the last block to end closes the loss. */
+ * experts of a segment a block; the last block to end closes the loss. 5.8 us for
+ * 512 runs of 896 experts: the latency of a read, of the ticket and of the partial
+ * losses. */
 template <bool WIDE>
 __global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs A) {
     __shared__ float fsum[16][kJoin];
@@ -280,10 +285,11 @@ struct BackwardArgs {
     uint32_t runs, span;
 };
 
-/* A row is stored twice over: its lanes store every expert that the token did
- * not choose, and lane r the one of route r, whose score it reads again (from
- * the cache) rather than through LDS: 27 us so with LDS rows of 64 KB a block
- * (two blocks a CU), 8192 tokens of 896 experts. */
+/* A row in registers again, its two sums, its gradient. Its lanes store every expert
+ * that the token did not choose, and lane r the one of route r, whose score it
+ * reads again (from the cache): handed over through LDS, rows of 64 KB a block
+ * left two blocks a CU and took 27 us for 8192 tokens of 896 experts, 19.2 here (3.1
+ * TB/s read and written; four waves' sums over their lanes hide the loads). */
 template <int J>
 __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(BackwardArgs A) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, E = A.E;
@@ -354,7 +360,8 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
 #pragma unroll
         for (int j = 0; j < J; j++) {
             const uint32_t q = lane + 64u * (uint32_t)j;
-            if ((j < whole_slots(J) || q < E) && !(chosen >> j & 1u)) out[q] = __fmul_rn(__fmul_rn(by, __fsub_rn(f[j], mean)), d[j]);
+            if ((j < whole_slots(J) || q < E) && !(chosen >> j & 1u))
+                out[q] = __fmul_rn(__fmul_rn(by, __fsub_rn(f[j], mean)), d[j]);
         }
     }
 }

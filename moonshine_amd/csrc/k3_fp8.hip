@@ -88,7 +88,8 @@ __device__ __forceinline__ float max8(const float (&v)[8]) {
 
 /* Sixteen lanes a block of 128 values, eight values a lane: one 16-byte load
  * (bf16), a maximum within a row of lanes, one 8-byte store. Scales: nblk of a
- * row, rows `stride` apart. Block q of the `blocks`, a row of lanes each. */
+ * row, rows `stride` apart. Block q of the `blocks`, a row of lanes each. Bound by
+ * memory: 8192 x 7168 in 30.8 us, 5.8 TB/s of bf16 read and codes written. */
 struct RowArgs {
     uint8_t *codes;
     float *scales;
@@ -117,7 +118,9 @@ __global__ __launch_bounds__(256) void rows_kernel(RowArgs A) {
 }
 
 /* One block of 256 threads a 128 x 128 block: thread t holds eight columns of
- * rows t / 16 + 16 m; rows past the last are left out. */
+ * rows t / 16 + 16 m; rows past the last are left out. The block stays in registers
+ * between its maximum and its codes, so memory is read once: 4100 x 7168 in 15.3
+ * us, 5.8 TB/s. */
 __global__ __launch_bounds__(256) void weight_kernel(uint8_t *__restrict__ codes,
                                                      float *__restrict__ scales,
                                                      const uint16_t *__restrict__ src,
@@ -222,7 +225,7 @@ __device__ __forceinline__ float act_f32(float g, float u, const Activation &A) 
 /* ---------------------------------------------------------------------- */
 
 /* A row of scales, 64 at a time by the lanes of a wave (those from base on):
- * loaded one by one, each block of columns would wait for its own. */
+ * loaded one at a time, each block of columns would wait for its own. */
 __device__ __forceinline__ float lane_scales(const float *row, uint32_t base, uint32_t n) {
     const uint32_t k = base + (threadIdx.x & 63u);
     return row[k < n ? k : n - 1u];
@@ -308,26 +311,34 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-/* A block of 512 threads encodes up to 64 blocks of 128 values into LDS: codes at
- * `codes`, scales at `scales` (LDS addresses). Loads first, so that what is
- * issued between the two halves does not stand in their way. */
+/* 16 lanes' part of an encoding: eight of a block's 128 values each, to codes and
+ * (the first lane) its scale at LDS addresses. */
+__device__ __forceinline__ void encode_lds(const float (&u)[8], uint32_t codes, uint32_t scale_at, bool first) {
+    float scale, inv;
+    fp8_scales(row_group_max<16>(max8(u)), scale, inv);
+    ds_write8(codes, fp8_codes8(u, inv));
+    if (first) ds_write4(scale_at, __float_as_uint(scale));
+}
+
+/* THREADS threads encode up to PER times as many pieces of eight values into LDS:
+ * codes at `codes`, scales at `scales` (LDS addresses). Loads first, so that what
+ * is issued between the two halves does not stand in their way. */
+template <uint32_t THREADS, uint32_t PER>
 struct TokenPart {
-    uint4 v[2];
+    uint4 v[PER];
     __device__ __forceinline__ void load(const uint16_t *x, uint32_t n) {
 #pragma unroll
-        for (uint32_t i = 0; i < 2u; i++) /* past the end the last ones again */
-            v[i] = ((const uint4 *)x)[min(threadIdx.x + 512u * i, 16u * n - 1u)];
+        for (uint32_t i = 0; i < PER; i++) /* past the end the last ones again */
+            v[i] = ((const uint4 *)x)[min(threadIdx.x + THREADS * i, 16u * n - 1u)];
     }
     __device__ __forceinline__ void encode(uint32_t n, uint32_t codes, uint32_t scales) const {
 #pragma unroll
-        for (uint32_t i = 0; i < 2u; i++) {
-            const uint32_t q = threadIdx.x + 512u * i;
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t q = threadIdx.x + THREADS * i;
             if (q >= 16u * n) continue; /* whole rows of 16 lanes */
-            float u[8], scale, inv;
+            float u[8];
             unpack8(v[i], u);
-            fp8_scales(row_group_max<16>(max8(u)), scale, inv);
-            ds_write8(codes + 8u * q, fp8_codes8(u, inv));
-            if ((q & 15u) == 0u) ds_write4(scales + (q >> 2), __float_as_uint(scale));
+            encode_lds(u, codes + 8u * q, scales + (q >> 2), (q & 15u) == 0u);
         }
     }
 };
@@ -367,7 +378,7 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
     const float *ws = P.scales + (uint64_t)(n0 / kBlock) * nblk;
     /* lane q: the scale of the wave's q-th block of 64 */
     float sw = ws[min(wave + 8u * (lane & 7u), nblk - 1u)];
-    TokenPart x[NT];
+    TokenPart<512u, 2u> x[NT]; /* 64 blocks */
 #pragma unroll
     for (uint32_t t = 0; t < NT; t++) x[t].load(P.x + (uint64_t)min(t, P.T - 1u) * P.K, min(64u, nblk));
     asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
@@ -431,42 +442,44 @@ struct OneExpertArgs {
     const float *weights;
     const uint16_t *x, *residual;
     uint16_t *out;
-    uint8_t *hq; /* [k, F] */
-    float *hs;   /* [k], hstride apart */
-    uint32_t hstride, H, F, E, k;
+    float *h; /* [T k, F] */
+    uint32_t H, F, E, k;
     Activation act;
 };
 
 /*
- * Gate and up of 128 columns for one route of a single token: 16 columns of each
- * a wave over the whole of K, 16 KB of weights in flight a wave. The 128 columns
- * are a scale block of the activation, encoded here. LDS: the rings, then the
- * token's codes and scales.
+ * Gate and up of one route of a token, WAVES times 16 columns a block: 16 columns of
+ * each a wave over the whole of K, RING blocks of 128 in flight. h is left in fp32,
+ * so that a block need not hold the 128 columns of one of its scales and one
+ * token's few columns reach every CU; the down kernel encodes it. LDS: the rings,
+ * then the token's codes and scales. Bound by the weights (hidden 7168, ffn 2048, 8
+ * experts: 41.8 us, 5.6 TB/s) and, of small layers, by the latency of the loads
+ * (2048, 512, 4 experts: 6.6 us).
  */
-constexpr int kGateUpRing = 4;
 constexpr uint32_t kOneHidden = 8192, kOneFfn = 4096; /* widths that a token's kernels hold in LDS */
-__global__ __launch_bounds__(512) void gateup_one_kernel(OneExpertArgs A) {
-    using Ring = WaveRing<2, kGateUpRing>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * Ring::BYTES + kOneHidden + kOneHidden / 32u];
-    __shared__ float red[8];
-    const uint32_t cols = A.F / kBlock, r = blockIdx.x / cols, col = blockIdx.x % cols, t = r / A.k;
-    TokenPart x;
+template <uint32_t WAVES, int RING, uint32_t MOST> /* H at most */
+__global__ __launch_bounds__(64 * WAVES) void gateup_one_kernel(OneExpertArgs A) {
+    using Ring = WaveRing<2, RING>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES * Ring::BYTES + MOST + MOST / 32u];
+    const uint32_t cols = A.F / (16u * WAVES), r = blockIdx.x / cols, t = r / A.k;
+    TokenPart<64u * WAVES, MOST / 8u / (64u * WAVES)> x;
     x.load(A.x + (uint64_t)t * A.H, A.H / kBlock);
     const uint32_t e = one_route(A.ids + t * A.k, r - t * A.k, A.k, A.E);
     if (e >= A.E) return;
     const k3_moe_fp8_expert ex = A.experts[e];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, nblk = A.H / kBlock;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t f0 = kBlock * col + 16u * wave;
-    const uint32_t codes = lds_addr(smem) + 8u * Ring::BYTES, scales = codes + A.H;
-    const float *gs = ex.gate_scales + (uint64_t)col * nblk, *us = ex.up_scales + (uint64_t)col * nblk;
+    const uint32_t f0 = 16u * (WAVES * (blockIdx.x % cols) + wave);
+    const uint32_t codes = lds_addr(smem) + WAVES * Ring::BYTES, scales = codes + A.H;
+    const uint64_t row = (uint64_t)(f0 / kBlock) * nblk;
+    const float *gs = ex.gate_scales + row, *us = ex.up_scales + row;
     float sg = lane_scales(gs, 0u, nblk), su = lane_scales(us, 0u, nblk);
     asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
     Ring ring;
     const uint8_t *const w[2] = {ex.gate_codes + (uint64_t)f0 * A.H, ex.up_codes + (uint64_t)f0 * A.H};
     ring.init(smem + Ring::BYTES * wave, w, 16u, A.H);
 #pragma unroll
-    for (uint32_t q = 0; q < kGateUpRing; q++) ring.fetch(min(q, nblk - 1u), q);
+    for (uint32_t q = 0; q < (uint32_t)RING; q++) ring.fetch(min(q, nblk - 1u), q);
     x.encode(nblk, codes, scales);
     asm volatile("" : "+v"(sg), "+v"(su)); /* waited for here, not in the loop */
     lds_barrier();
@@ -479,71 +492,76 @@ __global__ __launch_bounds__(512) void gateup_one_kernel(OneExpertArgs A) {
         after_wait(sx);
         const float fg = __fmul_rn(__uint_as_float(sx), scale_at(sg, k));
         const float fu = __fmul_rn(__uint_as_float(sx), scale_at(su, k));
-        ring.fetch(min(k + kGateUpRing, nblk - 1u), slot);
+        ring.fetch(min(k + RING, nblk - 1u), slot);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             gate[i] = fmaf(p[0][i], fg, gate[i]);
             up[i] = fmaf(p[1][i], fu, up[i]);
         }
-        slot = slot + 1u == (uint32_t)kGateUpRing ? 0u : slot + 1u;
+        slot = slot + 1u == (uint32_t)RING ? 0u : slot + 1u;
     }
     wait_vm<0>();
-    float h[4], m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        h[i] = act_f32(gate[i], up[i], A.act);
-        m = fmaxf(m, fabsf(h[i]));
-    }
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    if (lane == 0u) red[wave] = m;
-    __syncthreads();
     if ((lane & 15u) != 0u) return;
+    f32x4 h;
 #pragma unroll
-    for (int u = 0; u < 8; u++) m = fmaxf(m, red[u]);
-    float scale, inv;
-    fp8_scales(m, scale, inv);
-    *(uint32_t *)(A.hq + (uint64_t)r * A.F + f0 + 4u * g) =
-        e4m3x2_raw<true>(__fmul_rn(h[2], inv), __fmul_rn(h[3], inv),
-                         e4m3x2_raw<false>(__fmul_rn(h[0], inv), __fmul_rn(h[1], inv), 0u));
-    if (threadIdx.x == 0u) A.hs[(uint64_t)r * A.hstride + col] = scale;
+    for (int i = 0; i < 4; i++) h[i] = act_f32(gate[i], up[i], A.act);
+    *(f32x4 *)(A.h + (uint64_t)r * A.F + f0 + 4u * g) = h;
 }
 
 /*
- * A single token's output: 16 columns a block, a route a wave at a time (its
- * activation's codes in the wave's LDS), then the weighted
- * sum in rank order and the residual (as the batch's combine).
+ * A token's output: 16 columns a block, a route a wave at a time (its activation
+ * encoded into the wave's LDS under the first weight loads), then the weighted sum
+ * in rank order and the residual (as the batch's combine). 22.5 us for 8 routes of
+ * 7168 x 2048, 5.2 TB/s; 3.7 us for 4 of 2048 x 512.
  */
 constexpr int kDownRing = 3;
 template <uint32_t MOST> /* F at most: 2048 lets a CU hold two blocks */
 __global__ __launch_bounds__(512) void down_one_kernel(OneExpertArgs A) {
     using Ring = WaveRing<1, kDownRing>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * (Ring::BYTES + MOST)];
+    constexpr uint32_t kRow = MOST + 64u * (MOST / 2048u); /* codes and scales */
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * (Ring::BYTES + kRow)];
     __shared__ float y[32][16];
     __shared__ uint32_t live[32];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, nblk = A.F / kBlock;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = 16u * blockIdx.x;
-    uint8_t *mine = smem + (Ring::BYTES + MOST) * wave;
-    const uint32_t codes = lds_addr(mine) + Ring::BYTES;
+    uint8_t *mine = smem + (Ring::BYTES + kRow) * wave;
+    const uint32_t codes = lds_addr(mine) + Ring::BYTES, scales = codes + MOST;
     const uint32_t r0 = blockIdx.y * A.k; /* the token's first route */
     for (uint32_t r = wave; r < A.k; r += 8u) {
         const uint32_t e = one_route(A.ids + r0, r, A.k, A.E);
         if (lane == 0u) live[r] = e < A.E;
         if (e >= A.E) continue;
-        const uint8_t *h = A.hq + (uint64_t)(r0 + r) * A.F;
         const k3_moe_fp8_expert ex = A.experts[e];
         const float *ws = ex.down_scales + (uint64_t)(n0 / kBlock) * nblk;
         float f = lane_scales(ws, 0u, nblk); /* nblk <= 64 */
-        const float sx = lane_scales(A.hs + (uint64_t)(r0 + r) * A.hstride, 0u, nblk);
+        const f32x4 *h = (const f32x4 *)(A.h + (uint64_t)(r0 + r) * A.F);
+        constexpr uint32_t PER = MOST / 512u;
+        f32x4 v[PER][2];
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) { /* past the end the last ones again */
+            const uint32_t q = min(lane + 64u * i, A.F / 8u - 1u);
+            v[i][0] = h[2u * q], v[i][1] = h[2u * q + 1u];
+        }
         asm volatile("" ::: "memory"); /* issued before the weights, so that their wait leaves those out */
-        for (uint32_t o = 0; o < A.F; o += 1024u)
-            dma<16>(h + min(o + 16u * lane, A.F - 16u), mine + Ring::BYTES + o);
         Ring ring;
         const uint8_t *const w[1] = {ex.down_codes + (uint64_t)n0 * A.F};
         ring.init(mine, w, 16u, A.F);
 #pragma unroll
         for (uint32_t q = 0; q < kDownRing; q++) ring.fetch(min(q, nblk - 1u), q);
-        f = __fmul_rn(sx, f);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t q = lane + 64u * i;
+            if (q >= A.F / 8u) continue; /* whole rows of 16 lanes */
+            float u[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) u[j] = v[i][j >> 2][j & 3];
+            encode_lds(u, codes + 8u * q, scales + (q >> 2), (q & 15u) == 0u);
+        }
+        /* a wave's LDS operations are in order */
+        uint32_t sx = ds_read4<0>(scales + 4u * min(lane, nblk - 1u));
+        wait_lgkm<0>();
+        after_wait(sx);
+        f = __fmul_rn(__uint_as_float(sx), f);
         asm volatile("" : "+v"(f)); /* waited for here, not in the loop */
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         uint32_t slot = 0u;
@@ -607,9 +625,15 @@ struct TileLists {
  * them in a ring. A wave keeps its four weight fragments of a stage in
  * registers and streams the token fragments: four MFMAs with C = 0 each, whose
  * result goes into the fp32 accumulator with one fma per value under the factor
- * sx sw, one subtile later. Token scales
- * come four blocks at a time (16 bytes a token) into two buffers; the weights'
- * are held by the lanes of a wave, 64 blocks at a time, and read out by index.
+ * sx sw, one subtile later. Token scales come four blocks at a time (16 bytes a
+ * token) into two buffers; the weights' are held by the lanes of a wave, 64 blocks
+ * at a time, and read out by index.
+ *
+ * 4096 tokens, 7168 x 7168: 206 us, 2.04 PFLOP/s; gate/up and down of 4096 tokens
+ * (8 of 128 experts of 7168, 2048): 1.2 ms at 1.6 PFLOP/s and 0.72 ms at 1.34. The
+ * part holds its power there by its clock (1.75 to 2.0 GHz of 2.4): four fmas an
+ * MFMA on random data run at 3.5 PFLOP/s without any load or LDS. Tiles of fewer
+ * stages (down has 16) pay a block's start and its stores, some 5 us, more often.
  */
 template <int WN_, int TI_, int STAGES_>
 struct Tile {
@@ -759,8 +783,7 @@ struct TileRun {
             if constexpr (TL == 1) fetch<0, C::D>(smem, ahead, to);
             next = slot;
             slot = slot + 1u == (uint32_t)C::STAGES ? 0u : slot + 1u;
-            const float sw_0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w0), (int)(s & 63u)));
-            const float sw_1 = Two ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w1), (int)(s & 63u))) : sw_0;
+            const float sw_0 = scale_at(w0, s), sw_1 = Two ? scale_at(w1, s) : sw_0;
             static_for<TL>([&](auto J) {
                 constexpr int j = decltype(J)::value;
                 constexpr bool last = j + 1 == TL;
@@ -1073,7 +1096,9 @@ __global__ __launch_bounds__(512, 2) void experts_tile_kernel(TileArgs P) {
 }
 
 /* Output of a product whose K was split: the parts in their order. A block adds
- * one accumulator (token subtile j, fragment i) of every wave of a tile. */
+ * one accumulator (token subtile j, fragment i) of every wave of a tile, so that
+ * all CUs read: 4.2 us for 37 tokens of 7168 x 7168 in four parts (the last block of
+ * a tile alone would read its 128 KB in 5 us). */
 template <class C>
 __global__ __launch_bounds__(C::THREADS) void join_kernel(TileArgs P) {
     const uint32_t w = blockIdx.x / (4u * C::TI), ji = blockIdx.x % (4u * C::TI);
@@ -1136,7 +1161,8 @@ __device__ __forceinline__ void list_tiles(const TileLists &Q, uint32_t &row, ui
         total += tiles_of[w];
     }
     const uint32_t to = (uint32_t)(at >> (16u * cls)) & 0xffffu;
-    ExpertTile *const low = cls & 1u ? Q.tiles[1] : Q.tiles[0], *const high = cls & 1u ? Q.tiles[3] : Q.tiles[2];
+    ExpertTile *const low = cls & 1u ? Q.tiles[1] : Q.tiles[0];
+    ExpertTile *const high = cls & 1u ? Q.tiles[3] : Q.tiles[2];
     ExpertTile *const list = cls & 2u ? high : low;
     for (uint32_t i = 0; i < many; i++) {
         u32x4_8 *const t = (u32x4_8 *)(list + to + i);
@@ -1168,7 +1194,9 @@ __global__ __launch_bounds__(1024) void tiles_kernel(TileLists Q, const uint32_t
 /* Up to 1024 tokens: the plan (k3_moe_route_plan's order) and the tiles as block
  * 0's work, while the others encode the tokens' rows: five launches in one. Thread
  * t < T of block 0 holds token t's routes; an expert's rows are the set bits of
- * its masks, a word for each 64 tokens: WORDS of them at most. */
+ * its masks, a word for each 64 tokens: WORDS of them at most. 7.5 us for 61 tokens of
+ * 8 routes (three barriers, the ids' and descriptors' latency, two scans); six
+ * launches took 23 us. */
 constexpr uint32_t kSmallPlan = 1024, kFewWords = 4096, kMostWords = 16384;
 struct PlanArgs {
     TileLists lists;
@@ -1217,6 +1245,20 @@ __global__ __launch_bounds__(1024) void small_plan_kernel(PlanArgs A) {
     }
 }
 
+/* Whether a few tokens go through the experts one by one, in two launches. Tiles
+ * take four and read an expert once however many tokens chose it: 14 us or some
+ * 64 MB of weights read again, by the number of experts that T tokens choose if
+ * each chooses at random. (us, one by one and by tiles; hidden 2048, ffn 512, 4 of 64
+ * experts: 2 tokens 11.1 and 26.1, 8 tokens 22.4 and 32.1; 7168, 2048, 8 of 128:
+ * 2 tokens 126 and 134, 4 tokens level, 8 tokens 451 and 413.) */
+bool one_by_one(uint32_t T, const k3_moe_shape &s) {
+    if (T > 64u || s.hidden > kOneHidden || s.ffn > kOneFfn) return false;
+    double miss = 1.0; /* of an expert by all tokens */
+    for (uint32_t t = 0; t < T; t++) miss *= 1.0 - (double)s.top_k / s.expert_count;
+    const double again = (double)T * s.top_k - s.expert_count * (1.0 - miss);
+    return T == 1u || again * 3.0 * s.hidden * s.ffn < 64e6;
+}
+
 struct Fp8Workspace {
     uint32_t *ids;
     float *weights;                /* the layer's routes */
@@ -1226,7 +1268,7 @@ struct Fp8Workspace {
     TileLists lists;
     uint32_t tile_cap; /* most tiles of all classes */
     uint8_t *xq, *hq;
-    float *xs, *hs;
+    float *xs, *hs, *h;
     uint16_t *y;
     void *router;
     size_t router_bytes, bytes;
@@ -1266,6 +1308,7 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
     w.xs = (float *)take(4u * (size_t)T * scale_stride(s.hidden));
     w.hq = take(routes * s.ffn);
     w.hs = (float *)take(4u * routes * scale_stride(s.ffn));
+    w.h = (float *)take(one_by_one(T, s) ? 4u * routes * s.ffn : 0u);
     w.y = (uint16_t *)take(2u * routes * s.hidden);
     w.router_bytes = k3_moe_router_scratch_bytes(T, s.expert_count);
     w.router = take(w.router_bytes);
@@ -1327,7 +1370,8 @@ Cut cut_of(uint32_t T, uint32_t N, uint32_t K) {
         const TileCost &c = kTileCost[i];
         const uint32_t tt = (T + c.bt - 1u) / c.bt, tn = (N + c.bn - 1u) / c.bn;
         const uint64_t tiles = (uint64_t)tt * tn, padded = tiles * c.bt * c.bn;
-        for (uint32_t want = 1u; want <= groups && want <= 16u && (want == 1u || tiles * want <= 768u); want++) {
+        for (uint32_t want = 1u; want <= groups && want <= 16u; want++) {
+            if (want > 1u && tiles * want > 768u) break;
             const uint32_t span = 4u * ((groups + want - 1u) / want);
             const uint32_t splits = (4u * groups + span - 1u) / span;
             if (splits != want) continue; /* the same cut as a smaller number's */
@@ -1356,20 +1400,6 @@ bool launch_dense(TileArgs A, const Cut &q, hipStream_t st) {
     return hipGetLastError() == hipSuccess;
 }
 
-/* Whether a few tokens go through the experts one by one, in two launches. Tiles
- * take four and read an expert once however many tokens chose it: 14 us or some
- * 64 MB of weights read again, by the number of experts that T tokens choose if
- * each chooses at random. (us, one by one and by tiles; hidden 2048, ffn 512, 4 of 64
- * experts: 2 tokens 11.1 and 26.1, 8 tokens 22.4 and 32.1; 7168, 2048, 8 of 128:
- * 2 tokens 126 and 134, 4 tokens level, 8 tokens 451 and 413.) */
-bool one_by_one(uint32_t T, const k3_moe_shape &s) {
-    if (T > 64u || s.hidden > kOneHidden || s.ffn > kOneFfn) return false;
-    double miss = 1.0; /* of an expert by all tokens */
-    for (uint32_t t = 0; t < T; t++) miss *= 1.0 - (double)s.top_k / s.expert_count;
-    const double again = (double)T * s.top_k - s.expert_count * (1.0 - miss);
-    return T == 1u || again * 3.0 * s.hidden * s.ffn < 64e6;
-}
-
 /* The expert stage on given routes. */
 bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, const void *residual,
                      const uint32_t *ids, const float *wts, const k3_moe_fp8_expert *experts,
@@ -1377,9 +1407,17 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
     const uint32_t H = s.hidden, F = s.ffn, E = s.expert_count, k = s.top_k;
     if (one_by_one(T, s)) {
         const OneExpertArgs A{experts, ids, wts, (const uint16_t *)hidden, (const uint16_t *)residual,
-                              (uint16_t *)output, ws.hq, ws.hs, scale_stride(F), H, F, E, k,
+                              (uint16_t *)output, ws.h, H, F, E, k,
                               activation_of(s)};
-        hipLaunchKernelGGL(gateup_one_kernel, dim3(T * k * (F / kBlock)), dim3(512), 0, st, A);
+        /* the waves' columns over the whole chip while they are few (8 experts of
+         * 7168, 2048: 4 a block 41.8 us, 8 a block 48.9), 8 sharing a token's
+         * codes where there are many (8 tokens of 2048, 512, 4 experts: 22 us, 1 a
+         * block 27) */
+        const uint32_t all = T * k * (F / 16u), waves = all <= 512u && H <= 2048u ? 1u : all <= 1024u ? 4u : 8u;
+        const auto gateup = waves == 1u   ? gateup_one_kernel<1u, 16, 2048u>
+                            : waves == 4u ? gateup_one_kernel<4u, 8, kOneHidden>
+                                          : gateup_one_kernel<8u, 4, kOneHidden>;
+        hipLaunchKernelGGL(gateup, dim3(T * k * (F / (16u * waves))), dim3(64u * waves), 0, st, A);
         if (F <= 2048u)
             hipLaunchKernelGGL(down_one_kernel<2048u>, dim3(H / 16u, T), dim3(512), 0, st, A);
         else
@@ -1446,7 +1484,8 @@ extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scale
                                                     void *stream) {
     const uint64_t blocks = ((uint64_t)rows + kBlock - 1u) / kBlock * (columns / kBlock);
     if (!codes || !scales || !src || rows == 0u || columns == 0u || columns % kBlock != 0u ||
-        blocks >= (1ull << 24) || /* 2^32 threads */ ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
+        blocks >= (1ull << 24) || /* 2^32 threads */
+        ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
         ((uintptr_t)scales % 4u) != 0u)
         return false;
     hipLaunchKernelGGL(weight_kernel, dim3((uint32_t)blocks), dim3(256), 0, (hipStream_t)stream,
@@ -1474,7 +1513,8 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
         return false;
     /* blocks of one launch read all of the input and write their own columns */
     const uintptr_t in = (uintptr_t)input, to = (uintptr_t)output;
-    if (to < in + 2u * (uint64_t)vector_count * columns && in < to + 2u * (uint64_t)vector_count * rows) return false;
+    if (to < in + 2u * (uint64_t)vector_count * columns && in < to + 2u * (uint64_t)vector_count * rows)
+        return false;
     const size_t need = fp8_scratch_bytes(vector_count, rows, columns);
     if (need != 0u && (!scratch || scratch_bytes < need || ((uintptr_t)scratch % 256u) != 0u))
         return false;
