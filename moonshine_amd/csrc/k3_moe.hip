@@ -277,8 +277,9 @@ __device__ __forceinline__ float bf16_round(float v) { return bf16_to_f32(f32_to
  * a token costs one memory round trip. H % 8 == 0, rows 16-byte aligned. */
 constexpr uint32_t kCombineThreads = 128;
 
-/* ONCE: a token's repeated ids are skipped too (the plan gives them no row). */
-template <bool ONCE>
+/* ONCE: a token's repeated ids are skipped too (the plan gives them no row). K: k
+ * at most. */
+template <bool ONCE, int K>
 __global__ __launch_bounds__(128) void combine_kernel(
         uint16_t *__restrict__ out, const uint16_t *__restrict__ y,
         const uint16_t *__restrict__ residual, const uint32_t *__restrict__ ids,
@@ -287,9 +288,9 @@ __global__ __launch_bounds__(128) void combine_kernel(
     const uint32_t d = 8u * (blockIdx.x * kCombineThreads + threadIdx.x);
     if (!ONCE && d >= H) return;
     const uint64_t r0 = (uint64_t)t * k;
-    uint4 yv[32];
-    float w[32];
-    bool live[32];
+    uint4 yv[K];
+    float w[K];
+    bool live[K];
     uint32_t again = 0u; /* ranks that repeat an earlier one's id */
     if constexpr (ONCE) {
         const uint32_t lane = threadIdx.x & 63u, id = lane < k ? ids[r0 + lane] : E;
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(128) void combine_kernel(
         if (d >= H) return;
     }
 #pragma unroll
-    for (int r = 0; r < 32; r++) { /* route 0 stands in for r >= k */
+    for (int r = 0; r < K; r++) { /* route 0 stands in for r >= k */
         const uint64_t route = r0 + ((uint32_t)r < k ? (uint32_t)r : 0u);
         yv[r] = *(const uint4 *)(y + route * H + d);
         w[r] = wts[route];
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(128) void combine_kernel(
 #pragma unroll
     for (int i = 0; i < 8; i++) c[i] = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 32; r++) {
+    for (int r = 0; r < K; r++) {
         if (!live[r]) continue;
         const uint32_t u[4] = {yv[r].x, yv[r].y, yv[r].z, yv[r].w};
 #pragma unroll
@@ -341,12 +342,11 @@ bool k3::launch_combine(void *output, const uint16_t *y, const void *residual, c
                         const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E,
                         bool once, hipStream_t st) {
     const dim3 grid((H / 8u + kCombineThreads - 1u) / kCombineThreads, T);
-    if (once)
-        hipLaunchKernelGGL(combine_kernel<true>, grid, dim3(kCombineThreads), 0, st, (uint16_t *)output,
-                           y, (const uint16_t *)residual, ids, weights, H, k, E);
-    else
-        hipLaunchKernelGGL(combine_kernel<false>, grid, dim3(kCombineThreads), 0, st,
-                           (uint16_t *)output, y, (const uint16_t *)residual, ids, weights, H, k, E);
+    const auto combine = !once    ? combine_kernel<false, 32>
+                         : k <= 8u ? combine_kernel<true, 8>
+                                   : combine_kernel<true, 32>;
+    hipLaunchKernelGGL(combine, grid, dim3(kCombineThreads), 0, st, (uint16_t *)output, y,
+                       (const uint16_t *)residual, ids, weights, H, k, E);
     return hipGetLastError() == hipSuccess;
 }
 
