@@ -421,8 +421,8 @@ bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const vo
  * aligned (wider stores where the output and rows allow them); vector_count <=
  * 65535. scratch (256-byte aligned device memory):
  * k3_moe_fp8_128_scratch_bytes(vector_count, rows, columns) bytes, 0 where none
- * is needed (scratch may then be NULL). An output that overlaps the input is
- * refused.
+ * is needed (scratch may then be NULL); scratch of more vectors serves fewer. An
+ * output that overlaps the input is refused.
  */
 size_t k3_moe_fp8_128_scratch_bytes(uint32_t vector_count, uint32_t rows, uint32_t columns);
 bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, const float *scales,
@@ -452,8 +452,8 @@ typedef struct {
  * repeats an earlier rank's of its token, adds nothing, whatever its weight.
  * output may be hidden or residual itself. hidden and ffn multiples
  * of 128 up to 65536; output, hidden and residual 16-byte aligned; the workspace
- * 256-byte aligned, k3_moe_fp8_workspace_bytes(shape, T) bytes, no state kept
- * in it between calls; token_count <= 65535. expert_ids and expert_weights of
+ * 256-byte aligned, k3_moe_fp8_workspace_bytes(shape, T) bytes (those of more tokens serve
+ * fewer), no state kept in it between calls; token_count <= 65535. expert_ids and expert_weights of
  * the layer are optional copies of the routes.
  */
 size_t k3_moe_fp8_workspace_bytes(const k3_moe_shape *shape, uint32_t token_count);

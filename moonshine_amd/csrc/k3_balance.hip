@@ -366,11 +366,22 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
     }
 }
 
+/* Two blocks a CU read a batch (their partial sums are another eighth of the
+ * reads at 8192 tokens), four write its gradient. */
+constexpr uint32_t kPartBlocks = 512, kBackBlocks = 1024;
+/* Joins of a whole segment a block: of up to 16 runs, and where 16 experts a block
+ * would be more blocks than the chip holds at once (30 segments of 300 tokens,
+ * 1024 experts: loss 54 us so, 18.5 here). */
+constexpr uint32_t kFewRuns = 16, kJoinBlocks = 512;
+
 /* Runs a segment is cut into: about `blocks` in all, of `waves` tokens at
  * least. */
-void runs_of(uint32_t S, uint32_t L, uint32_t blocks, uint32_t waves, uint32_t &runs, uint32_t &span) {
+uint32_t most_runs(uint32_t S, uint32_t L, uint32_t blocks, uint32_t waves) {
     const uint32_t want = (blocks + S - 1u) / S, most = (L + waves - 1u) / waves;
-    runs = want < most ? want : most;
+    return want < most ? want : most;
+}
+void runs_of(uint32_t S, uint32_t L, uint32_t blocks, uint32_t waves, uint32_t &runs, uint32_t &span) {
+    runs = most_runs(S, L, blocks, waves);
     span = (L + runs - 1u) / runs;
     runs = (L + span - 1u) / span;
 }
@@ -388,7 +399,8 @@ size_t carve(BalanceArgs &A, void *base) {
         off += align256(n);
         return q;
     };
-    const size_t parts = (size_t)A.S * A.runs;
+    /* grows with the length: scratch of longer segments serves shorter ones */
+    const size_t parts = (size_t)A.S * most_runs(A.S, A.L, kPartBlocks, kWaves);
     A.part_mean = (float *)take(4u * parts * A.E);
     A.part_count = (uint32_t *)take(4u * parts * A.E);
     A.part_live = (uint32_t *)take(4u * parts);
@@ -396,14 +408,6 @@ size_t carve(BalanceArgs &A, void *base) {
     A.ticket = (uint32_t *)take(4u);
     return off;
 }
-
-/* Two blocks a CU read a batch (their partial sums are another eighth of the
- * reads at 8192 tokens), four write its gradient. */
-constexpr uint32_t kPartBlocks = 512, kBackBlocks = 1024;
-/* Joins of a whole segment a block: of up to 16 runs, and where 16 experts a block
- * would be more blocks than the chip holds at once (30 segments of 300 tokens,
- * 1024 experts: loss 54 us so, 18.5 here). */
-constexpr uint32_t kFewRuns = 16, kJoinBlocks = 512;
 
 /* f(integral_constant<int, J>) for the least J here with E <= 64 J */
 template <int J = 1, class F>

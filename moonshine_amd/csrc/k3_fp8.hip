@@ -1251,8 +1251,9 @@ __global__ __launch_bounds__(1024) void small_plan_kernel(PlanArgs A) {
  * each chooses at random. (us, one by one and by tiles; hidden 2048, ffn 512, 4 of 64
  * experts: 2 tokens 11.1 and 26.1, 8 tokens 22.4 and 32.1; 7168, 2048, 8 of 128:
  * 2 tokens 126 and 134, 4 tokens level, 8 tokens 451 and 413.) */
+constexpr uint32_t kOneTokensMost = 64;
 bool one_by_one(uint32_t T, const k3_moe_shape &s) {
-    if (T > 64u || s.hidden > kOneHidden || s.ffn > kOneFfn) return false;
+    if (T > kOneTokensMost || s.hidden > kOneHidden || s.ffn > kOneFfn) return false;
     double miss = 1.0; /* of an expert by all tokens */
     for (uint32_t t = 0; t < T; t++) miss *= 1.0 - (double)s.top_k / s.expert_count;
     const double again = (double)T * s.top_k - s.expert_count * (1.0 - miss);
@@ -1306,10 +1307,15 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
     w.lists.count = (uint32_t *)take(4u * kClasses);
     w.xq = take((size_t)T * s.hidden);
     w.xs = (float *)take(4u * (size_t)T * scale_stride(s.hidden));
+    const size_t from = off;
     w.hq = take(routes * s.ffn);
     w.hs = (float *)take(4u * routes * scale_stride(s.ffn));
-    w.h = (float *)take(one_by_one(T, s) ? 4u * routes * s.ffn : 0u);
     w.y = (uint16_t *)take(2u * routes * s.hidden);
+    /* tokens that go one by one need h instead; room for it whenever fewer tokens
+     * might, so that a workspace sized for more tokens serves them */
+    w.h = (float *)w.hq;
+    const size_t few = align256(4u * (size_t)(T < kOneTokensMost ? T : kOneTokensMost) * s.top_k * s.ffn);
+    if (s.hidden <= kOneHidden && s.ffn <= kOneFfn && off < from + few) off = from + few;
     w.router_bytes = k3_moe_router_scratch_bytes(T, s.expert_count);
     w.router = take(w.router_bytes);
     w.bytes = off;
@@ -1344,8 +1350,16 @@ bool launch_rows(const RowArgs &A, hipStream_t st) {
 struct Cut {
     int tile; /* 0 .. 4: Half32, Half64, Half128, Tile128, Tile256 */
     uint32_t tiles_t, tiles_n, splits, span;
-    size_t part_bytes;
 };
+
+/* Memory for the parts: no cut takes more, and the room kept for them grows with
+ * the tokens only, so that scratch sized for more tokens serves fewer. */
+constexpr size_t kMostParts = 32u << 20;
+constexpr uint32_t kMostSplits = 16;
+size_t parts_room(uint32_t T, uint32_t N) {
+    const uint64_t most = (T + 255ull) / 256u * ((N + 255ull) / 256u) * (65536u * 4u * kMostSplits);
+    return most < kMostParts ? most : kMostParts;
+}
 
 /*
  * The cheapest of all cuts, by what tiles cost on the part: nanoseconds of a
@@ -1370,8 +1384,8 @@ Cut cut_of(uint32_t T, uint32_t N, uint32_t K) {
         const TileCost &c = kTileCost[i];
         const uint32_t tt = (T + c.bt - 1u) / c.bt, tn = (N + c.bn - 1u) / c.bn;
         const uint64_t tiles = (uint64_t)tt * tn, padded = tiles * c.bt * c.bn;
-        for (uint32_t want = 1u; want <= groups && want <= 16u; want++) {
-            if (want > 1u && tiles * want > 768u) break;
+        for (uint32_t want = 1u; want <= groups && want <= kMostSplits; want++) {
+            if (want > 1u && (tiles * want > 768u || padded * want * 4u > kMostParts)) break;
             const uint32_t span = 4u * ((groups + want - 1u) / want);
             const uint32_t splits = (4u * groups + span - 1u) / span;
             if (splits != want) continue; /* the same cut as a smaller number's */
@@ -1380,7 +1394,7 @@ Cut cut_of(uint32_t T, uint32_t N, uint32_t K) {
             if (splits > 1u) ns += 3000u + padded * splits * 8u / 5000u;
             if (ns < least) {
                 least = ns;
-                best = Cut{i, tt, tn, splits, span, splits > 1u ? align256(padded * splits * 4u) : 0u};
+                best = Cut{i, tt, tn, splits, span};
             }
         }
     }
@@ -1462,7 +1476,7 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
     if (one_launch(T, rows)) return 0u; /* encoded by the product's own kernel */
     return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols)) +
-           cut_of(T, rows, cols).part_bytes;
+           parts_room(T, rows);
 }
 
 }  // namespace k3

@@ -8,6 +8,8 @@ import torch
 
 import _fp8 as R
 from moonshine_amd import _lib, balance, fp8
+from moonshine_amd._lib import K3MoeNativeShape
+from moonshine_amd.native import NativeConfig, routed_shape
 from moonshine_amd.synth import ACT_SITU, ACT_SWIGLU
 
 P = ctypes.c_void_p(1 << 20)  # never dereferenced: the checks fail first
@@ -35,7 +37,8 @@ def test_scratch_holds_the_encoded_rows(T, N, K):
 
 def test_scratch_refuses():
     f = _lib.lib().k3_moe_fp8_128_scratch_bytes
-    for bad in ((0, 1, 128), (65536, 1, 128), (1, 0, 128), (20, (1 << 24) + 1, 128), (20, 1, (1 << 24) + 128), (1, 1, 0), (1, 1, 64), (1, 1, 192)):
+    for bad in ((0, 1, 128), (65536, 1, 128), (1, 0, 128), (20, (1 << 24) + 1, 128),
+                (20, 1, (1 << 24) + 128), (1, 1, 0), (1, 1, 64), (1, 1, 192)):
         assert f(*bad) == 0
 
 
@@ -53,7 +56,8 @@ def test_product_refuses():
     L = _lib.lib()
     big = 1 << 40
     good = [P, P, P, P, 5, 64, 256, P, big]
-    for at, bad in ((0, None), (1, None), (2, None), (3, None), (4, 0), (4, 65536), (5, 0), (5, (1 << 24) + 1), (6, 0),
+    for at, bad in ((0, None), (1, None), (2, None), (3, None), (4, 0), (4, 65536), (5, 0),
+                    (5, (1 << 24) + 1), (6, 0),
                     (6, 64), (6, 200), (0, P.value + 1), (1, P.value + 8), (2, P.value + 2),
                     (3, P.value + 8)):
         args = list(good)
@@ -128,3 +132,26 @@ def test_wrappers_refuse_tensors_that_are_not_on_the_gpu():
         fp8.product(x, x, x)
     with pytest.raises(ValueError):
         balance.balance_loss(torch.zeros((2, 8)), torch.zeros((2, 1), dtype=torch.int32), 1.0)
+
+
+def test_scratch_for_more_serves_fewer():
+    """Sizes grow with the tokens: memory for the most tokens is enough for any."""
+    L = _lib.lib()
+    steps = list(range(1, 80)) + list(range(80, 1200, 7)) + [4096, 8191, 20000, 65535]
+    for n, k in ((16, 128), (576, 2048), (4096, 7168), (4100, 7168), (7168, 7168), (20000, 512)):
+        sizes = [L.k3_moe_fp8_128_scratch_bytes(t, n, k) for t in steps]
+        assert sizes == sorted(sizes), (n, k)
+    for kw in (dict(hidden=256, experts=8, top_k=2, ffn=128), dict(hidden=128, experts=64, top_k=6, ffn=2048),
+               dict(hidden=7168, experts=128, top_k=8, ffn=2048),
+               dict(hidden=8320, experts=4, top_k=4, ffn=256)):
+        s = ctypes.byref(fp8.shape(scaling_factor=1.0, activation=ACT_SWIGLU, **kw))
+        sizes = [L.k3_moe_fp8_workspace_bytes(s, t) for t in steps]
+        assert sizes == sorted(sizes), kw
+    for cfg in (NativeConfig("a", 1, 1024, 512, 64, 4, 256, 768),
+                NativeConfig("b", 1, 7168, 3584, 64, 4, 256, 4096)):
+        s = ctypes.byref(K3MoeNativeShape(routed_shape(cfg), cfg.hidden, cfg.shared, cfg.eps))
+        sizes = [L.k3_moe_native_workspace_bytes(s, t) for t in steps]
+        assert sizes == sorted(sizes), cfg
+    for segments in (1, 3, 40, 600):
+        sizes = [L.k3_moe_balance_scratch_bytes(segments, t, 64) for t in range(1, 9000, 13)]
+        assert sizes == sorted(sizes), segments
