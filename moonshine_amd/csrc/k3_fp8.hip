@@ -352,35 +352,42 @@ struct OneArgs {
 };
 
 /*
- * T <= NT tokens times a weight, 16 rows a block: its eight waves take every
- * eighth block of columns and add up through LDS in one order. The tokens are
- * encoded 64 blocks of columns at a time, by the block, under the first weight
- * loads; column c of the products is token min(c, NT - 1). Each block encodes the
- * tokens anew, which costs more the more blocks and tokens there are. us, here
- * and by tiles with a launch for the codes and one for the parts of K: 2048 x
- * 7168, 1 token 5.7 and 12.4, 4 tokens 7.4 and 12.4, 8 tokens 9.8 and 12.4; 7168
- * x 7168 12.7, 17.5, 22.6 and 20.3 (one token's weights at 4.1 TB/s and, of 2048
- * rows, 2.6: the first loads' latency is half of it).
+ * NT tokens (the last group's may be fewer) times a weight, 16 rows a block: its
+ * eight waves take every eighth block of columns and add up through LDS in one
+ * order. The tokens are encoded CHUNK blocks of columns at a time, by the block,
+ * under the first weight loads; column c of the products is token min(c, NT - 1).
+ * Each block encodes the tokens anew, which costs more the more blocks, tokens and
+ * columns there are. us, here and by tiles with a launch for the codes and one for
+ * the parts of K: 2048 x 7168, 1 token 5.7 and 12.4, 4 tokens 7.4 and 12.4, 8
+ * tokens 9.8 and 12.4; 7168 x 7168 12.7, 17.5, 22.6 and 20.3 (one token's weights
+ * at 4.1 TB/s and, of 2048 rows, 2.6: the first loads' latency is half of it); by 16
+ * tokens, from a graph: 512 x 2048, 16 tokens 5.9 and 7.8, 128 tokens 6.4 and 8.4; 1024
+ * x 4096, 64 tokens 8.6 and 9.4; 256 x 7168, 16 tokens 13.4 and 9.2.
  */
 constexpr int kOneRing = 4;
-constexpr uint32_t kOneTokens = 8;
-inline bool one_launch(uint32_t T, uint32_t N) { return T <= 4u || (T <= kOneTokens && N <= 4096u); }
-template <uint32_t NT>
+inline bool one_launch(uint32_t T, uint32_t N, uint32_t K) {
+    if (T <= 8u) return T <= 4u || N <= 4096u;
+    return K <= 4096u && (T + 15ull) / 16u * ((N + 15u) / 16u) <= 256u;
+}
+template <uint32_t NT, uint32_t CHUNK> /* blocks of columns encoded at a time: 64 or 32 */
 __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
     using Ring = WaveRing<1, kOneRing>;
-    constexpr uint32_t TOKEN = 64u * (kBlock + 4u); /* codes, then scales */
+    constexpr uint32_t TOKEN = CHUNK * (kBlock + 4u); /* codes, then scales */
+    static_assert(CHUNK == 64u || CHUNK == 32u, "whole turns of the waves, whole loads");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[8u * Ring::BYTES + NT * TOKEN];
     __shared__ float sums[8][NT][16];
+    const uint32_t t0 = NT * blockIdx.y, T = min(NT, P.T - t0);
     const uint32_t lane = threadIdx.x & 63u, nblk = P.K / kBlock, n0 = 16u * blockIdx.x;
     const uint32_t c = lane & 15u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t codes = lds_addr(smem) + 8u * Ring::BYTES;
     const uint32_t mine = codes + TOKEN * min(c, NT - 1u);
     const float *ws = P.scales + (uint64_t)(n0 / kBlock) * nblk;
-    /* lane q: the scale of the wave's q-th block of 64 */
+    /* lane q: the scale of the wave's q-th block of a chunk */
     float sw = ws[min(wave + 8u * (lane & 7u), nblk - 1u)];
-    TokenPart<512u, 2u> x[NT]; /* 64 blocks */
+    TokenPart<512u, CHUNK / 32u> x[NT];
 #pragma unroll
-    for (uint32_t t = 0; t < NT; t++) x[t].load(P.x + (uint64_t)min(t, P.T - 1u) * P.K, min(64u, nblk));
+    for (uint32_t t = 0; t < NT; t++)
+        x[t].load(P.x + (uint64_t)(t0 + min(t, T - 1u)) * P.K, min(CHUNK, nblk));
     asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
     Ring ring;
     const uint8_t *const w[1] = {P.codes + (uint64_t)n0 * P.K};
@@ -389,22 +396,22 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
     for (uint32_t q = 0; q < kOneRing; q++) ring.fetch(min(wave + 8u * q, nblk - 1u), q);
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     uint32_t slot = 0u;
-    for (uint32_t base = 0; base < nblk; base += 64u) {
-        const uint32_t n = min(64u, nblk - base);
+    for (uint32_t base = 0; base < nblk; base += CHUNK) {
+        const uint32_t n = min(CHUNK, nblk - base);
         if (base != 0u) {
             sw = ws[min(base + wave + 8u * (lane & 7u), nblk - 1u)];
 #pragma unroll
             for (uint32_t t = 0; t < NT; t++)
-                x[t].load(P.x + (uint64_t)min(t, P.T - 1u) * P.K + kBlock * base, n);
+                x[t].load(P.x + (uint64_t)(t0 + min(t, T - 1u)) * P.K + kBlock * base, n);
             lds_barrier(); /* the codes before have been read */
         }
 #pragma unroll
-        for (uint32_t t = 0; t < NT; t++) x[t].encode(n, codes + TOKEN * t, codes + TOKEN * t + 64u * kBlock);
+        for (uint32_t t = 0; t < NT; t++) x[t].encode(n, codes + TOKEN * t, codes + TOKEN * t + CHUNK * kBlock);
         asm volatile("" : "+v"(sw)); /* waited for here, not in the loop */
         lds_barrier();
         for (uint32_t k = wave, q = 0; k < n; k += 8u, q++) {
             f32x4 p[1];
-            uint32_t sx = ds_read4<64 * kBlock>(mine + 4u * k);
+            uint32_t sx = ds_read4<CHUNK * kBlock>(mine + 4u * k);
             ring.products(p, slot, mine + kBlock * k); /* waits for sx too */
             after_wait(sx);
             const float f = __fmul_rn(__uint_as_float(sx), scale_at(sw, q));
@@ -420,11 +427,11 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
         for (uint32_t r = 0; r < 4u; r++) sums[wave][c][4u * (lane >> 4) + r] = acc[r];
     __syncthreads();
     const uint32_t t = threadIdx.x >> 4, n = n0 + (threadIdx.x & 15u);
-    if (t < NT && t < P.T && n < P.N) {
+    if (t < T && n < P.N) {
         float v = 0.0f;
 #pragma unroll
         for (int u = 0; u < 8; u++) v = __fadd_rn(v, sums[u][t][threadIdx.x & 15u]);
-        P.out[(uint64_t)t * P.N + n] = f32_to_bf16(v);
+        P.out[(uint64_t)(t0 + t) * P.N + n] = f32_to_bf16(v);
     }
 }
 
@@ -1474,7 +1481,7 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
 }  // namespace
 
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
-    if (one_launch(T, rows)) return 0u; /* encoded by the product's own kernel */
+    if (one_launch(T, rows, cols)) return 0u; /* encoded by the product's own kernel */
     return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols)) +
            parts_room(T, rows);
 }
@@ -1534,18 +1541,16 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
         return false;
     const hipStream_t st = (hipStream_t)stream;
     const bool wide = rows % 4u == 0u && ((uintptr_t)output % 8u) == 0u;
-    if (one_launch(vector_count, rows)) {
+    if (one_launch(vector_count, rows, columns)) {
         const OneArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, vector_count, rows,
                         columns};
-        const dim3 grid((rows + 15u) / 16u);
-        if (vector_count == 1u)
-            hipLaunchKernelGGL(product_one_kernel<1u>, grid, dim3(512), 0, st, A);
-        else if (vector_count == 2u)
-            hipLaunchKernelGGL(product_one_kernel<2u>, grid, dim3(512), 0, st, A);
-        else if (vector_count <= 4u)
-            hipLaunchKernelGGL(product_one_kernel<4u>, grid, dim3(512), 0, st, A);
-        else
-            hipLaunchKernelGGL(product_one_kernel<8u>, grid, dim3(512), 0, st, A);
+        const auto product = vector_count == 1u   ? product_one_kernel<1u, 64u>
+                             : vector_count == 2u ? product_one_kernel<2u, 64u>
+                             : vector_count <= 4u ? product_one_kernel<4u, 64u>
+                             : vector_count <= 8u ? product_one_kernel<8u, 64u>
+                                                  : product_one_kernel<16u, 32u>;
+        const dim3 grid((rows + 15u) / 16u, vector_count <= 8u ? 1u : (vector_count + 15u) / 16u);
+        hipLaunchKernelGGL(product, grid, dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
     TileArgs B{};

@@ -65,10 +65,10 @@ def test_product_refuses():
         assert not L.k3_moe_fp8_128_gemm_bf16(*args, None), (at, bad)
     for at in (P.value + 16, P.value - 2, P.value + 2 * 5 * 256 - 2):  # an output over the input
         assert not L.k3_moe_fp8_128_gemm_bf16(at, P, P, P, 5, 64, 256, P, big, None), at
-    need = L.k3_moe_fp8_128_scratch_bytes(300, 64, 256)
+    need = L.k3_moe_fp8_128_scratch_bytes(300, 640, 256)
     assert need > 0
     for at, n in ((None, need), (P, need - 1), (P.value + 128, need)):
-        assert not L.k3_moe_fp8_128_gemm_bf16(P, P, P, P, 300, 64, 256, at, n, None)
+        assert not L.k3_moe_fp8_128_gemm_bf16(P, P, P, P, 300, 640, 256, at, n, None)
 
 
 def test_experts_refuse():

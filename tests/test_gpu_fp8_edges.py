@@ -22,6 +22,35 @@ def test_product_of_few_tokens(cuda, T, rows, cols):
     check_product(cuda, T, rows, cols, 7 * T + rows)
 
 
+# tokens and rows at the edges of groups of 16 in one launch, and of its bounds
+@pytest.mark.parametrize("T,rows,cols", [
+    (9, 16, 128), (9, 4096, 128), (15, 17, 4096), (16, 2048, 1152), (17, 31, 2048), (31, 512, 1024), (48, 1365, 384),
+    (64, 1024, 4096), (255, 256, 256), (256, 256, 128), (257, 256, 128), (4096, 16, 256), (4097, 16, 256)])
+def test_product_by_groups_of_16(cuda, T, rows, cols):
+    check_product(cuda, T, rows, cols, T + rows + 5)
+
+
+# tokens at the edges of 16-, 32-, 64- and 128-row tiles
+@pytest.mark.parametrize("T", [9, 16, 17, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129, 257])
+@pytest.mark.parametrize("rows,cols", [(4100, 128), (130, 4224), (4352, 640)])
+def test_product_tiles(cuda, T, rows, cols):
+    check_product(cuda, T, rows, cols, 11 * T + rows)
+
+
+@pytest.mark.parametrize("T", [20, 150, 300])
+def test_product_tiles_output_alignment(cuda, T):
+    """Outputs at 2, 8 and 16 bytes past a boundary, rows of 8 and of 4 columns: the same bits."""
+    x = normal((T, 256), T).to(cuda)
+    for rows in (4104, 4100, 4101):
+        wq, ws = fp8.quantize_weight(normal((rows, 256), T + 1, 0.02).to(cuda))
+        want = fp8.product(x, wq, ws)
+        for at in (1, 4, 8):
+            room = torch.full((T * rows + 16,), 3.0, dtype=torch.bfloat16, device=cuda)
+            fp8.product(x, wq, ws, out=room[at:at + T * rows].view(T, rows))
+            assert torch.equal(room[at:at + T * rows].view(T, rows), want)
+            assert (room[:at] == 3).all() and (room[at + T * rows:] == 3).all()
+
+
 # K whole and in 2 to 16 parts, the last one shorter; every height of tile
 @pytest.mark.parametrize("T,rows,cols", [
     (9, 130, 16384), (20, 257, 7296), (33, 1030, 2176), (37, 4100, 4224), (70, 129, 8192), (97, 2050, 1664),
