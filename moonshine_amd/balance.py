@@ -50,7 +50,8 @@ def router_backward(logits, ids, counts, live_tokens, coefficient, segments=1, m
                     dloss=None, dweights=None, scaling_factor=1.0, out=None):
     """The gradient by the logits, f32 [T, E]: of dloss (f32 [] on the device, or None for 1) times
     the loss, plus that of the route weights (scores of the ids, renormalized, times
-    scaling_factor) with gradient dweights f32 [T, k], or None for the loss alone."""
+    scaling_factor) with gradient dweights f32 [T, k], or None for the loss alone. out may be
+    logits itself."""
     device, x, i, m, T, E, k = _batch(logits, ids, segments, mask)
     c, n = _dense(counts, "counts", _I32, 2, device), _dense(live_tokens, "live_tokens", _I32, 1, device)
     if counts.shape != (segments, E) or live_tokens.shape != (segments,):
@@ -64,9 +65,11 @@ def router_backward(logits, ids, counts, live_tokens, coefficient, segments=1, m
             raise ValueError(f"dweights: {tuple(dweights.shape)}, wanted {(T, k)}")
     if out is None:
         out = logits.new_empty((T, E))
-    to = _dense(out, "out", _F32, 2, device)
-    if out.shape != (T, E):
-        raise ValueError(f"out: {tuple(out.shape)}, wanted {(T, E)}")
+        to = out.data_ptr()
+    else:
+        to = _dense(out, "out", _F32, 2, device)
+        if out.shape != (T, E):
+            raise ValueError(f"out: {tuple(out.shape)}, wanted {(T, E)}")
     _call(lib().k3_moe_router_backward_f32, device, to, x, i, c, n, m, dl, dw, segments, T // segments,
           E, k, coefficient, scaling_factor)
     return out

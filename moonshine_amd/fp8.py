@@ -77,7 +77,8 @@ def quantize_weight(w):
 
 
 def product(x, codes, scales, out=None):
-    """bf16 [T, cols] times an encoded weight [rows, cols] -> bf16 [T, rows]."""
+    """bf16 [T, cols] times an encoded weight [rows, cols] -> bf16 [T, rows]; out, if given, must
+    not overlap x."""
     at = _dense(x, "x", _BF16, 2)
     device = x.get_device()
     w, s = _dense(codes, "codes", _CODES, 2, device), _dense(scales, "scales", _F32, 2, device)
@@ -113,6 +114,14 @@ def _rows(t, name, shape, device):
     return at
 
 
+def _output(out, hidden, device):
+    """The output, a new one if None, and its address."""
+    if out is None:
+        out = hidden.new_empty(hidden.shape)
+        return out, out.data_ptr()
+    return out, _rows(out, "out", hidden.shape, device)
+
+
 def _workspace(shape, T, like):
     n = lib().k3_moe_fp8_workspace_bytes(ctypes.byref(shape), T)
     if n == 0:
@@ -124,7 +133,8 @@ def experts(hidden, ids, weights, table, shape, residual=None, out=None):
     """The expert stage on given routes: bf16 [T, H] -> bf16 [T, H].
 
     ids (int32) and weights (float32): [T, top_k]; table: int64 [E, 6] device
-    tensor of the experts' addresses (Fp8ExpertStore.table)."""
+    tensor of the experts' addresses (Fp8ExpertStore.table). out may be hidden or
+    residual itself."""
     x = _dense(hidden, "hidden", _BF16, 2)
     T, H = hidden.shape
     device = hidden.get_device()
@@ -137,9 +147,7 @@ def experts(hidden, ids, weights, table, shape, residual=None, out=None):
     if table.shape != (shape.expert_count, 6):
         raise ValueError("table: [experts, 6] is wanted")
     res = _rows(residual, "residual", hidden.shape, device)
-    if out is None:
-        out = hidden.new_empty((T, H))
-    to = _rows(out, "out", hidden.shape, device)
+    out, to = _output(out, hidden, device)
     keep, room, n = _workspace(shape, T, hidden)
     _call(lib().k3_moe_fp8_experts_bf16, device, to, x, res, i, w, t, ctypes.byref(shape), T, room, n)
     return out
@@ -205,9 +213,7 @@ class Fp8RoutedMoE:
         if H != self.shape.hidden:
             raise ValueError(f"hidden: {H} wide, the shape {self.shape.hidden}")
         res = _rows(residual, "residual", hidden.shape, device)
-        if out is None:
-            out = hidden.new_empty((T, H))
-        to = _rows(out, "out", hidden.shape, device)
+        out, to = _output(out, hidden, device)
         copies = []
         for t, name, dtypes in ((ids, "ids", _I32), (weights, "weights", _F32)):
             copies.append(None if t is None else _dense(t, name, dtypes, 2, device))
