@@ -435,8 +435,8 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
     }
 }
 
-/* Route r of a single token: its id, or E (none: from E on, or an earlier
- * one's). All ids come with one load. */
+/* Route r of a token: its id, or E (none: from E on, or an earlier one's). All ids
+ * come with one load. */
 __device__ __forceinline__ uint32_t one_route(const uint32_t *ids, uint32_t r, uint32_t k, uint32_t E) {
     const uint32_t lane = threadIdx.x & 63u, id = lane < k ? ids[lane] : E;
     const uint32_t e = (uint32_t)__builtin_amdgcn_readlane((int)id, (int)r);
@@ -875,9 +875,10 @@ __device__ __forceinline__ bool xcd_work(uint32_t L, uint32_t works, uint32_t &w
     return j8 < per && w < works;
 }
 
-/* Block L of the `tiles` row tiles (list: the experts') x P.tiles_n column blocks. */
+/* Work of `block` among `tiles` row tiles (list: the experts') x P.tiles_n column
+ * blocks (dense: x parts of K). LDS: bytes of smem. */
 template <class C, int MODE, uint32_t LDS>
-__device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uint32_t L8, uint32_t tiles,
+__device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uint32_t block, uint32_t tiles,
                                            const ExpertTile *list) {
     static_assert(MODE != kGateUp || C::WN == 4, "a gate/up block holds whole scale blocks");
     TileRun<C> R;
@@ -886,7 +887,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
     R.wn = R.wave % C::WN, R.wt = R.wave / C::WN;
     const uint32_t L = R.lane, K = P.K, nblk = K / kBlock;
     uint32_t w;
-    if (!xcd_work(L8, tiles * P.tiles_n * (MODE == kDense ? P.splits : 1u), w)) return;
+    if (!xcd_work(block, tiles * P.tiles_n * (MODE == kDense ? P.splits : 1u), w)) return;
     const uint32_t split = MODE == kDense ? w % P.splits : 0u; /* a part of K */
     if constexpr (MODE == kDense) w /= P.splits;
     uint32_t row0, rows, col;
