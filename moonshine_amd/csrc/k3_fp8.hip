@@ -987,6 +987,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
             __syncthreads();
             static_for<C::TI>([&](auto J) {
                 constexpr int j = decltype(J)::value;
+                if (32u * j >= rows) return;
                 const uint32_t r = 16u * (2u * j + R.wt) + c;
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; i++) {
@@ -1024,6 +1025,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
         uint8_t *rowbuf = smem + 16u * C::BT;   /* [BT][128] */
         static_for<C::TI>([&](auto J) {
             constexpr int j = decltype(J)::value;
+            if (32u * j >= rows) return; /* tokens that the tile has not */
             float m = 0.0f;
 #pragma unroll
             for (int i = 0; i < 2; i++)
@@ -1040,6 +1042,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
         __syncthreads();
         static_for<C::TI>([&](auto J) {
             constexpr int j = decltype(J)::value;
+            if (32u * j >= rows) return;
             const uint32_t r = 16u * (2u * j + R.wt) + c;
             float scale, inv;
             fp8_scales(fmaxf(fmaxf(red[r], red[C::BT + r]), fmaxf(red[2u * C::BT + r], red[3u * C::BT + r])),
