@@ -1139,8 +1139,9 @@ typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8))); /* two
 
 /* By a block of 1024 threads, thread e with expert e's n rows and descriptor (ex):
  * each class's tiles in expert order. `row` is the expert's first row; FIRST: it is
- * the sum of the earlier experts' n, and set here. The four classes' tiles are counted in 16
- * bits each of one word (65535 tokens of 32 routes are 9215 tiles at most). */
+ * the sum of the earlier experts' n, and set here. The four classes' tiles are
+ * counted in 16 bits each of one word (65535 tokens of 32 routes are 9215 tiles at
+ * most). */
 template <bool FIRST>
 __device__ __forceinline__ void list_tiles(const TileLists &Q, uint32_t &row, uint32_t n,
                                            u32x4_8 ex0, u32x4_8 ex1, u32x4_8 ex2) {
