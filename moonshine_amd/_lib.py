@@ -45,13 +45,6 @@ class K3MoeExpert(ctypes.Structure):
     ]
 
 
-class K3MoeFp8Expert(ctypes.Structure):
-    """k3_moe_fp8_expert (include/k3_moe.h)."""
-
-    _fields_ = [(n, _p) for n in ("gate_codes", "gate_scales", "down_codes", "down_scales",
-                                  "up_codes", "up_scales")]
-
-
 class K3MoeStaticWeight(ctypes.Structure):
     """k3_moe_static_weight (include/k3_moe.h)."""
 

@@ -23,7 +23,6 @@
  * c, so one factor scales all four.
  */
 #include "k3_device.h"
-#include "k3_fp8.h"
 #include "k3_internal.h"
 #include "k3_lds.h"
 #include "../../include/k3_moe.h"
@@ -1483,14 +1482,13 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
            launch_combine(output, ws.y, residual, ids, wts, T, H, k, E, true, st);
 }
 
-}  // namespace
-
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
     if (one_launch(T, rows, cols)) return 0u; /* encoded by the product's own kernel */
     return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols)) +
            parts_room(T, rows);
 }
 
+}  // namespace
 }  // namespace k3
 
 using namespace k3;

@@ -11,7 +11,6 @@
 #include "../../include/k3_moe.h"
 #include "../../include/k3_rocm_ops.h"
 #include "k3_decode.h"
-#include "k3_fp8.h"
 #include "k3_internal.h"
 #include "k3_topk.h"
 
