@@ -133,8 +133,9 @@ def experts(hidden, ids, weights, table, shape, residual=None, out=None):
     """The expert stage on given routes: bf16 [T, H] -> bf16 [T, H].
 
     ids (int32) and weights (float32): [T, top_k]; table: int64 [E, 6] device
-    tensor of the experts' addresses (Fp8ExpertStore.table). out may be hidden or
-    residual itself."""
+    tensor of the experts' addresses (Fp8ExpertStore.table; of a table made elsewhere
+    only the layout can be checked: codes at multiples of 16 bytes, scales of 4, on
+    hidden's device). out may be hidden or residual itself."""
     x = _dense(hidden, "hidden", _BF16, 2)
     T, H = hidden.shape
     device = hidden.get_device()
@@ -157,14 +158,18 @@ class Fp8ExpertStore:
     """All experts of one layer in FP8-128, and the device table of them.
 
     gate, up: (codes [E, F, H], scales [E, F / 128, H / 128]); down: (codes
-    [E, H, F], scales [E, H / 128, F / 128])."""
+    [E, H, F], scales [E, H / 128, F / 128]). Codes start at multiples of 16 bytes: a
+    matrix that lies elsewhere in a checkpoint's buffer is to be copied out first."""
 
     def __init__(self, gate, down, up):
         E, F, H = gate[0].shape
         for (codes, scales), name, rows, cols in ((gate, "gate", F, H), (down, "down", H, F),
                                                   (up, "up", F, H)):
-            _dense(codes, name, _CODES, 3, gate[0].get_device())
-            _dense(scales, name + " scales", _F32, 3, gate[0].get_device())
+            at = _dense(codes, name, _CODES, 3, gate[0].get_device())
+            scales_at = _dense(scales, name + " scales", _F32, 3, gate[0].get_device())
+            # the kernels load 16 codes at once; every expert's start as its matrix does
+            if at % 16 != 0 or scales_at % 4 != 0:
+                raise ValueError(f"{name}: codes at a multiple of 16 bytes and scales of 4 are wanted")
             if (rows % BLOCK != 0 or cols % BLOCK != 0 or codes.shape != (E, rows, cols)
                     or scales.shape != (E, rows // BLOCK, cols // BLOCK)):
                 raise ValueError(f"{name}: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
