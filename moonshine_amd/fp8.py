@@ -204,6 +204,8 @@ class Fp8RoutedMoE:
         self.cfg, self.shape, self.store = cfg, make_shape(cfg), store
         if (store.experts, store.hidden, store.ffn) != (cfg.experts, cfg.hidden, cfg.ffn):
             raise ValueError("the store's sizes are not the configuration's")
+        if store.table.device != router_weight.device:
+            raise ValueError(f"the store is on {store.table.device}, router_weight on {router_weight.device}")
         _dense(router_weight, "router_weight", _BF16, 2)
         _dense(router_bias, "router_bias", _F32, 1, router_weight.get_device())
         if router_weight.shape != (cfg.experts, cfg.hidden) or router_bias.shape != (cfg.experts,):

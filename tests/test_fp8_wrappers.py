@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from moonshine_amd import fp8
+from moonshine_amd.synth import Config
 
 E, F, H = 2, 128, 256
 
@@ -39,3 +40,14 @@ def test_store_refuses_codes_off_a_boundary_of_16_bytes(anywhere, name, at, dtyp
     m[name] = view_of_blob(codes, at).view(dtype), scales
     with pytest.raises(ValueError, match=name):
         fp8.Fp8ExpertStore(**m)
+
+
+def test_layer_refuses_a_store_on_another_device(anywhere):
+    m = matrices()
+    store = fp8.Fp8ExpertStore(**m)
+    router = torch.zeros((E, H), dtype=torch.bfloat16), torch.zeros(E)
+    cfg = Config("small", 1, H, E, 1, F)
+    fp8.Fp8RoutedMoE(cfg, *router, store)
+    store.table = store.table.to("meta")
+    with pytest.raises(ValueError, match="meta"):
+        fp8.Fp8RoutedMoE(cfg, *router, store)
