@@ -3,7 +3,10 @@
 balance_loss gives the balance loss of a batch with its per-expert counts and
 mean scores; router_backward the gradient of that loss, and of the route
 weights, by the router's logits. torch is used only for device memory and
-streams; each call takes its scratch from torch's allocator for itself.
+streams; each call takes its scratch from torch's allocator for itself. Autograd
+does not see them: logits that require a gradient are refused while gradients are
+recorded, rather than a loss returned that has none. In an autograd.Function,
+balance_loss goes in forward and router_backward, with dloss, in backward.
 """
 import torch
 

@@ -6,7 +6,9 @@ encoded weight, experts and Fp8RoutedMoE run routed experts held in it
 tensors. torch is used only for device memory and streams: everything runs in
 libk3moe.so, on the tensors' device and its current stream. Each call takes its
 scratch from torch's allocator for itself, so calls on different streams, and
-captured graphs, share none.
+captured graphs, share none. Autograd sees none of them: an input that requires a
+gradient is refused while gradients are recorded (quantizers give codes, which
+have none, and take any).
 """
 import ctypes
 
@@ -21,7 +23,7 @@ _CODES = (torch.float8_e4m3fn, torch.uint8)
 _BF16, _F32, _I32, _I64, _U8 = (torch.bfloat16,), (torch.float32,), (torch.int32,), (torch.int64,), (torch.uint8,)
 
 
-def _dense(t, name, dtypes, dim, device=None):
+def _layout(t, name, dtypes, dim, device=None):
     """The address of a contiguous tensor of one of `dtypes` on GPU `device` (any, if None)."""
     if (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and t.is_contiguous()
             and t.is_cuda and (device is None or t.get_device() == device)):
@@ -30,6 +32,21 @@ def _dense(t, name, dtypes, dim, device=None):
         f"{name}: a contiguous tensor of {dim} dimensions and {' or '.join(map(str, dtypes))} on GPU "
         f"{'' if device is None else device} is wanted"
         + (f", not {t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else ""))
+
+
+def _no_gradient(t, name):
+    """Refuses a tensor whose gradient autograd would be asked for: it would be missing in silence."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and autograd gets none through this call: pass "
+                         f"{name}.detach(), or call it under torch.no_grad() or in an autograd.Function")
+
+
+def _dense(t, name, dtypes, dim, device=None):
+    """_layout of a call's input that no gradient is wanted for."""
+    at = _layout(t, name, dtypes, dim, device)
+    if t.requires_grad:
+        _no_gradient(t, name)
+    return at
 
 
 # a call costs the host several microseconds, so device and stream are asked for directly
@@ -56,7 +73,7 @@ def _scratch(like, n):
 
 
 def _quantize(fn, x, block_rows):
-    at = _dense(x, "x", _BF16, 2)
+    at = _layout(x, "x", _BF16, 2)  # codes have no gradient, a weight to encode may require one
     rows, cols = x.shape
     if rows == 0 or cols == 0 or cols % BLOCK != 0:
         raise ValueError(f"x: {tuple(x.shape)}, columns in blocks of {BLOCK} are wanted")
@@ -165,8 +182,8 @@ class Fp8ExpertStore:
         E, F, H = gate[0].shape
         for (codes, scales), name, rows, cols in ((gate, "gate", F, H), (down, "down", H, F),
                                                   (up, "up", F, H)):
-            at = _dense(codes, name, _CODES, 3, gate[0].get_device())
-            scales_at = _dense(scales, name + " scales", _F32, 3, gate[0].get_device())
+            at = _layout(codes, name, _CODES, 3, gate[0].get_device())
+            scales_at = _layout(scales, name + " scales", _F32, 3, gate[0].get_device())
             # the kernels load 16 codes at once; every expert's start as its matrix does
             if at % 16 != 0 or scales_at % 4 != 0:
                 raise ValueError(f"{name}: codes at a multiple of 16 bytes and scales of 4 are wanted")
@@ -206,8 +223,8 @@ class Fp8RoutedMoE:
             raise ValueError("the store's sizes are not the configuration's")
         if store.table.device != router_weight.device:
             raise ValueError(f"the store is on {store.table.device}, router_weight on {router_weight.device}")
-        _dense(router_weight, "router_weight", _BF16, 2)
-        _dense(router_bias, "router_bias", _F32, 1, router_weight.get_device())
+        _layout(router_weight, "router_weight", _BF16, 2)
+        _layout(router_bias, "router_bias", _F32, 1, router_weight.get_device())
         if router_weight.shape != (cfg.experts, cfg.hidden) or router_bias.shape != (cfg.experts,):
             raise ValueError(f"router_weight {tuple(router_weight.shape)}, router_bias {tuple(router_bias.shape)}")
         self.router_weight, self.router_bias = router_weight, router_bias
@@ -215,6 +232,8 @@ class Fp8RoutedMoE:
     def forward(self, hidden, residual=None, out=None, ids=None, weights=None):
         """ids, weights: optional [T, top_k] tensors that receive the routes."""
         device = self.router_weight.get_device()
+        _no_gradient(self.router_weight, "router_weight")
+        _no_gradient(self.router_bias, "router_bias")
         x = _dense(hidden, "hidden", _BF16, 2, device)
         T, H = hidden.shape
         if H != self.shape.hidden:

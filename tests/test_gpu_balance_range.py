@@ -47,3 +47,31 @@ def test_gradient_of_low_scores(cuda, level, dloss, routes):
     off = (got - want).abs()
     bound = 1024 * U * size * sig * (1 - sig) + 1e-38
     assert torch.isfinite(got).all() and (off <= bound).all(), (off / bound).max()
+
+
+def test_in_an_autograd_function(cuda):
+    """balance_loss and router_backward as a Function: the gradient that autograd hands on is the
+    call's own, and without the Function logits that require a gradient are refused."""
+    class Balance(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, logits, ids, coef):
+            loss, counts, _, live = balance.balance_loss(logits, ids, coef)
+            ctx.save_for_backward(logits, ids, counts, live)
+            ctx.coef = coef
+            return loss
+
+        @staticmethod
+        def backward(ctx, dloss):
+            logits, ids, counts, live = ctx.saved_tensors
+            return balance.router_backward(logits, ids, counts, live, ctx.coef, dloss=dloss), None, None
+
+    g = torch.Generator().manual_seed(3)
+    logits = torch.randn((50, 24), generator=g).to(cuda).requires_grad_()
+    ids = logits.detach().topk(3, 1).indices.to(torch.int32)
+    with pytest.raises(ValueError, match="requires a gradient"):
+        balance.balance_loss(logits, ids, 0.4)
+    (1.5 * Balance.apply(logits, ids, 0.4)).backward()
+    x = logits.detach()
+    _, counts, _, live = balance.balance_loss(x, ids, 0.4)
+    want = balance.router_backward(x, ids, counts, live, 0.4, dloss=torch.tensor(1.5, device=cuda))
+    assert torch.equal(logits.grad, want) and want.abs().max() > 0
