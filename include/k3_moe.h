@@ -450,11 +450,12 @@ typedef struct {
  * encoded from fp32. residual may be NULL. experts is a DEVICE array of
  * expert_count descriptors. A route whose id is not below expert_count, or
  * repeats an earlier rank's of its token, adds nothing, whatever its weight.
- * output may be hidden or residual itself. hidden and ffn multiples
- * of 128 up to 65536; output, hidden and residual 16-byte aligned; the workspace
- * 256-byte aligned, k3_moe_fp8_workspace_bytes(shape, T) bytes (those of more tokens serve
- * fewer), no state kept in it between calls; token_count <= 65535. expert_ids and expert_weights of
- * the layer are optional copies of the routes.
+ * output may be hidden or residual itself; one over part of the residual is
+ * refused. hidden and ffn multiples of 128 up to 65536; output, hidden and
+ * residual 16-byte aligned; the workspace 256-byte aligned,
+ * k3_moe_fp8_workspace_bytes(shape, T) bytes (those of more tokens serve fewer),
+ * no state kept in it between calls; token_count <= 65535. expert_ids and
+ * expert_weights of the layer are optional copies of the routes.
  */
 size_t k3_moe_fp8_workspace_bytes(const k3_moe_shape *shape, uint32_t token_count);
 bool k3_moe_fp8_experts_bf16(void *output, const void *hidden, const void *residual,

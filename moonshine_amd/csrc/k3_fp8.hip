@@ -1536,8 +1536,7 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
         ((uintptr_t)output % 2u) != 0u)
         return false;
     /* blocks of one launch read all of the input and write their own columns */
-    const uintptr_t in = (uintptr_t)input, to = (uintptr_t)output;
-    if (to < in + 2u * (uint64_t)vector_count * columns && in < to + 2u * (uint64_t)vector_count * rows)
+    if (overlap(output, 2u * (uint64_t)vector_count * rows, input, 2u * (uint64_t)vector_count * columns))
         return false;
     const size_t need = fp8_scratch_bytes(vector_count, rows, columns);
     if (need != 0u && (!scratch || scratch_bytes < need || ((uintptr_t)scratch % 256u) != 0u))
@@ -1583,8 +1582,12 @@ namespace {
 bool fp8_args_ok(const void *output, const void *hidden, const void *residual,
                  const k3_moe_fp8_expert *experts, const k3_moe_shape *shape, uint32_t T,
                  const void *workspace) {
-    return output && hidden && experts && workspace && fp8_shape_ok(shape, T) &&
-           (((uintptr_t)output | (uintptr_t)hidden | (uintptr_t)residual) % 16u) == 0u &&
+    if (!output || !hidden || !experts || !workspace || !fp8_shape_ok(shape, T)) return false;
+    /* the last kernel's blocks read the residual and write the output, each its own
+     * columns of a token; hidden has been read by then */
+    const uint64_t bytes = 2u * (uint64_t)T * shape->hidden;
+    if (residual && residual != output && overlap(output, bytes, residual, bytes)) return false;
+    return (((uintptr_t)output | (uintptr_t)hidden | (uintptr_t)residual) % 16u) == 0u &&
            ((uintptr_t)experts % 8u) == 0u && ((uintptr_t)workspace % 256u) == 0u;
 }
 

@@ -91,6 +91,12 @@ bool launch_combine(void *output, const uint16_t *y, const void *residual, const
                     const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E, bool once,
                     hipStream_t stream);
 
+/* Whether two ranges of bytes have one in common. */
+inline bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+    const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;
+    return p < q + b_bytes && q < p + a_bytes;
+}
+
 /* Counter-based generator of the synthetic expert store. */
 __host__ __device__ inline uint64_t mix64(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;

@@ -1,0 +1,55 @@
+"""Outputs that share memory with an input: the buffer itself where the call allows it, any other
+overlap refused before a launch, neighbours allowed. (A refused call's memory is all its own, so
+the call would only race.)"""
+import pytest
+import torch
+
+from moonshine_amd import fp8
+from moonshine_amd.synth import ACT_SWIGLU
+from test_gpu_fp8 import layer, make_store, normal
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("T", [2, 40, 300])
+@pytest.mark.parametrize("rows", [1, -1])
+def test_experts_refuse_an_output_over_part_of_the_residual(cuda, T, rows):
+    E, H, F, k = 4, 128, 128, 2
+    store = make_store(cuda, E, H, F, 2)
+    x = normal((T, H), 1).to(cuda)
+    ids = torch.arange(k, dtype=torch.int32, device=cuda).repeat(T, 1)
+    w = torch.ones((T, k), device=cuda)
+    sh = fp8.shape(H, E, k, F, 1.0, ACT_SWIGLU)
+    room = normal((2 * T + 2, H), 3).to(cuda)
+    before = room.clone()
+    r = room[1:T + 1]
+    with pytest.raises(RuntimeError):
+        fp8.experts(x, ids, w, store.table, sh, r, out=room[1 + rows:T + 1 + rows])
+    with pytest.raises(RuntimeError):  # half a row
+        flat = room.view(-1)[H + H // 2:]
+        fp8.experts(x, ids, w, store.table, sh, r, out=flat[:T * H].view(T, H))
+    moe, y = layer(cuda, T, E=4, H=128, F=128, k=2)
+    with pytest.raises(RuntimeError):
+        moe.forward(y, r, out=room[1 + rows:T + 1 + rows])
+    assert torch.equal(room, before)
+    want = fp8.experts(x, ids, w, store.table, sh, r)
+    fp8.experts(x, ids, w, store.table, sh, r, out=room[T + 1:2 * T + 1])  # right behind it
+    assert torch.equal(room[T + 1:2 * T + 1], want) and torch.equal(r, before[1:T + 1])
+    fp8.experts(x, ids, w, store.table, sh, r, out=r)
+    assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("T", [2, 40, 300])
+def test_experts_over_the_hidden_rows(cuda, T):
+    """Every hidden row has been read before an output is written: any overlap is as good."""
+    E, H, F, k = 4, 128, 128, 2
+    store = make_store(cuda, E, H, F, 2)
+    ids = torch.arange(k, dtype=torch.int32, device=cuda).repeat(T, 1)
+    w = torch.ones((T, k), device=cuda)
+    sh = fp8.shape(H, E, k, F, 1.0, ACT_SWIGLU)
+    for at in (0, 1, 2):
+        room = normal((T + 2, H), 3).to(cuda)
+        x = room[1:T + 1]
+        want = fp8.experts(x, ids, w, store.table, sh)
+        fp8.experts(x, ids, w, store.table, sh, out=room[at:T + at])
+        assert torch.equal(room[at:T + at], want)
