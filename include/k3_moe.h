@@ -508,7 +508,7 @@ bool k3_moe_balance_loss_f32(float *loss, uint32_t *counts, float *mean_scores,
  * with f[s, e] = E counts[s, e] / (k N[s]); the ids and counts are constants,
  * as the choice of experts has no gradient. counts and live_tokens are
  * k3_moe_balance_loss_f32's. Rows of tokens that are not live are 0.
- * logits_gradient may be logits itself.
+ * logits_gradient may be logits itself; one over part of it is refused.
  */
 bool k3_moe_router_backward_f32(float *logits_gradient, const float *logits,
                                 const uint32_t *expert_ids, const uint32_t *counts,

@@ -17,6 +17,7 @@
  * partial loss in one order whichever block it is.
  */
 #include "k3_device.h"
+#include "k3_internal.h"
 #include "../../include/k3_moe.h"
 
 #include <hip/hip_runtime.h>
@@ -479,6 +480,9 @@ extern "C" bool k3_moe_router_backward_f32(float *logits_gradient, const float *
         (weight_gradient && !expert_ids) || !batch_ok(segments, length, expert_count) ||
         top_k == 0u || top_k > 32u || top_k > expert_count || !(scaling_factor > 0.0f))
         return false;
+    /* a wave reads its row whole before it writes it, and no other row */
+    const uint64_t bytes = 4ull * segments * length * expert_count;
+    if (logits_gradient != logits && overlap(logits_gradient, bytes, logits, bytes)) return false;
     BackwardArgs A{logits_gradient, logits, expert_ids, counts, live_tokens, mask, loss_gradient,
                    weight_gradient, segments, length, expert_count, top_k, coefficient,
                    scaling_factor, 0u, 0u};

@@ -4,7 +4,7 @@ the call would only race.)"""
 import pytest
 import torch
 
-from moonshine_amd import fp8
+from moonshine_amd import balance, fp8
 from moonshine_amd.synth import ACT_SWIGLU
 from test_gpu_fp8 import layer, make_store, normal
 
@@ -53,3 +53,24 @@ def test_experts_over_the_hidden_rows(cuda, T):
         want = fp8.experts(x, ids, w, store.table, sh)
         fp8.experts(x, ids, w, store.table, sh, out=room[at:T + at])
         assert torch.equal(room[at:T + at], want)
+
+
+@pytest.mark.parametrize("T,E", [(2, 8), (70, 200)])
+def test_router_gradient_refuses_part_of_the_logits(cuda, T, E):
+    g = torch.Generator().manual_seed(T)
+    room = torch.randn(2 * T * E + 2 * E, generator=g).to(cuda)
+    logits = room[E:E + T * E].view(T, E)
+    ids = logits.topk(2, 1).indices.to(torch.int32)
+    before = room.clone()
+    _, counts, _, live = balance.balance_loss(logits, ids, 0.3)
+
+    def gradient(at):
+        return balance.router_backward(logits, ids, counts, live, 0.3, out=room[at:at + T * E].view(T, E))
+
+    for at in (0, E - 1, E + 1, 2 * E, T * E):
+        with pytest.raises(RuntimeError):
+            gradient(at)
+    assert torch.equal(room, before)
+    want = balance.router_backward(logits, ids, counts, live, 0.3)
+    assert torch.equal(gradient(E + T * E), want) and torch.equal(logits, before[E:E + T * E].view(T, E))
+    assert torch.equal(gradient(E), want)
