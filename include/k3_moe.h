@@ -401,7 +401,8 @@ bool k3_moe_proj_mfma_bf16(void *output, const void *weights, const float *scale
  */
 
 /* Token rows: codes [rows, columns], scales f32 [rows, columns / 128].
- * columns % 128 == 0; src 16-byte, codes 8-byte, scales 4-byte aligned. */
+ * columns % 128 == 0; src 16-byte, codes 8-byte, scales 4-byte aligned, none over
+ * another (refused). */
 bool k3_moe_fp8_128_quantize_rows_bf16(uint8_t *codes, float *scales, const void *src,
                                        uint32_t rows, uint32_t columns, void *stream);
 

@@ -1493,12 +1493,20 @@ size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
 
 using namespace k3;
 
+/* Blocks read their values and write codes and scales in no order. */
+static bool encoded_apart(const uint8_t *codes, const float *scales, const void *src, uint64_t values,
+                          uint64_t scale_count) {
+    return !overlap(codes, values, src, 2u * values) && !overlap(scales, 4u * scale_count, src, 2u * values) &&
+           !overlap(codes, values, scales, 4u * scale_count);
+}
+
 extern "C" bool k3_moe_fp8_128_quantize_rows_bf16(uint8_t *codes, float *scales, const void *src,
                                                   uint32_t rows, uint32_t columns, void *stream) {
     const uint64_t blocks = (uint64_t)rows * (columns / kBlock);
     if (!codes || !scales || !src || rows == 0u || columns == 0u || columns % kBlock != 0u ||
         blocks > (1ull << 34) || ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
-        ((uintptr_t)scales % 4u) != 0u)
+        ((uintptr_t)scales % 4u) != 0u ||
+        !encoded_apart(codes, scales, src, (uint64_t)rows * columns, blocks))
         return false;
     return launch_rows(row_args(codes, scales, src, rows, columns, columns / kBlock), (hipStream_t)stream);
 }
@@ -1510,7 +1518,8 @@ extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scale
     if (!codes || !scales || !src || rows == 0u || columns == 0u || columns % kBlock != 0u ||
         blocks >= (1ull << 24) || /* 2^32 threads */
         ((uintptr_t)src % 16u) != 0u || ((uintptr_t)codes % 8u) != 0u ||
-        ((uintptr_t)scales % 4u) != 0u)
+        ((uintptr_t)scales % 4u) != 0u ||
+        !encoded_apart(codes, scales, src, (uint64_t)rows * columns, blocks))
         return false;
     hipLaunchKernelGGL(weight_kernel, dim3((uint32_t)blocks), dim3(256), 0, (hipStream_t)stream,
                        codes, scales, (const uint16_t *)src, rows, columns);

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from moonshine_amd import balance, fp8
+from moonshine_amd._lib import lib
 from moonshine_amd.synth import ACT_SWIGLU
 from test_gpu_fp8 import layer, make_store, normal
 
@@ -74,3 +75,28 @@ def test_router_gradient_refuses_part_of_the_logits(cuda, T, E):
     want = balance.router_backward(logits, ids, counts, live, 0.3)
     assert torch.equal(gradient(E + T * E), want) and torch.equal(logits, before[E:E + T * E].view(T, E))
     assert torch.equal(gradient(E), want)
+
+
+@pytest.mark.parametrize("entry", ["k3_moe_fp8_128_quantize_rows_bf16", "k3_moe_fp8_128_quantize_weight_bf16"])
+def test_quantizers_refuse_codes_or_scales_over_the_values(cuda, entry):
+    """Blocks of 128 values end before others are read: codes in the values' place would be read
+    as values."""
+    rows, cols = 200, 256
+    src = normal((rows, cols), 1).to(cuda)
+    n = 2 * rows * cols
+    room = torch.zeros(4 * n, dtype=torch.uint8, device=cuda)
+    room[n:2 * n] = src.view(torch.uint8).view(-1)
+    before, base = room.clone(), room.data_ptr()
+    run = lambda codes, scales, x=base + n: getattr(lib(), entry)(  # noqa: E731
+        codes, scales, x, rows, cols, torch.cuda.current_stream().cuda_stream)
+    away = base + 3 * n
+    for codes, scales in ((base + n, away), (base + n + n // 2, away), (base + n // 2 + 8, away),
+                          (base, base + n + 64), (base, base + n - 4), (base, base + 64)):
+        assert not run(codes, scales), (codes - base, scales - base)
+    assert torch.equal(room, before)
+    assert run(base + n // 2, away) and run(base + 2 * n, away)  # right before and behind the values
+    f = fp8.quantize_rows if "rows" in entry else fp8.quantize_weight
+    codes, scales = f(src)
+    for at in (n // 2, 2 * n):
+        assert torch.equal(room[at:at + n // 2], codes.view(torch.uint8).view(-1))
+    assert torch.equal(room[3 * n:3 * n + 4 * scales.numel()], scales.view(torch.uint8).view(-1))
