@@ -343,8 +343,12 @@ typedef struct {
     const k3_moe_expert  *experts;        /* [E], on the latent */
 } k3_moe_native_weights;
 
-/* Bytes of workspace k3_moe_native_forward_bf16 needs for token_count rows. */
+/* Bytes of workspace k3_moe_native_forward_bf16 needs for token_count rows: with
+ * bf16 and Q8-128 weights, and with the given ones, whose FP8-128 projections
+ * take scratch beside that (only kind is read of each). */
 size_t k3_moe_native_workspace_bytes(const k3_moe_native_shape *shape, uint32_t token_count);
+size_t k3_moe_native_weights_workspace_bytes(const k3_moe_native_weights *weights,
+                                             const k3_moe_native_shape *shape, uint32_t token_count);
 
 /* The layer above; expert_ids/expert_weights (nullable, [T, k]) receive
  * the routes. output, x and residual rows 16-byte aligned; precision as

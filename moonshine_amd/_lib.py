@@ -105,6 +105,8 @@ SIGNATURES = {
     "k3_rocm_add_bf16": (_b, [_p, _p, _p, _u64, _p]),
     "k3_moe_workspace_bytes": (_sz, [ctypes.POINTER(K3MoeShape), _u32]),
     "k3_moe_native_workspace_bytes": (_sz, [ctypes.POINTER(K3MoeNativeShape), _u32]),
+    "k3_moe_native_weights_workspace_bytes": (_sz, [ctypes.POINTER(K3MoeNativeWeights),
+                                                    ctypes.POINTER(K3MoeNativeShape), _u32]),
     "k3_moe_native_forward_bf16": (_b, [_p, _p, _p, ctypes.POINTER(K3MoeNativeWeights),
                                         ctypes.POINTER(K3MoeNativeShape), _u32, _u32, _p, _p,
                                         _p, _sz, _p, _p]),

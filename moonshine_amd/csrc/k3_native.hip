@@ -31,10 +31,11 @@ struct NativeWorkspace {
     void *experts;
     size_t expert_bytes, bytes;
     void *fp8[2]; /* scratch of the FP8-128 projections: the side stream's and the main one's */
-    size_t fp8_bytes;
+    size_t fp8_bytes[2];
 };
 
-NativeWorkspace carve(void *base, const k3_moe_native_shape &s, uint32_t T) {
+/* W (nullable: bf16 and Q8-128 weights): scratch is kept for its FP8-128 weights only. */
+NativeWorkspace carve(void *base, const k3_moe_native_shape &s, const k3_moe_native_weights *W, uint32_t T) {
     NativeWorkspace w{};
     uint8_t *p = (uint8_t *)base;
     size_t off = 0;
@@ -60,12 +61,19 @@ NativeWorkspace carve(void *base, const k3_moe_native_shape &s, uint32_t T) {
     w.sum = (uint16_t *)take(2u * T * H);
     w.expert_bytes = k3_moe_workspace_bytes(&s.routed, T);
     w.experts = take(w.expert_bytes);
-    const size_t fp8[4] = {k3_moe_fp8_128_scratch_bytes(T, (uint32_t)D, (uint32_t)H),
-                           k3_moe_fp8_128_scratch_bytes(T, (uint32_t)H, (uint32_t)D),
-                           k3_moe_fp8_128_scratch_bytes(T, (uint32_t)S, (uint32_t)H),
-                           k3_moe_fp8_128_scratch_bytes(T, (uint32_t)H, (uint32_t)S)};
-    for (size_t n : fp8) w.fp8_bytes = n > w.fp8_bytes ? n : w.fp8_bytes;
-    for (void *&q : w.fp8) q = take(w.fp8_bytes);
+    if (W) {
+        const auto widen = [&](int side, const k3_moe_static_weight &v, size_t rows, size_t cols) {
+            if (v.kind != K3_MOE_STATIC_FP8_128) return;
+            const size_t n = k3_moe_fp8_128_scratch_bytes(T, (uint32_t)rows, (uint32_t)cols);
+            if (n > w.fp8_bytes[side]) w.fp8_bytes[side] = n;
+        };
+        widen(0, W->routed_down, D, H);
+        widen(0, W->shared_gate, S, H);
+        widen(0, W->shared_up, S, H);
+        widen(1, W->routed_up, H, D);
+        widen(1, W->shared_down, H, S);
+    }
+    for (int side = 0; side < 2; side++) w.fp8[side] = take(w.fp8_bytes[side]);
     w.bytes = off;
     return w;
 }
@@ -91,7 +99,7 @@ bool project(const k3_moe_static_weight &w, void *out, const void *in, uint32_t 
              uint32_t precision, const NativeWorkspace &ws, int side, hipStream_t st) {
     if (w.kind == K3_MOE_STATIC_FP8_128)
         return k3_moe_fp8_128_gemm_bf16(out, (const uint8_t *)w.data, (const float *)w.scales, in, T,
-                                        w.rows, w.columns, ws.fp8[side], ws.fp8_bytes, st);
+                                        w.rows, w.columns, ws.fp8[side], ws.fp8_bytes[side], st);
     const bool q8 = w.kind == K3_MOE_STATIC_Q8_128;
     if (precision != K3_MOE_EXACT && T >= kProjMfmaMinTokens &&
         k3::proj_mfma_supported(T, w.rows, w.columns, q8, w.data, in))
@@ -111,11 +119,25 @@ bool shape_ok(const k3_moe_native_shape *s) {
 
 }  // namespace
 
+namespace {
+
+size_t workspace_bytes_of(const k3_moe_native_shape *shape, const k3_moe_native_weights *W, uint32_t T) {
+    if (!shape_ok(shape) || T == 0u || T > 65535u) return 0u;
+    if (k3_moe_workspace_bytes(&shape->routed, T) == 0u) return 0u;
+    return carve(nullptr, *shape, W, T).bytes;
+}
+
+}  // namespace
+
 extern "C" size_t k3_moe_native_workspace_bytes(const k3_moe_native_shape *shape,
                                                 uint32_t token_count) {
-    if (!shape_ok(shape) || token_count == 0u || token_count > 65535u) return 0u;
-    if (k3_moe_workspace_bytes(&shape->routed, token_count) == 0u) return 0u;
-    return carve(nullptr, *shape, token_count).bytes;
+    return workspace_bytes_of(shape, nullptr, token_count);
+}
+
+extern "C" size_t k3_moe_native_weights_workspace_bytes(const k3_moe_native_weights *weights,
+                                                        const k3_moe_native_shape *shape,
+                                                        uint32_t token_count) {
+    return weights ? workspace_bytes_of(shape, weights, token_count) : 0u;
 }
 
 /* Fork/join events of the shared-stream form: created once per host thread
@@ -167,7 +189,7 @@ extern "C" bool k3_moe_native_forward_bf16(void *output, const void *hidden, con
         !static_ok(W.shared_down, H, S))
         return false;
     if ((((uintptr_t)output | (uintptr_t)hidden | (uintptr_t)residual) % 16u) != 0u) return false;
-    const NativeWorkspace ws = carve(workspace, s, T);
+    const NativeWorkspace ws = carve(workspace, s, &W, T);
     if (workspace_bytes < ws.bytes || ((uintptr_t)workspace % kAlign) != 0u) return false;
     const hipStream_t st = (hipStream_t)stream;
     /* the side stream takes the latent projection and the shared expert's

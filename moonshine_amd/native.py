@@ -131,7 +131,8 @@ class NativeLayer:
         return sum(w.nbytes for w in self.statics().values())
 
     def workspace(self, tokens):
-        need = lib().k3_moe_native_workspace_bytes(ctypes.byref(self.shape), tokens)
+        need = lib().k3_moe_native_weights_workspace_bytes(ctypes.byref(self.weights),
+                                                           ctypes.byref(self.shape), tokens)
         if need == 0:
             raise ValueError("unsupported native shape or token count")
         if self._ws is None or self._ws.numel() < need:
