@@ -1363,12 +1363,19 @@ struct Cut {
     uint32_t tiles_t, tiles_n, splits, span;
 };
 
-/* Memory for the parts: no cut takes more, and the room kept for them grows with
- * the tokens only, so that scratch sized for more tokens serves fewer. */
+/* Memory for the parts of K, which no cut exceeds: up to 16 parts, 768 blocks, and
+ * tiles of 32, 64 or 128 rows for up to as many tokens (the cost rule alone picks
+ * nothing larger: replayed for 6.5 million sizes up to 7424 x 8192, 4200 tokens, and
+ * 20 million up to the limits). It grows with the tokens only, so that scratch sized
+ * for more of them serves fewer. 7168 x 7168: 12 MiB up to 32 tokens, 32 from 65 on. */
 constexpr size_t kMostParts = 32u << 20;
-constexpr uint32_t kMostSplits = 16;
-size_t parts_room(uint32_t T, uint32_t N) {
-    const uint64_t most = (T + 255ull) / 256u * ((N + 255ull) / 256u) * (65536u * 4u * kMostSplits);
+constexpr uint32_t kMostSplits = 16, kMostCutBlocks = 768;
+size_t parts_room(uint32_t T, uint32_t N, uint32_t K) {
+    const uint64_t groups = (K / kBlock + 3u) / 4u, splits = groups < kMostSplits ? groups : kMostSplits;
+    if (splits < 2u) return 0u;
+    const uint64_t height = T <= 32u ? 32u : T <= 64u ? 64u : T <= 128u ? 128u : (T + 255ull) / 256u * 256u;
+    const uint64_t width = (N + 255ull) / 256u * 256u * splits, cut = 128u * kMostCutBlocks;
+    const uint64_t most = 4u * height * (width < cut ? width : cut);
     return most < kMostParts ? most : kMostParts;
 }
 
@@ -1390,13 +1397,14 @@ constexpr TileCost kTileCost[5] = {{128, 32, 420, 340}, {128, 64, 490, 390}, {12
 Cut cut_of(uint32_t T, uint32_t N, uint32_t K) {
     const uint32_t groups = (K / kBlock + 3u) / 4u;
     Cut best{};
+    const uint64_t room = parts_room(T, N, K);
     uint64_t least = ~0ull;
     for (int i = 0; i < 5; i++) {
         const TileCost &c = kTileCost[i];
         const uint32_t tt = (T + c.bt - 1u) / c.bt, tn = (N + c.bn - 1u) / c.bn;
         const uint64_t tiles = (uint64_t)tt * tn, padded = tiles * c.bt * c.bn;
         for (uint32_t want = 1u; want <= groups && want <= kMostSplits; want++) {
-            if (want > 1u && (tiles * want > 768u || padded * want * 4u > kMostParts)) break;
+            if (want > 1u && (tiles * want > kMostCutBlocks || padded * want * 4u > room)) break;
             const uint32_t span = 4u * ((groups + want - 1u) / want);
             const uint32_t splits = (4u * groups + span - 1u) / span;
             if (splits != want) continue; /* the same cut as a smaller number's */
@@ -1485,7 +1493,7 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
     if (one_launch(T, rows, cols)) return 0u; /* encoded by the product's own kernel */
     return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols)) +
-           parts_room(T, rows);
+           parts_room(T, rows, cols);
 }
 
 }  // namespace
