@@ -424,7 +424,7 @@ bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scales, const vo
  * the blocks depends on the call's sizes only. columns % 128 == 0; rows and
  * columns <= 2^24; input and codes 16-byte, scales 4-byte, output 2-byte
  * aligned (wider stores where the output and rows allow them); vector_count <=
- * 65535. scratch (256-byte aligned device memory):
+ * 65535, vector_count * rows <= 2^38. scratch (256-byte aligned device memory):
  * k3_moe_fp8_128_scratch_bytes(vector_count, rows, columns) bytes, 0 where none
  * is needed (scratch may then be NULL); scratch of more vectors serves fewer. An
  * output that overlaps the input is refused.

@@ -1424,7 +1424,6 @@ template <class C>
 bool launch_dense(TileArgs A, const Cut &q, hipStream_t st) {
     A.tiles_t = q.tiles_t, A.tiles_n = q.tiles_n, A.splits = q.splits, A.span = q.span;
     const uint32_t tiles = q.tiles_t * q.tiles_n;
-    if ((uint64_t)tiles * q.splits >= (1u << 23)) return false; /* 2^32 threads: outputs of 2^33 values */
     hipLaunchKernelGGL(product_tile_kernel<C>, dim3(8u * ((tiles * q.splits + 7u) / 8u)),
                        dim3(C::THREADS), 0, st, A);
     if (q.splits == 1u) return hipGetLastError() == hipSuccess;
@@ -1490,6 +1489,14 @@ bool run_fp8_experts(const Fp8Workspace &ws, void *output, const void *hidden, c
            launch_combine(output, ws.y, residual, ids, wts, T, H, k, E, true, st);
 }
 
+/* 2^38 outputs (512 GiB) are half as many tiles as a launch takes: 2^23 blocks of 512
+ * threads are 2^32. */
+constexpr uint64_t kMostOutputs = 1ull << 38;
+bool product_ok(uint32_t T, uint32_t rows, uint32_t cols) {
+    return T != 0u && T <= 65535u && rows != 0u && rows <= kMostAxis && cols != 0u &&
+           cols % kBlock == 0u && cols <= kMostAxis && (uint64_t)T * rows <= kMostOutputs;
+}
+
 size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
     if (one_launch(T, rows, cols)) return 0u; /* encoded by the product's own kernel */
     return align256((size_t)T * cols) + align256(4u * (size_t)T * scale_stride(cols)) +
@@ -1497,6 +1504,9 @@ size_t fp8_scratch_bytes(uint32_t T, uint32_t rows, uint32_t cols) {
 }
 
 }  // namespace
+
+bool fp8_product_fits(uint32_t T, uint32_t rows, uint32_t cols) { return product_ok(T, rows, cols); }
+
 }  // namespace k3
 
 using namespace k3;
@@ -1536,9 +1546,7 @@ extern "C" bool k3_moe_fp8_128_quantize_weight_bf16(uint8_t *codes, float *scale
 
 extern "C" size_t k3_moe_fp8_128_scratch_bytes(uint32_t vector_count, uint32_t rows,
                                                uint32_t columns) {
-    if (vector_count == 0u || vector_count > 65535u || rows == 0u || rows > kMostAxis ||
-        columns == 0u || columns % kBlock != 0u || columns > kMostAxis)
-        return 0u;
+    if (!product_ok(vector_count, rows, columns)) return 0u;
     return fp8_scratch_bytes(vector_count, rows, columns);
 }
 
@@ -1546,9 +1554,7 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
                                          const void *input, uint32_t vector_count, uint32_t rows,
                                          uint32_t columns, void *scratch, size_t scratch_bytes,
                                          void *stream) {
-    if (!output || !codes || !scales || !input || vector_count == 0u || vector_count > 65535u ||
-        rows == 0u || rows > kMostAxis || columns == 0u || columns % kBlock != 0u ||
-        columns > kMostAxis ||
+    if (!output || !codes || !scales || !input || !product_ok(vector_count, rows, columns) ||
         (((uintptr_t)codes | (uintptr_t)input) % 16u) != 0u || ((uintptr_t)scales % 4u) != 0u ||
         ((uintptr_t)output % 2u) != 0u)
         return false;

@@ -91,6 +91,9 @@ bool launch_combine(void *output, const uint16_t *y, const void *residual, const
                     const float *weights, uint32_t T, uint32_t H, uint32_t k, uint32_t E, bool once,
                     hipStream_t stream);
 
+/* Whether k3_moe_fp8_128_gemm_bf16 takes a product of this size. */
+bool fp8_product_fits(uint32_t T, uint32_t rows, uint32_t cols);
+
 /* Whether two ranges of bytes have one in common. */
 inline bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
     const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;

@@ -32,6 +32,7 @@ struct NativeWorkspace {
     size_t expert_bytes, bytes;
     void *fp8[2]; /* scratch of the FP8-128 projections: the side stream's and the main one's */
     size_t fp8_bytes[2];
+    bool fp8_fits; /* the products take these sizes */
 };
 
 /* W (nullable: bf16 and Q8-128 weights): scratch is kept for its FP8-128 weights only. */
@@ -61,12 +62,14 @@ NativeWorkspace carve(void *base, const k3_moe_native_shape &s, const k3_moe_nat
     w.sum = (uint16_t *)take(2u * T * H);
     w.expert_bytes = k3_moe_workspace_bytes(&s.routed, T);
     w.experts = take(w.expert_bytes);
+    const auto widen = [&](int side, const k3_moe_static_weight &v, size_t rows, size_t cols) {
+        if (v.kind != K3_MOE_STATIC_FP8_128) return;
+        w.fp8_fits &= k3::fp8_product_fits(T, (uint32_t)rows, (uint32_t)cols);
+        const size_t n = k3_moe_fp8_128_scratch_bytes(T, (uint32_t)rows, (uint32_t)cols);
+        if (n > w.fp8_bytes[side]) w.fp8_bytes[side] = n;
+    };
+    w.fp8_fits = true;
     if (W) {
-        const auto widen = [&](int side, const k3_moe_static_weight &v, size_t rows, size_t cols) {
-            if (v.kind != K3_MOE_STATIC_FP8_128) return;
-            const size_t n = k3_moe_fp8_128_scratch_bytes(T, (uint32_t)rows, (uint32_t)cols);
-            if (n > w.fp8_bytes[side]) w.fp8_bytes[side] = n;
-        };
         widen(0, W->routed_down, D, H);
         widen(0, W->shared_gate, S, H);
         widen(0, W->shared_up, S, H);
@@ -82,8 +85,7 @@ bool static_ok(const k3_moe_static_weight &w, uint32_t rows, uint32_t cols) {
     if (!w.data || w.rows != rows || w.columns != cols) return false;
     if (w.kind == K3_MOE_STATIC_BF16) return true;
     if (w.kind == K3_MOE_STATIC_FP8_128 &&
-        (((uintptr_t)w.data % 16u) != 0u || ((uintptr_t)w.scales % 4u) != 0u ||
-         rows > (1u << 24) || cols > (1u << 24)))
+        (((uintptr_t)w.data % 16u) != 0u || ((uintptr_t)w.scales % 4u) != 0u))
         return false; /* as the product would: refused before the block's first launch */
     return w.kind <= K3_MOE_STATIC_FP8_128 && w.scales && cols % 128u == 0u;
 }
@@ -124,7 +126,8 @@ namespace {
 size_t workspace_bytes_of(const k3_moe_native_shape *shape, const k3_moe_native_weights *W, uint32_t T) {
     if (!shape_ok(shape) || T == 0u || T > 65535u) return 0u;
     if (k3_moe_workspace_bytes(&shape->routed, T) == 0u) return 0u;
-    return carve(nullptr, *shape, W, T).bytes;
+    const NativeWorkspace ws = carve(nullptr, *shape, W, T);
+    return ws.fp8_fits ? ws.bytes : 0u;
 }
 
 }  // namespace
@@ -190,7 +193,7 @@ extern "C" bool k3_moe_native_forward_bf16(void *output, const void *hidden, con
         return false;
     if ((((uintptr_t)output | (uintptr_t)hidden | (uintptr_t)residual) % 16u) != 0u) return false;
     const NativeWorkspace ws = carve(workspace, s, &W, T);
-    if (workspace_bytes < ws.bytes || ((uintptr_t)workspace % kAlign) != 0u) return false;
+    if (!ws.fp8_fits || workspace_bytes < ws.bytes || ((uintptr_t)workspace % kAlign) != 0u) return false;
     const hipStream_t st = (hipStream_t)stream;
     /* the side stream takes the latent projection and the shared expert's
      * gate/up (both need only x); the main stream routes meanwhile */

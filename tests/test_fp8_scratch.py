@@ -1,8 +1,11 @@
 """Scratch of the FP8-128 product (CPU): the encoded rows, and room for parts of K only where K
 can be cut."""
+import ctypes
+
 import pytest
 
 from moonshine_amd import _lib
+from moonshine_amd._lib import K3MoeNativeShape, K3MoeNativeWeights, K3MoeShape, K3MoeStaticWeight
 
 MIB = 1 << 20
 
@@ -39,7 +42,27 @@ def test_parts_of_few_rows(tokens):
 
 def test_grows_with_the_tokens():
     steps = [*range(1, 300), *range(300, 4200, 61), 8191, 40000, 65535]
-    for rows in (1, 130, 256, 1030, 4096, 7168, 50000, 1 << 24):
+    for rows in (1, 130, 256, 1030, 4096, 7168, 50000, 1 << 22):
         for cols in (128, 640, 1664, 2176, 4096, 8192, 65536, 1 << 24):
             sizes = [scratch(t, rows, cols) for t in steps]
             assert sizes == sorted(sizes), (rows, cols)
+
+
+def test_outputs_past_a_launch_are_refused_with_the_sizes():
+    """2^38 outputs are the most; the size is 0 as for every size that the product refuses."""
+    assert scratch(16384, 1 << 24, 128) > 0 and scratch(65535, 1 << 22, 128) > 0
+    for tokens, rows in ((16385, 1 << 24), (65535, 1 << 24), (65535, (1 << 22) + 65), (32768, (1 << 23) + 1)):
+        assert scratch(tokens, rows, 128) == 0, (tokens, rows)
+
+
+def test_block_refuses_such_an_output_with_its_size():
+    """The native block asks before its first launch, by the same rule."""
+    shape = K3MoeNativeShape(K3MoeShape(512, 8, 2, 256, 1.0, 0, 1.0, 1.0), 1024, 1 << 24, 1e-5)
+    w = K3MoeNativeWeights()
+    for name, rows, cols in (("routed_down", 512, 1024), ("routed_up", 1024, 512),
+                             ("shared_gate", 1 << 24, 1024), ("shared_up", 1 << 24, 1024),
+                             ("shared_down", 1024, 1 << 24)):
+        setattr(w, name, K3MoeStaticWeight(2, rows, cols, 1 << 20, 1 << 20))
+    size = lambda t: _lib.lib().k3_moe_native_weights_workspace_bytes(  # noqa: E731
+        ctypes.byref(w), ctypes.byref(shape), t)
+    assert size(16384) > 0 and size(16385) == 0
