@@ -49,8 +49,14 @@ def _dense(t, name, dtypes, dim, device=None):
     return at
 
 
-# a call costs the host several microseconds, so device and stream are asked for directly
-_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+def _public_stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# a call costs the host several microseconds, so device and stream are asked for directly where torch
+# has these names; they are not public, and a build may lack them
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
 def _call(fn, device, *args):

@@ -1,5 +1,8 @@
 """What moonshine_amd.fp8 and moonshine_amd.balance refuse by themselves, on CPU
 tensors that stand in for the GPU's: nothing is launched."""
+import importlib.util
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -112,3 +115,14 @@ def test_an_input_that_requires_a_gradient_is_refused(stopped, call, leaves):
 def test_a_weight_that_requires_a_gradient_is_encoded(stopped):
     with pytest.raises(Called):
         calls("x")["quantize"]()
+
+
+def test_imports_without_torchs_private_names(monkeypatch):
+    """The package loads, and asks for device and stream by torch's public functions."""
+    for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    spec = importlib.util.spec_from_file_location("moonshine_amd._fp8_again", fp8.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: SimpleNamespace(cuda_stream=7 + device))
+    assert again._device is torch.cuda.current_device and again._stream(3) == 10

@@ -1,5 +1,5 @@
-"""FP8-128 products in scratch of exactly their size: the bits of a call with room to spare,
-and nothing written behind it."""
+"""FP8-128 calls' scratch and stream: products in scratch of exactly their size give the bits of a
+call with room to spare and write nothing behind it."""
 import pytest
 import torch
 
@@ -28,3 +28,10 @@ def test_exact_scratch(cuda, T, rows, cols):
     assert torch.equal(out, fp8.product(x, codes, scales)) and (room[need:] == 0x5a).all()
     if need > 0:
         assert not run(need - 1)
+
+
+def test_public_stream_is_the_one_asked_for_directly(cuda):
+    device = torch.cuda.current_device()
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            assert fp8._public_stream(device) == fp8._stream(device) == stream.cuda_stream
