@@ -34,8 +34,9 @@ constexpr uint32_t kBackWaves = 4;
 
 inline size_t align256(size_t v) { return (v + 255u) & ~(size_t)255u; }
 
-/* sigma(x) = 1 / (1 + t), t = e^-x, to a few ulp of itself; 0 where t overflows
- * (x < -88.7). */
+/* sigma(x) = 1 / (1 + t), t = e^-x, to (8 + 2 |x|) 2^-24 of itself: the exponent is one
+ * rounded product, off by |x| 2^-24 of t, the rest a few ulp. 0 where it would be under
+ * 2^-126 (x < -87.33), which the hardware's reciprocal gives as 0. */
 __device__ __forceinline__ float exp_neg(float x) {
     return __builtin_amdgcn_exp2f(__fmul_rn(x, -1.44269504088896341f));
 }

@@ -75,3 +75,17 @@ def test_in_an_autograd_function(cuda):
     _, counts, _, live = balance.balance_loss(x, ids, 0.4)
     want = balance.router_backward(x, ids, counts, live, 0.4, dloss=torch.tensor(1.5, device=cuda))
     assert torch.equal(logits.grad, want) and want.abs().max() > 0
+
+
+def test_where_scores_end(cuda):
+    """Scores just over 2^-126 have their shares; under it they are 0, and so is all that follows."""
+    E, k = 8, 2
+    ids = torch.arange(k, dtype=torch.int32, device=cuda).repeat(3, 1)
+    for level, ends in ((-87.3, False), (-87.4, True), (-88.5, True), (-120.0, True)):
+        logits = torch.full((3, E), level, device=cuda)
+        loss, counts, mean, live = balance.balance_loss(logits, ids, 1.0)
+        grad = balance.router_backward(logits, ids, counts, live, 1.0, dweights=torch.ones((3, k), device=cuda))
+        if ends:
+            assert loss.item() == 0 and (mean == 0).all() and (grad == 0).all()
+        else:  # equal scores: shares of 1 / E, within 392 u
+            assert ((mean.cpu().double() - 1 / E).abs() <= 392 * U / E).all()
