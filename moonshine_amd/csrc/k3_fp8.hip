@@ -11,7 +11,7 @@
  *   join_kernel           the parts of K of a product that was cut
  *   gateup_one_kernel     one token: act(gate . x, up . x) of its routes,
  *   down_one_kernel       their down products and weighted sum
- *   small_plan_kernel     up to 256 tokens: their rows, and the experts' tiles
+ *   small_plan_kernel     up to 1024 tokens: their rows, and the experts' tiles
  *   tiles_kernel          the experts' tiles by k3_moe_route_plan's counts
  *   experts_tile_kernel   gate/up of all tiles; y[route] = bf16(down . h)
  *
@@ -233,11 +233,10 @@ __device__ __forceinline__ float act_f32(float g, float u, const Activation &A) 
 /* one token                                                               */
 /* ---------------------------------------------------------------------- */
 
-/* A row of scales, 64 at a time by the lanes of a wave (those from base on):
- * loaded one at a time, each block of columns would wait for its own. */
-__device__ __forceinline__ float lane_scales(const float *row, uint32_t base, uint32_t n) {
-    const uint32_t k = base + (threadIdx.x & 63u);
-    return row[k < n ? k : n - 1u];
+/* A row of up to 64 scales by the lanes of a wave: loaded one at a time, each block
+ * of columns would wait for its own. */
+__device__ __forceinline__ float lane_scales(const float *row, uint32_t n) {
+    return row[min(threadIdx.x & 63u, n - 1u)];
 }
 __device__ __forceinline__ float scale_at(float scales, uint32_t k) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), (int)(k & 63u)));
@@ -489,7 +488,7 @@ __global__ __launch_bounds__(64 * WAVES) void gateup_one_kernel(OneExpertArgs A)
     const uint32_t codes = lds_addr(smem) + WAVES * Ring::BYTES, scales = codes + A.H;
     const uint64_t row = (uint64_t)(f0 / kBlock) * nblk;
     const float *gs = ex.gate_scales + row, *us = ex.up_scales + row;
-    float sg = lane_scales(gs, 0u, nblk), su = lane_scales(us, 0u, nblk);
+    float sg = lane_scales(gs, nblk), su = lane_scales(us, nblk);
     asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
     Ring ring;
     const uint8_t *const w[2] = {ex.gate_codes + (uint64_t)f0 * A.H, ex.up_codes + (uint64_t)f0 * A.H};
@@ -549,7 +548,7 @@ __global__ __launch_bounds__(512) void down_one_kernel(OneExpertArgs A) {
         if (e >= A.E) continue;
         const k3_moe_fp8_expert ex = A.experts[e];
         const float *ws = ex.down_scales + (uint64_t)(n0 / kBlock) * nblk;
-        float f = lane_scales(ws, 0u, nblk); /* nblk <= 64 */
+        float f = lane_scales(ws, nblk); /* nblk <= 64 */
         const f32x4 *h = (const f32x4 *)(A.h + (uint64_t)(r0 + r) * A.F);
         constexpr uint32_t PER = MOST / 512u;
         f32x4 v[PER][2];
@@ -612,15 +611,16 @@ struct ExpertTile {
     uint32_t row, n, index, many;
     k3_moe_fp8_expert ex;
 };
-/* Rows of each but the last of an expert's tiles: all of up to 128 rows in one,
- * more in equal steps of 32 rows, at most 256. */
+/* Rows of each but the last of an expert's tiles: all of up to 128 rows in one, more
+ * in as few tiles of at most 256 as hold them, of whole steps of 32 rows. The last has
+ * what is left: of 1345 rows (six tiles) 65, of 1793 (eight) one. */
 __device__ __forceinline__ uint32_t tile_height(uint32_t n) {
     const uint32_t steps = (n + 31u) / 32u, many = (n + 255u) / 256u;
     return n > 128u ? 32u * ((steps + many - 1u) / many) : n;
 }
 
-/* Tile classes by an expert's rows: up to 32, 64 and 128 (one tile), more (tiles
- * of up to 256, of equal length in 32-row steps). */
+/* Tile classes by an expert's rows: up to 32, 64 and 128 (one tile), more (tiles of
+ * up to 256 by tile_height). */
 constexpr int kClasses = 4;
 
 struct TileLists {
@@ -965,7 +965,8 @@ __device__ __forceinline__ void tile_block(const TileArgs &P, uint8_t *smem, uin
     for (int j = 0; j < C::TI; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    /* lists hold no tile of fewer than TI / 2 steps of 32 rows */
+    /* a loop for each number of 32-row steps from TI / 2 on: fewer steps (an expert's
+     * last tile) take that one, with the last row in the place of those it has not */
     const uint32_t steps = (rows + 31u) / 32u;
     bool done = false;
     static_for<C::TI / 2>([&](auto Q) {
