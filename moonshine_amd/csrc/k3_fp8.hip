@@ -1338,7 +1338,7 @@ Fp8Workspace carve(void *base, const k3_moe_shape &s, uint32_t T) {
     w.h = (float *)w.hq;
     const size_t few = align256(4u * (size_t)(T < kOneTokensMost ? T : kOneTokensMost) * s.top_k * s.ffn);
     if (s.hidden <= kOneHidden && s.ffn <= kOneFfn && off < from + few) off = from + few;
-    w.router_bytes = k3_moe_router_scratch_bytes(T, s.expert_count);
+    w.router_bytes = router_scratch_up_to(T, s.expert_count);
     w.router = take(w.router_bytes);
     w.bytes = off;
     return w;

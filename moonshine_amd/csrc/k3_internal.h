@@ -49,6 +49,7 @@ constexpr uint32_t kRouterMaxSlices = 16;
  * 2048 at 79 tokens 8.3 against 19.2), the certified one's start is the same. */
 constexpr uint32_t kCertifiedMinTokens = 80;
 uint32_t router_slice_cap(uint32_t T, uint32_t E);              /* for sizing approx */
+size_t router_scratch_up_to(uint32_t T, uint32_t E); /* k3_moe_router_bf16's, of any number of tokens up to T */
 uint32_t router_slices(uint32_t T, uint32_t E, uint32_t H);     /* <= the cap */
 bool router_certified_supported(uint32_t tokens, uint32_t experts, uint32_t hidden,
                                 uint32_t top_k, const void *router_weight, const void *x);

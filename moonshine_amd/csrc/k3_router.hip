@@ -801,6 +801,19 @@ extern "C" size_t k3_moe_router_scratch_bytes(uint32_t token_count, uint32_t exp
            up256(4ull * expert_count);
 }
 
+/* The slices end where the tiles do, so that more tokens may take less (896 experts: 512
+ * tokens 16 slices' 29.4 MB, 513 tokens 25.7): the largest is at the last token of a row
+ * of tiles, or at T. From 512 tiles on there is one slice. */
+size_t k3::router_scratch_up_to(uint32_t T, uint32_t E) {
+    size_t most = k3_moe_router_scratch_bytes(T, E);
+    const uint32_t cols = (E + kRT - 1u) / kRT;
+    for (uint32_t t = kRT; t < T && t / kRT * cols <= 512u; t += kRT) {
+        const size_t n = k3_moe_router_scratch_bytes(t, E);
+        if (n > most) most = n;
+    }
+    return most;
+}
+
 extern "C" bool k3_moe_router_bf16(uint32_t *expert_ids, float *expert_weights,
                                    const void *hidden, const void *router_weight,
                                    const void *router_bias, uint32_t token_count,

@@ -66,3 +66,18 @@ def test_block_refuses_such_an_output_with_its_size():
     size = lambda t: _lib.lib().k3_moe_native_weights_workspace_bytes(  # noqa: E731
         ctypes.byref(w), ctypes.byref(shape), t)
     assert size(16384) > 0 and size(16385) == 0
+
+
+@pytest.mark.parametrize("experts", [1, 8, 64, 128, 200, 512, 896, 1024])
+def test_layer_workspace_for_more_tokens_serves_fewer(experts):
+    """The router's part grows in K slices that end at 512 tiles: at each row of tiles, and everywhere."""
+    for top_k, hidden, ffn in ((1, 128, 128), (8, 2048, 4096), (32, 8320, 128)):
+        if top_k > experts:
+            continue
+        s = ctypes.byref(K3MoeShape(hidden, experts, top_k, ffn, 1.0, 0, 4.0, 25.0))
+        steps = [*range(1, 2100), *range(2100, 65536, 29), *(128 * m + 1 for m in range(16, 512)), 65535]
+        sizes = {t: _lib.lib().k3_moe_fp8_workspace_bytes(s, t) for t in steps}
+        ordered = [sizes[t] for t in sorted(sizes)]
+        assert ordered == sorted(ordered), (experts, top_k)
+        for t in (1, 100, 512, 2049):
+            assert sizes[t] > _lib.lib().k3_moe_router_scratch_bytes(t, experts) > 0
