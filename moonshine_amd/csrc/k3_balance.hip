@@ -299,9 +299,9 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
     const uint32_t i0 = run * A.span, i1 = min(i0 + A.span, A.L);
     const uint32_t n = A.live[s];
     const uint32_t *counts = A.counts + (uint64_t)s * E;
-    /* f times the factor that the loss has in common: 0 without live tokens. Not the
-     * factor times 1 / Z: scores near 2^-126 and a large loss_gradient would take that
-     * past fp32 where the gradient, with slope / Z <= 1, is far inside. */
+    /* f, and the factor that the loss has in common: both 0 without live tokens. The
+     * factor does not meet 1 / Z before the slope has: scores near 2^-126 and a large
+     * loss_gradient would take that past fp32, while slope / Z <= 1. */
     const float per = n ? __fdiv_rn((float)E, __fmul_rn((float)A.k, (float)n)) : 0.0f;
     float share = n ? __fdiv_rn(__fdiv_rn(A.coef, (float)A.S), (float)n) : 0.0f;
     if (A.dloss) share = __fmul_rn(share, *A.dloss);
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
 #pragma unroll
     for (int j = 0; j < J; j++) {
         const uint32_t e = lane + 64u * (uint32_t)j;
-        f[j] = e < E ? __fmul_rn(__fmul_rn((float)counts[e], per), share) : 0.0f;
+        f[j] = e < E ? __fmul_rn((float)counts[e], per) : 0.0f;
     }
     for (uint32_t i = i0 + wave; i < i1; i += kBackWaves) {
         const uint64_t t = (uint64_t)s * A.L + i;
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
             e = lane_route(id, A.k, E);
             if (e < E) {
                 xe = A.logits[t * E + e];
-                fe = __fmul_rn(__fmul_rn((float)counts[e], per), share);
+                fe = __fmul_rn((float)counts[e], per);
                 dw = A.dw[t * A.k + lane];
             }
         }
@@ -360,13 +360,14 @@ __global__ __launch_bounds__(64 * kBackWaves) void router_backward_kernel(Backwa
             const float add = __fmul_rn(__fdiv_rn(A.scale, den), __fsub_rn(dw, m));
             const float d = slope_of(u, p);
             if (e < E)
-                out[e] = __fadd_rn(__fmul_rn(__fsub_rn(fe, mean), __fmul_rn(d, inv)), __fmul_rn(add, d));
+                out[e] = __fadd_rn(__fmul_rn(__fmul_rn(share, __fsub_rn(fe, mean)), __fmul_rn(d, inv)),
+                                   __fmul_rn(add, d));
         }
 #pragma unroll
         for (int j = 0; j < J; j++) {
             const uint32_t q = lane + 64u * (uint32_t)j;
             if ((j < whole_slots(J) || q < E) && !(chosen >> j & 1u))
-                out[q] = __fmul_rn(__fsub_rn(f[j], mean), __fmul_rn(d[j], inv));
+                out[q] = __fmul_rn(__fmul_rn(share, __fsub_rn(f[j], mean)), __fmul_rn(d[j], inv));
         }
     }
 }

@@ -42,10 +42,13 @@ def _no_gradient(t, name):
 
 
 def _dense(t, name, dtypes, dim, device=None):
-    """_layout of a call's input that no gradient is wanted for."""
+    """_layout of a call's input that no gradient is wanted for; written out for the usual tensor, as
+    a call has up to nine of them."""
+    if (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and t.is_contiguous()
+            and t.is_cuda and (device is None or t.get_device() == device) and not t.requires_grad):
+        return t.data_ptr()
     at = _layout(t, name, dtypes, dim, device)
-    if t.requires_grad:
-        _no_gradient(t, name)
+    _no_gradient(t, name)
     return at
 
 
