@@ -1,4 +1,5 @@
-"""The K3-native block with FP8-128 and mixed static weights in a workspace of exactly its size."""
+"""The K3-native block with FP8-128 and mixed static weights: in a workspace of exactly its size, and
+captured (the FP8-128 layer too)."""
 import ctypes
 
 import pytest
@@ -6,7 +7,7 @@ import torch
 
 from moonshine_amd import native as N
 from moonshine_amd._lib import lib
-from test_gpu_fp8 import normal
+from test_gpu_fp8 import layer, normal
 
 pytestmark = pytest.mark.gpu
 NAMES = ("routed_down", "routed_up", "shared_gate", "shared_up", "shared_down")
@@ -49,3 +50,51 @@ def test_exact_workspace(cuda, fp8, T, shared_stream):
     blk.workspace = lambda tokens: room[:need - 256]
     with pytest.raises(RuntimeError):
         blk.forward(x, r, shared_stream=stream)
+
+
+@pytest.mark.parametrize("T", [1, 5, 100])
+@pytest.mark.parametrize("shared_stream", [False, True])
+def test_replayed(cuda, T, shared_stream):
+    """The block captured on one or two streams: every replay is the eager call, which runs between."""
+    blk = block(cuda, T, NAMES)
+    x, r = normal((T, 1024), T).to(cuda), normal((T, 1024), T + 1).to(cuda)
+    ids, w = torch.zeros((T, 4), dtype=torch.int32, device=cuda), torch.zeros((T, 4), device=cuda)
+    side = torch.cuda.Stream()
+    stream = side.cuda_stream if shared_stream else None
+    blk.forward(x, r, shared_stream=stream)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = blk.forward(x, r, ids=ids, weights=w, shared_stream=stream)
+    for n in range(4):
+        v = normal((T, 1024), 50 + n).to(cuda)
+        x.copy_(v)
+        g.replay()
+        got = out.clone(), ids.clone(), w.clone()
+        eager = torch.zeros_like(ids), torch.zeros_like(w)
+        want = blk.forward(v, r, ids=eager[0], weights=eager[1], shared_stream=stream)
+        torch.cuda.synchronize()
+        for a, b in zip(got, (want, *eager)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_layer_replayed_with_its_routes(cuda, T):
+    """The FP8-128 layer's copies of the routes are part of the graph."""
+    moe, x = layer(cuda, T)
+    ids = torch.zeros((T, moe.cfg.top_k), dtype=torch.int32, device=cuda)
+    w = torch.zeros((T, moe.cfg.top_k), device=cuda)
+    moe.forward(x, x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = moe.forward(x, x, ids=ids, weights=w)
+    for n in range(4):
+        v = normal(x.shape, 60 + n).to(cuda)
+        x.copy_(v)
+        g.replay()
+        got = out.clone(), ids.clone(), w.clone()
+        eager = torch.zeros_like(ids), torch.zeros_like(w)
+        want = moe.forward(v, v, ids=eager[0], weights=eager[1])
+        torch.cuda.synchronize()
+        for a, b in zip(got, (want, *eager)):
+            assert torch.equal(a, b)
