@@ -526,6 +526,51 @@ bool k3_moe_router_backward_f32(float *logits_gradient, const float *logits,
                                 uint32_t top_k, float coefficient, float scaling_factor,
                                 void *stream);
 
+/* ---- the routed experts in training ------------------------------------- */
+
+/*
+ * bf16 products grouped by expert, and their gradients. Rows offsets[e] ..
+ * offsets[e + 1] - 1 of `rows` are expert e's (offsets [E + 1] on the device,
+ * ascending: k3_moe_route_plan's, with its token_index and route_index as indices
+ * below); an expert may have any number of them, none too. W is [E, N, K], N
+ * out_columns and K columns.
+ *   product:          output[to(r)]  = bf16(W[e] . input[from(r)])                [N]
+ *   input gradient:   output[to(r)]  = bf16(W[e]^T . output_gradient[from(r)])    [K]
+ *   weight gradient:  output[e, n, k] (+)= sum over e's rows r of
+ *                         output_gradient[from(r), n] input[from'(r), k]
+ * from and to are the indices given, or r itself where they are NULL. A row that
+ * an index picks from the *_rows of its tensor on is a row of zeros, and one that
+ * output_index sends there is not written; the rows of output to which no row is
+ * sent stay as they are, as do rows from offsets[E] on. An output index must not send
+ * two rows to one. Products are exact and summed in fp32, in an order set by the sizes
+ * and the number of an expert's rows.
+ * The weight gradient's output is f32 or bf16 [E, N, K]; an expert without rows has
+ * gradient 0. accumulate (f32 only) adds to what output holds.
+ * N and K multiples of 8 up to 32768; rows <= 65535 * 32, *_rows picked by an index
+ * <= 65535; E <= 1024; at most 2^23 tiles of 256 x 256; tensors 16-byte aligned; an
+ * output over an operand is refused. No scratch. The reference only serves; it has
+ * no counterpart.
+ */
+bool k3_moe_grouped_product_bf16(void *output, const void *input, const void *weights,
+                                 const uint32_t *offsets, const uint32_t *input_index,
+                                 const uint32_t *output_index, uint32_t rows, uint32_t input_rows,
+                                 uint32_t output_rows, uint32_t expert_count, uint32_t out_columns,
+                                 uint32_t columns, void *stream);
+bool k3_moe_grouped_input_gradient_bf16(void *output, const void *output_gradient,
+                                        const void *weights, const uint32_t *offsets,
+                                        const uint32_t *gradient_index,
+                                        const uint32_t *output_index, uint32_t rows,
+                                        uint32_t gradient_rows, uint32_t output_rows,
+                                        uint32_t expert_count, uint32_t out_columns,
+                                        uint32_t columns, void *stream);
+bool k3_moe_grouped_weight_gradient_bf16(void *output, bool f32, bool accumulate,
+                                         const void *output_gradient, const void *input,
+                                         const uint32_t *offsets, const uint32_t *gradient_index,
+                                         const uint32_t *input_index, uint32_t rows,
+                                         uint32_t gradient_rows, uint32_t input_rows,
+                                         uint32_t expert_count, uint32_t out_columns,
+                                         uint32_t columns, void *stream);
+
 /*
  * Synthetic resident expert store for benchmarks and tests: fills `bytes`
  * of device memory at `base` with the counter-based generator

@@ -145,6 +145,12 @@ SIGNATURES = {
                                      _sz, _p]),
     "k3_moe_router_backward_f32": (_b, [_p, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
                                         _f, _f, _p]),
+    "k3_moe_grouped_product_bf16": (_b, [_p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32,
+                                         _u32, _p]),
+    "k3_moe_grouped_input_gradient_bf16": (_b, [_p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
+                                                _u32, _u32, _p]),
+    "k3_moe_grouped_weight_gradient_bf16": (_b, [_p, _b, _b, _p, _p, _p, _p, _p, _u32, _u32, _u32,
+                                                 _u32, _u32, _u32, _p]),
 }
 
 _lib = None
