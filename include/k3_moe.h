@@ -437,6 +437,17 @@ bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, const float *s
                               const void *input, uint32_t vector_count, uint32_t rows,
                               uint32_t columns, void *scratch, size_t scratch_bytes, void *stream);
 
+/*
+ * The same product of rows that are encoded already (k3_moe_fp8_128_quantize_rows_bf16's or
+ * k3_moe_residual_norm_bf16's codes and scales, scales [vector_count, columns / 128]): the
+ * same bits for the same codes. input_codes 16-byte, input_scales 4-byte aligned;
+ * otherwise as above.
+ */
+bool k3_moe_fp8_128_encoded_gemm_bf16(void *output, const uint8_t *codes, const float *scales,
+                                      const uint8_t *input_codes, const float *input_scales,
+                                      uint32_t vector_count, uint32_t rows, uint32_t columns,
+                                      void *scratch, size_t scratch_bytes, void *stream);
+
 /* One routed expert with FP8-128 weights: codes and scales of each matrix.
  * Codes 16-byte, scales 4-byte aligned. */
 typedef struct {
@@ -570,6 +581,75 @@ bool k3_moe_grouped_weight_gradient_bf16(void *output, bool f32, bool accumulate
                                          uint32_t gradient_rows, uint32_t input_rows,
                                          uint32_t expert_count, uint32_t out_columns,
                                          uint32_t columns, void *stream);
+
+/*
+ * The activation between the two products, times the route weights, and its gradient.
+ * gate_up is [rows, 2 F], a row gate's F columns and then up's; w(r) =
+ * route_weights[route_index[r]] (route_index NULL: r itself; route_weights NULL: 1; a
+ * route that is none of `routes`: 0); act(g, u) as k3_moe_activation, in fp32:
+ *   output[r]            = bf16(w(r) act(g[r], u[r]))                         [F]
+ *   gate_up_gradient[r]  = bf16(w(r) dh[r] d act / d g), bf16(w(r) dh[r] d act / d u)
+ *   weight_gradient[route_index[r]] = sum_f dh[r, f] act(g[r, f], u[r, f])    fp32
+ * with dh = output_gradient. weight_gradient ([routes], NULL: not wanted) is 0 for a
+ * route without a row. Rows from offsets[E] on are left as they are; no two rows have one
+ * route. gate_up_gradient may be gate_up itself; any other overlap of an output is
+ * refused. F a multiple of 8 up to 32768; rows, routes <= 65535 * 32; E <= 1024;
+ * tensors 16-byte, the others 4-byte aligned.
+ */
+bool k3_moe_gated_rows_bf16(void *output, const void *gate_up, const uint32_t *offsets,
+                            const uint32_t *route_index, const float *route_weights, uint32_t rows,
+                            uint32_t routes, uint32_t expert_count, uint32_t ffn,
+                            uint32_t activation, float beta, float linear_beta, void *stream);
+bool k3_moe_gated_rows_backward_bf16(void *gate_up_gradient, float *weight_gradient,
+                                     const void *output_gradient, const void *gate_up,
+                                     const uint32_t *offsets, const uint32_t *route_index,
+                                     const float *route_weights, uint32_t rows, uint32_t routes,
+                                     uint32_t expert_count, uint32_t ffn, uint32_t activation,
+                                     float beta, float linear_beta, void *stream);
+
+/*
+ * A token's rows [T k, hidden] (of its routes, in rank order) added up as the layer does:
+ *   output[t] = bf16(residual[t] + bf16(sum_r w[t, r] rows[t k + r]))
+ * over the routes that k3_moe_route_plan keeps; rows of the others are not added, whatever
+ * they hold. expert_weights NULL: 1, for rows that their weights are in already, and for
+ * the routes' gradients of the token; residual NULL: none. output may be residual itself;
+ * another overlap of it with rows or residual is refused. hidden a multiple of 8 up to
+ * 65536, T <= 65535, k <= 32; output, rows and residual 16-byte aligned.
+ */
+bool k3_moe_combine_bf16(void *output, const void *rows, const void *residual,
+                         const void *expert_ids, const void *expert_weights, uint32_t token_count,
+                         uint32_t top_k, uint32_t expert_count, uint32_t hidden, void *stream);
+
+/* ---- the norm before the layer ------------------------------------------- */
+
+/*
+ * RMS norm with the residual's addition, and its gradient:
+ *   total  = bf16(input + residual)                  (residual NULL: input, and total NULL)
+ *   rstd   = 1 / sqrt(mean(total^2) + epsilon)       f32 [rows]
+ *   normed = bf16(n),  n = total rstd weight
+ *   codes, scales = the FP8-128 encoding of n, from fp32 (columns % 128 == 0)
+ * normed, codes with scales and rstd may be NULL where not wanted. total and normed may
+ * each be input or residual itself; another overlap of an output is refused. The gradient, of
+ * normed_gradient (dn) and, if it is not NULL, total_gradient (dt):
+ *   input_gradient  = bf16(dt + rstd (dn weight - total rstd^2 mean(dn weight total)))
+ *   weight_gradient = sum over rows of dn total rstd                  f32 [columns]
+ * input_gradient is the residual's too, and may be any one of normed_gradient, total and
+ * total_gradient itself. Sums are fp32 in an order set by the sizes. columns a
+ * multiple of 8 up to 32768, rows <= 65535 * 32; weight bf16 [columns]; bf16 tensors
+ * 16-byte, codes 8-byte, the others 4-byte aligned; scratch 256-byte aligned,
+ * k3_moe_residual_norm_scratch_bytes(rows, columns) bytes (those of more rows serve
+ * fewer).
+ */
+bool k3_moe_residual_norm_bf16(void *total, void *normed, uint8_t *codes, float *scales,
+                               float *rstd, const void *input, const void *residual,
+                               const void *weight, uint32_t rows, uint32_t columns, float epsilon,
+                               void *stream);
+size_t k3_moe_residual_norm_scratch_bytes(uint32_t rows, uint32_t columns);
+bool k3_moe_residual_norm_backward_bf16(void *input_gradient, float *weight_gradient,
+                                        const void *normed_gradient, const void *total,
+                                        const void *weight, const float *rstd,
+                                        const void *total_gradient, uint32_t rows, uint32_t columns,
+                                        void *scratch, size_t scratch_bytes, void *stream);
 
 /*
  * Synthetic resident expert store for benchmarks and tests: fills `bytes`

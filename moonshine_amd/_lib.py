@@ -135,6 +135,7 @@ SIGNATURES = {
     "k3_moe_fp8_128_quantize_weight_bf16": (_b, [_p, _p, _p, _u32, _u32, _p]),
     "k3_moe_fp8_128_scratch_bytes": (_sz, [_u32, _u32, _u32]),
     "k3_moe_fp8_128_gemm_bf16": (_b, [_p, _p, _p, _p, _u32, _u32, _u32, _p, _sz, _p]),
+    "k3_moe_fp8_128_encoded_gemm_bf16": (_b, [_p, _p, _p, _p, _p, _u32, _u32, _u32, _p, _sz, _p]),
     "k3_moe_fp8_workspace_bytes": (_sz, [ctypes.POINTER(K3MoeShape), _u32]),
     "k3_moe_fp8_experts_bf16": (_b, [_p, _p, _p, _p, _p, _p, ctypes.POINTER(K3MoeShape), _u32,
                                      _p, _sz, _p]),
@@ -151,6 +152,14 @@ SIGNATURES = {
                                                 _u32, _u32, _p]),
     "k3_moe_grouped_weight_gradient_bf16": (_b, [_p, _b, _b, _p, _p, _p, _p, _p, _u32, _u32, _u32,
                                                  _u32, _u32, _u32, _p]),
+    "k3_moe_gated_rows_bf16": (_b, [_p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _f, _f, _p]),
+    "k3_moe_gated_rows_backward_bf16": (_b, [_p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32,
+                                             _u32, _f, _f, _p]),
+    "k3_moe_combine_bf16": (_b, [_p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _p]),
+    "k3_moe_residual_norm_bf16": (_b, [_p, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _f, _p]),
+    "k3_moe_residual_norm_scratch_bytes": (_sz, [_u32, _u32]),
+    "k3_moe_residual_norm_backward_bf16": (_b, [_p, _p, _p, _p, _p, _p, _p, _u32, _u32, _p, _sz,
+                                                _p]),
 }
 
 _lib = None

@@ -23,6 +23,7 @@
  * c, so one factor scales all four.
  */
 #include "k3_device.h"
+#include "k3_fp8.h"
 #include "k3_internal.h"
 #include "k3_lds.h"
 #include "../../include/k3_moe.h"
@@ -30,60 +31,20 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace k3 {
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kBlock = 128;                /* values of a block */
 /* A tile's 256 rows, and a batch's 65535, are addressed by 32 bits. */
 constexpr uint32_t kMostAxis = 1u << 24, kMostWidth = 1u << 16;
-constexpr float kTop = 448.0f;                  /* largest e4m3 */
-constexpr float kLeast = 0x1.cp-118f;           /* 448 * 2^-126 */
 
 inline size_t align256(size_t v) { return (v + 255u) & ~(size_t)255u; }
 /* Scales of a row inside the library: whole groups of four. */
 inline uint32_t scale_stride(uint32_t cols) { return (cols / kBlock + 3u) & ~3u; }
-
-/* Scale and its inverse of a block with maximum a. */
-__device__ __forceinline__ void fp8_scales(float a, float &scale, float &inv) {
-    a = fmaxf(a, kLeast);
-    scale = __fdiv_rn(a, kTop);
-    inv = __fdiv_rn(kTop, a);
-}
-
-/* Eight values as codes. v inv is at most 448 (1 + 2^-23), which rounds to
- * 448; NaN (and inf x 0) gives a NaN code. */
-__device__ __forceinline__ uint2 fp8_codes8(const float (&v)[8], float inv) {
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const float *u = v + 4 * h;
-        w[h] = e4m3x2_raw<true>(__fmul_rn(u[2], inv), __fmul_rn(u[3], inv),
-                                e4m3x2_raw<false>(__fmul_rn(u[0], inv), __fmul_rn(u[1], inv), 0u));
-    }
-    return make_uint2(w[0], w[1]);
-}
-
-__device__ __forceinline__ void unpack8(const uint4 &p, float (&v)[8]) {
-    const uint32_t d[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[2 * i] = bf16_lo(d[i]);
-        v[2 * i + 1] = bf16_hi(d[i]);
-    }
-}
-__device__ __forceinline__ void load8(const uint16_t *src, float (&v)[8]) {
-    unpack8(*(const uint4 *)src, v);
-}
-
-__device__ __forceinline__ float max8(const float (&v)[8]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
-    return m;
-}
 
 /* Sixteen lanes a block of 128 values, eight values a lane: one 16-byte load
  * (bf16), a maximum within a row of lanes, one 8-byte store. Scales: nblk of a
@@ -190,20 +151,6 @@ __device__ __forceinline__ void store_rows(uint16_t *out, const f32x4 &v, uint32
     if (n + 1u < N) p[1] = (uint16_t)(u.x >> 16);
     if (n + 2u < N) p[2] = (uint16_t)u.y;
     if (n + 3u < N) p[3] = (uint16_t)(u.y >> 16);
-}
-
-/* tanh within 16 u of itself (u = 2^-24): its odd series below 1/4 (the term left
- * out is under u / 6 there), the exponential above (2 / (e + 1) to 3.6 u, of 0.245). */
-__device__ __forceinline__ float tanh_f32(float y) {
-    const float a = fabsf(y), z = __fmul_rn(a, a);
-    float p = 2.1869488536155203e-2f;
-    p = fmaf(p, z, -5.3968253968253968e-2f);
-    p = fmaf(p, z, 1.3333333333333333e-1f);
-    p = fmaf(p, z, -3.3333333333333333e-1f);
-    const float lo = fmaf(__fmul_rn(a, z), p, a);
-    const float e = __builtin_amdgcn_exp2f(__fmul_rn(a, 2.88539008177792681f)); /* e^2a */
-    const float hi = fmaf(-2.0f, __builtin_amdgcn_rcpf(__fadd_rn(e, 1.0f)), 1.0f);
-    return copysignf(a < 0.25f ? lo : hi, y);
 }
 
 /* The activation and SiTU's constants: by = 1 / beta (at most the largest number,
@@ -330,9 +277,34 @@ __device__ __forceinline__ void encode_lds(const float (&u)[8], uint32_t codes, 
 
 /* THREADS threads encode up to PER times as many pieces of eight values into LDS:
  * codes at `codes`, scales at `scales` (LDS addresses). Loads first, so that what
- * is issued between the two halves does not stand in their way. */
+ * is issued between the two halves does not stand in their way. ENCODED: the tokens
+ * come as codes with their scales and are copied. */
+template <uint32_t THREADS, uint32_t PER, bool ENCODED = false>
+struct TokenPart;
 template <uint32_t THREADS, uint32_t PER>
-struct TokenPart {
+struct TokenPart<THREADS, PER, true> {
+    uint2 v[PER];
+    float s[PER];
+    __device__ __forceinline__ void load(const uint8_t *x, const float *scales, uint32_t n) {
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t q = min(threadIdx.x + THREADS * i, 16u * n - 1u);
+            v[i] = ((const uint2 *)x)[q];
+            s[i] = scales[q >> 4];
+        }
+    }
+    __device__ __forceinline__ void encode(uint32_t n, uint32_t codes, uint32_t scales) const {
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t q = threadIdx.x + THREADS * i;
+            if (q >= 16u * n) continue;
+            ds_write8(codes + 8u * q, v[i]);
+            if ((q & 15u) == 0u) ds_write4(scales + (q >> 2), __float_as_uint(s[i]));
+        }
+    }
+};
+template <uint32_t THREADS, uint32_t PER>
+struct TokenPart<THREADS, PER, false> {
     uint4 v[PER];
     __device__ __forceinline__ void load(const uint16_t *x, uint32_t n) {
 #pragma unroll
@@ -355,7 +327,9 @@ struct OneArgs {
     uint16_t *out;
     const uint8_t *codes;
     const float *scales;
-    const uint16_t *x;
+    const uint16_t *x;      /* or, encoded, */
+    const uint8_t *xq;
+    const float *xs;
     uint32_t T, N, K;
 };
 
@@ -377,7 +351,7 @@ inline bool one_launch(uint32_t T, uint32_t N, uint32_t K) {
     if (T <= 8u) return T <= 4u || N <= 4096u;
     return K <= 4096u && (T + 15ull) / 16u * ((N + 15u) / 16u) <= 256u;
 }
-template <uint32_t NT, uint32_t CHUNK> /* blocks of columns encoded at a time: 64 or 32 */
+template <uint32_t NT, uint32_t CHUNK, bool ENCODED> /* blocks of columns encoded at a time: 64 or 32 */
 __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
     using Ring = WaveRing<1, kOneRing>;
     constexpr uint32_t TOKEN = CHUNK * (kBlock + 4u); /* codes, then scales */
@@ -392,10 +366,16 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
     const float *ws = P.scales + (uint64_t)(n0 / kBlock) * nblk;
     /* lane q: the scale of the wave's q-th block of a chunk */
     float sw = ws[min(wave + 8u * (lane & 7u), nblk - 1u)];
-    TokenPart<512u, CHUNK / 32u> x[NT];
+    TokenPart<512u, CHUNK / 32u, ENCODED> x[NT];
+    auto load = [&](uint32_t block, uint32_t n) {
 #pragma unroll
-    for (uint32_t t = 0; t < NT; t++)
-        x[t].load(P.x + (uint64_t)(t0 + min(t, T - 1u)) * P.K, min(CHUNK, nblk));
+        for (uint32_t t = 0; t < NT; t++) {
+            const uint64_t row = t0 + min(t, T - 1u), at = row * P.K + kBlock * block;
+            if constexpr (ENCODED) x[t].load(P.xq + at, P.xs + row * nblk + block, n);
+            else x[t].load(P.x + at, n);
+        }
+    };
+    load(0u, min(CHUNK, nblk));
     asm volatile("" ::: "memory"); /* issued before the weights, so that their waits leave those out */
     Ring ring;
     const uint8_t *const w[1] = {P.codes + (uint64_t)n0 * P.K};
@@ -408,9 +388,7 @@ __global__ __launch_bounds__(512) void product_one_kernel(OneArgs P) {
         const uint32_t n = min(CHUNK, nblk - base);
         if (base != 0u) {
             sw = ws[min(base + wave + 8u * (lane & 7u), nblk - 1u)];
-#pragma unroll
-            for (uint32_t t = 0; t < NT; t++)
-                x[t].load(P.x + (uint64_t)(t0 + min(t, T - 1u)) * P.K + kBlock * base, n);
+            load(base, n);
             lds_barrier(); /* the codes before have been read */
         }
 #pragma unroll
@@ -1368,6 +1346,17 @@ bool launch_rows(const RowArgs &A, hipStream_t st) {
     return hipGetLastError() == hipSuccess;
 }
 
+/* Scales [T, nblk] as rows `stride` apart, which tiles read four at a time. */
+__global__ __launch_bounds__(256) void spread_scales_kernel(float *__restrict__ to,
+                                                            const float *__restrict__ from, uint32_t T,
+                                                            uint32_t nblk, uint32_t stride) {
+    const uint64_t n = (uint64_t)T * stride;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += 256ull * gridDim.x) {
+        const uint64_t t = i / stride, b = i % stride;
+        to[i] = b < nblk ? from[t * nblk + b] : 0.0f;
+    }
+}
+
 /* How a product of more tokens is cut: its tile, and K in `splits` parts of `span`
  * blocks. */
 struct Cut {
@@ -1562,43 +1551,62 @@ extern "C" size_t k3_moe_fp8_128_scratch_bytes(uint32_t vector_count, uint32_t r
     return fp8_scratch_bytes(vector_count, rows, columns);
 }
 
-extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, const float *scales,
-                                         const void *input, uint32_t vector_count, uint32_t rows,
-                                         uint32_t columns, void *scratch, size_t scratch_bytes,
-                                         void *stream) {
-    if (!output || !codes || !scales || !input || !product_ok(vector_count, rows, columns) ||
-        (((uintptr_t)codes | (uintptr_t)input) % 16u) != 0u || ((uintptr_t)scales % 4u) != 0u ||
-        ((uintptr_t)output % 2u) != 0u)
+namespace {
+
+/* The product of rows in bf16 (input), or encoded (xq, xs with a scale for each block). */
+bool run_product(void *output, const uint8_t *codes, const float *scales, const void *input,
+                 const uint8_t *xq, const float *xs, uint32_t T, uint32_t rows, uint32_t columns,
+                 void *scratch, size_t scratch_bytes, hipStream_t st) {
+    if (!output || !codes || !scales || !product_ok(T, rows, columns) ||
+        (((uintptr_t)codes | (uintptr_t)input | (uintptr_t)xq) % 16u) != 0u ||
+        (((uintptr_t)scales | (uintptr_t)xs) % 4u) != 0u || ((uintptr_t)output % 2u) != 0u)
         return false;
     /* blocks of one launch read all of the input and write their own columns */
-    if (overlap(output, 2u * (uint64_t)vector_count * rows, input, 2u * (uint64_t)vector_count * columns))
+    const uint64_t bytes = 2u * (uint64_t)T * rows, values = (uint64_t)T * columns;
+    if (input ? overlap(output, bytes, input, 2u * values)
+              : overlap(output, bytes, xq, values) || overlap(output, bytes, xs, values / kBlock * 4u))
         return false;
-    const size_t need = fp8_scratch_bytes(vector_count, rows, columns);
+    const size_t need = fp8_scratch_bytes(T, rows, columns);
     if (need != 0u && (!scratch || scratch_bytes < need || ((uintptr_t)scratch % 256u) != 0u))
         return false;
-    const hipStream_t st = (hipStream_t)stream;
     const bool wide = rows % 4u == 0u && ((uintptr_t)output % 8u) == 0u;
-    if (one_launch(vector_count, rows, columns)) {
-        const OneArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, vector_count, rows,
+    if (one_launch(T, rows, columns)) {
+        const OneArgs A{(uint16_t *)output, codes, scales, (const uint16_t *)input, xq, xs, T, rows,
                         columns};
-        const auto product = vector_count == 1u   ? product_one_kernel<1u, 64u>
-                             : vector_count == 2u ? product_one_kernel<2u, 64u>
-                             : vector_count <= 4u ? product_one_kernel<4u, 64u>
-                             : vector_count <= 8u ? product_one_kernel<8u, 64u>
-                                                  : product_one_kernel<16u, 32u>;
-        const dim3 grid((rows + 15u) / 16u, vector_count <= 8u ? 1u : (vector_count + 15u) / 16u);
+        const auto pick = [&](auto encoded) {
+            constexpr bool E = decltype(encoded)::value;
+            return T == 1u   ? product_one_kernel<1u, 64u, E>
+                   : T == 2u ? product_one_kernel<2u, 64u, E>
+                   : T <= 4u ? product_one_kernel<4u, 64u, E>
+                   : T <= 8u ? product_one_kernel<8u, 64u, E>
+                             : product_one_kernel<16u, 32u, E>;
+        };
+        const auto product = input ? pick(std::false_type{}) : pick(std::true_type{});
+        const dim3 grid((rows + 15u) / 16u, T <= 8u ? 1u : (T + 15u) / 16u);
         hipLaunchKernelGGL(product, grid, dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
     TileArgs B{};
-    uint8_t *xq = (uint8_t *)scratch;
-    float *xs = (float *)(xq + align256((size_t)vector_count * columns));
-    B.codes = codes, B.scales = scales, B.xq = xq, B.xs = xs, B.xstride = scale_stride(columns);
-    B.part = (f32x4 *)((uint8_t *)xs + align256(4u * (size_t)vector_count * B.xstride));
-    B.out = (uint16_t *)output, B.T = vector_count, B.N = rows, B.K = columns, B.wide = wide;
+    uint8_t *const codes_at = (uint8_t *)scratch;
+    float *const scales_at = (float *)(codes_at + align256((size_t)T * columns));
+    B.codes = codes, B.scales = scales, B.xstride = scale_stride(columns);
+    B.part = (f32x4 *)((uint8_t *)scales_at + align256(4u * (size_t)T * B.xstride));
+    B.out = (uint16_t *)output, B.T = T, B.N = rows, B.K = columns, B.wide = wide;
     B.wide16 = rows % 8u == 0u && ((uintptr_t)output % 16u) == 0u;
-    if (!launch_rows(row_args(xq, xs, input, vector_count, columns, B.xstride), st)) return false;
-    const Cut q = cut_of(vector_count, rows, columns);
+    if (input) {
+        B.xq = codes_at, B.xs = scales_at;
+        if (!launch_rows(row_args(codes_at, scales_at, input, T, columns, B.xstride), st)) return false;
+    } else {
+        B.xq = xq, B.xs = xs;
+        if (columns / kBlock != B.xstride || ((uintptr_t)xs % 16u) != 0u) { /* read four at a time */
+            const uint64_t n = ((uint64_t)T * B.xstride + 255u) / 256u;
+            hipLaunchKernelGGL(spread_scales_kernel, dim3((uint32_t)(n < 4096u ? n : 4096u)), dim3(256), 0,
+                               st, scales_at, xs, T, columns / kBlock, B.xstride);
+            if (hipGetLastError() != hipSuccess) return false;
+            B.xs = scales_at;
+        }
+    }
+    const Cut q = cut_of(T, rows, columns);
     switch (q.tile) {
     case 0: return launch_dense<Half32>(B, q, st);
     case 1: return launch_dense<Half64>(B, q, st);
@@ -1606,6 +1614,26 @@ extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, con
     case 3: return launch_dense<Tile128>(B, q, st);
     default: return launch_dense<Tile256>(B, q, st);
     }
+}
+
+}  // namespace
+
+extern "C" bool k3_moe_fp8_128_gemm_bf16(void *output, const uint8_t *codes, const float *scales,
+                                         const void *input, uint32_t vector_count, uint32_t rows,
+                                         uint32_t columns, void *scratch, size_t scratch_bytes,
+                                         void *stream) {
+    return input && run_product(output, codes, scales, input, nullptr, nullptr, vector_count, rows, columns,
+                                scratch, scratch_bytes, (hipStream_t)stream);
+}
+
+extern "C" bool k3_moe_fp8_128_encoded_gemm_bf16(void *output, const uint8_t *codes,
+                                                 const float *scales, const uint8_t *input_codes,
+                                                 const float *input_scales, uint32_t vector_count,
+                                                 uint32_t rows, uint32_t columns, void *scratch,
+                                                 size_t scratch_bytes, void *stream) {
+    return input_codes && input_scales &&
+           run_product(output, codes, scales, nullptr, input_codes, input_scales, vector_count, rows, columns,
+                       scratch, scratch_bytes, (hipStream_t)stream);
 }
 
 extern "C" size_t k3_moe_fp8_workspace_bytes(const k3_moe_shape *shape, uint32_t token_count) {

@@ -151,11 +151,16 @@ struct Tile {
     static constexpr int DA = 4, DB = B_CHUNKS < WAVES ? 1 : B_CHUNKS / WAVES, D = DA + DB;
     static constexpr uint32_t LDS = STAGES * STAGE;
     static_assert(LDS <= 160u * 1024u, "LDS");
-    /* Two stages: P's place is free once its fragments are in registers, so after a
-     * second barrier in mid-stage it takes the P of two stages on. */
+    /* Two stages: P, and the first 128 q (four subtiles of a wave, which take half of Q's
+     * loads), are in registers or done with before the fourth subtile's products, so behind
+     * a second barrier there their places take those of two stages on; the other q's follow
+     * in the next stage. */
     static constexpr bool EARLY = STAGES == 2;
-    static constexpr int PREADS = PCOLS ? 4 : 2, QREADS = QCOLS ? 4 : 2; /* of a subtile */
+    static_assert(!EARLY || (TI == 8 && WAVES == 8), "two panels of 128 q");
+    static constexpr int HALF = EARLY ? DB / 2 : 0; /* loads of the first panel */
+    static constexpr int QREADS = QCOLS ? 4 : 2;    /* of a subtile */
     static __device__ __forceinline__ uint32_t b_chunk(uint32_t wave, uint32_t q) {
+        if constexpr (EARLY) return 16u * (q / HALF) + HALF * wave + q % HALF;
         return B_CHUNKS < WAVES ? wave % B_CHUNKS : DB * wave + q;
     }
 };
@@ -223,7 +228,7 @@ struct TileRun {
     /* weight gradient: row (of the tensor) z of a stage is held by lane z */
     const uint32_t *p_index, *q_index;
     uint32_t row, rows, p_rows, q_rows, p_bytes, q_bytes;
-    uint32_t p_row, q_row;
+    uint32_t p_row, q_row, q_late; /* P's, Q's first and second panel's next rows */
     uint32_t stages, wave, lane, wn, wt;
 
     /* the row that this lane holds of stage s, as the index has it; and ~0 in the place of
@@ -264,7 +269,8 @@ struct TileRun {
             const uint32_t ch = C::b_chunk(wave, Q - C::DA);
             const uint8_t *src;
             if constexpr (C::DIR == kWeight)
-                src = picked<C::BQ>(q_base, q_row, q_bytes, q_at[Q - C::DA], ch);
+                src = picked<128u>(q_base, Q - C::DA < C::HALF ? q_row : q_late, q_bytes, q_at[Q - C::DA],
+                                   ch & 15u);
             else
                 src = kDepth * now < q_end[Q - C::DA] ? q_base + q_stride * now + q_at[Q - C::DA]
                                                       : (const uint8_t *)&zero_piece;
@@ -293,7 +299,7 @@ struct TileRun {
         else
             p_lo = base + 8192u * wn + lo, p_hi = base + 8192u * wn + hi;
         if constexpr (C::QCOLS)
-            q_lo = base + C::A + (col_slot<C::BQ>(lane) ^ 32u * wt);
+            q_lo = base + C::A + (col_slot<128u>(lane) ^ 32u * wt);
         else
             q_lo = base + C::A + 2048u * wt + lo, q_hi = base + C::A + 2048u * wt + hi;
         Fragment<C::PCOLS> pf[4];
@@ -312,11 +318,11 @@ struct TileRun {
         auto read_q = [&](auto J) {
             constexpr int j = decltype(J)::value;
             if constexpr (C::QCOLS) {
-                const uint32_t a = (q_lo + st) ^ (64u * j);
+                const uint32_t a = (q_lo + st) ^ (64u * (j & 3));
                 static_for<2>([&](auto H) {
-                    constexpr int h = decltype(H)::value;
-                    qf[j & 1].v[h][0] = ds_read_tr<(int)C::BQ * 64 * h>(a);
-                    qf[j & 1].v[h][1] = ds_read_tr<(int)C::BQ * (64 * h + 8)>(a);
+                    constexpr int h = decltype(H)::value, panel = 16384 * (j >> 2);
+                    qf[j & 1].v[h][0] = ds_read_tr<panel + 128 * 64 * h>(a);
+                    qf[j & 1].v[h][1] = ds_read_tr<panel + 128 * (64 * h + 8)>(a);
                 });
             } else {
                 qf[j & 1].v[0] = ds_read16<4096 * j>(q_lo + st);
@@ -333,19 +339,22 @@ struct TileRun {
         uint32_t p_next = 0u, q_next = 0u;
         if constexpr (picks) {
             p_row = live_row(stage_row(p_index, 0u), p_rows, 0u);
-            q_row = live_row(stage_row(q_index, 0u), q_rows, 0u);
+            q_row = q_late = live_row(stage_row(q_index, 0u), q_rows, 0u);
             p_next = live_row(stage_row(p_index, 1u), p_rows, 1u);
             q_next = live_row(stage_row(q_index, 1u), q_rows, 1u);
         }
 #pragma unroll
         for (int s = 0; s < C::STAGES - 1; s++) fetch<0, C::D>(smem, (uint32_t)s, (uint32_t)s);
-        if constexpr (picks) {
-            p_row = p_next, q_row = q_next;
-            p_next = live_row(stage_row(p_index, 2u), p_rows, 2u);
+        if constexpr (C::EARLY) {
+            if constexpr (picks) p_row = p_next, q_row = q_late = q_next;
+            if constexpr (picks) {
+                p_next = live_row(stage_row(p_index, 2u), p_rows, 2u);
+                q_next = live_row(stage_row(q_index, 2u), q_rows, 2u);
+            }
+            fetch<0, C::DA + C::HALF>(smem, 1u, 1u);
+            if constexpr (picks) p_row = p_next, q_row = q_next;
         }
-        if constexpr (C::EARLY) fetch<0, C::DA>(smem, 1u, 1u);
-        if constexpr (picks) p_row = p_next;
-        wait_vm<C::EARLY ? C::DA : C::D *(C::STAGES - 2)>();
+        wait_vm<C::EARLY ? C::DA + C::HALF : C::D *(C::STAGES - 2)>();
         barrier();
         static_for<4>([&](auto I) {
             read_p(I, std::integral_constant<int, 0>{});
@@ -357,7 +366,7 @@ struct TileRun {
             const uint32_t ahead = s + C::STAGES - 1u, to = next;
             if constexpr (picks) { /* ahead of this stage's loads, so that their wait is theirs */
                 p_next = stage_row(p_index, s + 3u);
-                q_next = stage_row(q_index, s + 2u);
+                q_next = stage_row(q_index, s + 3u);
                 asm volatile("" ::: "memory");
             }
             if constexpr (TL == 1) fetch<0, C::D>(smem, ahead, to);
@@ -372,7 +381,7 @@ struct TileRun {
                 qf[j & 1].ready();
                 if constexpr (last) {
                     /* this wave's loads of stage s + 1; later ones stay out */
-                    wait_vm<C::EARLY ? C::DA : C::D *(C::STAGES - 2)>();
+                    wait_vm<!C::EARLY ? C::D *(C::STAGES - 2) : TL == 4 ? 0 : C::DA + C::HALF>();
                     barrier();
                     st = C::STAGE * slot;
                 }
@@ -386,19 +395,24 @@ struct TileRun {
                         __builtin_amdgcn_sched_barrier(0);
                         /* the loads ahead, spread over the products before the last
                          * subtile's: at once they would keep the waves from their reads */
-                        constexpr int half = 8 * ((TL + 1) / 2), at = 8 * j + 4 * h + i;
+                        constexpr int at = 8 * j + 4 * h + i;
                         if constexpr (TL == 1) {
                         } else if constexpr (C::EARLY) {
-                            if constexpr (at == half - 1) barrier();
-                            static_for<C::DB>([&](auto Q) {
-                                if constexpr (decltype(Q)::value * (half - 1) / C::DB == at)
-                                    fetch_one<C::DA + decltype(Q)::value>(smem, ahead, to);
+                            /* four subtiles: the stage's end is the second barrier */
+                            constexpr int mid = 25, end = TL == 4 ? 32 : 8 * (TL - 1);
+                            static_for<C::DB - C::HALF>([&](auto Q) {
+                                constexpr int q = decltype(Q)::value;
+                                if constexpr (q * 24 / (C::DB - C::HALF) == at)
+                                    fetch_one<C::DA + C::HALF + q>(smem, ahead, to);
                             });
-                            static_for<C::DA>([&](auto Q) {
-                                if constexpr (half - 1 + decltype(Q)::value * (8 * (TL - 1) - half) / C::DA == at)
-                                    fetch_one<decltype(Q)::value>(smem, s + 2u, to ^ 1u);
+                            if constexpr (at == mid && TL != 4) barrier();
+                            static_for<C::DA + C::HALF>([&](auto Q) {
+                                constexpr int q = decltype(Q)::value;
+                                if constexpr (mid + q * (end - mid) / (C::DA + C::HALF) == at)
+                                    fetch_one<q>(smem, s + 2u, to ^ 1u);
                             });
                         } else {
+                            constexpr int half = 8 * ((TL + 1) / 2);
                             static_for<C::D>([&](auto Q) {
                                 if constexpr (decltype(Q)::value * half / C::D == at)
                                     fetch_one<decltype(Q)::value>(smem, ahead, to);
@@ -409,7 +423,8 @@ struct TileRun {
                 if constexpr (last) read_q(std::integral_constant<int, 0>{});
             });
             if constexpr (picks) {
-                p_row = live_row(p_next, p_rows, s + 3u), q_row = live_row(q_next, q_rows, s + 2u);
+                q_late = q_row;
+                p_row = live_row(p_next, p_rows, s + 3u), q_row = live_row(q_next, q_rows, s + 3u);
             }
         }
         wait_lgkm<0>(); /* the reads past the end: their registers stay taken till here */
@@ -579,7 +594,8 @@ __global__ __launch_bounds__(512, 2) void grouped_weight_kernel(GroupArgs A) {
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         R.p_at[q] = 2u * min(8u * col_dma_piece<C::BP>(L, C::DA * R.wave + (uint32_t)q), A.P - 8u - p0);
-        R.q_at[q] = 2u * min(8u * col_dma_piece<C::BQ>(L, C::b_chunk(R.wave, (uint32_t)q)), A.Q - 8u - q0);
+        const uint32_t ch = C::b_chunk(R.wave, (uint32_t)q);
+        R.q_at[q] = 2u * min(128u * (ch >> 4) + 8u * col_dma_piece<128u>(L, ch & 15u), A.Q - 8u - q0);
     }
     const uint32_t high_q = min(C::BQ, A.Q - q0), width = min(C::BP, A.P - p0);
     f32x4 acc[C::TI][4];

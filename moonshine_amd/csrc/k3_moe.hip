@@ -304,7 +304,7 @@ __global__ __launch_bounds__(128) void combine_kernel(
     for (int r = 0; r < K; r++) { /* route 0 stands in for r >= k */
         const uint64_t route = r0 + ((uint32_t)r < k ? (uint32_t)r : 0u);
         yv[r] = *(const uint4 *)(y + route * H + d);
-        w[r] = wts[route];
+        w[r] = wts ? wts[route] : 1.0f;
         live[r] = ((uint32_t)r < k) & (ids[route] < E) & !(again >> r & 1u);
     }
     const uint64_t o = (uint64_t)t * H + d;
@@ -489,6 +489,24 @@ extern "C" bool k3_moe_workspace_init(void *workspace, size_t workspace_bytes, v
     if (!workspace || workspace_bytes == 0u) return false;
     (void)stream;
     return true;
+}
+
+extern "C" bool k3_moe_combine_bf16(void *output, const void *rows, const void *residual,
+                                    const void *expert_ids, const void *expert_weights,
+                                    uint32_t token_count, uint32_t top_k, uint32_t expert_count,
+                                    uint32_t hidden, void *stream) {
+    const uint64_t bytes = 2u * (uint64_t)token_count * hidden;
+    if (!output || !rows || !expert_ids || !rows_aligned(output, rows, residual) ||
+        (((uintptr_t)expert_ids | (uintptr_t)expert_weights) % 4u) != 0u || token_count == 0u ||
+        token_count > 65535u || top_k == 0u || top_k > 32u || expert_count == 0u || hidden == 0u ||
+        hidden % 8u != 0u || hidden > 65536u ||
+        /* blocks write their own columns of a token while others read its rows */
+        overlap(output, bytes, rows, bytes * top_k) ||
+        (residual && residual != output && overlap(output, bytes, residual, bytes)))
+        return false;
+    return launch_combine(output, (const uint16_t *)rows, residual, (const uint32_t *)expert_ids,
+                          (const float *)expert_weights, token_count, hidden, top_k, expert_count, true,
+                          (hipStream_t)stream);
 }
 
 extern "C" size_t k3_moe_plan_scratch_bytes(uint32_t token_count, uint32_t expert_count) {

@@ -1,7 +1,7 @@
 """FP8-128 on torch tensors: e4m3 codes with an fp32 scale for each block of 128.
 
 quantize_rows and quantize_weight encode, product multiplies bf16 rows with an
-encoded weight, experts and Fp8RoutedMoE run routed experts held in it
+encoded weight (product_encoded, encoded rows), experts and Fp8RoutedMoE run routed experts held in it
 (include/k3_moe.h has the definitions). Codes are float8_e4m3fn (or uint8)
 tensors. torch is used only for device memory and streams: everything runs in
 libk3moe.so, on the tensors' device and its current stream. Each call takes its
@@ -122,6 +122,31 @@ def product(x, codes, scales, out=None):
     n = L.k3_moe_fp8_128_scratch_bytes(T, N, K) if T > 1 else 0
     keep, room = _scratch(x, n)
     _call(L.k3_moe_fp8_128_gemm_bf16, device, to, w, s, at, T, N, K, room, n)
+    return out
+
+
+def product_encoded(x_codes, x_scales, codes, scales, out=None):
+    """product of rows that are encoded already (quantize_rows', or norm.residual_norm's): codes [T,
+    cols], scales [T, cols / 128] -> bf16 [T, rows]; out must not overlap them."""
+    at = _dense(x_codes, "x_codes", _CODES, 2)
+    device = x_codes.get_device()
+    xs = _dense(x_scales, "x_scales", _F32, 2, device)
+    w, s = _dense(codes, "codes", _CODES, 2, device), _dense(scales, "scales", _F32, 2, device)
+    (T, K), (N, K2) = x_codes.shape, codes.shape
+    if K != K2 or x_scales.shape != (T, K // BLOCK) or scales.shape != (-(-N // BLOCK), K // BLOCK):
+        raise ValueError(f"product of {tuple(x_codes.shape)}, scales {tuple(x_scales.shape)}, with "
+                         f"{tuple(codes.shape)}, scales {tuple(scales.shape)}")
+    if out is None:
+        out = x_codes.new_empty((T, N), dtype=torch.bfloat16)
+        to = out.data_ptr()
+    else:
+        to = _dense(out, "out", _BF16, 2, device)
+        if out.shape != (T, N):
+            raise ValueError(f"out: {tuple(out.shape)}, wanted {(T, N)}")
+    L = lib()
+    n = L.k3_moe_fp8_128_scratch_bytes(T, N, K) if T > 1 else 0
+    keep, room = _scratch(x_codes, n)
+    _call(L.k3_moe_fp8_128_encoded_gemm_bf16, device, to, w, s, at, xs, T, N, K, room, n)
     return out
 
 
@@ -264,5 +289,5 @@ class Fp8RoutedMoE:
         return experts(hidden, ids, weights, self.store.table, self.shape, residual, out)
 
 
-__all__ = ["quantize_rows", "quantize_weight", "product", "shape", "experts", "Fp8ExpertStore",
+__all__ = ["quantize_rows", "quantize_weight", "product", "product_encoded", "shape", "experts", "Fp8ExpertStore",
            "Fp8RoutedMoE"]
