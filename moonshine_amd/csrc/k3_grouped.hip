@@ -56,8 +56,28 @@ struct GroupArgs {
     bool accumulate;
 };
 
-/* Read by the lanes whose z, or row, lies past the end. */
-__device__ const uint4 zero_piece = {0u, 0u, 0u, 0u};
+/*
+ * Memory for loads to LDS by 32-bit offsets: a lane's address is one register (of 64-bit
+ * addresses their arithmetic took a fifth of a stage), and what lies at `bytes` or beyond
+ * reads as zeros, as the ends of a reduction have to.
+ */
+constexpr uint32_t kNowhere = 0xfffffff0u;
+struct Range {
+    const uint8_t *base;
+    uint32_t bytes;
+    __device__ __forceinline__ Range() {}
+    __device__ __forceinline__ Range(const void *p, uint64_t size)
+        : base((const uint8_t *)p), bytes((uint32_t)(size < kNowhere ? size : kNowhere)) {}
+    template <int Bytes>
+    __device__ __forceinline__ void load(uint32_t at, uint8_t *lds) const {
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)bytes, 0x00027000);
+        if constexpr (Bytes == 16)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)lds, 16, (int)at, 0, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)lds, 4, (int)at, 0, 0, 0);
+    }
+};
 
 __device__ __forceinline__ uint2 bf16x4(const f32x4 &v) {
     return make_uint2(f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
@@ -219,62 +239,98 @@ struct Fragment<true> {
     }
 };
 
+/*
+ * The rows that an operand of a weight gradient picks by an index. A wave loads z = 8 wave .. + 8
+ * of a stage; their indices come through LDS as well, by a load of its own that the waits
+ * count like any other (one to registers the compiler would wait for with all others out),
+ * into a ring of stages.
+ */
+struct Picks {
+    static constexpr uint32_t kRing = 4, SLOT = 256, BYTES = SLOT * kRing; /* a load fills a slot */
+    const uint32_t *index; /* from the tile's first row on; NULL: rows as they lie, nothing is read */
+    uint32_t rows, at;     /* at: this lane's place among the indices of a stage */
+    uint8_t *held;         /* this wave's */
+
+    __device__ __forceinline__ void fetch(uint32_t now, uint32_t slot) const {
+        Range(index + kDepth * now, index ? 4u * (uint64_t)(rows - kDepth * now) : 0u)
+            .load<4>(at, held + SLOT * slot);
+    }
+};
+
 template <class C>
 struct TileRun {
-    /* load q of stage s: base + stride s + at[q], while kDepth s is below end[q] */
+    /* Load q of stage s is from at[q], in p or q moved on by s strides (both an operand's whole
+     * extent from there). Operands of rows: of z, which lies inside them, those below Z;
+     * p_z and q_z are an even q's, ^ 32 an odd one's. */
     const uint8_t *p_base, *q_base;
-    uint64_t p_stride, q_stride;
-    uint32_t p_at[C::DA], q_at[C::DB], p_end[C::DA], q_end[C::DB];
-    /* weight gradient: row (of the tensor) z of a stage is held by lane z */
-    const uint32_t *p_index, *q_index;
-    uint32_t row, rows, p_rows, q_rows, p_bytes, q_bytes;
-    uint32_t p_row, q_row, q_late; /* P's, Q's first and second panel's next rows */
+    uint64_t p_bytes, q_bytes, p_stride, q_stride;
+    uint32_t p_at[C::DA], q_at[C::DB], p_z, q_z, Z;
+    /* weight gradient: at[q] is z's row times the row's bytes and the column's place */
+    Picks p_picks, q_picks;
+    uint32_t p_row_bytes, q_row_bytes, p_col[C::DA], q_col[C::DB], q_late[2]; /* q_late: q_at[2, 3] next */
     uint32_t stages, wave, lane, wn, wt;
 
-    /* the row that this lane holds of stage s, as the index has it; and ~0 in the place of
-     * one that is none, apart from its load so that this is not waited for at once */
-    __device__ __forceinline__ uint32_t stage_row(const uint32_t *index, uint32_t s) const {
-        const uint32_t r = row + min(kDepth * min(s, stages - 1u) + lane, rows - 1u);
-        return index ? index[r] : r;
+    __device__ __forceinline__ TileRun() {
+        lane = threadIdx.x & 63u;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        wn = wave % C::WN, wt = wave / C::WN;
     }
-    __device__ __forceinline__ uint32_t live_row(uint32_t r, uint32_t limit, uint32_t s) const {
-        return kDepth * min(s, stages - 1u) + lane < rows && r < limit ? r : ~0u;
+
+    /* z of load q among the wave's eight */
+    __device__ __forceinline__ uint32_t p_pick(int q) const { return 512u / C::BP * q + (lane >> 5); }
+    __device__ __forceinline__ uint32_t q_pick(int q) const { return 4u * (q & 1) + (lane >> 4); }
+    __device__ __forceinline__ void fetch_picks(uint32_t s) const {
+        const uint32_t now = min(s, stages - 1u), slot = s % Picks::kRing;
+        p_picks.fetch(now, slot);
+        q_picks.fetch(now, slot);
     }
-    template <uint32_t B>
-    __device__ __forceinline__ const uint8_t *picked(const uint8_t *base, uint32_t held, uint32_t bytes,
-                                                     uint32_t at, uint32_t ch) const {
-        uint32_t r = __builtin_amdgcn_readlane(held, ch * (512u / B));
-#pragma unroll
-        for (uint32_t i = 1; i < 512u / B; i++) {
-            const uint32_t o = __builtin_amdgcn_readlane(held, ch * (512u / B) + i);
-            if (lane / (B / 8u) >= i) r = o;
+    __device__ __forceinline__ void read_picks(uint32_t s, uint32_t (&p)[C::DA], uint32_t (&q)[2]) const {
+        const uint32_t slot = Picks::SLOT * (s % Picks::kRing);
+        const uint32_t p_from = lds_addr(p_picks.held) + slot + 4u * p_pick(0);
+        const uint32_t q_from = lds_addr(q_picks.held) + slot + 4u * q_pick(0);
+        static_for<C::DA>([&](auto Q) { p[decltype(Q)::value] = ds_read4<8 * decltype(Q)::value>(p_from); });
+        q[0] = ds_read4<0>(q_from), q[1] = ds_read4<16>(q_from);
+    }
+    /* A picked row's place: rows past the last, of the stage or of the tensor, lie past its end. The
+     * products are of 24 bits: a row of up to 65535, its bytes. */
+    __device__ __forceinline__ uint32_t place(const Picks &k, uint32_t read, uint32_t s, uint32_t z,
+                                              uint32_t row_bytes, uint32_t col) const {
+        const bool live = kDepth * min(s, stages - 1u) + z < k.rows;
+        const uint32_t r = k.index ? live ? min(read, kMostPicked) : kMostPicked : z;
+        return __umul24(r, row_bytes) + col;
+    }
+    __device__ __forceinline__ void set_picks(uint32_t s, uint32_t (&p)[C::DA], uint32_t (&q)[2]) {
+        if constexpr (C::DIR != kWeight) return;
+        else {
+        static_for<C::DA>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            after_wait(p[i]);
+            p_at[i] = place(p_picks, p[i], s, 8u * wave + p_pick(i), p_row_bytes, p_col[i]);
+        });
+        static_for<2>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            after_wait(q[i]);
+            const uint32_t row = place(q_picks, q[i], s, 8u * wave + q_pick(i), q_row_bytes, 0u);
+            q_at[i] = row + q_col[i];
+            q_late[i] = row + q_col[2 + i];
+        });
         }
-        const uint8_t *src = base + (uint64_t)r * bytes + at;
-        return r != ~0u ? src : (const uint8_t *)&zero_piece;
     }
+
     template <int Q>
     __device__ __forceinline__ void fetch_one(uint8_t *smem, uint32_t s, uint32_t slot) const {
         uint8_t *st = smem + C::STAGE * slot;
-        const uint32_t now = min(s, stages - 1u);
+        const uint32_t now = min(s, stages - 1u); /* past the end the last stage again: the waits count */
         if constexpr (Q < C::DA) {
-            const uint32_t ch = C::DA * wave + Q;
-            const uint8_t *src;
-            if constexpr (C::DIR == kWeight)
-                src = picked<C::BP>(p_base, p_row, p_bytes, p_at[Q], ch);
-            else
-                src = kDepth * now < p_end[Q] ? p_base + p_stride * now + p_at[Q]
-                                              : (const uint8_t *)&zero_piece;
-            dma<16>(src, st + 1024u * ch);
+            /* of columns, the reduction's end is the range's */
+            const Range r(p_base + p_stride * now, C::PCOLS ? p_bytes - p_stride * now : p_bytes);
+            const bool in = C::PCOLS || kDepth * now + (p_z ^ 32u * (Q & 1)) < Z;
+            r.template load<16>(in ? p_at[Q] : kNowhere, st + 1024u * (C::DA * wave + Q));
         } else {
-            const uint32_t ch = C::b_chunk(wave, Q - C::DA);
-            const uint8_t *src;
-            if constexpr (C::DIR == kWeight)
-                src = picked<128u>(q_base, Q - C::DA < C::HALF ? q_row : q_late, q_bytes, q_at[Q - C::DA],
-                                   ch & 15u);
-            else
-                src = kDepth * now < q_end[Q - C::DA] ? q_base + q_stride * now + q_at[Q - C::DA]
-                                                      : (const uint8_t *)&zero_piece;
-            dma<16>(src, st + C::A + 1024u * ch);
+            constexpr int q = Q - C::DA;
+            const Range r(q_base + q_stride * now, C::QCOLS ? q_bytes - q_stride * now : q_bytes);
+            const bool in = C::QCOLS || kDepth * now + (q_z ^ 32u * (C::DB > 1 ? q & 1 : 0)) < Z;
+            r.template load<16>(in ? q_at[q] : kNowhere, st + C::A + 1024u * C::b_chunk(wave, q));
         }
     }
     template <int FROM, int TO>
@@ -335,25 +391,27 @@ struct TileRun {
             asm volatile("" ::: "memory");
         };
         constexpr bool picks = C::DIR == kWeight;
-        static_assert(!picks || C::EARLY, "rows are held for P two stages on, Q one");
-        uint32_t p_next = 0u, q_next = 0u;
+        static_assert(!picks || C::EARLY, "rows are held for two stages on");
+        uint32_t p_next[C::DA], q_next[2];
+        auto rows_of_stage = [&](uint32_t s) {
+            read_picks(s, p_next, q_next);
+            wait_lgkm<0>();
+            set_picks(s, p_next, q_next);
+        };
         if constexpr (picks) {
-            p_row = live_row(stage_row(p_index, 0u), p_rows, 0u);
-            q_row = q_late = live_row(stage_row(q_index, 0u), q_rows, 0u);
-            p_next = live_row(stage_row(p_index, 1u), p_rows, 1u);
-            q_next = live_row(stage_row(q_index, 1u), q_rows, 1u);
+#pragma unroll
+            for (uint32_t s = 0; s < 3u; s++) fetch_picks(s);
+            wait_vm<0>();
+            rows_of_stage(0u);
+            q_at[2] = q_late[0], q_at[3] = q_late[1];
         }
 #pragma unroll
         for (int s = 0; s < C::STAGES - 1; s++) fetch<0, C::D>(smem, (uint32_t)s, (uint32_t)s);
-        if constexpr (C::EARLY) {
-            if constexpr (picks) p_row = p_next, q_row = q_late = q_next;
-            if constexpr (picks) {
-                p_next = live_row(stage_row(p_index, 2u), p_rows, 2u);
-                q_next = live_row(stage_row(q_index, 2u), q_rows, 2u);
-            }
-            fetch<0, C::DA + C::HALF>(smem, 1u, 1u);
-            if constexpr (picks) p_row = p_next, q_row = q_next;
+        if constexpr (picks) {
+            rows_of_stage(1u);
+            q_at[2] = q_late[0], q_at[3] = q_late[1];
         }
+        if constexpr (C::EARLY) fetch<0, C::DA + C::HALF>(smem, 1u, 1u);
         wait_vm<C::EARLY ? C::DA + C::HALF : C::D *(C::STAGES - 2)>();
         barrier();
         static_for<4>([&](auto I) {
@@ -364,10 +422,9 @@ struct TileRun {
         uint32_t slot = 0u, next = C::STAGES - 1;
         for (uint32_t s = 0; s < stages; s++) {
             const uint32_t ahead = s + C::STAGES - 1u, to = next;
-            if constexpr (picks) { /* ahead of this stage's loads, so that their wait is theirs */
-                p_next = stage_row(p_index, s + 3u);
-                q_next = stage_row(q_index, s + 3u);
-                asm volatile("" ::: "memory");
+            if constexpr (picks) { /* stage s + 2's have landed, s + 3's are loaded ahead of the rest */
+                read_picks(s + 2u, p_next, q_next);
+                fetch_picks(s + 3u);
             }
             if constexpr (TL == 1) fetch<0, C::D>(smem, ahead, to);
             next = slot;
@@ -379,6 +436,7 @@ struct TileRun {
                 wait_lgkm<last ? 0 : C::QREADS>(); /* the next subtile's reads stay out */
                 if constexpr (j == 0) static_for<4>([&](auto I) { pf[decltype(I)::value].ready(); });
                 qf[j & 1].ready();
+                if constexpr (picks && j == 0) set_picks(s + 2u, p_next, q_next);
                 if constexpr (last) {
                     /* this wave's loads of stage s + 1; later ones stay out */
                     wait_vm<!C::EARLY ? C::D *(C::STAGES - 2) : TL == 4 ? 0 : C::DA + C::HALF>();
@@ -422,10 +480,7 @@ struct TileRun {
                 });
                 if constexpr (last) read_q(std::integral_constant<int, 0>{});
             });
-            if constexpr (picks) {
-                q_late = q_row;
-                p_row = live_row(p_next, p_rows, s + 3u), q_row = live_row(q_next, q_rows, s + 3u);
-            }
+            if constexpr (picks) q_at[2] = q_late[0], q_at[3] = q_late[1];
         }
         wait_lgkm<0>(); /* the reads past the end: their registers stay taken till here */
         static_for<4>([&](auto I) { pf[decltype(I)::value].ready(); });
@@ -462,48 +517,35 @@ __device__ __forceinline__ void row_tile(const GroupArgs &A, uint8_t *smem, cons
                                          uint32_t col) {
     static_assert(C::LDS <= LDS && 2u * C::BP * C::BQ + 4u * C::BQ <= LDS, "stages; tile and rows");
     TileRun<C> R;
-    R.lane = threadIdx.x & 63u;
-    R.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    R.wn = R.wave % C::WN, R.wt = R.wave / C::WN;
     const uint32_t L = R.lane, p0 = C::BP * col;
-    R.stages = (A.Z + kDepth - 1u) / kDepth;
-    const uint64_t expert = (uint64_t)t.expert * A.P * A.Z;
-    R.p_base = (const uint8_t *)(A.p + expert);
-    if constexpr (C::PCOLS) { /* W[z, p] */
-        R.p_stride = 2u * kDepth * (uint64_t)A.P;
-        R.p_base += 2u * (uint64_t)p0;
-    } else {
-        R.p_stride = 2u * kDepth;
-        R.p_base += 2u * (uint64_t)p0 * A.Z;
-    }
+    R.stages = (A.Z + kDepth - 1u) / kDepth, R.Z = A.Z;
+    /* W[z, p] or W[p, z] */
+    const uint64_t first = C::PCOLS ? p0 : (uint64_t)p0 * A.Z, all = (uint64_t)A.P * A.Z;
+    R.p_stride = 2u * kDepth * (C::PCOLS ? (uint64_t)A.P : 1u);
+    R.p_base = (const uint8_t *)(A.p + t.expert * all + first);
+    R.p_bytes = 2u * (all - first);
+    R.p_z = 8u * a_dma_piece(L, 0u);
 #pragma unroll
     for (int q = 0; q < C::DA; q++) {
         const uint32_t ch = C::DA * R.wave + (uint32_t)q;
         if constexpr (C::PCOLS) {
-            const uint32_t z = col_dma_z<C::BP>(L, ch), piece = col_dma_piece<C::BP>(L, ch);
-            R.p_at[q] = 2u * (z * A.P + min(8u * piece, A.P - 8u - p0));
-            R.p_end[q] = A.Z > z ? A.Z - z : 0u;
+            const uint32_t piece = col_dma_piece<C::BP>(L, ch);
+            R.p_at[q] = 2u * (col_dma_z<C::BP>(L, ch) * A.P + min(8u * piece, A.P - 8u - p0));
         } else {
             const uint32_t h = ch & 1u, r = min(16u * (ch >> 1) + a_dma_row(L, h), A.P - 1u - p0);
-            const uint32_t z = 8u * a_dma_piece(L, h);
-            R.p_at[q] = 2u * (r * A.Z + z);
-            R.p_end[q] = A.Z > z ? A.Z - z : 0u;
+            R.p_at[q] = 2u * (r * A.Z + 8u * a_dma_piece(L, h));
         }
     }
-    R.q_base = (const uint8_t *)(A.q_index ? A.q : A.q + (uint64_t)t.row * A.Z);
     R.q_stride = 2u * kDepth;
+    R.q_base = (const uint8_t *)(A.q_index ? A.q : A.q + (uint64_t)t.row * A.Z);
+    R.q_bytes = 2u * (uint64_t)(A.q_index ? A.q_rows : t.rows) * A.Z;
+    R.q_z = 8u * a_dma_piece(L, C::b_chunk(R.wave, 0u) & 1u);
 #pragma unroll
     for (int q = 0; q < C::DB; q++) {
         const uint32_t ch = C::b_chunk(R.wave, (uint32_t)q), h = ch & 1u;
         uint32_t r = min(16u * (ch >> 1) + a_dma_row(L, h), t.rows - 1u);
-        const uint32_t z = 8u * a_dma_piece(L, h);
-        bool live = true;
-        if (A.q_index) {
-            r = A.q_index[t.row + r];
-            live = r < A.q_rows;
-        }
-        R.q_at[q] = 2u * (r * A.Z + z);
-        R.q_end[q] = live && A.Z > z ? A.Z - z : 0u;
+        if (A.q_index) r = A.q_index[t.row + r];
+        R.q_at[q] = !A.q_index || r < A.q_rows ? 2u * (r * A.Z + 8u * a_dma_piece(L, h)) : kNowhere;
     }
     f32x4 acc[C::TI][4];
     run_steps<C, LDS>(R, acc, smem, t.rows);
@@ -580,31 +622,36 @@ __global__ __launch_bounds__(512, 2) void grouped_weight_kernel(GroupArgs A) {
     const uint32_t grp = w / (4u * A.tiles_p), in = w % (4u * A.tiles_p);
     const uint32_t high = min(4u, A.tiles_q - 4u * grp);
     const uint32_t p0 = C::BP * (in / high), q0 = C::BQ * (4u * grp + in % high);
+    __shared__ uint8_t held[2][8][Picks::BYTES];
     TileRun<C> R;
-    R.lane = threadIdx.x & 63u;
-    R.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    R.wn = R.wave % C::WN, R.wt = R.wave / C::WN;
-    const uint32_t L = R.lane;
-    R.rows = rows_of(A.offsets, expert, A.R, R.row);
-    R.stages = (R.rows + kDepth - 1u) / kDepth;
-    R.p_index = A.p_index, R.q_index = A.q_index, R.p_rows = A.p_rows, R.q_rows = A.q_rows;
-    R.p_bytes = 2u * A.P, R.q_bytes = 2u * A.Q;
-    R.p_base = (const uint8_t *)(A.p + p0);
-    R.q_base = (const uint8_t *)(A.q + q0);
+    const uint32_t L = R.lane, at = L < 8u ? 4u * (8u * R.wave + L) : kNowhere;
+    uint32_t row;
+    const uint32_t rows = rows_of(A.offsets, expert, A.R, row);
+    R.stages = (rows + kDepth - 1u) / kDepth;
+    R.p_row_bytes = 2u * A.P, R.q_row_bytes = 2u * A.Q;
+    R.p_picks = Picks{A.p_index ? A.p_index + row : nullptr, rows, at, held[0][R.wave]};
+    R.q_picks = Picks{A.q_index ? A.q_index + row : nullptr, rows, at, held[1][R.wave]};
+    /* picked rows lie anywhere in the tensor, others move on with the stages */
+    R.p_stride = A.p_index ? 0u : (uint64_t)kDepth * R.p_row_bytes;
+    R.q_stride = A.q_index ? 0u : (uint64_t)kDepth * R.q_row_bytes;
+    R.p_base = (const uint8_t *)(A.p + (A.p_index ? 0u : (uint64_t)row * A.P) + p0);
+    R.q_base = (const uint8_t *)(A.q + (A.q_index ? 0u : (uint64_t)row * A.Q) + q0);
+    R.p_bytes = (uint64_t)(A.p_index ? A.p_rows : rows) * R.p_row_bytes - 2u * p0;
+    R.q_bytes = (uint64_t)(A.q_index ? A.q_rows : rows) * R.q_row_bytes - 2u * q0;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-        R.p_at[q] = 2u * min(8u * col_dma_piece<C::BP>(L, C::DA * R.wave + (uint32_t)q), A.P - 8u - p0);
+        R.p_col[q] = 2u * min(8u * col_dma_piece<C::BP>(L, C::DA * R.wave + (uint32_t)q), A.P - 8u - p0);
         const uint32_t ch = C::b_chunk(R.wave, (uint32_t)q);
-        R.q_at[q] = 2u * min(128u * (ch >> 4) + 8u * col_dma_piece<128u>(L, ch & 15u), A.Q - 8u - q0);
+        R.q_col[q] = 2u * min(128u * (ch >> 4) + 8u * col_dma_piece<128u>(L, ch & 15u), A.Q - 8u - q0);
     }
     const uint32_t high_q = min(C::BQ, A.Q - q0), width = min(C::BP, A.P - p0);
     f32x4 acc[C::TI][4];
     run_steps<C, C::LDS>(R, acc, smem, high_q);
     const uint32_t g = L >> 4, c = L & 15u;
-    const uint64_t at = ((uint64_t)expert * A.Q + q0) * A.P + p0;
+    const uint64_t to = ((uint64_t)expert * A.Q + q0) * A.P + p0;
     if constexpr (F32) {
         if (A.accumulate && R.stages == 0u) return;
-        float *out = (float *)A.out + at;
+        float *out = (float *)A.out + to;
         static_for<C::TI>([&](auto J) {
             constexpr int j = decltype(J)::value;
             const uint32_t r = 16u * (2u * j + R.wt) + c;
@@ -613,18 +660,18 @@ __global__ __launch_bounds__(512, 2) void grouped_weight_kernel(GroupArgs A) {
             for (uint32_t i = 0; i < 4u; i++) {
                 const uint32_t p = 64u * R.wn + 16u * i + 4u * g;
                 if (p >= width) continue;
-                f32x4 *to = (f32x4 *)(out + (uint64_t)r * A.P + p);
+                f32x4 *place = (f32x4 *)(out + (uint64_t)r * A.P + p);
                 f32x4 v = acc[j][i];
                 if (A.accumulate) {
-                    const f32x4 before = *to;
+                    const f32x4 before = *place;
 #pragma unroll
                     for (int k = 0; k < 4; k++) v[k] = __fadd_rn(before[k], v[k]);
                 }
-                *to = v;
+                *place = v;
             }
         });
     } else {
-        uint16_t *out = (uint16_t *)A.out + at;
+        uint16_t *out = (uint16_t *)A.out + to;
         constexpr uint32_t PIECES = C::BP / 8u;
         __syncthreads();
         static_for<C::TI>([&](auto J) {
