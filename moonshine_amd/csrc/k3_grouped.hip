@@ -41,7 +41,7 @@ typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 constexpr uint32_t kMostWidth = 1u << 15, kMostPicked = 65535, kMostRows = 65535u * 32u;
 constexpr uint32_t kDepth = 64; /* z of a stage */
 
-enum Direction { kProduct, kInput, kWeight };
+enum Direction { kProduct, kInput };
 
 struct GroupArgs {
     const uint16_t *p, *q;     /* the operands: W and rows; weight gradient: x and dy */
@@ -164,7 +164,7 @@ template <int DIR_, int WN_, int TI_, int STAGES_>
 struct Tile {
     static constexpr int DIR = DIR_, WN = WN_, TI = TI_, STAGES = STAGES_, WAVES = 2 * WN,
                          THREADS = 64 * WAVES;
-    static constexpr bool PCOLS = DIR != kProduct, QCOLS = DIR == kWeight;
+    static constexpr bool PCOLS = DIR != kProduct;
     static constexpr uint32_t BP = 64 * WN, BQ = 32 * TI;
     static constexpr uint32_t A = BP * kDepth * 2, B = BQ * kDepth * 2, STAGE = A + B;
     static constexpr uint32_t B_CHUNKS = 4 * TI; /* of 1 KB; fewer than the waves: some load the same */
@@ -178,7 +178,6 @@ struct Tile {
     static constexpr bool EARLY = STAGES == 2;
     static_assert(!EARLY || (TI == 8 && WAVES == 8), "two panels of 128 q");
     static constexpr int HALF = EARLY ? DB / 2 : 0; /* loads of the first panel */
-    static constexpr int QREADS = QCOLS ? 4 : 2;    /* of a subtile */
     static __device__ __forceinline__ uint32_t b_chunk(uint32_t wave, uint32_t q) {
         if constexpr (EARLY) return 16u * (q / HALF) + HALF * wave + q % HALF;
         return B_CHUNKS < WAVES ? wave % B_CHUNKS : DB * wave + q;
@@ -239,82 +238,20 @@ struct Fragment<true> {
     }
 };
 
-/*
- * The rows that an operand of a weight gradient picks by an index. A wave loads z = 8 wave .. + 8
- * of a stage; their indices come through LDS as well, by a load of its own that the waits
- * count like any other (one to registers the compiler would wait for with all others out),
- * into a ring of stages.
- */
-struct Picks {
-    static constexpr uint32_t kRing = 4, SLOT = 256, BYTES = SLOT * kRing; /* a load fills a slot */
-    const uint32_t *index; /* from the tile's first row on; NULL: rows as they lie, nothing is read */
-    uint32_t rows, at;     /* at: this lane's place among the indices of a stage */
-    uint8_t *held;         /* this wave's */
-
-    __device__ __forceinline__ void fetch(uint32_t now, uint32_t slot) const {
-        Range(index + kDepth * now, index ? 4u * (uint64_t)(rows - kDepth * now) : 0u)
-            .load<4>(at, held + SLOT * slot);
-    }
-};
-
 template <class C>
 struct TileRun {
-    /* Load q of stage s is from at[q], in p or q moved on by s strides (both an operand's whole
-     * extent from there). Operands of rows: of z, which lies inside them, those below Z;
+    /* Load q of stage s is from at[q], in p or q moved on by s strides (of q 128 bytes), in an
+     * extent of so many bytes. Operands of rows: of z, which lies inside them, those below Z;
      * p_z and q_z are an even q's, ^ 32 an odd one's. */
     const uint8_t *p_base, *q_base;
-    uint64_t p_bytes, q_bytes, p_stride, q_stride;
+    uint64_t p_bytes, q_bytes, p_stride;
     uint32_t p_at[C::DA], q_at[C::DB], p_z, q_z, Z;
-    /* weight gradient: at[q] is z's row times the row's bytes and the column's place */
-    Picks p_picks, q_picks;
-    uint32_t p_row_bytes, q_row_bytes, p_col[C::DA], q_col[C::DB], q_late[2]; /* q_late: q_at[2, 3] next */
     uint32_t stages, wave, lane, wn, wt;
 
     __device__ __forceinline__ TileRun() {
         lane = threadIdx.x & 63u;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         wn = wave % C::WN, wt = wave / C::WN;
-    }
-
-    /* z of load q among the wave's eight */
-    __device__ __forceinline__ uint32_t p_pick(int q) const { return 512u / C::BP * q + (lane >> 5); }
-    __device__ __forceinline__ uint32_t q_pick(int q) const { return 4u * (q & 1) + (lane >> 4); }
-    __device__ __forceinline__ void fetch_picks(uint32_t s) const {
-        const uint32_t now = min(s, stages - 1u), slot = s % Picks::kRing;
-        p_picks.fetch(now, slot);
-        q_picks.fetch(now, slot);
-    }
-    __device__ __forceinline__ void read_picks(uint32_t s, uint32_t (&p)[C::DA], uint32_t (&q)[2]) const {
-        const uint32_t slot = Picks::SLOT * (s % Picks::kRing);
-        const uint32_t p_from = lds_addr(p_picks.held) + slot + 4u * p_pick(0);
-        const uint32_t q_from = lds_addr(q_picks.held) + slot + 4u * q_pick(0);
-        static_for<C::DA>([&](auto Q) { p[decltype(Q)::value] = ds_read4<8 * decltype(Q)::value>(p_from); });
-        q[0] = ds_read4<0>(q_from), q[1] = ds_read4<16>(q_from);
-    }
-    /* A picked row's place: rows past the last, of the stage or of the tensor, lie past its end. The
-     * products are of 24 bits: a row of up to 65535, its bytes. */
-    __device__ __forceinline__ uint32_t place(const Picks &k, uint32_t read, uint32_t s, uint32_t z,
-                                              uint32_t row_bytes, uint32_t col) const {
-        const bool live = kDepth * min(s, stages - 1u) + z < k.rows;
-        const uint32_t r = k.index ? live ? min(read, kMostPicked) : kMostPicked : z;
-        return __umul24(r, row_bytes) + col;
-    }
-    __device__ __forceinline__ void set_picks(uint32_t s, uint32_t (&p)[C::DA], uint32_t (&q)[2]) {
-        if constexpr (C::DIR != kWeight) return;
-        else {
-        static_for<C::DA>([&](auto I) {
-            constexpr int i = decltype(I)::value;
-            after_wait(p[i]);
-            p_at[i] = place(p_picks, p[i], s, 8u * wave + p_pick(i), p_row_bytes, p_col[i]);
-        });
-        static_for<2>([&](auto I) {
-            constexpr int i = decltype(I)::value;
-            after_wait(q[i]);
-            const uint32_t row = place(q_picks, q[i], s, 8u * wave + q_pick(i), q_row_bytes, 0u);
-            q_at[i] = row + q_col[i];
-            q_late[i] = row + q_col[2 + i];
-        });
-        }
     }
 
     template <int Q>
@@ -328,8 +265,8 @@ struct TileRun {
             r.template load<16>(in ? p_at[Q] : kNowhere, st + 1024u * (C::DA * wave + Q));
         } else {
             constexpr int q = Q - C::DA;
-            const Range r(q_base + q_stride * now, C::QCOLS ? q_bytes - q_stride * now : q_bytes);
-            const bool in = C::QCOLS || kDepth * now + (q_z ^ 32u * (C::DB > 1 ? q & 1 : 0)) < Z;
+            const Range r(q_base + 2u * kDepth * now, q_bytes);
+            const bool in = kDepth * now + (q_z ^ 32u * (C::DB > 1 ? q & 1 : 0)) < Z;
             r.template load<16>(in ? q_at[q] : kNowhere, st + C::A + 1024u * C::b_chunk(wave, q));
         }
     }
@@ -349,17 +286,14 @@ struct TileRun {
     __device__ __forceinline__ void run(f32x4 (&acc)[C::TI][4], uint8_t *smem) {
         const uint32_t g = lane >> 4, c = lane & 15u;
         const uint32_t base = lds_addr(smem), lo = a_slot(c, g), hi = a_slot(c, 4u + g);
-        uint32_t p_lo, p_hi = 0u, q_lo, q_hi = 0u;
+        uint32_t p_lo, p_hi = 0u;
         if constexpr (C::PCOLS)
             p_lo = base + (col_slot<C::BP>(lane) ^ 128u * wn);
         else
             p_lo = base + 8192u * wn + lo, p_hi = base + 8192u * wn + hi;
-        if constexpr (C::QCOLS)
-            q_lo = base + C::A + (col_slot<128u>(lane) ^ 32u * wt);
-        else
-            q_lo = base + C::A + 2048u * wt + lo, q_hi = base + C::A + 2048u * wt + hi;
+        const uint32_t q_lo = base + C::A + 2048u * wt + lo, q_hi = base + C::A + 2048u * wt + hi;
         Fragment<C::PCOLS> pf[4];
-        Fragment<C::QCOLS> qf[2];
+        Fragment<false> qf[2];
         uint32_t st = 0u;
         auto read_p = [&](auto I, auto H) {
             constexpr int i = decltype(I)::value, h = decltype(H)::value;
@@ -373,44 +307,16 @@ struct TileRun {
         };
         auto read_q = [&](auto J) {
             constexpr int j = decltype(J)::value;
-            if constexpr (C::QCOLS) {
-                const uint32_t a = (q_lo + st) ^ (64u * (j & 3));
-                static_for<2>([&](auto H) {
-                    constexpr int h = decltype(H)::value, panel = 16384 * (j >> 2);
-                    qf[j & 1].v[h][0] = ds_read_tr<panel + 128 * 64 * h>(a);
-                    qf[j & 1].v[h][1] = ds_read_tr<panel + 128 * (64 * h + 8)>(a);
-                });
-            } else {
-                qf[j & 1].v[0] = ds_read16<4096 * j>(q_lo + st);
-                qf[j & 1].v[1] = ds_read16<4096 * j>(q_hi + st);
-            }
+            qf[j & 1].v[0] = ds_read16<4096 * j>(q_lo + st);
+            qf[j & 1].v[1] = ds_read16<4096 * j>(q_hi + st);
         };
         auto barrier = [] {
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         };
-        constexpr bool picks = C::DIR == kWeight;
-        static_assert(!picks || C::EARLY, "rows are held for two stages on");
-        uint32_t p_next[C::DA], q_next[2];
-        auto rows_of_stage = [&](uint32_t s) {
-            read_picks(s, p_next, q_next);
-            wait_lgkm<0>();
-            set_picks(s, p_next, q_next);
-        };
-        if constexpr (picks) {
-#pragma unroll
-            for (uint32_t s = 0; s < 3u; s++) fetch_picks(s);
-            wait_vm<0>();
-            rows_of_stage(0u);
-            q_at[2] = q_late[0], q_at[3] = q_late[1];
-        }
 #pragma unroll
         for (int s = 0; s < C::STAGES - 1; s++) fetch<0, C::D>(smem, (uint32_t)s, (uint32_t)s);
-        if constexpr (picks) {
-            rows_of_stage(1u);
-            q_at[2] = q_late[0], q_at[3] = q_late[1];
-        }
         if constexpr (C::EARLY) fetch<0, C::DA + C::HALF>(smem, 1u, 1u);
         wait_vm<C::EARLY ? C::DA + C::HALF : C::D *(C::STAGES - 2)>();
         barrier();
@@ -422,10 +328,6 @@ struct TileRun {
         uint32_t slot = 0u, next = C::STAGES - 1;
         for (uint32_t s = 0; s < stages; s++) {
             const uint32_t ahead = s + C::STAGES - 1u, to = next;
-            if constexpr (picks) { /* stage s + 2's have landed, s + 3's are loaded ahead of the rest */
-                read_picks(s + 2u, p_next, q_next);
-                fetch_picks(s + 3u);
-            }
             if constexpr (TL == 1) fetch<0, C::D>(smem, ahead, to);
             next = slot;
             slot = slot + 1u == (uint32_t)C::STAGES ? 0u : slot + 1u;
@@ -433,10 +335,9 @@ struct TileRun {
                 constexpr int j = decltype(J)::value;
                 constexpr bool last = j + 1 == TL;
                 if constexpr (!last) read_q(std::integral_constant<int, j + 1>{});
-                wait_lgkm<last ? 0 : C::QREADS>(); /* the next subtile's reads stay out */
+                wait_lgkm<last ? 0 : 2>(); /* the next subtile's reads stay out */
                 if constexpr (j == 0) static_for<4>([&](auto I) { pf[decltype(I)::value].ready(); });
                 qf[j & 1].ready();
-                if constexpr (picks && j == 0) set_picks(s + 2u, p_next, q_next);
                 if constexpr (last) {
                     /* this wave's loads of stage s + 1; later ones stay out */
                     wait_vm<!C::EARLY ? C::D *(C::STAGES - 2) : TL == 4 ? 0 : C::DA + C::HALF>();
@@ -480,7 +381,6 @@ struct TileRun {
                 });
                 if constexpr (last) read_q(std::integral_constant<int, 0>{});
             });
-            if constexpr (picks) q_at[2] = q_late[0], q_at[3] = q_late[1];
         }
         wait_lgkm<0>(); /* the reads past the end: their registers stay taken till here */
         static_for<4>([&](auto I) { pf[decltype(I)::value].ready(); });
@@ -536,7 +436,6 @@ __device__ __forceinline__ void row_tile(const GroupArgs &A, uint8_t *smem, cons
             R.p_at[q] = 2u * (r * A.Z + 8u * a_dma_piece(L, h));
         }
     }
-    R.q_stride = 2u * kDepth;
     R.q_base = (const uint8_t *)(A.q_index ? A.q : A.q + (uint64_t)t.row * A.Z);
     R.q_bytes = 2u * (uint64_t)(A.q_index ? A.q_rows : t.rows) * A.Z;
     R.q_z = 8u * a_dma_piece(L, C::b_chunk(R.wave, 0u) & 1u);
@@ -608,11 +507,206 @@ __global__ __launch_bounds__(512, 2) void grouped_rows_kernel(GroupArgs A) {
     else row_tile<Tile256<DIR>, LDS>(A, smem, t, col);
 }
 
-/* 256 x 256 of an expert's weight gradient: p its columns (x), q its rows (dy). */
+/* ---------------------------------------------------------------------- */
+/* weight gradient                                                         */
+/* ---------------------------------------------------------------------- */
+
+/*
+ * A block holds 128 of p (columns of x) x 256 of q (columns of dy), in four waves of 64 x 128,
+ * and two blocks lie on a CU: a reduction is as long as an expert has rows, often only a few
+ * stages, and one block's first loads and its stores (128 KB in f32) run under the other's products.
+ * A stage is 32 rows; q is kept as two panels of 128 columns.
+ */
+struct Weight {
+    static constexpr uint32_t BP = 128, BQ = 256, DEPTH = 32, STAGES = 3, WAVES = 4, THREADS = 256;
+    static constexpr uint32_t A = BP * DEPTH * 2, B = BQ * DEPTH * 2, STAGE = A + B, PANEL = B / 2;
+    static constexpr int DA = 2, DB = 4, D = DA + DB; /* loads of 1 KB, four rows of 128 columns, a wave */
+    static constexpr int TI = 8;                      /* subtiles of q of a wave */
+};
+
+/*
+ * The rows that an operand picks by an index. A wave loads rows 8 wave .. + 8 of a stage; their
+ * indices come through LDS as well, by a load of its own that the waits count like any other (one
+ * to registers the compiler would wait for with all others out), into a ring of stages.
+ */
+struct Picks {
+    static constexpr uint32_t kRing = 4, SLOT = 256, BYTES = SLOT * kRing; /* a load fills a slot */
+    const uint32_t *index; /* from the expert's first row on; NULL: rows as they lie, nothing is read */
+    uint32_t rows, at;     /* at: this lane's place among the indices of a stage */
+    uint8_t *held;         /* this wave's */
+
+    __device__ __forceinline__ void fetch(uint32_t now, uint32_t slot) const {
+        Range(index + Weight::DEPTH * now, index ? 4u * (uint64_t)(rows - Weight::DEPTH * now) : 0u)
+            .load<4>(at, held + SLOT * slot);
+    }
+    /* The places of this lane's two rows of a stage by the indices read: its row times the row's
+     * bytes. Rows past the expert's last, or the tensor's, lie past the range's end. The products
+     * are of 24 bits: a row of up to 65535, its bytes. */
+    __device__ __forceinline__ uint32_t place(uint32_t read, uint32_t now, uint32_t z, uint32_t row_bytes) const {
+        const bool live = Weight::DEPTH * now + z < rows;
+        return __umul24(index ? live ? min(read, kMostPicked) : kMostPicked : z, row_bytes);
+    }
+};
+
+struct WeightRun {
+    using C = Weight;
+    const uint8_t *p_base, *q_base; /* moved on by a stride each stage where rows lie in order */
+    uint64_t p_bytes, q_bytes, p_stride, q_stride;
+    Picks p, q;
+    uint32_t p_row_bytes, q_row_bytes, p_col[2], q_col[4]; /* the loads' columns */
+    uint32_t p_at[2], q_at[2];                             /* and rows, of the stage that is loaded */
+    uint32_t stages, wave, lane, wn, wt;
+
+    __device__ __forceinline__ WeightRun() {
+        lane = threadIdx.x & 63u;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        wn = wave % 2u, wt = wave / 2u;
+    }
+    __device__ __forceinline__ uint32_t clamped(uint32_t s) const { return min(s, stages - 1u); }
+    __device__ __forceinline__ void fetch_picks(uint32_t s) const {
+        p.fetch(clamped(s), s % Picks::kRing);
+        q.fetch(clamped(s), s % Picks::kRing);
+    }
+    __device__ __forceinline__ void read_picks(uint32_t s, uint32_t (&r)[4]) const {
+        const uint32_t at = Picks::SLOT * (s % Picks::kRing) + 4u * (lane >> 4);
+        r[0] = ds_read4<0>(lds_addr(p.held) + at), r[1] = ds_read4<16>(lds_addr(p.held) + at);
+        r[2] = ds_read4<0>(lds_addr(q.held) + at), r[3] = ds_read4<16>(lds_addr(q.held) + at);
+    }
+    __device__ __forceinline__ void set_rows(uint32_t s, uint32_t (&r)[4]) {
+        static_for<4>([&](auto I) { after_wait(r[decltype(I)::value]); });
+        const uint32_t now = clamped(s), z = 8u * wave + (lane >> 4);
+        p_at[0] = p.place(r[0], now, z, p_row_bytes), p_at[1] = p.place(r[1], now, z + 4u, p_row_bytes);
+        q_at[0] = q.place(r[2], now, z, q_row_bytes), q_at[1] = q.place(r[3], now, z + 4u, q_row_bytes);
+    }
+    /* Load Q of stage s; past the end the last stage again, so that the counts of the waits stay. */
+    template <int Q>
+    __device__ __forceinline__ void fetch_one(uint8_t *smem, uint32_t s, uint32_t slot) const {
+        uint8_t *st = smem + C::STAGE * slot;
+        const uint32_t now = clamped(s);
+        if constexpr (Q < C::DA) {
+            Range(p_base + p_stride * now, p_bytes - p_stride * now)
+                .load<16>(p_at[Q] + p_col[Q], st + 1024u * (2u * wave + Q));
+        } else {
+            constexpr int q = Q - C::DA;
+            Range(q_base + q_stride * now, q_bytes - q_stride * now)
+                .load<16>(q_at[q & 1] + q_col[q], st + C::A + C::PANEL * (q >> 1) + 1024u * (2u * wave + (q & 1)));
+        }
+    }
+    __device__ __forceinline__ void fetch(uint8_t *smem, uint32_t s, uint32_t slot) const {
+        static_for<C::D>([&](auto Q) { fetch_one<decltype(Q)::value>(smem, s, slot); });
+    }
+
+    /* acc[j] += the products over all stages, for the first 2 PAIRS subtiles of a wave, two a step, as
+     * in TileRun: a step's reads run under the products of the one before. */
+    template <int PAIRS>
+    __device__ __forceinline__ void run(f32x4 (&acc)[C::TI][4], uint8_t *smem) {
+        const uint32_t base = lds_addr(smem);
+        const uint32_t p_lo = base + (col_slot<128u>(lane) ^ 128u * wn);
+        const uint32_t q_lo = base + C::A + (col_slot<128u>(lane) ^ 32u * wt);
+        u32x2_t pf[4][2], qf[2][2][2];
+        uint32_t st = 0u;
+        auto read_p = [&](auto I) {
+            constexpr int i = decltype(I)::value;
+            const uint32_t a = (p_lo + st) ^ (32u * i);
+            pf[i][0] = ds_read_tr<0>(a), pf[i][1] = ds_read_tr<1024>(a);
+        };
+        auto read_q = [&](auto S) {
+            constexpr int step = decltype(S)::value;
+            static_for<2>([&](auto J) {
+                constexpr int j = 2 * step + decltype(J)::value, panel = C::PANEL * (j >> 2);
+                const uint32_t a = (q_lo + st) ^ (64u * (j & 3));
+                qf[step & 1][j & 1][0] = ds_read_tr<panel>(a), qf[step & 1][j & 1][1] = ds_read_tr<panel + 1024>(a);
+            });
+        };
+        auto whole = [](const u32x2_t (&v)[2]) {
+            return __builtin_bit_cast(bf16x8, u32x4_t{v[0].x, v[0].y, v[1].x, v[1].y});
+        };
+        auto barrier = [] {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        uint32_t next_rows[4];
+#pragma unroll
+        for (uint32_t s = 0; s < 3u; s++) fetch_picks(s);
+        wait_vm<0>();
+#pragma unroll
+        for (uint32_t s = 0; s < 2u; s++) {
+            read_picks(s, next_rows);
+            wait_lgkm<0>();
+            set_rows(s, next_rows);
+            fetch(smem, s, s);
+        }
+        wait_vm<C::D>(); /* stage 0 */
+        barrier();
+        static_for<4>(read_p);
+        read_q(std::integral_constant<int, 0>{});
+        uint32_t slot = 0u, to = 2u;
+        for (uint32_t s = 0; s < stages; s++) {
+            /* stage s + 2's rows have landed, s + 3's are loaded ahead of the rest */
+            read_picks(s + 2u, next_rows);
+            fetch_picks(s + 3u);
+            const uint32_t free = to;
+            to = slot;
+            slot = slot + 1u == C::STAGES ? 0u : slot + 1u;
+            static_for<PAIRS>([&](auto S) {
+                constexpr int step = decltype(S)::value;
+                constexpr bool last = step + 1 == PAIRS;
+                if constexpr (!last) read_q(std::integral_constant<int, step + 1>{});
+                wait_lgkm<last ? 0 : 4>();
+                if constexpr (step == 0) {
+                    static_for<4>([&](auto I) {
+                        after_wait(pf[decltype(I)::value][0]);
+                        after_wait(pf[decltype(I)::value][1]);
+                    });
+                    set_rows(s + 2u, next_rows);
+                }
+                static_for<2>([&](auto J) {
+                    after_wait(qf[step & 1][decltype(J)::value][0]);
+                    after_wait(qf[step & 1][decltype(J)::value][1]);
+                });
+                if constexpr (last) {
+                    wait_vm<C::D>(); /* stage s + 1 has landed; this stage's loads stay out */
+                    barrier();
+                    st = C::STAGE * slot;
+                }
+                static_for<2>([&](auto J) {
+                    constexpr int j = 2 * step + decltype(J)::value;
+                    static_for<4>([&](auto I) {
+                        constexpr int i = decltype(I)::value;
+                        acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(whole(pf[i]), whole(qf[step & 1][j & 1]),
+                                                                            acc[j][i], 0, 0, 0);
+                        if constexpr (last && (j & 1) == 1) read_p(I);
+                        __builtin_amdgcn_sched_barrier(0);
+                        /* the loads ahead, spread over the steps before the last */
+                        constexpr int at = 4 * j + i;
+                        static_for<C::D>([&](auto Q) {
+                            if constexpr (1 + decltype(Q)::value * (8 * (PAIRS - 1) - 1) / C::D == at)
+                                fetch_one<decltype(Q)::value>(smem, s + 2u, free);
+                        });
+                    });
+                });
+                if constexpr (last) read_q(std::integral_constant<int, 0>{});
+            });
+        }
+        wait_lgkm<0>(); /* the reads past the end: their registers stay taken till here */
+        static_for<4>([&](auto I) {
+            after_wait(pf[decltype(I)::value][0]);
+            after_wait(pf[decltype(I)::value][1]);
+        });
+        static_for<2>([&](auto J) {
+            after_wait(qf[0][decltype(J)::value][0]);
+            after_wait(qf[0][decltype(J)::value][1]);
+        });
+        wait_vm<0>(); /* the loads past the end land before the LDS is used again */
+    }
+};
+
 template <bool F32>
-__global__ __launch_bounds__(512, 2) void grouped_weight_kernel(GroupArgs A) {
-    using C = Tile<kWeight, 4, 8, 2>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
+__global__ __launch_bounds__(256, 2) void grouped_weight_kernel(GroupArgs A) {
+    using C = Weight;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[C::STAGES * C::STAGE];
+    __shared__ uint8_t held[2][C::WAVES][Picks::BYTES];
     const uint32_t works = A.E * A.tiles_p * A.tiles_q, each = (works + 7u) / 8u;
     uint32_t w = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= each || w >= works) return;
@@ -620,78 +714,85 @@ __global__ __launch_bounds__(512, 2) void grouped_weight_kernel(GroupArgs A) {
     w %= A.tiles_p * A.tiles_q;
     /* four q tiles at a time, along p */
     const uint32_t grp = w / (4u * A.tiles_p), in = w % (4u * A.tiles_p);
-    const uint32_t high = min(4u, A.tiles_q - 4u * grp);
-    const uint32_t p0 = C::BP * (in / high), q0 = C::BQ * (4u * grp + in % high);
-    __shared__ uint8_t held[2][8][Picks::BYTES];
-    TileRun<C> R;
+    const uint32_t many = min(4u, A.tiles_q - 4u * grp);
+    const uint32_t p0 = C::BP * (in / many), q0 = C::BQ * (4u * grp + in % many);
+    WeightRun R;
     const uint32_t L = R.lane, at = L < 8u ? 4u * (8u * R.wave + L) : kNowhere;
     uint32_t row;
     const uint32_t rows = rows_of(A.offsets, expert, A.R, row);
-    R.stages = (rows + kDepth - 1u) / kDepth;
+    R.stages = (rows + C::DEPTH - 1u) / C::DEPTH;
     R.p_row_bytes = 2u * A.P, R.q_row_bytes = 2u * A.Q;
-    R.p_picks = Picks{A.p_index ? A.p_index + row : nullptr, rows, at, held[0][R.wave]};
-    R.q_picks = Picks{A.q_index ? A.q_index + row : nullptr, rows, at, held[1][R.wave]};
+    R.p = Picks{A.p_index ? A.p_index + row : nullptr, rows, at, held[0][R.wave]};
+    R.q = Picks{A.q_index ? A.q_index + row : nullptr, rows, at, held[1][R.wave]};
     /* picked rows lie anywhere in the tensor, others move on with the stages */
-    R.p_stride = A.p_index ? 0u : (uint64_t)kDepth * R.p_row_bytes;
-    R.q_stride = A.q_index ? 0u : (uint64_t)kDepth * R.q_row_bytes;
+    R.p_stride = A.p_index ? 0u : (uint64_t)C::DEPTH * R.p_row_bytes;
+    R.q_stride = A.q_index ? 0u : (uint64_t)C::DEPTH * R.q_row_bytes;
     R.p_base = (const uint8_t *)(A.p + (A.p_index ? 0u : (uint64_t)row * A.P) + p0);
     R.q_base = (const uint8_t *)(A.q + (A.q_index ? 0u : (uint64_t)row * A.Q) + q0);
     R.p_bytes = (uint64_t)(A.p_index ? A.p_rows : rows) * R.p_row_bytes - 2u * p0;
     R.q_bytes = (uint64_t)(A.q_index ? A.q_rows : rows) * R.q_row_bytes - 2u * q0;
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-        R.p_col[q] = 2u * min(8u * col_dma_piece<C::BP>(L, C::DA * R.wave + (uint32_t)q), A.P - 8u - p0);
-        const uint32_t ch = C::b_chunk(R.wave, (uint32_t)q);
-        R.q_col[q] = 2u * min(128u * (ch >> 4) + 8u * col_dma_piece<128u>(L, ch & 15u), A.Q - 8u - q0);
+    for (uint32_t q = 0; q < 2u; q++) {
+        const uint32_t col = 8u * col_dma_piece<128u>(L, 2u * R.wave + q);
+        R.p_col[q] = 2u * min(col, A.P - 8u - p0);
+        R.q_col[q] = 2u * min(col, A.Q - 8u - q0);
+        R.q_col[2u + q] = 2u * min(128u + col, A.Q - 8u - q0);
     }
-    const uint32_t high_q = min(C::BQ, A.Q - q0), width = min(C::BP, A.P - p0);
+    const uint32_t high = min(C::BQ, A.Q - q0), width = min(C::BP, A.P - p0);
     f32x4 acc[C::TI][4];
-    run_steps<C, C::LDS>(R, acc, smem, high_q);
+#pragma unroll
+    for (int j = 0; j < C::TI; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (R.stages != 0u) {
+        if (high <= 128u) R.run<2>(acc, smem);
+        else R.run<4>(acc, smem);
+    }
     const uint32_t g = L >> 4, c = L & 15u;
     const uint64_t to = ((uint64_t)expert * A.Q + q0) * A.P + p0;
-    if constexpr (F32) {
-        if (A.accumulate && R.stages == 0u) return;
-        float *out = (float *)A.out + to;
-        static_for<C::TI>([&](auto J) {
+    /* through LDS for stores of whole rows (64-byte pieces straight from the accumulators took 10 us for
+     * 256 x 256): f32 128 rows at a time, bf16 all; piece p of row r lies at p ^ r modulo 16 */
+    constexpr uint32_t ROW = F32 ? 512u : 256u, HIGH = F32 ? 128u : 256u, PIECES = ROW / 16u;
+    static_assert(ROW * HIGH <= sizeof smem, "the part of the tile");
+    if (F32 && A.accumulate && R.stages == 0u) return;
+    static_for<C::BQ / HIGH>([&](auto H) {
+        constexpr int part = decltype(H)::value, JS = HIGH / 32;
+        __syncthreads();
+        static_for<JS>([&](auto J) {
             constexpr int j = decltype(J)::value;
             const uint32_t r = 16u * (2u * j + R.wt) + c;
-            if (r >= high_q) return;
 #pragma unroll
             for (uint32_t i = 0; i < 4u; i++) {
-                const uint32_t p = 64u * R.wn + 16u * i + 4u * g;
-                if (p >= width) continue;
-                f32x4 *place = (f32x4 *)(out + (uint64_t)r * A.P + p);
-                f32x4 v = acc[j][i];
+                const f32x4 &v = acc[JS * part + j][i];
+                const uint32_t n = 16u * R.wn + 4u * i + g; /* of four columns */
+                if constexpr (F32)
+                    *(f32x4 *)(smem + ROW * r + 16u * (n ^ (r & 15u))) = v;
+                else
+                    *(uint2 *)(smem + ROW * r + 16u * (n >> 1 ^ (r & 15u)) + 8u * (n & 1u)) = bf16x4(v);
+            }
+        });
+        __syncthreads();
+        const uint32_t piece = threadIdx.x % PIECES;
+        if ((F32 ? 4u : 8u) * piece >= width) return;
+#pragma unroll 4
+        for (uint32_t r = threadIdx.x / PIECES; r < HIGH; r += C::THREADS / PIECES) {
+            const uint32_t q = HIGH * part + r;
+            if (q >= high) break;
+            const uint4 v = *(const uint4 *)(smem + ROW * r + 16u * (piece ^ (r & 15u)));
+            if constexpr (F32) {
+                f32x4 *place = (f32x4 *)((float *)A.out + to + (uint64_t)q * A.P + 4u * piece);
+                f32x4 sum = __builtin_bit_cast(f32x4, v);
                 if (A.accumulate) {
                     const f32x4 before = *place;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = __fadd_rn(before[k], v[k]);
+                    for (int k = 0; k < 4; k++) sum[k] = __fadd_rn(before[k], sum[k]);
                 }
-                *place = v;
+                __builtin_nontemporal_store(sum, place);
+            } else {
+                *(uint4 *)((uint16_t *)A.out + to + (uint64_t)q * A.P + 8u * piece) = v;
             }
-        });
-    } else {
-        uint16_t *out = (uint16_t *)A.out + to;
-        constexpr uint32_t PIECES = C::BP / 8u;
-        __syncthreads();
-        static_for<C::TI>([&](auto J) {
-            constexpr int j = decltype(J)::value;
-            if (32u * j >= high_q) return;
-            const uint32_t r = 16u * (2u * j + R.wt) + c;
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; i++) {
-                const uint32_t p = 8u * R.wn + 2u * i + (g >> 1);
-                *(uint2 *)(smem + 16u * (PIECES * r + (p ^ (r & (PIECES - 1u)))) + 8u * (g & 1u)) =
-                    bf16x4(acc[j][i]);
-            }
-        });
-        __syncthreads();
-        const uint32_t p = threadIdx.x % PIECES;
-        if (8u * p >= width) return;
-        for (uint32_t r = threadIdx.x / PIECES; r < high_q; r += C::THREADS / PIECES)
-            *(uint4 *)(out + (uint64_t)r * A.P + 8u * p) =
-                *(const uint4 *)(smem + 16u * (PIECES * r + (p ^ (r & (PIECES - 1u)))));
-    }
+        }
+    });
 }
 
 /* ---------------------------------------------------------------------- */
@@ -787,10 +888,10 @@ extern "C" bool k3_moe_grouped_weight_gradient_bf16(void *output, bool f32, bool
     A.p_index = input_index, A.q_index = gradient_index, A.p_rows = input_rows, A.q_rows = gradient_rows;
     A.out = output, A.R = rows, A.E = expert_count, A.P = columns, A.Q = out_columns;
     A.accumulate = accumulate;
-    A.tiles_p = (columns + 255u) / 256u, A.tiles_q = (out_columns + 255u) / 256u;
+    A.tiles_p = (columns + Weight::BP - 1u) / Weight::BP, A.tiles_q = (out_columns + Weight::BQ - 1u) / Weight::BQ;
     const uint64_t blocks = 8u * (((uint64_t)expert_count * A.tiles_p * A.tiles_q + 7u) / 8u);
     if (blocks >= 1u << 23) return false;
     const auto kernel = f32 ? grouped_weight_kernel<true> : grouped_weight_kernel<false>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(512), 0, (hipStream_t)stream, A);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(Weight::THREADS), 0, (hipStream_t)stream, A);
     return hipGetLastError() == hipSuccess;
 }
