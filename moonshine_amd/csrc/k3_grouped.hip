@@ -100,61 +100,62 @@ __device__ __forceinline__ uint32_t rows_of(const uint32_t *offsets, uint32_t e,
     return end > begin ? end - begin : 0u;
 }
 
-__device__ __forceinline__ uint32_t tiles_of(uint32_t n) { return (n + 255u) / 256u; }
-
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t a = __shfl_up(v, o, 64);
-        if ((int)lane >= o) v += a;
-    }
+/* Sums over the lanes up to each. */
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false); /* row_shr 1, 2, 4, 8 */
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false); /* row_bcast 15, 31 */
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
     return v;
 }
 
 struct RowTile {
-    uint32_t expert, row, rows, many, index, n; /* n: the expert's rows, in `many` tiles */
+    uint32_t expert, row, rows, n; /* n: all rows of the expert */
 };
 
 /*
- * Row tile and column of work `block` among all experts' row tiles x tiles_p columns,
- * found by every wave for itself from the offsets: each lane counts the tiles of
- * up to 16 consecutive experts, and the lanes then take those of the one that holds the
- * tile. About 1 us, where a launch that lists the tiles takes 4. An expert's tiles
+ * Row tile and column of work `block` among all experts' row tiles (of MOST rows at most) x
+ * tiles_p columns, found by every wave for itself from the offsets: each lane counts the
+ * tiles of up to 16 consecutive experts, and the lanes then take those of the one that holds
+ * the tile. About 1 us, where a launch that lists the tiles takes 4. An expert's tiles
  * of one column are neighbours, as they read the same weights; XCD x (blocks x,
  * x + 8, ...) takes a contiguous range of the works. False past the end.
  */
+template <uint32_t MOST>
 __device__ __forceinline__ bool find_tile(const GroupArgs &A, uint32_t block, RowTile &t,
                                           uint32_t &col) {
     const uint32_t lane = threadIdx.x & 63u, per = (A.E + 63u) / 64u;
-    uint32_t mine = 0u;
+    uint32_t mine = 0u, begin = 0u, n = 0u;
     for (uint32_t i = 0; i < per; i++) {
         const uint32_t e = lane * per + i;
-        uint32_t begin;
-        if (e < A.E) mine += tiles_of(rows_of(A.offsets, e, A.R, begin));
+        n = e < A.E ? rows_of(A.offsets, e, A.R, begin) : 0u;
+        mine += (n + MOST - 1u) / MOST;
     }
-    const uint32_t upto = wave_scan(mine, lane);
-    const uint32_t total = __builtin_amdgcn_readlane(upto, 63);
-    const uint32_t works = total * A.tiles_p, each = (works + 7u) / 8u;
+    const uint32_t upto = wave_scan(mine);
+    const uint32_t works = __builtin_amdgcn_readlane(upto, 63) * A.tiles_p, each = (works + 7u) / 8u;
     const uint32_t w = (block & 7u) * each + (block >> 3);
     if ((block >> 3) >= each || w >= works) return false;
     const uint32_t tile = w / A.tiles_p; /* an expert's tiles x columns, before its order is set */
     const uint32_t owner = __builtin_ctzll(__ballot(upto > tile));
-    const uint32_t before = __builtin_amdgcn_readlane(upto - mine, owner);
-    const uint32_t e = owner * per + lane;
-    uint32_t begin = 0u, n = 0u;
-    if (lane < per && e < A.E) n = rows_of(A.offsets, e, A.R, begin);
-    const uint32_t many = tiles_of(n), to = before + wave_scan(many, lane);
-    const uint32_t at = __builtin_ctzll(__ballot(to > tile));
+    uint32_t at = owner, first = __builtin_amdgcn_readlane(upto - mine, owner), many = mine;
+    if (per > 1u) {
+        const uint32_t e = owner * per + lane;
+        n = lane < per && e < A.E ? rows_of(A.offsets, e, A.R, begin) : 0u;
+        many = (n + MOST - 1u) / MOST;
+        const uint32_t to = first + wave_scan(many);
+        at = __builtin_ctzll(__ballot(to > tile));
+        first = __builtin_amdgcn_readlane(to - many, at);
+    }
     t.n = __builtin_amdgcn_readlane(n, at);
-    t.many = __builtin_amdgcn_readlane(many, at);
-    t.expert = owner * per + at;
-    const uint32_t first = __builtin_amdgcn_readlane(to, at) - t.many;
+    many = __builtin_amdgcn_readlane(many, at);
+    t.expert = per > 1u ? owner * per + at : at;
     const uint32_t local = (tile - first) * A.tiles_p + w % A.tiles_p;
-    const uint32_t height = tile_height(t.n);
-    t.index = local % t.many;
-    col = local / t.many;
-    t.row = __builtin_amdgcn_readlane(begin, at) + height * t.index;
-    t.rows = t.n > height * t.index ? min(height, t.n - height * t.index) : 0u;
+    const uint32_t height = MOST == 256u ? tile_height(t.n) : MOST, index = local % many;
+    col = local / many;
+    t.row = __builtin_amdgcn_readlane(begin, at) + height * index;
+    t.rows = min(height, t.n - height * index);
     return true;
 }
 
@@ -500,11 +501,66 @@ __global__ __launch_bounds__(512, 2) void grouped_rows_kernel(GroupArgs A) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[LDS];
     RowTile t;
     uint32_t col;
-    if (!find_tile(A, blockIdx.x, t, col) || t.rows == 0u) return;
+    if (!find_tile<256u>(A, blockIdx.x, t, col)) return;
     if (t.n <= 32u) row_tile<Tile32<DIR>, LDS>(A, smem, t, col);
     else if (t.n <= 64u) row_tile<Tile64<DIR>, LDS>(A, smem, t, col);
     else if (t.n <= 128u) row_tile<Tile128<DIR>, LDS>(A, smem, t, col);
     else row_tile<Tile256<DIR>, LDS>(A, smem, t, col);
+}
+
+/*
+ * A product of few rows: up to 16 of an expert x 16 of p a block, whose eight waves share z: pairs
+ * of 32, so that a wave reads whole 128-byte lines, straight into the registers of the MFMA
+ * layout, and add up through LDS in one order. More blocks than tiles of 256 p, and
+ * no stage to fill: bound by the latency of two loads, then by the weights' stream.
+ */
+__global__ __launch_bounds__(512) void grouped_few_kernel(GroupArgs A) {
+    __shared__ f32x4 sums[8][64];
+    RowTile t;
+    uint32_t col;
+    if (!find_tile<16u>(A, blockIdx.x, t, col)) return;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u, n0 = 16u * col;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint16_t *w = A.p + (uint64_t)t.expert * A.P * A.Z + (uint64_t)min(n0 + c, A.P - 1u) * A.Z;
+    uint32_t r = t.row + min(c, t.rows - 1u), to = r;
+    if (A.to) to = A.to[r];
+    bool row = true;
+    if (A.q_index) {
+        r = A.q_index[r];
+        row = r < A.q_rows;
+    }
+    const uint16_t *x = A.q + (uint64_t)(row ? r : 0u) * A.Z;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int DEEP = 4; /* pairs under way */
+    for (uint32_t k = 64u * wave; k < A.Z; k += 512u * DEEP) {
+        u32x4_t a[DEEP][2], b[DEEP][2];
+#pragma unroll
+        for (int i = 0; i < DEEP; i++)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) {
+                const uint32_t z = k + 512u * (uint32_t)i + 32u * h + 8u * g;
+                a[i][h] = b[i][h] = u32x4_t{0u, 0u, 0u, 0u};
+                if (z < A.Z) { /* 8 of z, a multiple of 8 */
+                    a[i][h] = __builtin_nontemporal_load((const u32x4_t *)(w + z));
+                    if (row) b[i][h] = *(const u32x4_t *)(x + z);
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < DEEP; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[i][h]),
+                                                              __builtin_bit_cast(bf16x8, b[i][h]), acc, 0, 0, 0);
+    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0u) return;
+#pragma unroll
+    for (int v = 1; v < 8; v++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = __fadd_rn(acc[i], sums[v][lane][i]);
+    if (c < t.rows && n0 + 4u * g < A.P && (!A.to || to < A.to_rows))
+        *(uint2 *)((uint16_t *)A.out + (uint64_t)to * A.P + n0 + 4u * g) = bf16x4(acc);
 }
 
 /* ---------------------------------------------------------------------- */
@@ -810,6 +866,12 @@ bool picks_ok(const uint32_t *index, uint32_t have, uint32_t rows) {
     return (uintptr_t)index % 4u == 0u && (index ? have != 0u && have <= kMostPicked : have >= rows);
 }
 
+/* Most blocks of a product that goes 16 rows x 16 columns a block. us, so and by tiles of 256
+ * columns, rows of experts chosen at random: 1024 x 2048, 4 of 64 experts, 4 rows (256 blocks) 5.1 and
+ * 15.6, 8 rows 8.0 and 16.4, 16 rows (1024) 15.3 and 16.9, 32 rows 22.0 and 18.3; 2048 x 512, 8
+ * rows (1024) 5.8 and 7.0, 16 rows 12.5 and 7.1; 7168 x 2048, 8 rows (3584) 44.9 and 36.9. */
+constexpr uint64_t kFewBlocks = 1024;
+
 template <int DIR>
 bool launch_rows(void *output, const void *input, const void *weights, const uint32_t *offsets,
                  const uint32_t *input_index, const uint32_t *output_index, uint32_t rows,
@@ -830,9 +892,16 @@ bool launch_rows(void *output, const void *input, const void *weights, const uin
     A.p = (const uint16_t *)weights, A.q = (const uint16_t *)input, A.offsets = offsets;
     A.q_index = input_index, A.to = output_index, A.q_rows = input_rows, A.to_rows = output_rows;
     A.out = output, A.R = rows, A.E = experts, A.P = P, A.Z = Z;
+    /* n rows are in at most 1 + n / 16 tiles of 16, of experts that have rows */
+    const uint32_t used = experts < rows ? experts : rows;
+    const uint64_t few = (uint64_t)(rows / 16u + used) * ((P + 15u) / 16u);
+    if (DIR == kProduct && few <= kFewBlocks) {
+        A.tiles_p = (P + 15u) / 16u;
+        hipLaunchKernelGGL(grouped_few_kernel, dim3((uint32_t)few + 8u), dim3(512), 0, st, A);
+        return hipGetLastError() == hipSuccess;
+    }
     A.tiles_p = (P + 255u) / 256u;
-    /* n rows are in at most 1 + n / 256 tiles, of experts that have rows */
-    const uint64_t tiles = rows / 256u + (experts < rows ? experts : rows);
+    const uint64_t tiles = rows / 256u + used;
     const uint64_t blocks = tiles * A.tiles_p + 8u;
     if (blocks >= 1u << 23) return false; /* 2^32 threads */
     hipLaunchKernelGGL(grouped_rows_kernel<DIR>, dim3((uint32_t)blocks), dim3(512), 0, st, A);
