@@ -177,8 +177,8 @@ struct Tile {
      * a second barrier there their places take those of two stages on; the other q's follow
      * in the next stage. */
     static constexpr bool EARLY = STAGES == 2;
-    static_assert(!EARLY || (TI == 8 && WAVES == 8), "two panels of 128 q");
     static constexpr int HALF = EARLY ? DB / 2 : 0; /* loads of the first panel */
+    static_assert(!EARLY || (TI == 8 && HALF * WAVES == 16), "two panels of 128 q");
     static __device__ __forceinline__ uint32_t b_chunk(uint32_t wave, uint32_t q) {
         if constexpr (EARLY) return 16u * (q / HALF) + HALF * wave + q % HALF;
         return B_CHUNKS < WAVES ? wave % B_CHUNKS : DB * wave + q;
@@ -488,24 +488,23 @@ __device__ __forceinline__ void row_tile(const GroupArgs &A, uint8_t *smem, cons
     }
 }
 
-template <int DIR> using Tile32 = Tile<DIR, 4, 1, 4>;
-template <int DIR> using Tile64 = Tile<DIR, 4, 2, 3>;
-template <int DIR> using Tile128 = Tile<DIR, 4, 4, 3>;
-template <int DIR> using Tile256 = Tile<DIR, 4, 8, 2>;
-
-/* A block's class goes by the rows of its expert: a CU holds one block of any, so the
- * largest's registers and LDS cost the others nothing. */
-template <int DIR>
-__global__ __launch_bounds__(512, 2) void grouped_rows_kernel(GroupArgs A) {
-    constexpr uint32_t LDS = Tile128<DIR>::LDS;
+/* Tiles of 64 WN columns. A block's class goes by the rows of its expert: a CU holds one block
+ * of any, so the largest's registers and LDS cost the others nothing. */
+template <int DIR, int WN>
+__global__ __launch_bounds__(128 * WN, WN / 2) void grouped_rows_kernel(GroupArgs A) {
+    using Tile32 = Tile<DIR, WN, 1, 4>;
+    using Tile64 = Tile<DIR, WN, 2, 3>;
+    using Tile128 = Tile<DIR, WN, 4, 3>;
+    using Tile256 = Tile<DIR, WN, 8, 2>;
+    constexpr uint32_t LDS = Tile128::LDS;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[LDS];
     RowTile t;
     uint32_t col;
     if (!find_tile<256u>(A, blockIdx.x, t, col)) return;
-    if (t.n <= 32u) row_tile<Tile32<DIR>, LDS>(A, smem, t, col);
-    else if (t.n <= 64u) row_tile<Tile64<DIR>, LDS>(A, smem, t, col);
-    else if (t.n <= 128u) row_tile<Tile128<DIR>, LDS>(A, smem, t, col);
-    else row_tile<Tile256<DIR>, LDS>(A, smem, t, col);
+    if (t.n <= 32u) row_tile<Tile32, LDS>(A, smem, t, col);
+    else if (t.n <= 64u) row_tile<Tile64, LDS>(A, smem, t, col);
+    else if (t.n <= 128u) row_tile<Tile128, LDS>(A, smem, t, col);
+    else row_tile<Tile256, LDS>(A, smem, t, col);
 }
 
 /*
@@ -872,6 +871,17 @@ bool picks_ok(const uint32_t *index, uint32_t have, uint32_t rows) {
  * rows (1024) 5.8 and 7.0, 16 rows 12.5 and 7.1; 7168 x 2048, 8 rows (3584) 44.9 and 36.9. */
 constexpr uint64_t kFewBlocks = 1024;
 
+/* Tiles of 128 columns instead of 256, where these leave half of the CUs without one: `used`
+ * experts have up to 128 rows each, if these are spread evenly, and so one row tile. us, of 256 and
+ * of 128 columns (N x K): product of 1040 x 1096, 24 experts, 24 rows 10.5 and 7.4, 384 rows 18.0 and
+ * 12.7, 3000 rows 31.4 and 23.6, but 6000 rows 33.2 and 40.9; input gradient of 2048 x 512, 64
+ * experts, 244 rows 18.1 and 14.7, 8000 rows 46.0 and 33.5; with more tiles, product of 1024 x
+ * 1024, 40 experts (160), 366 rows 14.4 and 17.9, of 1024 x 2048, 64 experts (256), 244 rows 23.7
+ * and 29.6. */
+bool narrow_tiles(uint32_t used, uint32_t rows, uint32_t P) {
+    return (uint64_t)used * ((P + 255u) / 256u) <= 128u && rows <= 128u * used;
+}
+
 template <int DIR>
 bool launch_rows(void *output, const void *input, const void *weights, const uint32_t *offsets,
                  const uint32_t *input_index, const uint32_t *output_index, uint32_t rows,
@@ -900,11 +910,15 @@ bool launch_rows(void *output, const void *input, const void *weights, const uin
         hipLaunchKernelGGL(grouped_few_kernel, dim3((uint32_t)few + 8u), dim3(512), 0, st, A);
         return hipGetLastError() == hipSuccess;
     }
-    A.tiles_p = (P + 255u) / 256u;
     const uint64_t tiles = rows / 256u + used;
+    const bool narrow = narrow_tiles(used, rows, P);
+    A.tiles_p = narrow ? (P + 127u) / 128u : (P + 255u) / 256u;
     const uint64_t blocks = tiles * A.tiles_p + 8u;
     if (blocks >= 1u << 23) return false; /* 2^32 threads */
-    hipLaunchKernelGGL(grouped_rows_kernel<DIR>, dim3((uint32_t)blocks), dim3(512), 0, st, A);
+    if (narrow)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_rows_kernel<DIR, 2>), dim3((uint32_t)blocks), dim3(256), 0, st, A);
+    else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_rows_kernel<DIR, 4>), dim3((uint32_t)blocks), dim3(512), 0, st, A);
     return hipGetLastError() == hipSuccess;
 }
 
