@@ -647,8 +647,15 @@ struct WeightRun {
                 .load<16>(q_at[q & 1] + q_col[q], st + C::A + C::PANEL * (q >> 1) + 1024u * (2u * wave + (q & 1)));
         }
     }
-    __device__ __forceinline__ void fetch(uint8_t *smem, uint32_t s, uint32_t slot) const {
-        static_for<C::D>([&](auto Q) { fetch_one<decltype(Q)::value>(smem, s, slot); });
+    /* Loads FROM .. TO of a stage to its slot, s < 3; and of the first two. */
+    template <int FROM, int TO>
+    __device__ __forceinline__ void fetch_stage(uint8_t *smem, uint32_t s) const {
+        static_for<TO - FROM>([&](auto Q) { fetch_one<FROM + decltype(Q)::value>(smem, s, s); });
+    }
+    template <int FROM, int TO>
+    __device__ __forceinline__ void fetch(uint8_t *smem) const {
+        fetch_stage<FROM, TO>(smem, 0u);
+        fetch_stage<FROM, TO>(smem, 1u);
     }
 
     /* acc[j] += the products over all stages, for the first 2 PAIRS subtiles of a wave, two a step, as
@@ -681,18 +688,30 @@ struct WeightRun {
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         };
-        uint32_t next_rows[4];
+        /* the first stages of an operand whose rows lie in order are under way while the other's
+         * indices are waited for */
+        uint32_t next_rows[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (uint32_t s = 0; s < 3u; s++) fetch_picks(s);
-        wait_vm<0>();
-#pragma unroll
-        for (uint32_t s = 0; s < 2u; s++) {
-            read_picks(s, next_rows);
+        set_rows(0u, next_rows);
+        if (!p.index) fetch<0, C::DA>(smem);
+        if (!q.index) fetch<C::DA, C::D>(smem);
+        if (p.index || q.index) {
+            if (!q.index) wait_vm<2 * C::DB>();
+            else if (!p.index) wait_vm<2 * C::DA>();
+            else wait_vm<0>();
+            uint32_t rows[2][4];
+            read_picks(0u, rows[0]);
+            read_picks(1u, rows[1]);
             wait_lgkm<0>();
-            set_rows(s, next_rows);
-            fetch(smem, s, s);
+            static_for<2>([&](auto S) {
+                constexpr uint32_t s = decltype(S)::value;
+                set_rows(s, rows[s]);
+                if (p.index) fetch_stage<0, C::DA>(smem, s);
+                if (q.index) fetch_stage<C::DA, C::D>(smem, s);
+            });
         }
-        wait_vm<C::D>(); /* stage 0 */
+        wait_vm<0>(); /* stages 0 and 1, which came close behind it */
         barrier();
         static_for<4>(read_p);
         read_q(std::integral_constant<int, 0>{});
