@@ -384,6 +384,14 @@ __device__ __forceinline__ uint32_t e4m3x2_raw(float a, float b, uint32_t old) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)old, Hi);
 }
 
+/* Two values rounded to bf16 (nearest even) by the part's packed conversion: f32_to_bf16's bits in
+ * one instruction instead of twelve, except that a NaN's payload is not specified. */
+__device__ __forceinline__ uint32_t bf16_pack2(float lo, float hi) {
+    typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+    typedef float f32x2_v __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_v{lo, hi}, bf16x2_v));
+}
+
 /* Two values rounded to bf16 (nearest even) by the part's packed
  * conversion, back as fp32; f32_to_bf16's values except that a NaN's
  * payload is not specified. */

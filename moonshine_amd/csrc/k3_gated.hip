@@ -71,12 +71,9 @@ __device__ __forceinline__ float gated_value(float g, float u, const GatedArgs &
     }
 }
 
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-    return f32_to_bf16(lo) | (uint32_t)f32_to_bf16(hi) << 16;
-}
 __device__ __forceinline__ void store8(uint16_t *to, const float (&v)[8]) {
-    *(uint4 *)to = make_uint4(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]),
-                              bf16_pair(v[6], v[7]));
+    *(uint4 *)to = make_uint4(bf16_pack2(v[0], v[1]), bf16_pack2(v[2], v[3]), bf16_pack2(v[4], v[5]),
+                              bf16_pack2(v[6], v[7]));
 }
 
 /* The wave's row, its route (routes: none) and weight; false past the last expert's rows. */

@@ -80,8 +80,7 @@ struct Range {
 };
 
 __device__ __forceinline__ uint2 bf16x4(const f32x4 &v) {
-    return make_uint2(f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
-                      f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16);
+    return make_uint2(bf16_pack2(v[0], v[1]), bf16_pack2(v[2], v[3]));
 }
 
 /* Rows of each but the last of an expert's tiles: all of up to 128 rows in one, more

@@ -30,11 +30,9 @@ struct NormArgs {
     float eps;
 };
 
-__device__ __forceinline__ uint32_t pair(float lo, float hi) {
-    return f32_to_bf16(lo) | (uint32_t)f32_to_bf16(hi) << 16;
-}
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-    return make_uint4(pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7]));
+    return make_uint4(bf16_pack2(v[0], v[1]), bf16_pack2(v[2], v[3]), bf16_pack2(v[4], v[5]),
+                      bf16_pack2(v[6], v[7]));
 }
 
 /* Sum over the THREADS threads of a row, the same order for each; red: its
