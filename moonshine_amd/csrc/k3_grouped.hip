@@ -775,14 +775,21 @@ struct WeightRun {
     }
 };
 
+/* XCD x (blocks x, x + 8, ...; it has an L2 of its own) takes runs of 16 tiles, which share operands, and
+ * the XCDs take the runs in turn, so that experts with many rows fall to all of them. us, in one
+ * contiguous range an XCD and so: 4096 tokens, 8 of 32 experts of 4096 x 7168 (bf16), rows spread evenly
+ * 1925 and 1945, by a skewed router 2279 and 1948; 1000 tokens, 4 of 64 of 1024 x 2048, 70 and
+ * 65, skewed 78 and 68 (runs of 64 tiles 71 and 84, of 4 66 and 66). */
+constexpr uint32_t kRun = 16;
+
 template <bool F32>
 __global__ __launch_bounds__(256, 2) void grouped_weight_kernel(GroupArgs A) {
     using C = Weight;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[C::STAGES * C::STAGE];
     __shared__ uint8_t held[2][C::WAVES][Picks::BYTES];
-    const uint32_t works = A.E * A.tiles_p * A.tiles_q, each = (works + 7u) / 8u;
-    uint32_t w = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= each || w >= works) return;
+    const uint32_t turn = blockIdx.x >> 3;
+    uint32_t w = (turn / kRun * 8u + (blockIdx.x & 7u)) * kRun + turn % kRun;
+    if (w >= A.E * A.tiles_p * A.tiles_q) return;
     const uint32_t expert = w / (A.tiles_p * A.tiles_q);
     w %= A.tiles_p * A.tiles_q;
     /* four q tiles at a time, along p */
@@ -990,7 +997,8 @@ extern "C" bool k3_moe_grouped_weight_gradient_bf16(void *output, bool f32, bool
     A.out = output, A.R = rows, A.E = expert_count, A.P = columns, A.Q = out_columns;
     A.accumulate = accumulate;
     A.tiles_p = (columns + Weight::BP - 1u) / Weight::BP, A.tiles_q = (out_columns + Weight::BQ - 1u) / Weight::BQ;
-    const uint64_t blocks = 8u * (((uint64_t)expert_count * A.tiles_p * A.tiles_q + 7u) / 8u);
+    const uint64_t all = 8u * kRun; /* whole turns of the XCDs */
+    const uint64_t blocks = ((uint64_t)expert_count * A.tiles_p * A.tiles_q + all - 1u) / all * all;
     if (blocks >= 1u << 23) return false;
     const auto kernel = f32 ? grouped_weight_kernel<true> : grouped_weight_kernel<false>;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(Weight::THREADS), 0, (hipStream_t)stream, A);
