@@ -141,6 +141,13 @@ __global__ __launch_bounds__(256) void zero_kernel(float *__restrict__ to, uint3
     if (i < n) to[i] = 0.0f;
 }
 
+/* Whether an output lies over what rows are found by, or over the route weights. */
+bool over_routes(const void *output, uint64_t bytes, const GatedArgs &A) {
+    return overlap(output, bytes, A.offsets, 4u * (uint64_t)(A.E + 1u)) ||
+           (A.route_index && overlap(output, bytes, A.route_index, 4u * (uint64_t)A.R)) ||
+           (A.route_weights && overlap(output, bytes, A.route_weights, 4u * (uint64_t)A.routes));
+}
+
 bool gated_args(GatedArgs &A, const void *gate_up, const uint32_t *offsets, const uint32_t *route_index,
                 const float *route_weights, uint32_t rows, uint32_t routes, uint32_t experts, uint32_t ffn,
                 uint32_t activation, float beta, float linear_beta) {
@@ -172,7 +179,7 @@ extern "C" bool k3_moe_gated_rows_bf16(void *output, const void *gate_up, const 
     if (!output || (uintptr_t)output % 16u != 0u ||
         !gated_args(A, gate_up, offsets, route_index, route_weights, rows, routes, expert_count, ffn, activation,
                     beta, linear_beta) ||
-        overlap(output, bytes, gate_up, 2u * bytes))
+        overlap(output, bytes, gate_up, 2u * bytes) || over_routes(output, bytes, A))
         return false;
     A.out = (uint16_t *)output;
     const auto kernel = activation == K3_MOE_ACT_SWIGLU ? gated_kernel<true> : gated_kernel<false>;
@@ -197,10 +204,11 @@ extern "C" bool k3_moe_gated_rows_backward_bf16(void *gate_up_gradient, float *w
         /* each value's place is read by the lane that writes there: the gradient may take gate_up's */
         (gate_up_gradient != gate_up && overlap(gate_up_gradient, 2u * bytes, gate_up, 2u * bytes)) ||
         overlap(gate_up_gradient, 2u * bytes, output_gradient, bytes) ||
+        over_routes(gate_up_gradient, 2u * bytes, A) ||
         (weight_gradient && (overlap(weight_gradient, grads, gate_up_gradient, 2u * bytes) ||
                              overlap(weight_gradient, grads, gate_up, 2u * bytes) ||
                              overlap(weight_gradient, grads, output_gradient, bytes) ||
-                             (route_weights && overlap(weight_gradient, grads, route_weights, grads)))))
+                             over_routes(weight_gradient, grads, A))))
         return false;
     A.out = (uint16_t *)gate_up_gradient, A.weight_gradient = weight_gradient;
     A.dh = (const uint16_t *)output_gradient;

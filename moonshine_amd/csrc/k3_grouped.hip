@@ -890,6 +890,14 @@ bool picks_ok(const uint32_t *index, uint32_t have, uint32_t rows) {
     return (uintptr_t)index % 4u == 0u && (index ? have != 0u && have <= kMostPicked : have >= rows);
 }
 
+/* Whether an output lies over the offsets or an index, which tiles read while others write. */
+bool over_plan(const void *output, uint64_t bytes, const uint32_t *offsets, uint32_t experts,
+               const uint32_t *index, const uint32_t *other, uint32_t rows) {
+    return overlap(output, bytes, offsets, 4u * (uint64_t)(experts + 1u)) ||
+           (index && overlap(output, bytes, index, 4u * (uint64_t)rows)) ||
+           (other && overlap(output, bytes, other, 4u * (uint64_t)rows));
+}
+
 /* Most blocks of a product that goes 16 rows x 16 columns a block. us, so and by tiles of 256
  * columns, rows of experts chosen at random: 1024 x 2048, 4 of 64 experts, 4 rows (256 blocks) 5.1 and
  * 15.6, 8 rows 8.0 and 16.4, 16 rows (1024) 15.3 and 16.9, 32 rows 22.0 and 18.3; 2048 x 512, 8
@@ -921,7 +929,8 @@ bool launch_rows(void *output, const void *input, const void *weights, const uin
     const uint64_t out = 2u * (uint64_t)output_rows * P;
     /* tiles read all of a row while others write */
     if (overlap(output, out, input, 2u * (uint64_t)input_rows * Z) ||
-        overlap(output, out, weights, 2u * (uint64_t)experts * N * K))
+        overlap(output, out, weights, 2u * (uint64_t)experts * N * K) ||
+        over_plan(output, out, offsets, experts, input_index, output_index, rows))
         return false;
     GroupArgs A{};
     A.p = (const uint16_t *)weights, A.q = (const uint16_t *)input, A.offsets = offsets;
@@ -989,7 +998,8 @@ extern "C" bool k3_moe_grouped_weight_gradient_bf16(void *output, bool f32, bool
         return false;
     const uint64_t values = (uint64_t)expert_count * out_columns * columns, out = (f32 ? 4u : 2u) * values;
     if (overlap(output, out, output_gradient, 2u * (uint64_t)gradient_rows * out_columns) ||
-        overlap(output, out, input, 2u * (uint64_t)input_rows * columns))
+        overlap(output, out, input, 2u * (uint64_t)input_rows * columns) ||
+        over_plan(output, out, offsets, expert_count, gradient_index, input_index, rows))
         return false;
     GroupArgs A{};
     A.p = (const uint16_t *)input, A.q = (const uint16_t *)output_gradient, A.offsets = offsets;

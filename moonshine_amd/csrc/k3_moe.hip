@@ -502,7 +502,9 @@ extern "C" bool k3_moe_combine_bf16(void *output, const void *rows, const void *
         hidden % 8u != 0u || hidden > 65536u ||
         /* blocks write their own columns of a token while others read its rows */
         overlap(output, bytes, rows, bytes * top_k) ||
-        (residual && residual != output && overlap(output, bytes, residual, bytes)))
+        (residual && residual != output && overlap(output, bytes, residual, bytes)) ||
+        overlap(output, bytes, expert_ids, 4u * (uint64_t)token_count * top_k) ||
+        (expert_weights && overlap(output, bytes, expert_weights, 4u * (uint64_t)token_count * top_k)))
         return false;
     return launch_combine(output, (const uint16_t *)rows, residual, (const uint32_t *)expert_ids,
                           (const float *)expert_weights, token_count, hidden, top_k, expert_count, true,

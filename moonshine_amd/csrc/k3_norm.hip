@@ -299,12 +299,18 @@ extern "C" bool k3_moe_residual_norm_backward_bf16(void *input_gradient, float *
         (((uintptr_t)weight_gradient | (uintptr_t)rstd) % 4u) != 0u || (uintptr_t)scratch % 256u != 0u)
         return false;
     const uint64_t n = 2u * (uint64_t)rows * columns;
-    for (const void *in : {normed_gradient, total, total_gradient})
-        if (in && in != input_gradient && overlap(input_gradient, n, in, n)) return false;
-    if (overlap(input_gradient, n, weight, 2u * (uint64_t)columns) ||
-        overlap(input_gradient, n, rstd, 4u * (uint64_t)rows) ||
-        overlap(input_gradient, n, weight_gradient, 4u * (uint64_t)columns))
-        return false;
+    const uint64_t parts = k3_moe_residual_norm_scratch_bytes(rows, columns);
+    const struct { const void *p; uint64_t bytes; } outs[] = {
+        {input_gradient, n}, {weight_gradient, 4u * (uint64_t)columns}, {scratch, parts}};
+    for (int i = 0; i < 3; i++) {
+        for (int j = i + 1; j < 3; j++)
+            if (overlap(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) return false;
+        for (const void *in : {normed_gradient, total, total_gradient})
+            if (in && !(i == 0 && in == input_gradient) && overlap(outs[i].p, outs[i].bytes, in, n)) return false;
+        if (overlap(outs[i].p, outs[i].bytes, weight, 2u * (uint64_t)columns) ||
+            overlap(outs[i].p, outs[i].bytes, rstd, 4u * (uint64_t)rows))
+            return false;
+    }
     const NormBackArgs A{(uint16_t *)input_gradient, (float *)scratch, (const uint16_t *)normed_gradient,
                          (const uint16_t *)total, (const uint16_t *)weight, (const uint16_t *)total_gradient,
                          rstd, rows, columns};

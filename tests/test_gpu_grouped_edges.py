@@ -216,3 +216,64 @@ def test_refused_over_its_operands(cuda):
     assert torch.equal(room, before)
     got = grouped.product(rows, w, o, out=room[8:16])  # between them
     equal(got, R.by_rows(rows.cpu(), w.cpu(), o.cpu(), None, False)[0])
+
+
+def test_both_operands_picked(cuda):
+    """A weight gradient whose rows both come by indices, some more than once; more tiles than a turn of the
+    XCDs, of part tiles and of experts with no row, one, and more than a stage."""
+    counts = [1, 0, 31, 33, 200, 64, 97]
+    E, N, K, have = len(counts), 520, 1416, 50
+    offsets = torch.tensor([0] + counts, dtype=torch.int32).cumsum(0).to(torch.int32)
+    g = torch.Generator().manual_seed(1)
+    i, j = (torch.randint(0, have, (sum(counts),), generator=g).to(torch.int32) for _ in range(2))
+    j[3], i[100] = -1, have
+    dy, x = R.whole((have, N), 2), R.whole((have, K), 3)
+    want = R.by_weights(dy, x, offsets, i, j)[0]
+    o, i, j = offsets.to(cuda), i.to(cuda), j.to(cuda)
+    for dtype in (torch.float32, torch.bfloat16):
+        equal(grouped.weight_gradient(dy.to(cuda), x.to(cuda), o, dy_index=i, x_index=j, dtype=dtype), want)
+    out = torch.ones((E, N, K), device=cuda)
+    equal(grouped.weight_gradient(dy.to(cuda), x.to(cuda), o, dy_index=i, x_index=j, out=out, accumulate=True), want + 1)
+
+
+@pytest.mark.parametrize("K", [2040, 2048, 2056, 4104, 8200])
+@pytest.mark.parametrize("n", [1, 16, 17])
+def test_few_rows_of_long_reductions(cuda, n, K):
+    E, N = 3, 40
+    offsets = torch.tensor([0, n, n, n + 1], dtype=torch.int32)
+    w, x = R.whole((E, N, K), 1), R.whole((n + 1, K), 2)
+    equal(grouped.product(x.to(cuda), w.to(cuda), offsets.to(cuda)), R.by_rows(x, w, offsets, None, False)[0])
+
+
+@pytest.mark.parametrize("E,rows", [(15, 15), (16, 16), (16, 32), (32, 4096), (32, 4097), (33, 4096)])
+def test_where_one_kind_of_tile_takes_over_from_another(cuda, E, rows):
+    """1024 columns: up to 1024 blocks of 16 x 16, up to 128 tiles of 256 columns and rows for one row tile
+    an expert, and more; all rows of one expert, and spread."""
+    wide, inner = 1024, 72
+    spread = [rows * e // E for e in range(E + 1)]
+    for values in (spread, [0] * (E - 1) + [0, rows]):
+        offsets = torch.tensor(values, dtype=torch.int32)
+        x = R.whole((rows, inner), 1)
+        w = R.whole((E, wide, inner), 2)
+        equal(grouped.product(x.to(cuda), w.to(cuda), offsets.to(cuda)), R.by_rows(x, w, offsets, None, False)[0])
+        w = w.transpose(1, 2).contiguous()
+        equal(grouped.input_gradient(x.to(cuda), w.to(cuda), offsets.to(cuda)), R.by_rows(x, w, offsets, None, True)[0])
+
+
+@pytest.mark.parametrize("n", [4, 40])
+def test_the_largest_tensor_that_an_index_picks_from(cuda, n):
+    """65535 rows of 32768 values, just under 4 GiB: its last row, and the first that it has not."""
+    rows, wide, inner = 65535, 32768, 8
+    big = torch.zeros((rows, wide), dtype=torch.bfloat16, device=cuda)
+    ends = R.whole((2, wide), 1)
+    big[0], big[-1] = ends[0].to(cuda), ends[1].to(cuda)
+    index = torch.tensor(([65534, 65535, 0, -1] * n)[:n], dtype=torch.int32)
+    at = torch.tensor(([1, 2, 0, -1] * n)[:n], dtype=torch.int32)  # the same of `ends`
+    offsets = torch.tensor([0, n], dtype=torch.int32)
+    o, i = offsets.to(cuda), index.to(cuda)
+    w, d = R.whole((1, inner, wide), 2), R.whole((n, inner), 3)
+    equal(grouped.product(big, w.to(cuda), o, index=i), R.by_rows(ends, w, offsets, at, False)[0])
+    equal(grouped.weight_gradient(d.to(cuda), big, o, x_index=i), R.by_weights(d, ends, offsets, None, at)[0])
+    equal(grouped.weight_gradient(big, d.to(cuda), o, dy_index=i), R.by_weights(ends, d, offsets, at, None)[0])
+    w = w.transpose(1, 2).contiguous()
+    equal(grouped.input_gradient(big, w.to(cuda), o, index=i), R.by_rows(ends, w, offsets, at, True)[0])

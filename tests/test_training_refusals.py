@@ -1,6 +1,9 @@
 """What the training operators and the residual norm refuse (CPU): by the C entry points, on addresses
 that nothing reads, and by the wrappers, on CPU tensors that stand in for the GPU's."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -38,6 +41,7 @@ def by_rows(name, **change):
     dict(experts=0), dict(experts=1025),
     dict(n=0), dict(n=12), dict(n=32776), dict(k=0), dict(k=20), dict(k=32776),
     dict(output=address(2, 16)), dict(output=address(3, 16)), dict(input=address(1, 128)),
+    dict(output=address(4)), dict(output=address(5, 16)), dict(output=address(6)), dict(to=address(1, 252)),
 ])
 def test_products_refuse(name, change):
     assert not by_rows(name, **change)
@@ -53,6 +57,7 @@ WEIGHT = dict(output=address(1), f32=True, accumulate=False, dy=address(2), x=ad
     dict(x_index=address(6, 3)), dict(f32=False, accumulate=True), dict(rows=0), dict(dy_rows=0), dict(x_rows=65536),
     dict(dy_index=None, dy_rows=7), dict(x_index=None, x_rows=7), dict(experts=0), dict(experts=1025), dict(n=4),
     dict(k=4), dict(n=40000), dict(k=40000), dict(output=address(2, 16)), dict(output=address(3, 32)),
+    dict(output=address(4)), dict(output=address(5)), dict(output=address(6, 16)), dict(offsets=address(1, 400)),
 ])
 def test_weight_gradient_refuses(change):
     assert not lib().k3_moe_grouped_weight_gradient_bf16(*dict(WEIGHT, **change).values(), None)
@@ -64,7 +69,8 @@ GATED_CHANGES = [
     dict(gate_up=None), dict(offsets=None), dict(gate_up=address(2, 8)), dict(offsets=address(3, 1)),
     dict(route=address(4, 2)), dict(weights=address(5, 1)), dict(rows=0), dict(rows=65535 * 32 + 1), dict(routes=0),
     dict(experts=0), dict(experts=1025), dict(ffn=0), dict(ffn=12), dict(ffn=32776), dict(act=2), dict(beta=0.0),
-    dict(beta=float("nan")), dict(linear=-1.0)]
+    dict(beta=float("nan")), dict(linear=-1.0), dict(output=address(3)), dict(output=address(4, 16)),
+    dict(output=address(5, 16))]
 
 
 @pytest.mark.parametrize("change", GATED_CHANGES + [dict(output=None), dict(output=address(1, 4)),
@@ -76,7 +82,8 @@ def test_gated_refuses(change):
 @pytest.mark.parametrize("change", GATED_CHANGES + [
     dict(output=None), dict(output=address(1, 4)), dict(output=address(2, 16)), dict(output=address(7)),
     dict(dweights=address(8, 2)), dict(dweights=address(1, 64)), dict(dweights=address(2, 4)),
-    dict(dweights=address(7, 8)), dict(dweights=address(5)), dict(dh=None), dict(dh=address(7, 8))])
+    dict(dweights=address(7, 8)), dict(dweights=address(5)), dict(dweights=address(3, 8)),
+    dict(dweights=address(4, 28)), dict(dh=None), dict(dh=address(7, 8))])
 def test_gated_backward_refuses(change):
     a = dict(output=GATED["output"], dweights=address(8), dh=address(7))
     a.update({k: v for k, v in GATED.items() if k != "output"})
@@ -87,7 +94,7 @@ def test_gated_backward_refuses(change):
     dict(output=None), dict(rows=None), dict(ids=None), dict(output=address(1, 8)), dict(rows=address(2, 2)),
     dict(residual=address(3, 4)), dict(ids=address(4, 1)), dict(weights=address(5, 2)), dict(T=0), dict(T=65536),
     dict(k=0), dict(k=33), dict(E=0), dict(H=0), dict(H=12), dict(H=65544), dict(output=address(2, 16)),
-    dict(output=address(3, 16))])
+    dict(output=address(3, 16)), dict(output=address(4)), dict(output=address(5, 16))])
 def test_combine_refuses(change):
     a = dict(output=address(1), rows=address(2), residual=address(3), ids=address(4), weights=address(5), T=4, k=2,
              E=3, H=16)
@@ -118,7 +125,10 @@ def test_norm_refuses_a_call_for_nothing():
     dict(scratch=None), dict(scratch=address(8, 16)), dict(bytes=100), dict(rows=0), dict(cols=12), dict(cols=40000),
     dict(dx=address(1, 8)), dict(dt=address(7, 2)), dict(dweight=address(2, 2)), dict(rstd=address(6, 1)),
     dict(dx=address(3, 16)), dict(dx=address(4, 16)), dict(dx=address(7, 16)), dict(dx=address(5)),
-    dict(dweight=address(1, 16))])
+    dict(dweight=address(1, 16)), dict(dweight=address(8)), dict(dweight=address(3, 4)), dict(dweight=address(4)),
+    dict(dweight=address(5, 128)), dict(dweight=address(6, 12)), dict(dweight=address(7)), dict(scratch=address(1)),
+    dict(scratch=address(3)), dict(scratch=address(4, 256)), dict(scratch=address(5)), dict(scratch=address(6)),
+    dict(scratch=address(7, 512)), dict(dx=address(8, 256))])
 def test_norm_backward_refuses(change):
     a = dict(dx=address(1), dweight=address(2), dn=address(3), total=address(4), weight=address(5), rstd=address(6),
              dt=address(7), rows=4, cols=128, scratch=address(8), bytes=1 << 20)
@@ -138,9 +148,28 @@ def test_norm_scratch_grows_with_the_rows():
     dict(xs=address(5, 2)), dict(T=0), dict(T=65536), dict(cols=64), dict(output=address(4, 16)),
     dict(output=address(5)), dict(bytes=0), dict(scratch=None)])
 def test_encoded_product_refuses(change):
-    a = dict(output=address(1), codes=address(2), scales=address(3), x=address(4), xs=address(5), T=100, rows=256,
+    a = dict(output=address(1), codes=address(2), scales=address(3), x=address(4), xs=address(5), T=1000, rows=4096,
              cols=1024, scratch=address(6), bytes=1 << 30)
     assert not lib().k3_moe_fp8_128_encoded_gemm_bf16(*dict(a, **change).values(), None)
+
+
+def test_refused_calls_launch_nothing():
+    """Without a GPU a call that goes through fails as well, at its launch: the runtime's log tells the two
+    apart. In a process that sees no GPU."""
+    env = dict(os.environ, HIP_VISIBLE_DEVICES="-1", AMD_LOG_LEVEL="3")
+    launch = "__hipPushCallConfiguration"
+
+    def log(*command):
+        run = subprocess.run([sys.executable, *command], env=env, cwd=os.path.dirname(os.path.abspath(__file__)),
+                             capture_output=True, text=True, timeout=300)
+        return run.returncode, run.stdout + run.stderr
+
+    code, text = log("-c", "import conftest, test_training_refusals as t\n"
+                           "assert not t.by_rows('k3_moe_grouped_product_bf16')")
+    assert code == 0 and launch in text
+    code, text = log("-m", "pytest", "-q", "-s", "-p", "no:cacheprovider", "-k", "refuse and not wrappers and not launch",
+                     os.path.basename(__file__))
+    assert code == 0 and launch not in text, text[-2000:]
 
 
 # ---- wrappers -----------------------------------------------------------------------------------
