@@ -6,7 +6,13 @@
  * A row is held by THREADS threads in CHUNKS pieces of eight values each, from
  * its one read to its writes: piece t + THREADS j is thread t's, so 16 lanes hold
  * the 128 values of an FP8-128 block. Rows of up to 2048 values go four to a block, a wave
- * each, without a barrier. Bound by memory.
+ * each, without a barrier; longer ones take as many threads as leave two pieces to each, four past
+ * 16384 values. Bound by memory: 8 bytes a value either way (residual in, sum out; both
+ * gradients in), 7 with codes in place of the normed rows. us, rows x columns, forward and backward
+ * (a large copy moves 5.2 TB/s): 32768 x 1024 44 and 51, 16384 x 2176 46 and 55, 8192 x 7168 83 (5.6
+ * TB/s) and 97, of which the join of the weight's gradient 5; 4096 x 16384 95 and 107; 2048 x 32768
+ * 106 and 142. With four pieces a thread 16384 x 2176 took 56 and 72, 8192 x 7168 88 and 98,
+ * 4096 x 16384 105 and 204: fewer waves were under way, and of 1024 threads registers spilled.
  */
 #include "k3_device.h"
 #include "k3_fp8.h"
@@ -113,7 +119,9 @@ __global__ __launch_bounds__(THREADS < 256u ? 256u : THREADS) void norm_kernel(N
  * s rstd^2 mean(d weight s)) and dweight = sum over rows d s rstd. A block takes every
  * gridDim.x-th row (of its rows of a wave each, ROWS of them at once) and keeps the sums
  * of its columns in registers; they go to `parts`, a row for each block, and
- * norm_join_kernel adds those in their order.
+ * norm_join_kernel adds those in their order. The sum's own gradient is loaded only behind the
+ * sums' terms, under the wait for the row's sum: loaded with the others it took registers that cost
+ * a wave (8192 x 7168 99.6 and 97.8 us).
  */
 struct NormBackArgs {
     uint16_t *dx;
@@ -123,39 +131,57 @@ struct NormBackArgs {
     uint32_t rows, cols;
 };
 
+/* A row by offsets of 32 bits: pieces past its end, and all of no tensor, read as zeros and are not
+ * written, without a branch; 64-bit addresses and the branches of a row's pieces took 60 registers. */
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_range(const void *base, uint64_t at, uint32_t cols) {
+    return __builtin_amdgcn_make_buffer_rsrc((uint16_t *)base + at, 0, base ? (int)(2u * cols) : 0, 0x00027000);
+}
+__device__ __forceinline__ uint4 piece(__amdgpu_buffer_rsrc_t row, uint32_t p) {
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(row, (int)(16u * p), 0, 0));
+}
+__device__ __forceinline__ void put_piece(__amdgpu_buffer_rsrc_t row, uint32_t p, const uint4 &v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), row, (int)(16u * p), 0, 0);
+}
+/* Unpacks of v from here on stay behind `behind`. */
+__device__ __forceinline__ void keep_packed(uint4 &v, float &behind) {
+    asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w), "+v"(behind));
+}
+
 template <uint32_t THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS < 256u ? 256u : THREADS) void norm_back_kernel(NormBackArgs A) {
     constexpr uint32_t ROWS = THREADS < 256u ? 256u / THREADS : 1u;
     __shared__ float red[2][THREADS / 64u];
     __shared__ float cols[ROWS > 1u ? ROWS : 1u][ROWS > 1u ? 8u * THREADS : 1u];
     const uint32_t t = threadIdx.x % THREADS, mine = threadIdx.x / THREADS, pieces = A.cols / 8u;
+    const __amdgpu_buffer_rsrc_t weight = row_range(A.weight, 0u, A.cols);
     float sums[CHUNKS][8];
     uint4 wv[CHUNKS];
 #pragma unroll
     for (int j = 0; j < CHUNKS; j++) {
         const uint32_t p = t + THREADS * (uint32_t)j;
-        wv[j] = p < pieces ? ((const uint4 *)A.weight)[p] : make_uint4(0u, 0u, 0u, 0u);
+        wv[j] = piece(weight, p);
 #pragma unroll
         for (int i = 0; i < 8; i++) sums[j][i] = 0.0f;
     }
     uint32_t turn = 0u;
-    for (uint32_t row = blockIdx.x * ROWS + mine; row < A.rows; row += gridDim.x * ROWS) {
+    for (uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * ROWS + mine); row < A.rows; row += gridDim.x * ROWS) {
         const uint64_t at = (uint64_t)row * A.cols;
+        const __amdgpu_buffer_rsrc_t d_row = row_range(A.d, at, A.cols), s_row = row_range(A.total, at, A.cols),
+                                     t_row = row_range(A.dtotal, at, A.cols), dx_row = row_range(A.dx, at, A.cols);
         uint4 dv[CHUNKS], sv[CHUNKS], tv[CHUNKS];
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
             const uint32_t p = t + THREADS * (uint32_t)j;
-            dv[j] = sv[j] = tv[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (p >= pieces) continue;
-            dv[j] = ((const uint4 *)(A.d + at))[p];
-            sv[j] = ((const uint4 *)(A.total + at))[p];
-            if (A.dtotal) tv[j] = ((const uint4 *)(A.dtotal + at))[p];
+            dv[j] = piece(d_row, p);
+            sv[j] = piece(s_row, p);
         }
         const float rstd = A.rstd[row];
         float dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
             float d[8], s[8], w[8];
+            keep_packed(dv[j], dot), keep_packed(sv[j], dot), keep_packed(wv[j], dot);
             unpack8(dv[j], d);
             unpack8(sv[j], s);
             unpack8(wv[j], w);
@@ -166,8 +192,18 @@ __global__ __launch_bounds__(THREADS < 256u ? 256u : THREADS) void norm_back_ker
                 sums[j][i] = fmaf(ds, rstd, sums[j][i]);
             }
         }
+#pragma unroll
+        for (int j = 0; j < CHUNKS; j++) {
+            if (j == 0) asm volatile("" : "+v"(dot) : : "memory"); /* not ahead of the loop above */
+            tv[j] = piece(t_row, t + THREADS * (uint32_t)j);
+        }
         dot = row_sum<THREADS>(dot, red[turn & 1u]); /* two places: one barrier a row */
         turn++;
+        /* unpacked anew below: kept over the sum, the floats would take twice the registers */
+#pragma unroll
+        for (int j = 0; j < CHUNKS; j++) {
+            keep_packed(dv[j], dot), keep_packed(sv[j], dot), keep_packed(wv[j], dot);
+        }
         const float back = __fmul_rn(__fmul_rn(rstd, rstd), __fdiv_rn(dot, (float)A.cols));
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
@@ -180,7 +216,7 @@ __global__ __launch_bounds__(THREADS < 256u ? 256u : THREADS) void norm_back_ker
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 d[i] = fmaf(rstd, fmaf(-s[i], back, __fmul_rn(d[i], w[i])), b[i]);
-            if (p < pieces) ((uint4 *)(A.dx + at))[p] = pack8(d);
+            put_piece(dx_row, p, pack8(d));
         }
     }
     float *part = A.parts + (uint64_t)blockIdx.x * A.cols;
@@ -234,10 +270,12 @@ bool norm_sizes_ok(uint32_t rows, uint32_t cols) {
     return rows != 0u && rows <= kMostRows && cols != 0u && cols % 8u == 0u && cols <= kMostColumns;
 }
 
-/* Blocks of the gradient: each keeps a row of sums, so no more than fill the chip. */
+/* Blocks of the gradient: each keeps a row of sums, so no more than the chip holds at once: three
+ * a CU of up to 512 threads, one of 1024. */
 uint32_t back_blocks(uint32_t rows, uint32_t cols) {
     const uint32_t groups = cols <= 2048u ? (rows + 3u) / 4u : rows;
-    return groups < 768u ? groups : 768u;
+    const uint32_t most = cols <= 8192u ? 768u : 256u;
+    return groups < most ? groups : most;
 }
 
 }  // namespace
@@ -276,7 +314,9 @@ extern "C" bool k3_moe_residual_norm_bf16(void *total, void *normed, uint8_t *co
     const dim3 four((rows + 3u) / 4u), one(rows);
     if (columns <= 512u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_kernel<64u, 1>), four, dim3(256), 0, st, A);
     else if (columns <= 2048u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_kernel<64u, 4>), four, dim3(256), 0, st, A);
-    else if (columns <= 8192u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_kernel<256u, 4>), one, dim3(256), 0, st, A);
+    else if (columns <= 4096u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_kernel<256u, 2>), one, dim3(256), 0, st, A);
+    else if (columns <= 8192u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_kernel<512u, 2>), one, dim3(512), 0, st, A);
+    else if (columns <= 16384u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_kernel<1024u, 2>), one, dim3(1024), 0, st, A);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_kernel<1024u, 4>), one, dim3(1024), 0, st, A);
     return hipGetLastError() == hipSuccess;
 }
@@ -319,7 +359,9 @@ extern "C" bool k3_moe_residual_norm_backward_bf16(void *input_gradient, float *
     const dim3 grid(blocks);
     if (columns <= 512u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_back_kernel<64u, 1>), grid, dim3(256), 0, st, A);
     else if (columns <= 2048u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_back_kernel<64u, 4>), grid, dim3(256), 0, st, A);
-    else if (columns <= 8192u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_back_kernel<256u, 4>), grid, dim3(256), 0, st, A);
+    else if (columns <= 4096u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_back_kernel<256u, 2>), grid, dim3(256), 0, st, A);
+    else if (columns <= 8192u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_back_kernel<512u, 2>), grid, dim3(512), 0, st, A);
+    else if (columns <= 16384u) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_back_kernel<1024u, 2>), grid, dim3(1024), 0, st, A);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_back_kernel<1024u, 4>), grid, dim3(1024), 0, st, A);
     hipLaunchKernelGGL(norm_join_kernel, dim3((columns + 31u) / 32u), dim3(1024), 0, st, weight_gradient,
                        (const float *)scratch, blocks, columns);

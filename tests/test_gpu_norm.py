@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 
 U, EPS = 2.0 ** -24, 1e-5
 SIZES = [(1, 8), (3, 24), (5, 128), (4, 512), (9, 520), (130, 640), (7, 2048), (6, 2056), (61, 7168), (3, 8192), (2, 8200),
-         (2, 16384), (1, 32768), (1000, 256), (801, 2176)]
+         (2, 16384), (1, 32768), (1000, 256), (801, 2176), (5, 4096), (770, 4104), (300, 8200), (3, 16392), (260, 16640)]
 
 
 def data(rows, cols):
