@@ -830,8 +830,14 @@ __global__ __launch_bounds__(256, 2) void grouped_weight_kernel(GroupArgs A) {
     }
     const uint32_t g = L >> 4, c = L & 15u;
     const uint64_t to = ((uint64_t)expert * A.Q + q0) * A.P + p0;
-    /* through LDS for stores of whole rows (64-byte pieces straight from the accumulators took 10 us for
-     * 256 x 256): f32 128 rows at a time, bf16 all; piece p of row r lies at p ^ r modulo 16 */
+    /* Through LDS for stores of whole rows (64-byte pieces straight from the accumulators took 10 us for
+     * 256 x 256): f32 128 rows at a time, bf16 all; piece p of row r lies at p ^ r modulo 16. The output
+     * passes the caches by, which the operands are read from again. us, so and as usual stores: f32, 4096
+     * tokens, 8 of 32 experts of 4096 x 7168, 2058 and 2204, 1000 tokens 814 and 1038, 4 of 16 of 4096
+     * x 7176, 1000 tokens, 528 and 645; bf16 100, 1000 and 4096 tokens of the first 299 and 349, 590 and
+     * 755, 1830 and 1885; but bf16 rows that end inside a 128-byte line are cut lines twice: 4 of 16
+     * of 4096 x 7176, 100 tokens, 396 and 266 (1000 tokens 345 and 468), 3 of 24 of 1040 x 1096, 1000
+     * tokens, 28.0 and 25.7. */
     constexpr uint32_t ROW = F32 ? 512u : 256u, HIGH = F32 ? 128u : 256u, PIECES = ROW / 16u;
     static_assert(ROW * HIGH <= sizeof smem, "the part of the tile");
     if (F32 && A.accumulate && R.stages == 0u) return;
@@ -854,24 +860,30 @@ __global__ __launch_bounds__(256, 2) void grouped_weight_kernel(GroupArgs A) {
         __syncthreads();
         const uint32_t piece = threadIdx.x % PIECES;
         if ((F32 ? 4u : 8u) * piece >= width) return;
+        const auto store = [&](auto nontemporal) {
 #pragma unroll 4
-        for (uint32_t r = threadIdx.x / PIECES; r < HIGH; r += C::THREADS / PIECES) {
-            const uint32_t q = HIGH * part + r;
-            if (q >= high) break;
-            const uint4 v = *(const uint4 *)(smem + ROW * r + 16u * (piece ^ (r & 15u)));
-            if constexpr (F32) {
-                f32x4 *place = (f32x4 *)((float *)A.out + to + (uint64_t)q * A.P + 4u * piece);
-                f32x4 sum = __builtin_bit_cast(f32x4, v);
-                if (A.accumulate) {
-                    const f32x4 before = *place;
+            for (uint32_t r = threadIdx.x / PIECES; r < HIGH; r += C::THREADS / PIECES) {
+                const uint32_t q = HIGH * part + r;
+                if (q >= high) break;
+                const u32x4_t v = *(const u32x4_t *)(smem + ROW * r + 16u * (piece ^ (r & 15u)));
+                if constexpr (F32) {
+                    f32x4 *place = (f32x4 *)((float *)A.out + to + (uint64_t)q * A.P + 4u * piece);
+                    f32x4 sum = __builtin_bit_cast(f32x4, v);
+                    if (A.accumulate) {
+                        const f32x4 before = *place;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) sum[k] = __fadd_rn(before[k], sum[k]);
+                        for (int k = 0; k < 4; k++) sum[k] = __fadd_rn(before[k], sum[k]);
+                    }
+                    __builtin_nontemporal_store(sum, place);
+                } else {
+                    u32x4_t *place = (u32x4_t *)((uint16_t *)A.out + to + (uint64_t)q * A.P + 8u * piece);
+                    if constexpr (decltype(nontemporal)::value) __builtin_nontemporal_store(v, place);
+                    else *place = v;
                 }
-                __builtin_nontemporal_store(sum, place);
-            } else {
-                *(uint4 *)((uint16_t *)A.out + to + (uint64_t)q * A.P + 8u * piece) = v;
             }
-        }
+        };
+        if (F32 || A.P % 64u == 0u) store(std::true_type{});
+        else store(std::false_type{});
     });
 }
 
