@@ -5,8 +5,8 @@
  *
  * A wave a row: each lane takes eight columns at a time of gate and of up, so
  * every load and store is 16 bytes, and the gradient by the route's weight is one sum over
- * the wave. Bound by memory: 6 bytes a value forward, 10 backward. 32768 rows of F = 2048: 78 and 117
- * us, 5.2 and 5.7 TB/s, where a large copy moves 5.2; 222 rows of F = 1024 4 and 6 us, a wave's
+ * the wave. Bound by memory: 6 bytes a value forward, 10 backward. 32768 rows of F = 2048: 67 and 114
+ * us, 6.0 and 5.9 TB/s, where a large copy moves 5.2; 222 rows of F = 1024 4 and 6 us, a wave's
  * latency.
  */
 #include "k3_device.h"
