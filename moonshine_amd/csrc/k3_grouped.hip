@@ -591,9 +591,10 @@ __global__ __launch_bounds__(512) void grouped_few_kernel(GroupArgs A) {
  * A stage is 32 rows; q is kept as two panels of 128 columns. 4000 rows of 64 experts of 2048 x 512
  * to bf16 32 us, 27 of which the 147 MB take as a large copy; 32768 rows of 32 experts of 4096 x 7168 to
  * f32 2060 to 2200 us by the card, 0.87 to 0.93 PFLOP/s (a large library product of such
- * operands 1.18), to bf16 1830. Bound by LDS: transposing reads of 96 KB at 199 bytes a clock and the
- * loads' 48 KB fill nine tenths of the 1024 clocks that two blocks' stage has of matrix instructions. Wave
- * tiles of 128 x 128 would read a third less, with one wave a SIMD to hide each wait.
+ * operands 1.18), to bf16 1850. Bound by power, operands and the stages' own waits: of the last, on
+ * zeros 1540 (the clock falls less), with the operands in L2 1610, with both 1265. Waves of 128 x 128, four of
+ * them and 256 x 256 a block, read a third less of LDS, but one block a CU leaves its waits and
+ * stores bare: 2030, on zeros 1970; 1000 tokens 790 and 645, 64 experts of 1024 x 2048 83 and 60.
  */
 struct Weight {
     static constexpr uint32_t BP = 128, BQ = 256, DEPTH = 32, STAGES = 3, WAVES = 4, THREADS = 256;
