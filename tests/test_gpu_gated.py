@@ -148,3 +148,25 @@ def test_infinities_and_nan_stay_in_their_row(cuda):
     want = (gu.double()[:, :F] * torch.sigmoid(gu.double()[:, :F]) * gu.double()[:, F:])
     assert torch.equal(h.isnan(), want.isnan()) and torch.equal(h.isinf(), want.isinf())
     assert h[0].isfinite().all() and h[3].isfinite().all()
+
+
+def test_past_32_bits(cuda):
+    """Rows past 4 GiB have the bits that they have alone: gated rows, their gradient, and their sum."""
+    rows, F, last = 65600, 32768, 2
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device=cuda)
+    alone = torch.tensor([0, last], dtype=torch.int32, device=cuda)
+    gu = torch.zeros((rows, 2 * F), dtype=torch.bfloat16, device=cuda)
+    gu[-last:] = R.normal((last, 2 * F), 1).to(cuda)
+    route = torch.arange(rows, dtype=torch.int32, device=cuda)
+    w = torch.rand((rows, 1), generator=torch.Generator().manual_seed(2)).to(cuda)
+    want = experts.gated(gu[-last:].clone(), alone, route[:last], w[-last:].clone(), ACT_SITU)
+    h = experts.gated(gu, offsets, route, w, ACT_SITU)
+    assert torch.equal(h[-last:], want) and not h[:-last].any()
+    dgu, dw = experts.gated_backward(want, gu[-last:].clone(), alone, route[:last], w[-last:].clone(), ACT_SITU)
+    big, bdw = experts.gated_backward(h, gu, offsets, route, w, ACT_SITU, out=gu)
+    assert torch.equal(big[-last:], dgu) and not big[:-last].any()
+    assert torch.equal(bdw[-last:], dw) and not bdw[:-last].any()
+    del gu, big
+    ids = torch.tensor([[0, 1]], dtype=torch.int32, device=cuda).expand(rows // 2, 2).contiguous()
+    out = experts.combine(h, ids, 2)
+    assert torch.equal(out[-1:], experts.combine(want, ids[:1].clone(), 2)) and not out[:-1].any()

@@ -197,3 +197,27 @@ def test_streams_and_graphs(cuda):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(again, want))
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_past_32_bits(cuda):
+    """Rows past 4 GiB of every tensor have the bits that they have alone."""
+    rows, cols = 131200, 16384
+    x, r = (torch.zeros((rows, cols), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    w = (1 + R.normal((cols,), 3, 0.2).float()).to(torch.bfloat16).to(cuda)
+    x[-3:], r[-3:] = R.normal((3, cols), 1).to(cuda), R.normal((3, cols), 2).to(cuda)
+    want = norm.residual_norm(x[-3:].clone(), w, EPS, residual=r[-3:].clone(), encode=True)
+    got = norm.residual_norm(x, w, EPS, residual=r, encode=True, total=x)
+    for a, b in zip(got, want):
+        assert torch.equal(a[-3:].view(torch.uint8), b.view(torch.uint8))
+    assert not got.normed[:-3].any()
+    dn, dt = R.normal((3, cols), 4).to(cuda), R.normal((3, cols), 5).to(cuda)
+    dx, dw = norm.residual_norm_backward(dn, want.total, w, want.rstd, dt)
+    r.zero_()
+    r[-3:] = dn
+    got.normed.zero_()
+    got.normed[-3:] = dt
+    big, bdw = norm.residual_norm_backward(r, x, w, got.rstd, got.normed, out=r)
+    assert torch.equal(big[-3:], dx) and not big[:-3].any()
+    # the weight's terms of the other rows are zeros: the three are added in another order
+    terms = (dn.double() * want.total.double() * want.rstd.double()[:, None]).abs().sum(0)
+    assert ((bdw - dw).double().abs() <= 8 * U * terms).all()
