@@ -593,8 +593,9 @@ __global__ __launch_bounds__(512) void grouped_few_kernel(GroupArgs A) {
  * f32 2060 to 2200 us by the card, 0.87 to 0.93 PFLOP/s (a large library product of such
  * operands 1.18), to bf16 1850. Bound by power, operands and the stages' own waits: of the last, on
  * zeros 1540 (the clock falls less), with the operands in L2 1610, with both 1265. Waves of 128 x 128, four of
- * them and 256 x 256 a block, read a third less of LDS, but one block a CU leaves its waits and
- * stores bare: 2030, on zeros 1970; 1000 tokens 790 and 645, 64 experts of 1024 x 2048 83 and 60.
+ * them and 256 x 256 a block, read a third less of LDS, but one wave a SIMD has its 250 instructions a
+ * stage to issue by itself and leaves its waits and stores bare: 1915, on zeros 1830; 1000 tokens 790
+ * and 645, 64 experts of 1024 x 2048 83 and 60.
  */
 struct Weight {
     static constexpr uint32_t BP = 128, BQ = 256, DEPTH = 32, STAGES = 3, WAVES = 4, THREADS = 256;
