@@ -138,6 +138,11 @@ def backward(doutput, saved, gate_up, down, dgate_up=None, ddown=None):
     """doutput bf16 [T, H] -> (dhidden bf16 [T, H], dweights f32 [T, top_k], dgate_up, ddown f32 as the
     weights). dgate_up and ddown, if given, are added to. The residual's gradient is doutput."""
     s, p = saved, saved.plan
+    (T, H), E, F = s.hidden.shape, p.experts, s.h.shape[1]
+    # a token that doutput lacks would be a row of zeros to the plan's indices
+    for t, name, shape in ((doutput, "doutput", (T, H)), (gate_up, "gate_up", (E, 2 * F, H)), (down, "down", (E, H, F))):
+        if t.shape != shape:
+            raise ValueError(f"{name}: {tuple(t.shape)}, wanted {shape}")
     dh = grouped.input_gradient(doutput, down, p.offsets, index=p.token_index)
     ddown = grouped.weight_gradient(doutput, s.h, p.offsets, dy_index=p.token_index, out=ddown,
                                     accumulate=ddown is not None)
