@@ -139,10 +139,17 @@ def backward(doutput, saved, gate_up, down, dgate_up=None, ddown=None):
     weights). dgate_up and ddown, if given, are added to. The residual's gradient is doutput."""
     s, p = saved, saved.plan
     (T, H), E, F = s.hidden.shape, p.experts, s.h.shape[1]
-    # a token that doutput lacks would be a row of zeros to the plan's indices
-    for t, name, shape in ((doutput, "doutput", (T, H)), (gate_up, "gate_up", (E, 2 * F, H)), (down, "down", (E, H, F))):
-        if t.shape != shape:
-            raise ValueError(f"{name}: {tuple(t.shape)}, wanted {shape}")
+    device = s.hidden.get_device()
+    # all before the first call: a token that doutput lacks would be a row of zeros to the plan's
+    # indices, and a gradient refused late would leave the other added to
+    for t, name, dtypes, shape in ((doutput, "doutput", _BF16, (T, H)), (gate_up, "gate_up", _BF16, (E, 2 * F, H)),
+                                   (down, "down", _BF16, (E, H, F)), (dgate_up, "dgate_up", _F32, (E, 2 * F, H)),
+                                   (ddown, "ddown", _F32, (E, H, F))):
+        if t is None and dtypes is _F32:
+            continue
+        at = _dense(t, name, dtypes, len(shape), device)
+        if t.shape != shape or at % 16 != 0:
+            raise ValueError(f"{name}: {tuple(t.shape)} at {at:#x}, wanted {shape} at a multiple of 16 bytes")
     dh = grouped.input_gradient(doutput, down, p.offsets, index=p.token_index)
     ddown = grouped.weight_gradient(doutput, s.h, p.offsets, dy_index=p.token_index, out=ddown,
                                     accumulate=ddown is not None)
