@@ -557,11 +557,11 @@ bool k3_moe_router_backward_f32(float *logits_gradient, const float *logits,
  * and the number of an expert's rows.
  * The weight gradient's output is f32 or bf16 [E, N, K]; an expert without rows has
  * gradient 0. accumulate (f32 only) adds to what output holds.
- * N and K multiples of 8 up to 32768; rows <= 65535 * 32, *_rows picked by an index
- * <= 65535; E <= 1024; less than 2^23 tiles of 16 rows x 16 or 256 x 128 columns (the
- * products) or of 128 x 256 values (the weight gradient); tensors 16-byte aligned; an output
- * over an operand, the offsets or an index is refused. No scratch. The reference only serves;
- * it has no counterpart.
+ * N and K multiples of 8 up to 32768; rows 1 to 65535 * 32 (of none, the caller's weight
+ * gradient is 0), *_rows picked by an index 1 to 65535; E <= 1024; less than 2^23 tiles of
+ * 16 rows x 16 or 256 x 128 columns (the products) or of 128 x 256 values (the weight
+ * gradient); tensors 16-byte aligned; an output over an operand, the offsets or an index is
+ * refused. No scratch. The reference only serves; it has no counterpart.
  */
 bool k3_moe_grouped_product_bf16(void *output, const void *input, const void *weights,
                                  const uint32_t *offsets, const uint32_t *input_index,
@@ -594,7 +594,7 @@ bool k3_moe_grouped_weight_gradient_bf16(void *output, bool f32, bool accumulate
  * with dh = output_gradient. weight_gradient ([routes], NULL: not wanted) is 0 for a
  * route without a row. Rows from offsets[E] on are left as they are; no two rows have one
  * route. gate_up_gradient may be gate_up itself; any other overlap of an output is
- * refused. F a multiple of 8 up to 32768; rows, routes <= 65535 * 32; E <= 1024;
+ * refused. F a multiple of 8 up to 32768; rows 1 to 65535 * 32, routes up to that; E <= 1024;
  * tensors 16-byte, the others 4-byte aligned.
  */
 bool k3_moe_gated_rows_bf16(void *output, const void *gate_up, const uint32_t *offsets,
@@ -615,7 +615,7 @@ bool k3_moe_gated_rows_backward_bf16(void *gate_up_gradient, float *weight_gradi
  * they hold. expert_weights NULL: 1, for rows that their weights are in already, and for
  * the routes' gradients of the token; residual NULL: none. output may be residual itself;
  * another overlap of it with an input is refused. hidden a multiple of 8 up to
- * 65536, T <= 65535, k <= 32; output, rows and residual 16-byte aligned.
+ * 65536, T 1 to 65535, k 1 to 32; output, rows and residual 16-byte aligned.
  */
 bool k3_moe_combine_bf16(void *output, const void *rows, const void *residual,
                          const void *expert_ids, const void *expert_weights, uint32_t token_count,
@@ -635,11 +635,11 @@ bool k3_moe_combine_bf16(void *output, const void *rows, const void *residual,
  *   input_gradient  = bf16(dt + rstd (dn weight - total rstd^2 mean(dn weight total)))
  *   weight_gradient = sum over rows of dn total rstd                  f32 [columns]
  * input_gradient is the residual's too, and may be any one of normed_gradient, total and
- * total_gradient itself; another overlap of an output, or of scratch, is refused. Sums are fp32 in an order set by the sizes. columns a
- * multiple of 8 up to 32768, rows <= 65535 * 32; weight bf16 [columns]; bf16 tensors
- * 16-byte, codes 8-byte, the others 4-byte aligned; scratch 256-byte aligned,
- * k3_moe_residual_norm_scratch_bytes(rows, columns) bytes (those of more rows serve
- * fewer).
+ * total_gradient itself; another overlap of an output, or of scratch, is refused. Squares and
+ * sums are fp32, in an order set by the sizes. columns a multiple of 8 up to 32768, rows 1 to
+ * 65535 * 32; weight bf16 [columns]; bf16 tensors 16-byte, codes 8-byte, the others 4-byte
+ * aligned; scratch 256-byte aligned, k3_moe_residual_norm_scratch_bytes(rows, columns) bytes
+ * (those of more rows serve fewer).
  */
 bool k3_moe_residual_norm_bf16(void *total, void *normed, uint8_t *codes, float *scales,
                                float *rstd, const void *input, const void *residual,

@@ -13,7 +13,8 @@ grouped.py and of gated, gated_backward and combine here, one after the other
 balance.router_backward. torch is used only for device memory and streams. Autograd
 does not see these calls: an input that requires a gradient is refused while
 gradients are recorded; in an autograd.Function, forward goes in forward and
-backward in backward.
+backward in backward. A batch of no tokens has empty outputs and weight gradients of
+zeros.
 """
 from dataclasses import dataclass
 
@@ -50,7 +51,8 @@ def gated(gate_up, offsets, route_index, weights, activation, beta=4.0, linear_b
         to = _dense(out, "out", _BF16, 2, device)
         if out.shape != (R, F):
             raise ValueError(f"out: {tuple(out.shape)}, wanted {(R, F)}")
-    _call(lib().k3_moe_gated_rows_bf16, device, to, at, o, i, w, R, routes, E, F, activation, beta, linear_beta)
+    if R != 0:
+        _call(lib().k3_moe_gated_rows_bf16, device, to, at, o, i, w, R, routes, E, F, activation, beta, linear_beta)
     return out
 
 
@@ -70,6 +72,8 @@ def gated_backward(dh, gate_up, offsets, route_index, weights, activation, beta=
         if out.shape != gate_up.shape:
             raise ValueError(f"out: {tuple(out.shape)}, wanted {tuple(gate_up.shape)}")
     dweights = weights.new_empty(weights.shape)
+    if R == 0:
+        return out, dweights.zero_()
     _call(lib().k3_moe_gated_rows_backward_bf16, device, to, dweights.data_ptr(), d, at, o, i, w, R, routes, E, F,
           activation, beta, linear_beta)
     return out, dweights
@@ -101,7 +105,8 @@ def combine(rows, ids, experts, residual=None, weights=None, out=None):
         to = _dense(out, "out", _BF16, 2, device)
         if out.shape != (T, H):
             raise ValueError(f"out: {tuple(out.shape)}, wanted {(T, H)}")
-    _call(lib().k3_moe_combine_bf16, device, to, at, r, i, w, T, k, experts, H)
+    if T != 0:
+        _call(lib().k3_moe_combine_bf16, device, to, at, r, i, w, T, k, experts, H)
     return out
 
 
@@ -126,7 +131,7 @@ def forward(hidden, ids, weights, gate_up, down, activation, beta=4.0, linear_be
         raise ValueError(f"gate_up {tuple(gate_up.shape)}, down {tuple(down.shape)}")
     if ids.shape != weights.shape or ids.shape[0] != hidden.shape[0]:
         raise ValueError(f"hidden {tuple(hidden.shape)}, ids {tuple(ids.shape)}, weights {tuple(weights.shape)}")
-    plan = grouped.route_plan(ids, E)
+    plan = grouped.route_plan(ids, E) if ids.shape[0] != 0 else grouped.no_routes(ids, E)
     gu = grouped.product(hidden, gate_up, plan.offsets, index=plan.token_index)
     h = gated(gu, plan.offsets, plan.route_index, weights, activation, beta, linear_beta)
     y = grouped.product(h, down, plan.offsets, to=plan.route_index)

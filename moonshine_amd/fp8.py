@@ -127,7 +127,7 @@ def product(x, codes, scales, out=None):
 
 def product_encoded(x_codes, x_scales, codes, scales, out=None):
     """product of rows that are encoded already (quantize_rows', or norm.residual_norm's): codes [T,
-    cols], scales [T, cols / 128] -> bf16 [T, rows]; out must not overlap them."""
+    cols], scales [T, cols / 128] -> bf16 [T, rows], empty for no rows; out must not overlap them."""
     at = _dense(x_codes, "x_codes", _CODES, 2)
     device = x_codes.get_device()
     xs = _dense(x_scales, "x_scales", _F32, 2, device)
@@ -143,6 +143,8 @@ def product_encoded(x_codes, x_scales, codes, scales, out=None):
         to = _dense(out, "out", _BF16, 2, device)
         if out.shape != (T, N):
             raise ValueError(f"out: {tuple(out.shape)}, wanted {(T, N)}")
+    if T == 0:
+        return out
     L = lib()
     n = L.k3_moe_fp8_128_scratch_bytes(T, N, K) if T > 1 else 0
     keep, room = _scratch(x_codes, n)

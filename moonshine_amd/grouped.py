@@ -8,7 +8,9 @@ requires a gradient is refused while gradients are recorded; in an
 autograd.Function, product goes in forward and the gradients in backward.
 
 Rows past the last expert's, and rows of an output that `to` sends nothing to, are
-left as they were: of an output made here they hold whatever its memory did.
+left as they were: of an output made here they hold whatever its memory did. Of no rows
+at all, outputs are empty and a weight gradient zeros (added up, out as it was), without a
+call of the library.
 """
 from dataclasses import dataclass
 
@@ -51,6 +53,13 @@ def route_plan(ids, experts):
     return RoutePlan(ids, experts, counts, offsets, token, route)
 
 
+def no_routes(ids, experts):
+    """The plan of no token's routes, ids int32 [0, top_k]."""
+    _dense(ids, "ids", _I32, 2)
+    none = ids.new_empty((0,))
+    return RoutePlan(ids, experts, ids.new_zeros((experts,)), ids.new_zeros((experts + 1,)), none, none)
+
+
 def _index(t, name, device):
     return None if t is None else _dense(t, name, _I32, 1, device)
 
@@ -59,6 +68,8 @@ def _rows(name, have, index, index_name):
     """Rows of the product by a tensor of `have` rows and an index (or None) of it."""
     if index is None:
         return have
+    if index.shape[0] == 0:
+        return 0
     if not 0 < have <= MOST_PICKED:
         raise ValueError(f"{name}: {have} rows; {index_name} picks from 1 to {MOST_PICKED}")
     return index.shape[0]
@@ -92,7 +103,8 @@ def _by_rows(fn, rows, name, weights, inner, outer, offsets, index, to, out):
         dst = _dense(out, "out", _BF16, 2, device)
         if out.shape[1] != width or (to is None and out.shape[0] < R):
             raise ValueError(f"out: {tuple(out.shape)}, wanted {(R, width)}")
-    _call(fn, device, dst, at, w, o, i, t, R, rows.shape[0], out.shape[0], E, N, K)
+    if R != 0:
+        _call(fn, device, dst, at, w, o, i, t, R, rows.shape[0], out.shape[0], E, N, K)
     return out
 
 
@@ -138,9 +150,11 @@ def weight_gradient(dy, x, offsets, dy_index=None, x_index=None, dtype=torch.flo
             raise ValueError(f"out: {tuple(out.shape)}, wanted {(E, N, K)}")
     if accumulate and dtype != torch.float32:
         raise ValueError("accumulate: a float32 out is wanted")
+    if R == 0:
+        return out if accumulate else out.zero_()
     _call(lib().k3_moe_grouped_weight_gradient_bf16, device, dst, dtype == torch.float32, accumulate, at, src,
           o, i, j, R, dy.shape[0], x.shape[0], E, N, K)
     return out
 
 
-__all__ = ["RoutePlan", "route_plan", "product", "input_gradient", "weight_gradient"]
+__all__ = ["RoutePlan", "route_plan", "no_routes", "product", "input_gradient", "weight_gradient"]

@@ -5,7 +5,8 @@ asked for, in FP8-128 for fp8.product_encoded; residual_norm_backward the gradie
 by the sum and by the norm's weight (include/k3_moe.h has the formulas). torch is
 used only for device memory and streams. Autograd does not see these calls: an
 input that requires a gradient is refused while gradients are recorded; in an
-autograd.Function, residual_norm goes in forward and the gradient in backward.
+autograd.Function, residual_norm goes in forward and the gradient in backward. Of no rows,
+outputs are empty and the weight's gradient zeros.
 """
 from typing import NamedTuple, Optional
 
@@ -69,7 +70,8 @@ def residual_norm(x, weight, epsilon, residual=None, normed=True, encode=False, 
         scales = x.new_empty((rows, cols // BLOCK), dtype=torch.float32)
         c, s = codes.data_ptr(), scales.data_ptr()
     rstd = x.new_empty((rows,), dtype=torch.float32)
-    _call(lib().k3_moe_residual_norm_bf16, device, t, n, c, s, rstd.data_ptr(), at, r, w, rows, cols, epsilon)
+    if rows != 0:
+        _call(lib().k3_moe_residual_norm_bf16, device, t, n, c, s, rstd.data_ptr(), at, r, w, rows, cols, epsilon)
     return Normed(x if residual is None else total, rstd, out, codes, scales)
 
 
@@ -90,6 +92,8 @@ def residual_norm_backward(dnormed, total, weight, rstd, dtotal=None, out=None):
     else:
         to = _like(out, "out", dnormed, device)
     dweight = dnormed.new_empty((cols,), dtype=torch.float32)
+    if rows == 0:
+        return out, dweight.zero_()
     L = lib()
     n = L.k3_moe_residual_norm_scratch_bytes(rows, cols)
     keep, room = _scratch(dnormed, n)
