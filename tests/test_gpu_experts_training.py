@@ -173,3 +173,73 @@ def test_no_row_at_all(cuda):
     assert torch.equal(out.cpu(), res)
     dx, dw, dgu, ddown = experts.backward(dout.to(cuda), saved, gu.to(cuda), down.to(cuda))
     assert not dx.any() and not dw.any() and not dgu.any() and not ddown.any()
+
+
+def slopes(g, u, act):
+    """The activation with its first and second derivatives, in 64 bits: v, (by g, by u), (gg, gu, uu)."""
+    g, u = g.clone().requires_grad_(), u.clone().requires_grad_()
+    v = activation(g, u, act)
+    by_g, by_u = torch.autograd.grad(v.sum(), (g, u), create_graph=True)
+    gg, gu = torch.autograd.grad(by_g.sum(), (g, u), retain_graph=True)
+    uu, = torch.autograd.grad(by_u.sum(), u, materialize_grads=True)  # SwiGLU's is 0
+    return v.detach(), (by_g.detach(), by_u.detach()), (gg, gu, uu)
+
+
+@pytest.mark.parametrize("act", [ACT_SITU, ACT_SWIGLU])
+@pytest.mark.parametrize("T,k,E,H,F", [(1, 2, 4, 64, 32), (7, 3, 5, 72, 40), (150, 2, 6, 264, 136), (600, 4, 8, 256, 128),
+                                       (90, 16, 896, 128, 64)])
+def test_each_value_within_its_roundings(cuda, act, T, k, E, H, F):
+    """Each value of a layer's outputs and gradients against the formula step by step in 64 bits. An error of
+    an input goes on by the magnitudes of the terms that it is in, and each step adds half a bf16 step of its
+    own value and Z fp32 steps of its terms' magnitudes (tests/_grouped.py; the activation, which
+    is within 2^-12 of its terms for these values, counts as a bf16 step more). Twice the sum, for the
+    products of errors."""
+    x, res, gu, down, ids, w, dout = problem(T, k, E, H, F, T + 1)
+    ids = ids.clone()
+    if T > 1:
+        ids[0, 1], ids[1, 0] = ids[0, 0], E
+    on = [t.to(cuda) for t in (x, ids, w, gu, down)]
+    out, saved = experts.forward(*on, act, residual=res.to(cuda))
+    got = dict(zip(("dx", "dw", "dgu", "ddown"), experts.backward(dout.to(cuda), saved, on[3], on[4])), out=out)
+    half, step = 2.0 ** -8, 2.0 ** -23
+    x, res, gu, down, w, dout = (t.double() for t in (x, res, gu, down, w, dout))
+    keep = live_routes(ids, E)
+    zeros = lambda *s: torch.zeros(s, dtype=torch.float64)  # noqa: E731
+    want = {n: zeros(*s) for n, s in dict(y=(T, H), dx=(T, H), dw=(T, k), dgu=(E, 2 * F, H), ddown=(E, H, F)).items()}
+    err = {n: torch.zeros_like(t) for n, t in want.items()}
+    for e in range(E):
+        t, r = torch.where((ids == e) & keep)
+        if len(t) == 0:
+            continue
+        n, wr = len(t), w[t, r][:, None]
+        z = x[t] @ gu[e].t()
+        ez = half * z.abs() + H * step * (x[t].abs() @ gu[e].abs().t())
+        (g, u), (eg, eu) = z.chunk(2, 1), ez.chunk(2, 1)
+        v, (by_g, by_u), (gg, gu_, uu) = slopes(g, u, act)
+        ev = by_g.abs() * eg + by_u.abs() * eu + half * v.abs()
+        h, eh = wr * v, wr * ev + half * (wr * v).abs()
+        y, ey = h @ down[e].t(), eh @ down[e].abs().t() + F * step * (h.abs() @ down[e].abs().t())
+        want["y"].index_add_(0, t, y)
+        err["y"].index_add_(0, t, ey + half * y.abs())
+        d = dout[t]
+        dh = d @ down[e]
+        edh = half * dh.abs() + H * step * (d.abs() @ down[e].abs())
+        want["dw"][t, r] = (dh * v).sum(1)
+        err["dw"][t, r] = (edh * v.abs() + dh.abs() * ev + F * step * (dh * v).abs()).sum(1)
+        dz = torch.cat([wr * dh * by_g, wr * dh * by_u], 1)
+        edz = torch.cat([wr * (edh * by_g.abs() + dh.abs() * (gg.abs() * eg + gu_.abs() * eu)),
+                         wr * (edh * by_u.abs() + dh.abs() * (gu_.abs() * eg + uu.abs() * eu))], 1)
+        edz = edz + 2 * half * dz.abs()
+        want["dgu"][e], want["ddown"][e] = dz.t() @ x[t], d.t() @ h
+        err["dgu"][e] = edz.t() @ x[t].abs() + n * step * (dz.abs().t() @ x[t].abs())
+        err["ddown"][e] = d.abs().t() @ eh + n * step * (d.abs().t() @ h.abs())
+        rows, size = dz @ gu[e], dz.abs() @ gu[e].abs()
+        want["dx"].index_add_(0, t, rows)
+        err["dx"].index_add_(0, t, edz @ gu[e].abs() + 2 * F * step * size + half * rows.abs())
+    for name in ("y", "dx"):  # the sum's own rounding
+        err[name] += (half + k * step) * want[name].abs()
+    want["out"] = want["y"] + res
+    err["out"] = err["y"] + half * want["out"].abs()
+    for name, value in got.items():
+        off, most = (value.cpu().double() - want[name]).abs(), 2 * err[name] + 2.0 ** -130
+        assert (off <= most).all(), (name, float((off / most).max()))
