@@ -32,8 +32,8 @@ struct GatedArgs {
     float beta, linear, by, by_linear; /* SiTU's bounds and their reciprocals */
 };
 
-/* sigmoid(g) and 1 - sigmoid(g), each to a few ulps of itself: of e^-|g|, so that neither is the
- * difference of numbers near 1. */
+/* sigmoid(g) and 1 - sigmoid(g), each to a few ulps of itself (0 where it is under 2^-126): of e^-|g|,
+ * so that neither is the difference of numbers near 1. */
 __device__ __forceinline__ void sigmoids(float g, float &s, float &rest) {
     const float e = __builtin_amdgcn_exp2f(__fmul_rn(fabsf(g), -1.44269504088896341f));
     const float big = __builtin_amdgcn_rcpf(__fadd_rn(1.0f, e)), small = __fmul_rn(e, big);

@@ -118,7 +118,11 @@ struct RowTile {
  * Row tile and column of work `block` among all experts' row tiles (of MOST rows at most) x
  * tiles_p columns, found by every wave for itself from the offsets: each lane counts the
  * tiles of up to 16 consecutive experts, and the lanes then take those of the one that holds
- * the tile. About 1 us, where a launch that lists the tiles takes 4. An expert's tiles
+ * the tile. About 1 us at 64 experts, where a launch that lists the tiles takes 4; past
+ * that a lane's experts are a load after the other: a launch that only looks its 256 tiles up takes 4.0 us
+ * of 64 experts, 3.7 of 128, 5.9 of 256, 13.5 of 512 and 31.5 of 896, and the products of 32 rows each of 64
+ * of them, 1024 x 512, 14.0 us of 64 and 42.7 of 896. Where most experts have rows it is less of the whole:
+ * 1024 rows of 613 of 896 experts of 1024 x 1024 230 us, of which their weights take 211. An expert's tiles
  * of one column are neighbours, as they read the same weights; XCD x (blocks x,
  * x + 8, ...) takes a contiguous range of the works. False past the end.
  */
@@ -500,9 +504,10 @@ __device__ __forceinline__ void row_tile(const GroupArgs &A, uint8_t *smem, cons
 /*
  * Tiles of 64 WN columns. A block's class goes by the rows of its expert: a CU holds one block
  * of any, so the largest's registers and LDS cost the others nothing. With few rows an expert bound by the
- * weights, read once: 488 rows of 32 experts of 7168 x 2048 165 us, 5.7 TB/s (a large read 6.1). With
- * many by the matrix units and what feeds them: 32768 rows of 4096 x 7168 1510 us, 1.27 PFLOP/s (a large
- * library product 1.45), the input gradient of 7168 x 2048 800 us, 1.20. A stage of 256 x 256 takes 1.14
+ * weights, read once: 488 rows of 32 experts of 7168 x 2048 170 us, 5.5 TB/s (a large read 6.1). With
+ * many by the matrix units and what feeds them: 32768 rows of 4096 x 7168 1570 us, 1.23 PFLOP/s (a large
+ * library product 1.45), the input gradient of 7168 x 2048 830 us, 1.16 (medians of forty calls once the
+ * clock has settled; the least 1505 and 807). A stage of 256 x 256 takes 1.14
  * us with its operands in L2, 1.37 from memory, and 1.01 of matrix instructions alone; more stages,
  * blocks that stay and load their next tile ahead (1690 us), other orders and staggered starts measured
  * level or slower.
@@ -529,7 +534,7 @@ __global__ __launch_bounds__(128 * WN, WN / 2) void grouped_rows_kernel(GroupArg
  * of 32, so that a wave reads whole 128-byte lines, straight into the registers of the MFMA
  * layout, and add up through LDS in one order. More blocks than tiles of 256 p, and
  * no stage to fill: bound by the latency of two loads, then by the weights' stream. 4 rows of 4 of 64
- * experts of 1024 x 2048 5.4 us, of which their 16.8 MB take 2.8 at 6.1 TB/s.
+ * experts of 1024 x 2048 5.9 us (5.3 from the caches), of which their 16.8 MB take 2.8 at 6.1 TB/s.
  */
 __global__ __launch_bounds__(512) void grouped_few_kernel(GroupArgs A) {
     __shared__ f32x4 sums[8][64];
@@ -936,19 +941,22 @@ bool over_plan(const void *output, uint64_t bytes, const uint32_t *offsets, uint
            (other && overlap(output, bytes, other, 4u * (uint64_t)rows));
 }
 
-/* Most blocks of a product that goes 16 rows x 16 columns a block. us, so and by tiles of 256
- * columns, rows of experts chosen at random: 1024 x 2048, 4 of 64 experts, 4 rows (256 blocks) 5.1 and
- * 15.6, 8 rows 8.0 and 16.4, 16 rows (1024) 15.3 and 16.9, 32 rows 22.0 and 18.3; 2048 x 512, 8
- * rows (1024) 5.8 and 7.0, 16 rows 12.5 and 7.1; 7168 x 2048, 8 rows (3584) 44.9 and 36.9. */
+/* Most blocks of a product that goes 16 rows x 16 columns a block. us, weights from memory, so, by tiles
+ * of 128 columns (narrow_tiles: what these products get instead) and of 256; rows of experts chosen at random
+ * of 64: 1024 x 2048, 4 rows (256 blocks) 5.9, 10.4 and 15.9, 8 rows (512) 9.0, 10.7 and 16.2, 16 rows
+ * (1088) 15.6, 14.6 and 20.8, 32 rows (2176) 21.9, 21.2 and 29.1; 2048 x 512, 4 rows (512) 4.5, 5.2 and 6.9,
+ * 8 rows (1024) 6.9, 5.9 and 7.1, 16 rows (2176) 10.8, 9.2 and 10.6; of 32, 7168 x 2048, 2 rows (896) 15.4,
+ * 11.6 and 16.4. Past 512 blocks the tiles of 128 are ahead by up to a quarter. */
 constexpr uint64_t kFewBlocks = 1024;
 
 /* Tiles of 128 columns instead of 256, where these leave half of the CUs without one: `used`
- * experts have up to 128 rows each, if these are spread evenly, and so one row tile. us, of 256 and
- * of 128 columns (N x K): product of 1040 x 1096, 24 experts, 24 rows 10.5 and 7.4, 384 rows 18.0 and
- * 12.7, 3000 rows 31.4 and 23.6, but 6000 rows 33.2 and 40.9; input gradient of 2048 x 512, 64
- * experts, 244 rows 18.1 and 14.7, 8000 rows 46.0 and 33.5; with more tiles, product of 1024 x
- * 1024, 40 experts (160), 366 rows 14.4 and 17.9, of 1024 x 2048, 64 experts (256), 244 rows 23.7
- * and 29.6. */
+ * experts have up to 128 rows each, if these are spread evenly, and so one row tile. us, weights from
+ * memory, of 256 and of 128 columns (N x K): product of 1040 x 1096, 24 experts, 24 rows 23.4 and 14.2, 384 rows
+ * 26.4 and 17.1, 3000 rows 35.9 and 26.3, but 6000 rows 40.8 and 52.7; its input gradient, 24 rows 16.9 and
+ * 11.8, 3000 rows 29.2 and 22.9, 6000 rows 33.6 and 47.6; input gradient of 2048 x 512, 64 experts, 244 rows
+ * 32.2 and 26.9, 8000 rows 48.9 and 38.6; with more tiles, product of 1024 x 1024, 40 experts (160), 64 rows
+ * 16.6 and 14.5, 366 rows 18.6 and 21.9, 1500 rows 20.0 and 24.7, of 1024 x 2048, 64 experts (256), 64 rows 46.7
+ * and 47.5, 244 rows 62.8 and 60.0. Weights that the caches hold give the same order. */
 bool narrow_tiles(uint32_t used, uint32_t rows, uint32_t P) {
     return (uint64_t)used * ((P + 255u) / 256u) <= 128u && rows <= 128u * used;
 }
